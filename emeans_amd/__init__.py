@@ -21,8 +21,9 @@ from typing import List, Optional, Tuple
 import numpy as np
 
 from . import model_file
-from ._lib import (EMH_IP, EMH_L2, EMH_PROF_EMA, EMH_PROF_SCATTER, EMH_PROF_SCREEN,
-                   Config as _CConfig, DedupConfig as _CDedupConfig,
+from ._lib import (EMH_ADAMW_BLOCK, EMH_BF16, EMH_F16, EMH_F32, EMH_F8, EMH_IP, EMH_L2,
+                   EMH_PROF_EMA, EMH_PROF_SCATTER, EMH_PROF_SCREEN, EMH_U32,
+                   AdamConfig as _CAdamConfig, AdamTensor as _CAdamTensor, Config as _CConfig, DedupConfig as _CDedupConfig,
                    DedupInput as _CDedupInput, DedupResult as _CDedupResult, EmeansHipError,
                    EmeansHipInvalid, EpochStats as _CEpoch, TrainInit as _CTrainInit,
                    TrainOut as _CTrainOut, check, lib)
@@ -33,12 +34,15 @@ __all__ = [
     "knn_self", "knn", "dedup", "dedup_with_neighbors", "make_assigner", "available_backends",
     "Backend", "BACKEND_NAME", "EmeansHipError", "EmeansHipInvalid",
     "GPU_KMAX", "KLONG", "NONE",
+    "AdamTensor", "AdamW", "F32", "U32", "F16", "BF16", "F8",
 ]
 
 BACKEND_NAME = "hip"
 GPU_KMAX = 16          # emeans-core/src/knn.rs:16: the screened top-k's largest k
 KLONG = 4096           # the exact top-k's largest k beyond GPU_KMAX (no CPU fallback)
 NONE = 0xFFFFFFFF      # emeans-core/src/knn.rs:19
+# What a buffer's elements are (HipDevice.wrap, zeros).
+F32, U32, F16, BF16, F8 = EMH_F32, EMH_U32, EMH_F16, EMH_BF16, EMH_F8
 
 
 def _metric(m) -> int:
@@ -195,8 +199,27 @@ class HipDevice:
     def sync(self):
         check(lib().emh_sync(self._ctx))
 
+    def zeros(self, n: int, kind: int) -> DevBuf:
+        """n zeros of any kind (F32 .. F8)."""
+        return self._new(lib().emh_zeros, n, kind, kind=kind)
+
+    _NP = {F32: np.float32, U32: np.uint32, F16: np.float16, BF16: np.uint16, F8: np.uint8}
+
+    def write(self, b: DevBuf, offset: int, v):
+        """b[offset ..] = v for a buffer of any kind (bf16 and f8 as raw bits)."""
+        v = np.ascontiguousarray(v, dtype=self._NP[b.kind])
+        check(lib().emh_write(self._ctx, b.h, offset, _p(v), v.size))
+
+    def read(self, b: DevBuf, rng=None) -> np.ndarray:
+        """The elements of a buffer of any kind (bf16 and f8 as raw bits)."""
+        lo, hi = rng if rng is not None else (0, len(b))
+        out = np.empty(max(hi - lo, 0), self._NP[b.kind])
+        check(lib().emh_read(self._ctx, b.h, lo, hi, _p(out)))
+        return out
+
     def wrap(self, ptr: int, length: int, kind: int) -> DevBuf:
-        """A non-owning view of device memory (e.g. a torch tensor's data_ptr())."""
+        """A non-owning view of device memory (e.g. a torch tensor's data_ptr())
+        of `length` elements of a kind (F32 .. F8)."""
         h = C.c_void_p()
         check(lib().emh_wrap(self._ctx, C.c_void_p(ptr), length, kind, C.byref(h)))
         return DevBuf(self, h, kind)
@@ -243,6 +266,25 @@ class HipDevice:
                    d: int, step: EmaStep):
         check(lib().emh_ema_update(self._ctx, positions.h, usage.h, sums.h, counts.h, k, d,
                                    step.alpha, step.decay, int(step.replace)))
+
+    # -- learning operators
+    def layer_norm(self, x: DevBuf, rows: int, d: int, weight: Optional[DevBuf],
+                   bias: Optional[DevBuf], y: DevBuf, mean: Optional[DevBuf] = None,
+                   rstd: Optional[DevBuf] = None, eps: float = 1e-5, ldx: int = 0, ldy: int = 0):
+        """y = (x - mean) rstd weight + bias of every row of x (rows x d, F32, F16
+        or BF16; ldx, ldy: row strides in elements, 0 = d). mean and rstd (F32,
+        rows entries) are what layer_norm_grad takes. y may be x."""
+        check(lib().emh_layer_norm(self._ctx, x.h, ldx, rows, d, _h(weight), _h(bias), eps, y.h,
+                                   ldy, _h(mean), _h(rstd)))
+
+    def layer_norm_grad(self, dy: DevBuf, x: DevBuf, rows: int, d: int, weight: Optional[DevBuf],
+                        mean: DevBuf, rstd: DevBuf, dx: Optional[DevBuf],
+                        dweight: Optional[DevBuf] = None, dbias: Optional[DevBuf] = None,
+                        lddy: int = 0, ldx: int = 0, lddx: int = 0):
+        """The gradients of layer_norm's rows (may be dy), weight and bias (F32
+        or x's kind) from that of its result; each may be None."""
+        check(lib().emh_layer_norm_grad(self._ctx, dy.h, lddy, x.h, ldx, rows, d, _h(weight),
+                                        mean.h, rstd.h, _h(dx), lddx, _h(dweight), _h(dbias)))
 
     # -- Assigner::assign (assign_all over assign_on)
     def assign(self, x, d: int, centroids, metric, chunk: int = 65536):
@@ -387,6 +429,62 @@ class HipDevice:
         2)) take the exact kernels alone even when the mode screens (default
         EXACT_BELOW); 0 screens every call the mode screens. Same bits."""
         check(lib().emh_set_exact_below(self._ctx, int(items)))
+
+
+def _h(b: Optional[DevBuf]):
+    return None if b is None else b.h
+
+
+@dataclass
+class AdamTensor:
+    """One tensor of an AdamW plan: param and grad (F32, F16 or BF16), the states
+    m and v (F32, or F8 with m_scale and v_scale: F32, an entry for every
+    AdamW.BLOCK elements), all zero to begin with; copy (F16 or BF16) gets
+    the new parameters rounded."""
+    param: DevBuf
+    grad: DevBuf
+    m: DevBuf
+    v: DevBuf
+    m_scale: Optional[DevBuf] = None
+    v_scale: Optional[DevBuf] = None
+    copy: Optional[DevBuf] = None
+    weight_decay: float = 0.0
+
+
+class AdamW:
+    """AdamW over many tensors in one launch: a plan that keeps their addresses
+    (and the buffers alive)."""
+    BLOCK = EMH_ADAMW_BLOCK
+
+    def __init__(self, dev: HipDevice, tensors: List[AdamTensor]):
+        self._h = None
+        self._dev, self._tensors = dev, list(tensors)
+        table = (_CAdamTensor * max(len(self._tensors), 1))()
+        for c, t in zip(table, self._tensors):
+            c.param, c.grad, c.m, c.v = t.param.h, t.grad.h, t.m.h, t.v.h
+            c.m_scale, c.v_scale, c.copy = _h(t.m_scale), _h(t.v_scale), _h(t.copy)
+            c.weight_decay = t.weight_decay
+        h = C.c_void_p()
+        check(lib().emh_adamw_create(dev._ctx, table, len(self._tensors), C.byref(h)))
+        self._h = h
+
+    def step(self, lr: float, step: int, beta1: float = 0.9, beta2: float = 0.999,
+             eps: float = 1e-8, grad_scale: float = 1.0):
+        """One step over all tensors; step counts from 1."""
+        cfg = _CAdamConfig(lr, beta1, beta2, eps, grad_scale, step)
+        check(lib().emh_adamw_step(self._h, C.byref(cfg)))
+
+    def close(self):
+        """Free the plan (not the tensors)."""
+        if self._h and self._dev._ctx:
+            check(lib().emh_adamw_destroy(self._h))
+        self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 def _train_init(k, d, init, state):

@@ -12,6 +12,8 @@ LIB_PATH = os.path.join(HERE, "libemeans_hip.so")
 
 EMH_OK, EMH_INVALID, EMH_ERROR = 0, 1, 2
 EMH_L2, EMH_IP = 0, 1
+EMH_F32, EMH_U32, EMH_F16, EMH_BF16, EMH_F8 = 0, 1, 2, 3, 4
+EMH_ADAMW_BLOCK = 256
 EMH_PROF_SCREEN, EMH_PROF_SCATTER, EMH_PROF_EMA = 0, 1, 2
 
 
@@ -79,6 +81,17 @@ class DedupResult(C.Structure):
                 ("split_components", C.c_uint64)]
 
 
+class AdamTensor(C.Structure):
+    _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("m", C.c_void_p),
+                ("v", C.c_void_p), ("m_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("copy", C.c_void_p), ("weight_decay", C.c_double)]
+
+
+class AdamConfig(C.Structure):
+    _fields_ = [("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double),
+                ("eps", C.c_double), ("grad_scale", C.c_double), ("step", C.c_uint64)]
+
+
 # name: (restype, argtypes). Every function is declared in include/emeans_hip.h.
 _vp, _sz, _i, _u32, _u64, _f, _d = (C.c_void_p, C.c_size_t, C.c_int, C.c_uint32, C.c_uint64,
                                      C.c_float, C.c_double)
@@ -102,6 +115,15 @@ SIGNATURES = {
     "emh_read_u32": (_i, [_vp, _vp, _sz, _sz, _vp]),
     "emh_free": (_i, [_vp, _vp]),
     "emh_wrap": (_i, [_vp, _vp, _sz, _i, _pp]),
+    "emh_zeros": (_i, [_vp, _sz, _i, _pp]),
+    "emh_write": (_i, [_vp, _vp, _sz, _vp, _sz]),
+    "emh_read": (_i, [_vp, _vp, _sz, _sz, _vp]),
+    "emh_layer_norm": (_i, [_vp, _vp, _sz, _sz, _sz, _vp, _vp, _f, _vp, _sz, _vp, _vp]),
+    "emh_layer_norm_grad": (_i, [_vp, _vp, _sz, _vp, _sz, _sz, _sz, _vp, _vp, _vp, _vp, _sz, _vp,
+                                 _vp]),
+    "emh_adamw_create": (_i, [_vp, _vp, _sz, _pp]),
+    "emh_adamw_step": (_i, [_vp, _vp]),
+    "emh_adamw_destroy": (_i, [_vp]),
     "emh_buf_ptr": (_vp, [_vp]),
     "emh_buf_len": (_sz, [_vp]),
     "emh_top1": (_i, [_vp, _vp, _sz, _vp, _sz, _sz, _vp, _vp, _sz, _i, _vp, _vp]),

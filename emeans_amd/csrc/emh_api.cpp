@@ -223,20 +223,21 @@ emh_buf* new_buf(emh_ctx* c, size_t len, int kind) {
   b->kind = kind;
   b->serial = ++g_serial;
   b->device = c->device;
-  if (len > 0 && len * 4 <= KEEP_BLOCK_MAX) {
+  const size_t bytes = emh::buf_bytes(len, kind);
+  if (len > 0 && bytes <= KEEP_BLOCK_MAX) {
     try {
-      b->ptr = take_kept(c, len * 4);
+      b->ptr = take_kept(c, bytes);
     } catch (...) {
       delete b;
       throw;
     }
   }
   if (len > 0 && !b->ptr) {
-    hipError_t e = hipMalloc(&b->ptr, len * 4);
+    hipError_t e = hipMalloc(&b->ptr, bytes);
     if (e != hipSuccess) {
       delete b;
       char m[256];
-      snprintf(m, sizeof m, "hipMalloc of %zu bytes failed: %s", len * 4, hipGetErrorString(e));
+      snprintf(m, sizeof m, "hipMalloc of %zu bytes failed: %s", bytes, hipGetErrorString(e));
       throw emh::Failure(m);
     }
   }
@@ -267,10 +268,13 @@ void check_device_flags(emh_ctx* c) {
   EMH_HIP(hipMemcpyAsync(w, c->small, sizeof w, hipMemcpyDeviceToHost, c->stream));
   EMH_HIP(hipStreamSynchronize(c->stream));
   bool bad_label = w[emh::SW_BAD_LABEL] != 0, bad_id = w[emh::SW_BAD_ID] != 0;
-  if (bad_label || bad_id) {
+  const bool bad_class = w[emh::SW_BAD_CLASS] != 0;
+  if (bad_label || bad_id || bad_class) {
     emh::launch_fill_u32(c, c->small + emh::SW_BAD_LABEL, 1, 0);
     emh::launch_fill_u32(c, c->small + emh::SW_BAD_ID, 1, 0);
+    emh::launch_fill_u32(c, c->small + emh::SW_BAD_CLASS, 1, 0);
     EMH_HIP(hipStreamSynchronize(c->stream));
+    EMH_ENSURE(!bad_class, "cross_entropy: label out of range");
     EMH_ENSURE(!bad_label, "scatter_add: label out of range");
     EMH_ENSURE(!bad_id, "row id out of range");
   }
@@ -354,7 +358,8 @@ int emh_destroy(emh_ctx* c) {
                             &c->xnorm, &c->bigj, &c->chunkcnt, &c->tickets,
                             &c->preview_ticket, &c->xsplit, &c->xsplit_norm, &c->csplit, &c->csplit_norm, &c->csplit_part,
                             &c->cmean, &c->tframe, &c->xpre, &c->xpre_norm, &c->tsplit, &c->tsplit_norm, &c->tsplit_part, &c->tally_cnt,
-                            &c->log5, &c->klong, &c->trun, &c->kpp, &c->iscore, &c->cnorm})
+                            &c->log5, &c->klong, &c->trun, &c->kpp, &c->iscore, &c->cnorm, &c->norm_part,
+                            &c->xent})
       s->release();
     for (emh::Pinned* s : {&c->pin_usage, &c->pin_plan, &c->pin_small, &c->pin_order[0],
                            &c->pin_order[1], &c->pin_lab[0], &c->pin_lab[1], &c->pin_sco[0],
@@ -429,21 +434,30 @@ static int zeros(emh_ctx* c, size_t len, int kind, emh_buf** out) {
     EMH_ENSURE(c && out, "null argument");
     use_device(c);
     emh_buf* b = new_buf(c, len, kind);
-    if (len > 0) emh::launch_fill_u32(c, (uint32_t*)b->ptr, len, 0);
+    if (len > 0) emh::launch_fill_u32(c, (uint32_t*)b->ptr, emh::buf_bytes(len, kind) / 4, 0);
     *out = b;
   });
 }
 int emh_zeros_f32(emh_ctx* c, size_t len, emh_buf** out) { return zeros(c, len, 0, out); }
 int emh_zeros_u32(emh_ctx* c, size_t len, emh_buf** out) { return zeros(c, len, 1, out); }
 
+int emh_zeros(emh_ctx* c, size_t len, int kind, emh_buf** out) {
+  if (kind < EMH_F32 || kind > EMH_F8)
+    return guard([&] { EMH_ENSURE(false, "kind %d must be 0 to 4", kind); });
+  return zeros(c, len, kind, out);
+}
+
+// kind < 0: any.
 static int write(emh_ctx* c, emh_buf* b, size_t off, const void* v, size_t len, int kind) {
   return guard([&] {
-    EMH_ENSURE(c && b && b->kind == kind, "buffer kind mismatch");
-    EMH_ENSURE(off + len <= b->len, "write past the buffer");
+    EMH_ENSURE(c && b && (kind < 0 || b->kind == kind), "buffer kind mismatch");
+    EMH_ENSURE(off <= b->len && len <= b->len - off, "write past the buffer");
     if (len == 0) return;
+    EMH_ENSURE(v, "null source");
     use_device(c);
     ++b->gen;
-    EMH_HIP(hipMemcpyAsync((char*)b->ptr + off * 4, v, len * 4, hipMemcpyHostToDevice,
+    const size_t e = emh::kind_bytes(b->kind);
+    EMH_HIP(hipMemcpyAsync((char*)b->ptr + off * e, v, len * e, hipMemcpyHostToDevice,
                            c->stream));
     EMH_HIP(hipStreamSynchronize(c->stream));
   });
@@ -455,13 +469,19 @@ int emh_write_u32(emh_ctx* c, emh_buf* b, size_t off, const uint32_t* v, size_t 
   return write(c, b, off, v, len, 1);
 }
 
+int emh_write(emh_ctx* c, emh_buf* b, size_t off, const void* v, size_t len) {
+  return write(c, b, off, v, len, -1);
+}
+
 static int read(emh_ctx* c, const emh_buf* b, size_t lo, size_t hi, void* dst, int kind) {
   return guard([&] {
-    EMH_ENSURE(c && b && b->kind == kind, "buffer kind mismatch");
+    EMH_ENSURE(c && b && (kind < 0 || b->kind == kind), "buffer kind mismatch");
     EMH_ENSURE(lo <= hi && hi <= b->len, "read past the buffer");
+    EMH_ENSURE(hi == lo || dst, "null destination");
     use_device(c);
+    const size_t e = emh::kind_bytes(b->kind);
     if (hi > lo)
-      EMH_HIP(hipMemcpyAsync(dst, (const char*)b->ptr + lo * 4, (hi - lo) * 4,
+      EMH_HIP(hipMemcpyAsync(dst, (const char*)b->ptr + lo * e, (hi - lo) * e,
                              hipMemcpyDeviceToHost, c->stream));
     check_device_flags(c);  // waits
   });
@@ -471,6 +491,9 @@ int emh_read_f32(emh_ctx* c, const emh_buf* b, size_t lo, size_t hi, float* dst)
 }
 int emh_read_u32(emh_ctx* c, const emh_buf* b, size_t lo, size_t hi, uint32_t* dst) {
   return read(c, b, lo, hi, dst, 1);
+}
+int emh_read(emh_ctx* c, const emh_buf* b, size_t lo, size_t hi, void* dst) {
+  return read(c, b, lo, hi, dst, -1);
 }
 
 int emh_free(emh_ctx* c, emh_buf* b) {
@@ -490,7 +513,7 @@ int emh_free(emh_ctx* c, emh_buf* b) {
     // A buffer whose address went out may be in use on streams of the
     // caller's own: hipFree waits for them.
     if (keep)
-      keep_block(c, p, b->len * 4);
+      keep_block(c, p, emh::buf_bytes(b->len, b->kind));
     else if (p)
       EMH_HIP(hipFree(p));
   });
@@ -499,7 +522,8 @@ int emh_free(emh_ctx* c, emh_buf* b) {
 int emh_wrap(emh_ctx* c, void* p, size_t len, int kind, emh_buf** out) {
   return guard([&] {
     EMH_ENSURE(c && out, "null argument");
-    EMH_ENSURE(kind == 0 || kind == 1, "kind must be 0 (f32) or 1 (u32)");
+    EMH_ENSURE(kind >= EMH_F32 && kind <= EMH_F8,
+               "kind %d must be 0 (f32), 1 (u32), 2 (f16), 3 (bf16) or 4 (f8)", kind);
     EMH_ENSURE(len == 0 || p, "null pointer");
     auto* b = new emh_buf;
     b->ptr = p;

@@ -44,6 +44,13 @@ struct Failure : std::runtime_error {
 
 void set_last_error(const std::string& m);
 
+// Bytes of an element of a buffer kind (EMH_F32 ..), and of a buffer of len
+// elements (whole words: fills write words).
+inline size_t kind_bytes(int kind) { return kind == EMH_F8 ? 1 : kind >= EMH_F16 ? 2 : 4; }
+inline size_t buf_bytes(size_t len, int kind) {
+  return (len * kind_bytes(kind) + 3) & ~(size_t)3;
+}
+
 // Device scratch that grows on demand and is reused by later calls.
 struct Scratch {
   void* ptr = nullptr;
@@ -156,6 +163,7 @@ enum SmallWord : int {
   SW_TICKET = 6,          // blocks of the scatter count kernel that have finished (reset by the last)
   SW_NBIG = 7,            // clusters of the current scatter with more rows than the per-column path takes
   SW_BAD_INIT = 8,        // set when a training run's initial centroids are not finite
+  SW_BAD_CLASS = 9,       // set when the cross entropy saw a label >= k that is not NONE
   SW_WORDS = 16,
 };
 // The rows whose fp16 lines a context may hold at once (emh_lines.h), besides a
@@ -188,7 +196,7 @@ constexpr int SCALE_ROWS_READ = 32;  // rows that the scale looks at (half beyon
 struct emh_buf {
   void* ptr = nullptr;
   size_t len = 0;   // elements
-  int kind = 0;     // 0 f32, 1 u32
+  int kind = 0;     // EMH_F32 ..
   bool owned = true;
   int device = -1;  // where the library allocated it
   // Which buffer and which contents, for the split rows a context keeps: a
@@ -243,6 +251,8 @@ struct emh_ctx {
   // carved from a block kept between calls, since hipFree waits for the
   // whole device, the other contexts' streams included.
   emh::Scratch trun, kpp, iscore, cnorm;
+  emh::Scratch norm_part;  // layer_norm_grad: the blocks' sums of dweight and dbias
+  emh::Scratch xent;       // cross_entropy's parts, gradients of a piece and laid-out operands
   emh::Scratch preview_ticket;  // k_mass_preview's last-block ticket (left at zero)
   // Host staging of the device loop: masses, plan, flags, epoch orders and
   // epoch labels/scores (double-buffered), results.

@@ -1,0 +1,51 @@
+// Launchers of the learning operators (layer norm, cross entropy, AdamW), and
+// the arguments that their entry points (emh_learn.cpp) have checked.
+#pragma once
+
+#include "emh_internal.h"
+
+namespace emh {
+
+// A row-major matrix or vector of a run-time kind.
+struct MatIn {
+  const void* p = nullptr;
+  size_t ld = 0;
+  int kind = EMH_F32;
+};
+struct MatOut {
+  void* p = nullptr;
+  size_t ld = 0;
+  int kind = EMH_F32;
+};
+
+// ---- emh_norm.hip
+void launch_layer_norm(emh_ctx* c, const MatIn& x, size_t rows, size_t d, const MatIn& weight,
+                       const MatIn& bias, float eps, const MatOut& y, float* mean, float* rstd);
+void launch_layer_norm_grad(emh_ctx* c, const MatIn& dy, const MatIn& x, size_t rows, size_t d,
+                            const MatIn& weight, const float* mean, const float* rstd,
+                            const MatOut& dx, const MatOut& dweight, const MatOut& dbias);
+
+// ---- emh_adamw.hip
+struct AdamTensor {  // as the kernel reads it
+  void* param;
+  const void* grad;
+  void* m;
+  void* v;
+  float* m_scale;  // 8-bit states: not null
+  float* v_scale;
+  void* copy;
+  uint64_t len;
+  double weight_decay;
+  int param_kind, grad_kind, copy_kind, pad;
+};
+struct AdamScalars {
+  float beta1, beta2, new1, new2;  // new = 1 - beta
+  float rate, inv2, eps, gscale;   // lr / (1 - beta1^t), 1 / (1 - beta2^t)
+  double lr;
+};
+constexpr size_t ADAM_CHUNK = 4096;  // elements of a workgroup's share of one tensor
+// chunks[i]: the tensor and the chunk in it that workgroup i takes.
+void launch_adamw(emh_ctx* c, const AdamTensor* tensors, const uint2* chunks, size_t nchunks,
+                  const AdamScalars& s);
+
+}  // namespace emh

@@ -1,0 +1,439 @@
+// Layer norm's forward and backward pass over the rows of a matrix.
+//
+// Forward, for a row x of d elements: mean = sum x / d, var = sum (x - mean)^2 /
+// d, y = (x - mean) rstd w + b. The row stays in registers between the two sums
+// and the result, so memory is read once; the second sum is over differences
+// (sum x^2 - mean^2 would cancel where a row's mean exceeds its spread).
+//
+// Backward, with h = (x - mean) rstd and g = dy w: dx = rstd (g - mean(g) - h
+// mean(g h)); dweight = sum over rows of dy h, dbias = sum of dy. A thread owns
+// the same columns in every row that its workgroup takes, so both sums over the
+// rows grow in its registers, in f32; a workgroup adds its groups' through LDS and leaves
+// one row of sums, and a second launch adds those. No atomics: the order of
+// every sum follows from the sizes.
+//
+// Bound by HBM: 2 (forward) and 3 (backward) elements moved per element.
+#include <algorithm>
+
+#include "emh_learn.h"
+#include "emh_types.h"
+
+namespace emh {
+namespace {
+
+struct NormArgs {
+  const void* x;
+  size_t ldx;
+  const void* dy;
+  size_t lddy;
+  size_t rows;
+  int d;
+  const void* w;
+  const void* b;
+  int wkind, bkind;
+  float eps;
+  void* y;  // forward: y; backward: dx
+  size_t ldy;
+  float* mean;
+  float* rstd;
+  float* part;  // backward: [block][2][d], or null
+};
+
+// Sums over the LPR lanes (threads, past a wave) that share a row, in all of
+// them. red: LDS, one float for every wave, and a row of the workgroup's groups
+// for each of the calls that may follow one another without a barrier.
+template <int LPR, int TB>
+__device__ __forceinline__ float row_sum(float v, float (*red)[TB / 64], int slot) {
+  v = lanes_sum<(LPR < 64 ? LPR : 64)>(v);
+  if constexpr (LPR > 64) {
+    const int w = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) red[slot][w] = v;
+    __syncthreads();
+    constexpr int NW = LPR / 64;
+    const int w0 = w / NW * NW;
+    v = 0.f;
+#pragma unroll
+    for (int i = 0; i < NW; i++) v += red[slot][w0 + i];
+  }
+  return v;
+}
+
+template <class T>
+__device__ __forceinline__ Vec<T> load_cols(const T* row, int col, int d) {
+  constexpr int N = VecOf<T>::N;
+  if (col + N <= d) return load_vec(row + col);
+  return load_some(row + min(col, d), d - col);
+}
+template <class T>
+__device__ __forceinline__ void store_cols(T* row, int col, int d, const float* v) {
+  constexpr int N = VecOf<T>::N;
+  if (col + N <= d)
+    store_vec(row + col, v);
+  else
+    store_some(row + min(col, d), v, d - col);
+}
+
+// Forward: LPR threads a row, NV vectors of 16 bytes a thread.
+template <class T, int LPR, int NV>
+__global__ __launch_bounds__(256) void k_norm(const NormArgs a) {
+  constexpr int N = VecOf<T>::N, TB = 256, G = TB / LPR;
+  __shared__ float red[4][TB / 64];
+  const int l = threadIdx.x % LPR, g = threadIdx.x / LPR;
+  const int d = a.d;
+  float w[NV * N], b[NV * N];
+#pragma unroll
+  for (int j = 0; j < NV; j++)
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+      const int col = (l + LPR * j) * N + e;
+      w[j * N + e] = a.w && col < d ? load_kind(a.w, a.wkind, col) : 1.f;
+      b[j * N + e] = a.b && col < d ? load_kind(a.b, a.bkind, col) : 0.f;
+    }
+  const float inv = 1.0f / (float)d;
+  int slot = 0;
+  // (The bound is the workgroup's: all its threads meet at row_sum's barriers.)
+  for (size_t r0 = (size_t)blockIdx.x * G; r0 < a.rows; r0 += (size_t)gridDim.x * G) {
+    const size_t row = r0 + g;
+    const bool live = row < a.rows;
+    const T* x = reinterpret_cast<const T*>(a.x) + (live ? row : 0) * a.ldx;
+    Vec<T> v[NV];
+#pragma unroll
+    for (int j = 0; j < NV; j++) v[j] = load_cols(x, (l + LPR * j) * N, d);
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; j++)
+#pragma unroll
+      for (int e = 0; e < N; e++) s += v[j].get(e);  // zeros past d
+    const float mean = row_sum<LPR, TB>(s, red, slot) * inv;
+    float q = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; j++)
+#pragma unroll
+      for (int e = 0; e < N; e++) {
+        const float o = v[j].get(e) - mean;
+        q = fmaf(o, (l + LPR * j) * N + e < d ? o : 0.f, q);
+      }
+    const float rstd = 1.0f / sqrtf(row_sum<LPR, TB>(q, red, slot ^ 1) * inv + a.eps);
+    slot ^= 2;
+    if (!live) continue;
+    T* y = reinterpret_cast<T*>(a.y) + row * a.ldy;
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+      float o[N];
+#pragma unroll
+      for (int e = 0; e < N; e++)
+        o[e] = fmaf((v[j].get(e) - mean) * rstd, w[j * N + e], b[j * N + e]);
+      store_cols(y, (l + LPR * j) * N, d, o);
+    }
+    if (l == 0 && a.mean) a.mean[row] = mean;
+    if (l == 0 && a.rstd) a.rstd[row] = rstd;
+  }
+}
+
+// Backward, TB threads: the next row's loads are in flight while a row's sums
+// are formed.
+template <class T, int LPR, int NV, int TB>
+__global__ __launch_bounds__(TB) void k_norm_grad(const NormArgs a) {
+  constexpr int N = VecOf<T>::N, G = TB / LPR;
+  __shared__ float red[4][TB / 64];
+  __shared__ float fold[G > 1 ? TB * NV * N : 1];
+  const int l = threadIdx.x % LPR, g = threadIdx.x / LPR;
+  const int d = a.d;
+  float w[NV * N], aw[NV * N], ab[NV * N];
+#pragma unroll
+  for (int j = 0; j < NV; j++)
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+      const int col = (l + LPR * j) * N + e;
+      w[j * N + e] = a.w && col < d ? load_kind(a.w, a.wkind, col) : 1.f;
+      aw[j * N + e] = ab[j * N + e] = 0.f;
+    }
+  const float inv = 1.0f / (float)d;
+  Vec<T> x[NV], dy[NV];
+  float mean, rstd;
+  auto fetch = [&](size_t row) __attribute__((always_inline)) {
+    const bool live = row < a.rows;
+    const size_t r = live ? row : 0;
+    const T* xp = reinterpret_cast<const T*>(a.x) + r * a.ldx;
+    const T* dp = reinterpret_cast<const T*>(a.dy) + r * a.lddy;
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+      x[j] = load_cols(xp, (l + LPR * j) * N, d);
+      dy[j] = load_cols(dp, (l + LPR * j) * N, d);
+    }
+    mean = a.mean[r];
+    rstd = a.rstd[r];
+  };
+  const size_t step = (size_t)gridDim.x * G;
+  int slot = 0;
+  size_t r0 = (size_t)blockIdx.x * G;
+  if (r0 < a.rows) fetch(r0 + g);
+  for (; r0 < a.rows; r0 += step) {
+    const size_t row = r0 + g;
+    const bool live = row < a.rows;
+    float h[NV * N], u[NV * N];
+    float c1 = 0.f, c2 = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; j++)
+#pragma unroll
+      for (int e = 0; e < N; e++) {
+        const int i = j * N + e;
+        const bool in = live && (l + LPR * j) * N + e < d;
+        h[i] = in ? (x[j].get(e) - mean) * rstd : 0.f;
+        const float t = in ? dy[j].get(e) : 0.f;
+        ab[i] += t;
+        aw[i] = fmaf(t, h[i], aw[i]);
+        u[i] = t * w[i];
+        c1 += u[i];
+        c2 = fmaf(u[i], h[i], c2);
+      }
+    const float rs = rstd;
+    if (r0 + step < a.rows) fetch(r0 + step + g);
+    c1 = row_sum<LPR, TB>(c1, red, slot) * inv;
+    c2 = row_sum<LPR, TB>(c2, red, slot ^ 1) * inv;
+    slot ^= 2;
+    if (live && a.y) {
+      T* o = reinterpret_cast<T*>(a.y) + row * a.ldy;
+#pragma unroll
+      for (int j = 0; j < NV; j++) {
+        float t[N];
+#pragma unroll
+        for (int e = 0; e < N; e++)
+          t[e] = rs * (u[j * N + e] - c1 - h[j * N + e] * c2);
+        store_cols(o, (l + LPR * j) * N, d, t);
+      }
+    }
+  }
+  if (!a.part) return;
+  // The groups' sums of a column, added by the first group: dweight, then dbias.
+#pragma unroll
+  for (int which = 0; which < 2; which++) {
+    float* v = which ? ab : aw;
+    if constexpr (G > 1) {
+      if (which) __syncthreads();
+#pragma unroll
+      for (int i = 0; i < NV * N; i++) fold[i * TB + threadIdx.x] = v[i];
+      __syncthreads();
+    }
+    if (g == 0) {
+      float* out = a.part + ((size_t)blockIdx.x * 2 + which) * d;
+#pragma unroll
+      for (int j = 0; j < NV; j++) {
+        float s[N];
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+          if constexpr (G > 1) {
+            s[e] = 0.f;
+            for (int k = 0; k < G; k++) s[e] += fold[(j * N + e) * TB + k * LPR + l];
+          } else {
+            s[e] = v[j * N + e];
+          }
+        }
+        const int col = (l + LPR * j) * N;
+#pragma unroll
+        for (int e = 0; e < N; e++)
+          if (col + e < d) out[col + e] = s[e];
+      }
+    }
+  }
+}
+
+// Rows too long for the registers of a workgroup: one workgroup a row, read
+// again for every step (from L2, mostly).
+template <class T>
+__global__ __launch_bounds__(256) void k_norm_wide(const NormArgs a) {
+  __shared__ float red[4][4];
+  const T* x = reinterpret_cast<const T*>(a.x) + (size_t)blockIdx.x * a.ldx;
+  T* y = reinterpret_cast<T*>(a.y) + (size_t)blockIdx.x * a.ldy;
+  float s = 0.f;
+  for (int i = threadIdx.x; i < a.d; i += 256) s += to_f32(x[i]);
+  const float mean = row_sum<256, 256>(s, red, 0) / (float)a.d;
+  float q = 0.f;
+  for (int i = threadIdx.x; i < a.d; i += 256) {
+    const float o = to_f32(x[i]) - mean;
+    q = fmaf(o, o, q);
+  }
+  const float rstd = 1.0f / sqrtf(row_sum<256, 256>(q, red, 1) / (float)a.d + a.eps);
+  for (int i = threadIdx.x; i < a.d; i += 256) {
+    const float h = (to_f32(x[i]) - mean) * rstd;
+    y[i] = from_f32<T>(fmaf(h, a.w ? load_kind(a.w, a.wkind, i) : 1.f,
+                            a.b ? load_kind(a.b, a.bkind, i) : 0.f));
+  }
+  if (threadIdx.x == 0 && a.mean) a.mean[blockIdx.x] = mean;
+  if (threadIdx.x == 0 && a.rstd) a.rstd[blockIdx.x] = rstd;
+}
+template <class T>
+__global__ __launch_bounds__(256) void k_norm_grad_wide(const NormArgs a) {
+  __shared__ float red[4][4];
+  const T* x = reinterpret_cast<const T*>(a.x) + (size_t)blockIdx.x * a.ldx;
+  const T* dy = reinterpret_cast<const T*>(a.dy) + (size_t)blockIdx.x * a.lddy;
+  T* o = reinterpret_cast<T*>(a.y) + (size_t)blockIdx.x * a.ldy;
+  const float mean = a.mean[blockIdx.x], rstd = a.rstd[blockIdx.x];
+  float c1 = 0.f, c2 = 0.f;
+  for (int i = threadIdx.x; i < a.d; i += 256) {
+    const float u = to_f32(dy[i]) * (a.w ? load_kind(a.w, a.wkind, i) : 1.f);
+    c1 += u;
+    c2 = fmaf(u, (to_f32(x[i]) - mean) * rstd, c2);
+  }
+  c1 = row_sum<256, 256>(c1, red, 0) / (float)a.d;
+  c2 = row_sum<256, 256>(c2, red, 1) / (float)a.d;
+  for (int i = threadIdx.x; i < a.d; i += 256) {
+    const float u = to_f32(dy[i]) * (a.w ? load_kind(a.w, a.wkind, i) : 1.f);
+    o[i] = from_f32<T>(rstd * (u - c1 - (to_f32(x[i]) - mean) * rstd * c2));
+  }
+}
+// Their sums over rows: a thread a column, blockIdx.y a share of the rows.
+template <class T>
+__global__ __launch_bounds__(256) void k_norm_cols(const NormArgs a) {
+  const int col = blockIdx.x * 256 + threadIdx.x;
+  if (col >= a.d) return;
+  const size_t per = (a.rows + gridDim.y - 1) / gridDim.y;
+  const size_t lo = blockIdx.y * per, hi = min(a.rows, lo + per);
+  float sw = 0.f, sb = 0.f;
+#pragma unroll 4
+  for (size_t r = lo; r < hi; r++) {
+    const float t = to_f32(reinterpret_cast<const T*>(a.dy)[r * a.lddy + col]);
+    const float h = (to_f32(reinterpret_cast<const T*>(a.x)[r * a.ldx + col]) - a.mean[r]) * a.rstd[r];
+    sw = fmaf(t, h, sw);
+    sb += t;
+  }
+  a.part[((size_t)blockIdx.y * 2) * a.d + col] = sw;
+  a.part[((size_t)blockIdx.y * 2 + 1) * a.d + col] = sb;
+}
+
+// out = the nparts rows of sums added: 64 columns a workgroup, 16 shares of the
+// rows in step and then one after another.
+__global__ __launch_bounds__(1024) void k_norm_sums(const float* __restrict__ part, int nparts,
+                                                    int d, void* dw, int dwkind, void* db,
+                                                    int dbkind) {
+  __shared__ float s[16][64];
+  const int c = threadIdx.x & 63, g = threadIdx.x >> 6;
+  const int col = blockIdx.x * 64 + c;
+  float v = 0.f;
+  if (col < 2 * d) {
+#pragma unroll 8
+    for (int i = g; i < nparts; i += 16) v += part[(size_t)i * 2 * d + col];
+  }
+  s[g][c] = v;
+  __syncthreads();
+  if (g != 0 || col >= 2 * d) return;
+  v = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; i++) v += s[i][c];
+  if (col < d) {
+    if (dw) store_kind(dw, dwkind, col, v);
+  } else if (db) {
+    store_kind(db, dbkind, col - d, v);
+  }
+}
+// No rows: the sums are zero.
+__global__ __launch_bounds__(256) void k_norm_zero(int d, void* dw, int dwkind, void* db,
+                                                   int dbkind) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= d) return;
+  if (dw) store_kind(dw, dwkind, i, 0.f);
+  if (db) store_kind(db, dbkind, i, 0.f);
+}
+
+template <class F>
+void by_kind(int kind, F&& f) {
+  if (kind == EMH_F32)
+    f(float{});
+  else if (kind == EMH_F16)
+    f(f16{});
+  else
+    f(bf16{});
+}
+template <int L, int V>
+struct Shape {
+  static constexpr int LPR = L, NV = V;
+};
+// The threads that share a row and the vectors each holds: the fewest that hold
+// the row. False: none does.
+template <class T, class F>
+bool by_shape(size_t d, F&& f) {
+  const size_t v = (d + VecOf<T>::N - 1) / VecOf<T>::N;
+  if (v <= 16)
+    f(Shape<16, 1>{});
+  else if (v <= 64)
+    f(Shape<64, 1>{});
+  else if (v <= 128)
+    f(Shape<64, 2>{});
+  else if (v <= 192)
+    f(Shape<64, 3>{});
+  else if (v <= 256)
+    f(Shape<64, 4>{});
+  else if (v <= 512)
+    f(Shape<256, 2>{});
+  else if (v <= 1024)
+    f(Shape<256, 4>{});
+  else
+    return false;
+  return true;
+}
+
+}  // namespace
+
+void launch_layer_norm(emh_ctx* c, const MatIn& x, size_t rows, size_t d, const MatIn& weight,
+                       const MatIn& bias, float eps, const MatOut& y, float* mean, float* rstd) {
+  if (rows == 0) return;
+  NormArgs a{};
+  a.x = x.p, a.ldx = x.ld, a.rows = rows, a.d = (int)d;
+  a.w = weight.p, a.wkind = weight.kind, a.b = bias.p, a.bkind = bias.kind;
+  a.eps = eps, a.y = y.p, a.ldy = y.ld, a.mean = mean, a.rstd = rstd;
+  by_kind(x.kind, [&](auto t) {
+    using T = decltype(t);
+    const bool held = by_shape<T>(d, [&](auto s) {
+      using S = decltype(s);
+      constexpr size_t G = 256 / S::LPR;
+      const size_t blocks = std::min((rows + G - 1) / G, (size_t)c->cus * 8);
+      k_norm<T, S::LPR, S::NV><<<dim3((unsigned)blocks), 256, 0, c->stream>>>(a);
+    });
+    if (!held) k_norm_wide<T><<<dim3((unsigned)rows), 256, 0, c->stream>>>(a);
+  });
+  EMH_HIP(hipGetLastError());
+}
+
+void launch_layer_norm_grad(emh_ctx* c, const MatIn& dy, const MatIn& x, size_t rows, size_t d,
+                            const MatIn& weight, const float* mean, const float* rstd,
+                            const MatOut& dx, const MatOut& dweight, const MatOut& dbias) {
+  NormArgs a{};
+  a.x = x.p, a.ldx = x.ld, a.dy = dy.p, a.lddy = dy.ld, a.rows = rows, a.d = (int)d;
+  a.w = weight.p, a.wkind = weight.kind, a.y = dx.p, a.ldy = dx.ld;
+  a.mean = const_cast<float*>(mean), a.rstd = const_cast<float*>(rstd);
+  const bool sums = dweight.p || dbias.p;
+  if (rows == 0) {
+    if (sums)
+      k_norm_zero<<<grid1(d, 256), 256, 0, c->stream>>>((int)d, dweight.p, dweight.kind, dbias.p,
+                                                        dbias.kind);
+    EMH_HIP(hipGetLastError());
+    return;
+  }
+  size_t parts = 0;
+  by_kind(x.kind, [&](auto t) {
+    using T = decltype(t);
+    const bool held = by_shape<T>(d, [&](auto s) {
+      using S = decltype(s);
+      // A workgroup a CU: as many waves as its registers allow, and the fewest
+      // rows of sums to write and add.
+      constexpr int TB = S::NV * VecOf<T>::N <= 16 ? 1024 : 512;
+      constexpr size_t G = TB / S::LPR;
+      parts = std::min((rows + G - 1) / G, (size_t)c->cus * (1024 / TB));
+      if (sums) a.part = (float*)c->norm_part.get(parts * 2 * d * 4);
+      k_norm_grad<T, S::LPR, S::NV, TB><<<dim3((unsigned)parts), TB, 0, c->stream>>>(a);
+    });
+    if (held) return;
+    if (sums) {  // before dx, which may overwrite dy
+      parts = std::min((rows + 15) / 16, (size_t)64);
+      a.part = (float*)c->norm_part.get(parts * 2 * d * 4);
+      k_norm_cols<T><<<dim3((unsigned)((d + 255) / 256), (unsigned)parts), 256, 0, c->stream>>>(a);
+    }
+    if (dx.p) k_norm_grad_wide<T><<<dim3((unsigned)rows), 256, 0, c->stream>>>(a);
+  });
+  if (sums)
+    k_norm_sums<<<grid1(2 * d, 64), 1024, 0, c->stream>>>(a.part, (int)parts, (int)d, dweight.p,
+                                                          dweight.kind, dbias.p, dbias.kind);
+  EMH_HIP(hipGetLastError());
+}
+
+}  // namespace emh

@@ -1,0 +1,122 @@
+// Loads and stores of the learning operators' element types, as f32 in
+// registers: vectors of up to 16 bytes from any address that an element may
+// have (the hardware takes unaligned global accesses).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace emh {
+
+// Sixteen and eight bytes at an element's alignment.
+struct __attribute__((packed, aligned(2))) Any16 {
+  uint32_t w[4];
+};
+struct __attribute__((packed, aligned(2))) Any8 {
+  uint32_t w[2];
+};
+
+typedef _Float16 f16;
+typedef __bf16 bf16;
+
+template <class T>
+struct VecOf {
+  static constexpr int N = 16 / sizeof(T);  // elements of a 16-byte vector
+};
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(f16 v) { return (float)v; }
+__device__ __forceinline__ float to_f32(bf16 v) { return (float)v; }
+template <class T>
+__device__ __forceinline__ T from_f32(float v) {
+  return (T)v;  // nearest, ties to even
+}
+
+// A 16-byte vector's raw bits and its elements.
+template <class T>
+struct Vec {
+  static constexpr int N = VecOf<T>::N;
+  uint4 raw;
+  __device__ __forceinline__ float get(int e) const {
+    if constexpr (sizeof(T) == 4) {
+      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+      return __uint_as_float(w[e]);
+    } else {
+      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+      const uint16_t b = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+      return to_f32(__builtin_bit_cast(T, b));
+    }
+  }
+};
+template <class T>
+__device__ __forceinline__ Vec<T> load_vec(const T* p) {
+  const Any16 a = *reinterpret_cast<const Any16*>(p);
+  return Vec<T>{make_uint4(a.w[0], a.w[1], a.w[2], a.w[3])};
+}
+// The elements p[0 .. left), left < N; the others zero.
+template <class T>
+__device__ __forceinline__ Vec<T> load_some(const T* p, int left) {
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int e = 0; e < VecOf<T>::N; e++) {
+    if (e >= left) continue;
+    if constexpr (sizeof(T) == 4)
+      w[e] = __float_as_uint(p[e]);
+    else
+      w[e >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, p[e]) << (16 * (e & 1));
+  }
+  return Vec<T>{make_uint4(w[0], w[1], w[2], w[3])};
+}
+template <class T>
+__device__ __forceinline__ void store_vec(T* p, const float* v) {
+  Any16 a;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) a.w[e] = __float_as_uint(v[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+      a.w[e] = (uint32_t)__builtin_bit_cast(uint16_t, from_f32<T>(v[2 * e])) |
+               (uint32_t)__builtin_bit_cast(uint16_t, from_f32<T>(v[2 * e + 1])) << 16;
+  }
+  *reinterpret_cast<Any16*>(p) = a;
+}
+template <class T>
+__device__ __forceinline__ void store_some(T* p, const float* v, int left) {
+#pragma unroll
+  for (int e = 0; e < VecOf<T>::N; e++)
+    if (e < left) p[e] = from_f32<T>(v[e]);
+}
+
+// Element i of a buffer whose kind is a run-time value (EMH_F32, EMH_F16,
+// EMH_BF16).
+__device__ __forceinline__ float load_kind(const void* p, int kind, size_t i) {
+  if (kind == EMH_F32) return reinterpret_cast<const float*>(p)[i];
+  if (kind == EMH_F16) return (float)reinterpret_cast<const f16*>(p)[i];
+  return (float)reinterpret_cast<const bf16*>(p)[i];
+}
+__device__ __forceinline__ void store_kind(void* p, int kind, size_t i, float v) {
+  if (kind == EMH_F32)
+    reinterpret_cast<float*>(p)[i] = v;
+  else if (kind == EMH_F16)
+    reinterpret_cast<f16*>(p)[i] = (f16)v;
+  else
+    reinterpret_cast<bf16*>(p)[i] = (bf16)v;
+}
+
+// Sums over groups of W consecutive lanes (W a power of two, at most 64), in
+// every lane.
+template <int W>
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+  for (int o = W / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+template <int W>
+__device__ __forceinline__ float lanes_max(float v) {
+#pragma unroll
+  for (int o = W / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  return v;
+}
+
+}  // namespace emh

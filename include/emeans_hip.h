@@ -36,8 +36,16 @@ extern "C" {
 #define EMH_IP 1
 
 typedef struct emh_ctx emh_ctx;
-/* A device buffer of f32 or u32 (Device::F / Device::U). */
+/* A device buffer of f32 or u32 (Device::F / Device::U), or of one of the
+ * narrower kinds that the learning operators take. */
 typedef struct emh_buf emh_buf;
+
+/* What a buffer's elements are. */
+#define EMH_F32 0
+#define EMH_U32 1
+#define EMH_F16 2  /* IEEE half precision */
+#define EMH_BF16 3 /* the upper half of an f32 */
+#define EMH_F8 4   /* e4m3: 4 exponent and 3 mantissa bits, largest 448, no infinities */
 
 /* Message of the last failed call on this thread (emeans-ffi/src/lib.rs:95-140). */
 const char* emh_last_error(void);
@@ -84,10 +92,15 @@ int emh_read_u32(emh_ctx* ctx, const emh_buf* b, size_t lo, size_t hi, uint32_t*
  * when it fails. */
 int emh_free(emh_ctx* ctx, emh_buf* b);
 /* A non-owning view of caller device memory (for example a torch tensor) as a
- * buffer; freeing the view does not free the memory. kind: 0 f32, 1 u32. */
+ * buffer; freeing the view does not free the memory. kind: EMH_F32 .. EMH_F8. */
 int emh_wrap(emh_ctx* ctx, void* dev_ptr, size_t len, int kind, emh_buf** out);
 void* emh_buf_ptr(const emh_buf* b);
 size_t emh_buf_len(const emh_buf* b);
+/* zeros, write and read for a buffer of any kind: v and dst hold the elements as
+ * the device does (bf16 and f8 as raw bits). */
+int emh_zeros(emh_ctx* ctx, size_t len, int kind, emh_buf** out);
+int emh_write(emh_ctx* ctx, emh_buf* b, size_t offset, const void* v, size_t len);
+int emh_read(emh_ctx* ctx, const emh_buf* b, size_t lo, size_t hi, void* dst);
 
 /* --------------------------------------------------------------------- ops */
 /* Device::top1 (core/mod.rs:97-112): for every selected position p in
@@ -329,6 +342,69 @@ int emh_internal_scores(emh_ctx* ctx, const emh_buf* x, size_t n, size_t d, cons
  * dots with thresholds). Queued; read out to wait. */
 int emh_dots(emh_ctx* ctx, const emh_buf* a, size_t m, const emh_buf* b, size_t nb, size_t d,
              emh_buf* out);
+
+/* ---------------------------------------------- learning operators */
+/* A training step on the rows and labels of a clustering (no counterpart in the
+ * reference): a layer norm, the cross entropy of a linear classifier over the
+ * clusters, their gradients, and the AdamW step. Matrices are row-major; a row
+ * stride (ld..., in elements, 0 = the row's length) may exceed the row. Buffers
+ * may start at any address that their element allows. All calls are queued;
+ * sums and statistics are held in f32 whatever the buffers' kinds. An output
+ * may be one of the inputs only where that is said; other overlaps are refused. */
+
+/* Layer norm of each row of x (rows x d, f32, f16 or bf16): y = (x - mean) rstd
+ * weight + bias, rstd = 1 / sqrt(mean((x - mean)^2) + eps). weight and bias (d
+ * entries, x's kind or f32) may be NULL (ones, zeros). y: x's kind, may be x.
+ * mean and rstd (f32, rows entries): for the gradient; both may be NULL. */
+int emh_layer_norm(emh_ctx* ctx, const emh_buf* x, size_t ldx, size_t rows, size_t d,
+                   const emh_buf* weight, const emh_buf* bias, float eps, emh_buf* y, size_t ldy,
+                   emh_buf* mean, emh_buf* rstd);
+/* Its gradient: dy and x (one kind), and mean and rstd as emh_layer_norm left
+ * them. With h = (x - mean) rstd and g = dy weight: dx = rstd (g - mean(g) - h
+ * mean(g h)) (x's kind, may be dy), dweight = sum over rows of dy h, dbias =
+ * sum of dy (d entries, f32 or x's kind, overwritten). Each of the three may
+ * be NULL. The sums' order depends on the sizes alone. */
+int emh_layer_norm_grad(emh_ctx* ctx, const emh_buf* dy, size_t lddy, const emh_buf* x, size_t ldx,
+                        size_t rows, size_t d, const emh_buf* weight, const emh_buf* mean,
+                        const emh_buf* rstd, emh_buf* dx, size_t lddx, emh_buf* dweight,
+                        emh_buf* dbias);
+
+/* One tensor of an AdamW step. param: f32, f16 or bf16; grad: f32, f16 or bf16,
+ * as long. copy (f16 or bf16, as long, may be NULL) gets the new parameters
+ * rounded, for a master copy in f32. States of 32 bits: m and v f32, the scales
+ * NULL. States of 8 bits: m and v f8, m_scale and v_scale f32 with an entry for
+ * every 256 elements (EMH_ADAMW_BLOCK): m = code m_scale, sqrt(v) = code v_scale;
+ * zeros to begin with. */
+#define EMH_ADAMW_BLOCK 256
+typedef struct emh_adamw_tensor {
+  emh_buf* param;
+  const emh_buf* grad;
+  emh_buf* m;
+  emh_buf* v;
+  emh_buf* m_scale;
+  emh_buf* v_scale;
+  emh_buf* copy;
+  double weight_decay;
+} emh_adamw_tensor;
+typedef struct emh_adamw_config {
+  double lr, beta1, beta2, eps;
+  double grad_scale; /* the gradients are multiplied by it */
+  uint64_t step;     /* 1 for the first */
+} emh_adamw_config;
+typedef struct emh_adamw emh_adamw;
+/* A plan over count tensors, which keeps their addresses: the buffers outlive it,
+ * and it its context's last step. No tensor that the step writes may overlap
+ * another. */
+int emh_adamw_create(emh_ctx* ctx, const emh_adamw_tensor* tensors, size_t count, emh_adamw** out);
+/* One step over all of them, in one launch: g = grad_scale grad, m = beta1 m + (1 - beta1) g,
+ * v = beta2 v + (1 - beta2) g^2, param = param (1 - lr weight_decay) - lr
+ * (m / (1 - beta1^step)) / (sqrt(v / (1 - beta2^step)) + eps), from the unrounded
+ * m and v. 8-bit states are rounded anew: a block's scale is its largest
+ * magnitude / 448, its values the nearest codes of value / scale (a positive v at least
+ * the least positive code; an element that is not finite gets a NaN and has no
+ * part in the scale). */
+int emh_adamw_step(emh_adamw* plan, const emh_adamw_config* cfg);
+int emh_adamw_destroy(emh_adamw* plan);
 
 /* ------------------------------------------------- host replay (no device) */
 /* The seeded host-side pieces of the device loop, exported so that callers and
