@@ -286,6 +286,25 @@ class HipDevice:
         check(lib().emh_layer_norm_grad(self._ctx, dy.h, lddy, x.h, ldx, rows, d, _h(weight),
                                         mean.h, rstd.h, _h(dx), lddx, _h(dweight), _h(dbias)))
 
+    def cross_entropy(self, x: DevBuf, n: int, d: int, w: DevBuf, k: int, labels: DevBuf,
+                      loss: DevBuf, lse: Optional[DevBuf] = None, scale: float = 1.0,
+                      ldx: int = 0, ldw: int = 0):
+        """loss[i] = lse[i] - z[i, labels[i]] with z = scale x w^T and lse the log
+        of its rows' sums of exponentials (x: n x d, w: k x d, one kind; labels:
+        U32, NONE for a row without one, whose loss is 0)."""
+        check(lib().emh_cross_entropy(self._ctx, x.h, ldx, n, d, w.h, ldw, k, labels.h, scale,
+                                      loss.h, _h(lse)))
+
+    def cross_entropy_grad(self, x: DevBuf, n: int, d: int, w: DevBuf, k: int, labels: DevBuf,
+                           lse: DevBuf, dx: Optional[DevBuf], dw: Optional[DevBuf],
+                           gloss: Optional[DevBuf] = None, scale: float = 1.0, ldx: int = 0,
+                           ldw: int = 0, lddx: int = 0, lddw: int = 0):
+        """The gradients of cross_entropy's losses weighted by gloss (F32), or of
+        the mean over the rows with a label, into dx (n x d) and dw (k x d), of
+        x's kind; either may be None."""
+        check(lib().emh_cross_entropy_grad(self._ctx, x.h, ldx, n, d, w.h, ldw, k, labels.h, scale,
+                                           lse.h, _h(gloss), _h(dx), lddx, _h(dw), lddw))
+
     # -- Assigner::assign (assign_all over assign_on)
     def assign(self, x, d: int, centroids, metric, chunk: int = 65536):
         x, c = _f32(x), _f32(centroids)

@@ -121,6 +121,9 @@ SIGNATURES = {
     "emh_layer_norm": (_i, [_vp, _vp, _sz, _sz, _sz, _vp, _vp, _f, _vp, _sz, _vp, _vp]),
     "emh_layer_norm_grad": (_i, [_vp, _vp, _sz, _vp, _sz, _sz, _sz, _vp, _vp, _vp, _vp, _sz, _vp,
                                  _vp]),
+    "emh_cross_entropy": (_i, [_vp, _vp, _sz, _sz, _sz, _vp, _sz, _sz, _vp, _f, _vp, _vp]),
+    "emh_cross_entropy_grad": (_i, [_vp, _vp, _sz, _sz, _sz, _vp, _sz, _sz, _vp, _f, _vp, _vp, _vp,
+                                    _sz, _vp, _sz]),
     "emh_adamw_create": (_i, [_vp, _vp, _sz, _pp]),
     "emh_adamw_step": (_i, [_vp, _vp]),
     "emh_adamw_destroy": (_i, [_vp]),

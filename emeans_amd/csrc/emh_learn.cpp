@@ -180,6 +180,95 @@ int emh_layer_norm_grad(emh_ctx* c, const emh_buf* dy, size_t lddy, const emh_bu
   });
 }
 
+}  // extern "C"
+
+namespace {
+struct XentCall {
+  emh::XentIn in;
+  Range x, w, labels;
+};
+XentCall check_xent(emh_ctx* c, const emh_buf* x, size_t ldx, size_t n, size_t d, const emh_buf* w,
+                    size_t ldw, size_t k, const emh_buf* labels, float scale) {
+  EMH_ENSURE(c, "null context");
+  EMH_ENSURE(d > 0 && d <= (size_t(1) << 24), "d must be 1 to 2^24");
+  EMH_ENSURE(k > 0 && k <= (size_t(1) << 30), "k must be 1 to 2^30");
+  EMH_ENSURE(n <= (size_t(1) << 30), "too many rows");
+  EMH_ENSURE(x && real_kind(x->kind), "x must be an f32, f16 or bf16 buffer");
+  EMH_ENSURE(w && w->kind == x->kind, "w must be of x's kind");
+  EMH_ENSURE(labels && labels->kind == EMH_U32, "labels must be a u32 buffer");
+  EMH_ENSURE(std::isfinite(scale), "scale must be finite");
+  XentCall t{};
+  t.x = check_matrix(x, n, d, ldx, "x");
+  t.w = check_matrix(w, k, d, ldw, "w");
+  t.labels = check_vector(labels, n, "labels");
+  t.in = {{x->ptr, ldx, x->kind}, {w->ptr, ldw, w->kind}, n, d, k, (const uint32_t*)labels->ptr,
+          scale};
+  return t;
+}
+void apart_from_inputs(const Range& r, const XentCall& t, const char* what) {
+  apart(r, t.x, what, "x");
+  apart(r, t.w, what, "w");
+  apart(r, t.labels, what, "labels");
+}
+}  // namespace
+
+extern "C" {
+
+int emh_cross_entropy(emh_ctx* c, const emh_buf* x, size_t ldx, size_t n, size_t d,
+                      const emh_buf* w, size_t ldw, size_t k, const emh_buf* labels, float scale,
+                      emh_buf* loss, emh_buf* lse) {
+  return guard([&] {
+    const XentCall t = check_xent(c, x, ldx, n, d, w, ldw, k, labels, scale);
+    const Range rl = check_f32(loss, n, "loss");
+    apart_from_inputs(rl, t, "loss");
+    if (lse) {
+      const Range rs = check_f32(lse, n, "lse");
+      apart_from_inputs(rs, t, "lse");
+      apart(rs, rl, "lse", "loss");
+    }
+    if (n == 0) return;
+    use_device(c);
+    ++loss->gen;
+    if (lse) ++lse->gen;
+    emh::launch_cross_entropy(c, t.in, (float*)loss->ptr, lse ? (float*)lse->ptr : nullptr);
+  });
+}
+
+int emh_cross_entropy_grad(emh_ctx* c, const emh_buf* x, size_t ldx, size_t n, size_t d,
+                           const emh_buf* w, size_t ldw, size_t k, const emh_buf* labels,
+                           float scale, const emh_buf* lse, const emh_buf* gloss, emh_buf* dx,
+                           size_t lddx, emh_buf* dw, size_t lddw) {
+  return guard([&] {
+    const XentCall t = check_xent(c, x, ldx, n, d, w, ldw, k, labels, scale);
+    const Range rs = check_f32(lse, n, "lse");
+    Range rg;
+    if (gloss) rg = check_f32(gloss, n, "gloss");
+    Range out[2];
+    emh_buf* o[2] = {dx, dw};
+    size_t* ld[2] = {&lddx, &lddw};
+    const char* name[2] = {"dx", "dw"};
+    for (int i = 0; i < 2; i++) {
+      if (!o[i]) continue;
+      EMH_ENSURE(o[i]->kind == x->kind, "%s must be of x's kind", name[i]);
+      out[i] = check_matrix(o[i], i ? k : n, d, *ld[i], name[i]);
+      apart_from_inputs(out[i], t, name[i]);
+      apart(out[i], rs, name[i], "lse");
+      apart(out[i], rg, name[i], "gloss");
+    }
+    apart(out[0], out[1], "dx", "dw");
+    if (!dx && !dw) return;
+    use_device(c);
+    emh::MatOut mo[2];
+    for (int i = 0; i < 2; i++) {
+      if (!o[i]) continue;
+      ++o[i]->gen;
+      mo[i] = {o[i]->ptr, *ld[i], o[i]->kind};
+    }
+    emh::launch_cross_entropy_grad(c, t.in, (const float*)lse->ptr,
+                                   gloss ? (const float*)gloss->ptr : nullptr, mo[0], mo[1]);
+  });
+}
+
 int emh_adamw_create(emh_ctx* c, const emh_adamw_tensor* tensors, size_t count, emh_adamw** out) {
   return guard([&] {
     EMH_ENSURE(c && out, "null argument");

@@ -25,6 +25,21 @@ void launch_layer_norm_grad(emh_ctx* c, const MatIn& dy, const MatIn& x, size_t 
                             const MatIn& weight, const float* mean, const float* rstd,
                             const MatOut& dx, const MatOut& dweight, const MatOut& dbias);
 
+// ---- emh_xent.hip
+// Rows x (n x d) against classes w (k x d, x's kind); labels: n, NONE where a row
+// has none.
+struct XentIn {
+  MatIn x, w;
+  size_t n, d, k;
+  const uint32_t* labels;
+  float scale;
+};
+constexpr uint32_t NO_LABEL = 0xFFFFFFFFu;
+void launch_cross_entropy(emh_ctx* c, const XentIn& in, float* loss, float* lse);
+// gloss (n entries): the gradients of the rows' losses, or null: of their mean.
+void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, const float* gloss,
+                               const MatOut& dx, const MatOut& dw);
+
 // ---- emh_adamw.hip
 struct AdamTensor {  // as the kernel reads it
   void* param;

@@ -369,6 +369,28 @@ int emh_layer_norm_grad(emh_ctx* ctx, const emh_buf* dy, size_t lddy, const emh_
                         const emh_buf* rstd, emh_buf* dx, size_t lddx, emh_buf* dweight,
                         emh_buf* dbias);
 
+/* Softmax cross entropy of the rows of x (n x d) against the classes of w
+ * (k x d; x's kind: f32, f16 or bf16), without keeping the n x k logits: with z_iv
+ * = scale x_i . w_v, lse[i] = log sum_v exp z_iv and loss[i] = lse[i] -
+ * z_i,labels[i] (f32, n entries each). labels: a u32 each, 0xFFFFFFFF for a
+ * row without one (loss 0); any other label >= k is an error at the next
+ * synchronizing call (the row counts as one without a label). lse may be NULL. */
+int emh_cross_entropy(emh_ctx* ctx, const emh_buf* x, size_t ldx, size_t n, size_t d,
+                      const emh_buf* w, size_t ldw, size_t k, const emh_buf* labels, float scale,
+                      emh_buf* loss, emh_buf* lse);
+/* Its gradients, with lse as emh_cross_entropy left it: of sum_i gloss[i] loss[i]
+ * (gloss f32, n entries), or, with gloss NULL, of the mean loss of the rows
+ * that have a label (zeros if none has). With g_iv = gloss[i] scale (exp(z_iv -
+ * lse[i]) - [v = labels[i]]), zero in rows without a label: dx_i = sum_v g_iv
+ * w_v (n x d), dw_v = sum_i g_iv x_i (k x d), both of x's kind, overwritten; either
+ * may be NULL. A row without a label has no part in dw, whatever it holds.
+ * The logits are computed again, for pieces of the classes. The sums' order
+ * depends on the sizes alone. */
+int emh_cross_entropy_grad(emh_ctx* ctx, const emh_buf* x, size_t ldx, size_t n, size_t d,
+                           const emh_buf* w, size_t ldw, size_t k, const emh_buf* labels,
+                           float scale, const emh_buf* lse, const emh_buf* gloss, emh_buf* dx,
+                           size_t lddx, emh_buf* dw, size_t lddw);
+
 /* One tensor of an AdamW step. param: f32, f16 or bf16; grad: f32, f16 or bf16,
  * as long. copy (f16 or bf16, as long, may be NULL) gets the new parameters
  * rounded, for a master copy in f32. States of 32 bits: m and v f32, the scales
