@@ -190,7 +190,7 @@ struct XentCall {
 XentCall check_xent(emh_ctx* c, const emh_buf* x, size_t ldx, size_t n, size_t d, const emh_buf* w,
                     size_t ldw, size_t k, const emh_buf* labels, float scale) {
   EMH_ENSURE(c, "null context");
-  EMH_ENSURE(d > 0 && d <= (size_t(1) << 24), "d must be 1 to 2^24");
+  EMH_ENSURE(d > 0 && d <= (size_t(1) << 21), "d must be 1 to 2^21");
   EMH_ENSURE(k > 0 && k <= (size_t(1) << 30), "k must be 1 to 2^30");
   EMH_ENSURE(n <= (size_t(1) << 30), "too many rows");
   EMH_ENSURE(x && real_kind(x->kind), "x must be an f32, f16 or bf16 buffer");

@@ -1,0 +1,294 @@
+// Tiles of products of two 16-bit matrices in f32, the core of the cross
+// entropy's four products (emh_xent.h): out(i, j) = sum over k of R(i, k) C(j, k).
+//
+// A workgroup owns a tile of TR rows x TC columns of the result. The depth goes by in
+// slabs of 64, each operand's slab (TR or TC by 64, 128 bytes a row) moved to LDS by
+// DMA into one of two stages. An operand lies in memory in one of two ways:
+//   DEEP  its rows run along the depth (x and w for the logits): a slab is 128
+//         bytes of each row, and a wave's operand is one 16-byte read a lane;
+//   WIDE  its rows run across it (w and x for the gradients: the depth is the
+//         class or the row): a slab is 64 rows of 2 T bytes, and the operand is two
+//         reads that transpose 4 x 16 elements on the way (ds_read_b64_tr_b16), so
+//         no operand is ever transposed in memory.
+// In LDS the 16-byte chunks of a row are XOR-swizzled so that neither kind of
+// read meets a bank twice: a DEEP row r's chunks by (r / 2) % 8 (two rows fill the
+// 64 banks: sixteen rows' equal chunks are sixteen different ones), a WIDE row's
+// by 4 (r % 4) (a transposing read takes 64 bytes of each of four rows).
+//
+// The columns are the MFMA's A and the rows its B, so that a lane holds one
+// row of each 32 x 32 block and four consecutive columns at a time.
+#pragma once
+
+#include "emh_dma.h"
+#include "emh_learn.h"
+#include "emh_types.h"
+
+namespace emh {
+namespace {
+
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef short v8s __attribute__((ext_vector_type(8)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef const v8s __attribute__((address_space(3)))* lds_v8s;
+typedef v4s __attribute__((address_space(3)))* lds_v4s;
+
+__device__ __forceinline__ v16f mfma16(f16, v8s a, v8s b, v16f c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a),
+                                                __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ v16f mfma16(bf16, v8s a, v8s b, v16f c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a),
+                                                 __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+}
+
+constexpr int SLAB = 64;  // depth of a slab
+
+// A workgroup's shape: waves of NWR x NWC, each WB x WA blocks of 32 x 32.
+template <int NWR_, int NWC_, int WB_, int WA_>
+struct TileShape {
+  static constexpr int NWR = NWR_, NWC = NWC_, WB = WB_, WA = WA_;
+  static constexpr int NW = NWR * NWC, THREADS = 64 * NW;
+  static constexpr int TR = NWR * WB * 32, TC = NWC * WA * 32;
+  static constexpr int RBYTES = TR * SLAB * 2, CBYTES = TC * SLAB * 2;
+  static constexpr int STAGE = RBYTES + CBYTES;
+  static constexpr int RD = RBYTES / (1024 * NW), CD = CBYTES / (1024 * NW);  // DMAs a wave
+};
+typedef TileShape<4, 2, 2, 4> TileL;  // 256 x 256, 8 waves
+typedef TileShape<2, 2, 2, 2> TileS;  // 128 x 128, 4 waves
+
+// One operand. f32 matrices come as two planes of fp16 (emh_xent.h).
+struct Operand {
+  const char* p[2];  // planes
+  uint32_t ld;       // bytes of a row in memory (16-byte multiples, rows 16-byte aligned)
+  uint32_t rows;     // rows there are: what lies past them (DEEP: of the tile, WIDE: of the
+                     // last slab) reads the last
+  uint32_t wide;     // WIDE: elements of a row that may be read (a multiple of 8)
+};
+
+struct TileIn {
+  Operand r, c;
+  uint32_t slabs;   // of the depth; one operand is zero past it
+  uint32_t passes;  // 1, or 3: planes (0, 0), (0, 1), (1, 0)
+  uint32_t rtiles, ctiles, splits;  // workgroups: rtiles ctiles splits
+};
+
+// Which tile, and which steps (pass, slab) of it, a workgroup takes.
+struct TileAt {
+  uint32_t rt, ct, split, s0, s1;
+};
+// Workgroups are dealt to the 8 XCDs in turn: every XCD takes a run of
+// consecutive items, in which the tiles of GROUP row tiles and a column tile follow each
+// other, so that what its 32 CUs read at a time is a few row and column
+// slabs, shared in its L2.
+__device__ __forceinline__ TileAt tile_at(const TileIn& t) {
+  const uint32_t nb = gridDim.x, bid = blockIdx.x;
+  const uint32_t xcd = bid & 7, q = bid >> 3, m = nb >> 3, rem = nb & 7;
+  uint32_t wi = xcd * m + min(xcd, rem) + q;
+  TileAt a;
+  const uint32_t tiles = t.rtiles * t.ctiles;
+  a.split = wi / tiles;
+  wi -= a.split * tiles;
+  constexpr uint32_t GROUP = 8;
+  const uint32_t per = GROUP * t.ctiles, g = wi / per;
+  const uint32_t have = min(GROUP, t.rtiles - g * GROUP);
+  wi -= g * per;
+  a.ct = wi / have;
+  a.rt = g * GROUP + wi % have;
+  const uint32_t steps = t.slabs * t.passes;
+  a.s0 = (uint32_t)((uint64_t)steps * a.split / t.splits);
+  a.s1 = (uint32_t)((uint64_t)steps * (a.split + 1) / t.splits);
+  return a;
+}
+
+__device__ __forceinline__ uint32_t deep_swz(uint32_t row) { return (row >> 1) & 7; }
+
+// A wave's DMAs of one operand's slab, and its reads of it.
+template <bool DEEP, int T, int ND, int NW>
+struct Side16 {
+  static constexpr uint32_t RB = 2 * T;         // WIDE: bytes of a row in LDS
+  static constexpr uint32_t LPR = RB / 16;      // ... lanes of a DMA that share it
+  uint32_t off[ND];                             // DEEP: row and chunk; WIDE: chunk
+  uint32_t krow[ND];                            // WIDE: row in the slab
+  uint32_t at[DEEP ? 1 : 4];                    // LDS reads (WIDE: by block)
+
+  // t0: the tile's first row (DEEP) or column (WIDE). w: the wave, uniform.
+  __device__ __forceinline__ void init(const Operand& o, uint32_t t0, int w) {
+    const uint32_t lane = threadIdx.x & 63;
+#pragma unroll
+    for (int j = 0; j < ND; j++) {
+      const uint32_t d = (uint32_t)(j * NW + w);
+      if constexpr (DEEP) {
+        const uint32_t row = d * 8 + (lane >> 3);
+        const uint32_t r = min(t0 + row, o.rows - 1) - t0;
+        off[j] = r * o.ld + (((lane & 7) ^ deep_swz(row)) << 4);
+      } else {
+        krow[j] = d * (64 / LPR) + lane / LPR;
+        const uint32_t chunk = (lane % LPR) ^ ((krow[j] & 3) << 2);
+        const uint32_t col = t0 + chunk * 8;
+        off[j] = (col < o.wide ? col : 0u) * 2;
+      }
+    }
+  }
+  // The wave's blocks begin at block b0 of the operand's tile.
+  __device__ __forceinline__ void init_reads(uint32_t lds, int b0) {
+    const uint32_t lane = threadIdx.x & 63;
+    if constexpr (DEEP) {
+      const uint32_t li = lane & 31, h = lane >> 5;
+      at[0] = lds + (uint32_t)b0 * 32 * 128 + li * 128 + ((h ^ deep_swz(li)) << 4);
+    } else {
+      const uint32_t g = lane >> 4, l = lane & 15;
+#pragma unroll
+      for (int a = 0; a < 4; a++) {
+        const uint32_t chunk = (uint32_t)(b0 + a) * 4 + (g & 1) * 2 + ((l & 3) >> 1);
+        at[a] = lds + (8 * (g >> 1) + (l >> 2)) * RB + (((chunk ^ ((l >> 2) << 2))) << 4) + (l & 1) * 8;
+      }
+    }
+  }
+  // DMA j of the slab that begins at `slab` (uniform) of the plane at p.
+  __device__ __forceinline__ void dma(int j, const char* p, const Operand& o, uint32_t slab,
+                                      uint32_t lds) const {
+    if constexpr (DEEP) {
+      dma16a(p + (size_t)slab * (SLAB * 2), off[j], lds);
+    } else {
+      const uint32_t last = o.rows - 1 - slab * SLAB;
+      dma16a(p + (size_t)slab * SLAB * o.ld, min(krow[j], last) * o.ld + off[j], lds);
+    }
+  }
+  // Block a's operand of MFMA step ks from the stage at `stage` (bytes).
+  __device__ __forceinline__ v8s read(uint32_t stage, int ks, int a) const {
+    if constexpr (DEEP) {
+      return *(lds_v8s)(uintptr_t)(((at[0] + stage) ^ (uint32_t)(ks << 5)) + (uint32_t)a * 32 * 128);
+    } else {
+      const uint32_t p = at[a] + stage + (uint32_t)ks * 16 * RB;
+      const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(uintptr_t)p);
+      const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(uintptr_t)(p + 4 * RB));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+};
+
+// The tile's sums into acc[column block][row block] of every wave.
+//
+// A step: the slab's four MFMA steps. Each column block's operand is replaced by the
+// next step's as soon as its MFMAs are issued. The last MFMA step's operands
+// are in registers before it begins, so its stage is free then: every wave has
+// waited for its own reads and DMAs (the next slab's) and met the others at the
+// barrier, and the DMAs of the slab after the next go out between its MFMAs.
+template <class T, class S, bool RDEEP, bool CDEEP>
+__device__ __forceinline__ void tile_sums(const TileIn& t, const TileAt& at, char* ring,
+                                          v16f (&acc)[S::WA][S::WB]) {
+  const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int wr = w % S::NWR, wc = w / S::NWR;
+  Side16<RDEEP, S::TR, S::RD, S::NW> R;
+  Side16<CDEEP, S::TC, S::CD, S::NW> C;
+  R.init(t.r, at.rt * S::TR, w);
+  C.init(t.c, at.ct * S::TC, w);
+  const uint32_t lds0 = lds_addr(ring);
+  R.init_reads(lds0, wr * S::WB);
+  C.init_reads(lds0 + S::RBYTES, wc * S::WA);
+  const size_t r0 = RDEEP ? (size_t)at.rt * S::TR * t.r.ld : 0;
+  const size_t c0 = CDEEP ? (size_t)at.ct * S::TC * t.c.ld : 0;
+  const uint32_t ldst = lds0 + (uint32_t)w * 1024;
+
+  // Load cursor: pass, slab and stage of the next DMAs; past the last step it
+  // stays there, and what it fetches again nothing reads.
+  uint32_t lpass = at.s0 / t.slabs, lslab = at.s0 % t.slabs, lleft = at.s1 - at.s0, lst = 0;
+  auto dma = [&](int q) __attribute__((always_inline)) {
+    if (q < S::RD)
+      R.dma(q, t.r.p[lpass == 2 ? 1 : 0] + r0, t.r, lslab,
+            ldst + lst + (uint32_t)q * S::NW * 1024);
+    else
+      C.dma(q - S::RD, t.c.p[lpass == 1 ? 1 : 0] + c0, t.c, lslab,
+            ldst + lst + S::RBYTES + (uint32_t)(q - S::RD) * S::NW * 1024);
+  };
+  auto advance = [&]() __attribute__((always_inline)) {
+    lst ^= S::STAGE;
+    if (lleft > 1) {
+      lleft--;
+      if (++lslab == t.slabs) {
+        lslab = 0;
+        lpass++;
+      }
+    }
+  };
+  static_assert((S::STAGE & (S::STAGE - 1)) == 0, "stages are toggled by XOR");
+
+#pragma unroll
+  for (int a = 0; a < S::WA; a++)
+#pragma unroll
+    for (int y = 0; y < S::WB; y++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) acc[a][y][r] = 0.f;
+
+  constexpr int PER = S::RD + S::CD;
+#pragma unroll
+  for (int s = 0; s < 2; s++) {
+#pragma unroll
+    for (int q = 0; q < PER; q++) dma(q);
+    advance();
+  }
+  wait_vm<PER>();  // the first slab is in, the second in flight
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  v8s rb[2][S::WB], ca[S::WA];
+#pragma unroll
+  for (int y = 0; y < S::WB; y++) rb[0][y] = R.read(0, 0, y);
+#pragma unroll
+  for (int a = 0; a < S::WA; a++) ca[a] = C.read(0, 0, a);
+  uint32_t st = 0;
+  for (uint32_t s = at.s0; s < at.s1; s++) {
+#pragma unroll
+    for (int ks = 0; ks < 4; ks++) {
+      if (ks == 3) {
+        wait_vm<0>();
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+      }
+      const uint32_t from = ks == 3 ? st ^ S::STAGE : st;
+#pragma unroll
+      for (int a = 0; a < S::WA; a++) {
+#pragma unroll
+        for (int y = 0; y < S::WB; y++)
+          acc[a][y] = mfma16(T{}, ca[a], rb[ks & 1][y], acc[a][y]);
+        __builtin_amdgcn_sched_barrier(0);
+        if (a == 0) {
+#pragma unroll
+          for (int y = 0; y < S::WB; y++) rb[(ks + 1) & 1][y] = R.read(from, (ks + 1) & 3, y);
+        }
+        ca[a] = C.read(from, (ks + 1) & 3, a);
+        if (ks == 3) {
+#pragma unroll
+          for (int q = a * PER / S::WA; q < (a + 1) * PER / S::WA; q++) dma(q);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    advance();
+    st ^= S::STAGE;
+  }
+  wait_vm<0>();  // the DMAs past the last step have landed
+  asm volatile("" ::: "memory");
+}
+
+// A lane's pair of fours of a block's columns, 8 q + 4 h .. + 3 of q = 2 p and
+// 2 p + 1, as eight consecutive ones: 16 p + 8 h .. + 7 (the lanes l and l + 32
+// swap halves).
+__device__ __forceinline__ void eight(const float* lo, const float* hi, float* out) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    // Lanes below 32 keep lo and take the partner's lo; the others keep hi and
+    // take the partner's hi.
+    const auto v = __builtin_amdgcn_permlane32_swap(__float_as_uint(lo[e]), __float_as_uint(hi[e]),
+                                                    false, false);
+    out[e] = __uint_as_float(v[0]);
+    out[4 + e] = __uint_as_float(v[1]);
+  }
+}
+
+}  // namespace
+}  // namespace emh

@@ -1,0 +1,98 @@
+// The cross entropy's products and what they share (emh_xent.hip,
+// emh_xent_logits.hip, emh_xent_grads.hip).
+//
+// z = scale x w^T, in tiles (emh_tile.h), twice: for every row's maximum and sum
+// of exponentials, and for the gradients of a piece of the classes, G = gloss
+// (softmax - onehot), which go to memory in 16 bits; then dx = G w and dw = G^T x,
+// times scale (and, for a mean, 1 / rows) in f32. A factor that all rows share is
+// left out of G: most rows' label has a G of nearly -1, which 16 bits hold
+// better than any product, whose rounding would be one error for all of them.
+//
+// Types. 16-bit rows and classes are the MFMA's operands as they are; G is
+// rounded once to their type (f16: times a power of two that brings the largest
+// possible element to 2^13 .. 2^14, or the gradients of a mean over many rows would be
+// subnormal). float32 operands are two planes of f16: a row times a power of two
+// 2^-e that brings its largest element to 2^13 .. 2^14, h = f16(x), l = f16(x - h),
+// which hold 22 bits and more of every element down to 2^-26 of the row's
+// largest; h h + h l + l h leaves out 2^-22 of a product at most, as f32's own
+// rounding would over a few terms, and takes three MFMAs of the f16 rate where
+// the f32 MFMA takes sixteen.
+// The exponents: z = sum 2^(ex_i + ew_v). The gradient products sum over the
+// class or the row, whose exponent then has to be in G: there are two G,
+//   Ga = G 2^(ew_v - ewmax + ga_i)  for dx_i = 2^(ewmax - ga_i) sum_v Ga w_v,
+//   Gb = G 2^(ex_i + gb)            for dw_v = 2^-gb sum_i Gb x_i,
+// with ga_i and gb such that the largest element is below 2^14: what is lost of
+// the others is 2^-39 of that.
+#pragma once
+
+#include "emh_learn.h"
+#include "emh_tile.h"
+
+namespace emh {
+
+// What a gradient call finds out about its rows, on the device.
+struct XentState {
+  uint32_t count;  // rows with a label
+  int uexp;        // largest exponent of |gloss_i| 2^ex_i over them (no gloss: of 2^ex_i), + BIAS
+  int ewmax;       // largest ew_v, + BIAS
+  uint32_t odd;    // a row without a label holds a value that is not finite
+};
+constexpr int XENT_BIAS = 4096;  // (so that zero is less than any)
+
+struct LogitArgs {
+  TileIn t;
+  uint32_t n, m;    // rows, classes of the piece
+  uint32_t col0, k; // its first class, all classes
+  const uint32_t* labels;
+  float s2;         // scale log2(e)
+  const int* ex;    // f32: exponents of the rows, and of the piece's classes
+  const int* ew;
+  float2* part;     // statistics: [part][row] (max, sum) of z log2(e)
+  float* zlabel;
+  const float* lse; // gradients
+  const float* gloss;
+  const XentState* st;
+  float scale;
+  char* g[4];       // G; f32: Ga's planes, Gb's planes
+  size_t ldg;       // bytes (rows and columns to full tiles)
+};
+// Bits of what a call is: which instantiation runs.
+void launch_logits(hipStream_t s, const LogitArgs& a, int kind, bool large, bool grads);
+
+struct ProdArgs {
+  TileIn t;
+  uint32_t rows, cols;  // of the result
+  bool dw;              // else dx
+  const uint32_t* labels;  // dx: rows without one are zero
+  uint32_t k;
+  const float* gloss;
+  const XentState* st;
+  float scale;
+  void* out;            // the result in its kind, or
+  size_t ldo;           // (elements)
+  float* part;          // one split's sums: [split][row][ldp] in f32
+  size_t ldp;
+  bool add;             // into what an earlier piece left
+  const uint32_t* when; // dw: where it is not zero, x is read from here
+  Operand alt;
+};
+void launch_prod(hipStream_t s, const ProdArgs& a, int kind, bool large);
+
+// A row's weight in G, the powers of two of G (see above) and the factor left for the
+// results: all from the call's state.
+struct RowScale {
+  float by;   // scale, and without gloss 1 / rows with a label
+  int gexp;   // f16: G's exponent; f32: gb
+  __device__ __forceinline__ void init(const XentState* st, const float* gloss, float scale) {
+    const uint32_t c = st->count;
+    by = gloss ? scale : c ? scale / (float)c : 0.f;
+    gexp = st->uexp ? 14 - (st->uexp - XENT_BIAS + 1) : 0;  // |weight_i| 2^ex_i < 2^(uexp + 1)
+  }
+};
+// The exponent that brings a row's weight below 2^14.
+__device__ __forceinline__ int row_exp(const float* gloss, uint32_t i) {
+  const float f = gloss ? fabsf(gloss[i]) : 1.f;
+  return f > 0.f && f < INFINITY ? 13 - ilogbf(f) : 0;
+}
+
+}  // namespace emh

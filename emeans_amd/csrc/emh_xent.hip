@@ -1,125 +1,161 @@
 // Softmax cross entropy of rows against a linear classifier's classes, and its
-// gradients, without an n x k matrix of logits.
-//
-// Every product is a tile of 64 x 64 dots, 4 x 4 a thread, over slabs of 16
-// columns in LDS, in f32.
+// gradients, without an n x k matrix of logits: which products run over what
+// (emh_xent.h), the operands laid out for them, and the joins of their parts.
 #include <algorithm>
+#include <cmath>
 
-#include "emh_learn.h"
-#include "emh_types.h"
+#include "emh_xent.h"
 
 namespace emh {
 namespace {
 
-constexpr float LOG2E = 1.44269504f, LN2 = 0.693147181f;
+constexpr float LN2 = 0.693147181f;
 
-// Element (i, k) of an operand at i si + k sk.
-struct Side {
-  const void* p;
-  int kind;
-  size_t si, sk, rows;
-};
-struct ProdArgs {
-  Side a, b;
-  size_t depth;
-  int mode;  // 0 statistics, 1 gradients of logits, 2 f32 out (+=), 3 out in kind
-  const uint32_t* labels;
-  float s2;  // scale log2(e)
-  float2* part;   // mode 0: [column tile][row]
-  float* zlabel;  // ... the label's logit times log2(e)
-  size_t col0;    // the first class of the piece
-  const float* lse;
-  const float* up;   // gloss, or one value for all rows
-  int up_each;
-  float scale;
-  void* out;
-  size_t ldo;
-  int okind, add;
-};
-
-__global__ __launch_bounds__(256) void k_prod(const ProdArgs g) {
-  __shared__ float A[16][68], B[16][68];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const size_t i0 = (size_t)blockIdx.y * 64, j0 = (size_t)blockIdx.x * 64;
-  float acc[4][4] = {};
-  for (size_t k0 = 0; k0 < g.depth; k0 += 16) {
-    for (int t = threadIdx.x; t < 1024; t += 256) {
-      // Neighbouring threads along the operand's contiguous direction.
-      const int kk = g.a.sk == 1 ? t & 15 : t >> 6, r = g.a.sk == 1 ? t >> 4 : t & 63;
-      const bool in = i0 + r < g.a.rows && k0 + kk < g.depth;
-      A[kk][r] = in ? load_kind(g.a.p, g.a.kind, (i0 + r) * g.a.si + (k0 + kk) * g.a.sk) : 0.f;
-      const int kb = g.b.sk == 1 ? t & 15 : t >> 6, q = g.b.sk == 1 ? t >> 4 : t & 63;
-      const bool inb = j0 + q < g.b.rows && k0 + kb < g.depth;
-      B[kb][q] = inb ? load_kind(g.b.p, g.b.kind, (j0 + q) * g.b.si + (k0 + kb) * g.b.sk) : 0.f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 16; k++)
-#pragma unroll
-      for (int u = 0; u < 4; u++)
-#pragma unroll
-        for (int v = 0; v < 4; v++) acc[u][v] = fmaf(A[k][ty * 4 + u], B[k][tx * 4 + v], acc[u][v]);
-    __syncthreads();
-  }
-#pragma unroll
-  for (int u = 0; u < 4; u++) {
-    const size_t i = i0 + ty * 4 + u;
-    const bool row = i < g.a.rows;
-    if (g.mode == 0) {
-      const uint32_t lab = row ? g.labels[i] : NO_LABEL;
-      float m = -INFINITY, s = 0.f;
-#pragma unroll
-      for (int v = 0; v < 4; v++) {
-        const size_t j = j0 + tx * 4 + v;
-        acc[u][v] = j < g.b.rows ? acc[u][v] * g.s2 : -INFINITY;
-        m = fmaxf(m, acc[u][v]);
-        if (row && j == lab) g.zlabel[i] = acc[u][v];
-      }
-      m = lanes_max<16>(m);
-      const float mm = m == -INFINITY ? 0.f : m;
-#pragma unroll
-      for (int v = 0; v < 4; v++) s += exp2f(acc[u][v] - mm);
-      s = lanes_sum<16>(s);
-      if (row && tx == 0) g.part[blockIdx.x * g.a.rows + i] = make_float2(m, s);
-      continue;
-    }
-    if (!row) continue;
-#pragma unroll
-    for (int v = 0; v < 4; v++) {
-      const size_t j = j0 + tx * 4 + v;
-      if (j >= g.b.rows) continue;
-      float o = acc[u][v];
-      if (g.mode == 1) {
-        const uint32_t lab = g.labels[i];
-        const float p = exp2f(o * g.s2 - g.lse[i] * LOG2E);
-        o = (p - (g.col0 + j == lab ? 1.f : 0.f)) * (g.up[g.up_each ? i : 0] * g.scale);
-        if (lab == NO_LABEL) o = 0.f;
-      }
-      if (g.mode == 3)
-        store_kind(g.out, g.okind, i * g.ldo + j, o);
-      else if (g.add)
-        reinterpret_cast<float*>(g.out)[i * g.ldo + j] += o;
-      else
-        reinterpret_cast<float*>(g.out)[i * g.ldo + j] = o;
-    }
+// Rows to 16-byte aligned rows of dp elements, the rest zero (dp a multiple of
+// SLAB). labels: rows without one become zeros. when: only if it is not zero.
+// A wave a row.
+template <class T>
+__global__ __launch_bounds__(256) void k_pack16(const T* x, size_t ld, size_t n, uint32_t d,
+                                                uint32_t dp, const uint32_t* labels, uint32_t k,
+                                                T* out, const uint32_t* when) {
+  if (when && *when == 0u) return;
+  const size_t i = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (i >= n) return;
+  const uint32_t lane = threadIdx.x & 63;
+  const T* row = x + i * ld;
+  const bool zero = labels && labels[i] >= k;
+  for (uint32_t c = lane * 8; c < dp; c += 512) {
+    Vec<T> v{make_uint4(0u, 0u, 0u, 0u)};
+    if (!zero && c < d) v = c + 8 <= d ? load_vec(row + c) : load_some(row + c, (int)(d - c));
+    *reinterpret_cast<uint4*>(out + i * dp + c) = v.raw;
   }
 }
 
-// The parts' maxima and sums joined, the rows' lse and loss. A label out of
-// range is recorded and counts as none.
-__global__ __launch_bounds__(256) void k_xent_join(const float2* part, size_t nparts, size_t n,
-                                                   const uint32_t* labels, size_t k,
-                                                   const float* zlabel, float* loss, float* lse,
-                                                   uint32_t* small) {
-  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+// f32 rows to planes of f16 (see emh_xent.h) and their exponents e (x = plane
+// 2^e). With st, what the gradients need to know: rows (labels given) their count
+// and the largest exponent of |gloss| 2^e, rows without a label become zeros;
+// classes the largest exponent. A wave a row.
+__global__ __launch_bounds__(256) void k_pack32(const float* x, size_t ld, size_t n, uint32_t d,
+                                                uint32_t dp, const uint32_t* labels, uint32_t k,
+                                                const float* gloss, f16* hi, f16* lo, int* ex,
+                                                XentState* st, uint32_t* small) {
+  const size_t i = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (i >= n) return;
-  float m = -INFINITY, s = 0.f;
-  for (size_t t = 0; t < nparts; t++) {
-    const float2 p = part[t * n + i];
-    const float b = fmaxf(m, p.x), mm = b == -INFINITY ? 0.f : b;
-    s = s * exp2f(m - mm) + p.y * exp2f(p.x - mm);
-    m = b;
+  const uint32_t lane = threadIdx.x & 63;
+  const float* row = x + i * ld;
+  const uint32_t lab = labels ? labels[i] : 0u;
+  const bool zero = labels && lab >= k;
+  float top = 0.f;
+  for (uint32_t c = lane * 4; c < d; c += 256) {
+    const Vec<float> v = c + 4 <= d ? load_vec(row + c) : load_some(row + c, (int)(d - c));
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const float m = fabsf(v.get(e));
+      top = fmaxf(top, m < INFINITY ? m : 0.f);
+    }
   }
+  top = lanes_max<64>(top);
+  const int e0 = !zero && top > 0.f ? max(ilogbf(top) - 13, -120) : 0;
+  const float by = ldexpf(1.f, -e0);
+  for (uint32_t c = lane * 4; c < dp; c += 256) {
+    Vec<float> v{make_uint4(0u, 0u, 0u, 0u)};
+    if (!zero && c < d) v = c + 4 <= d ? load_vec(row + c) : load_some(row + c, (int)(d - c));
+    uint16_t a[4], b[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const float t = v.get(e) * by;
+      const f16 h = (f16)t;
+      a[e] = __builtin_bit_cast(uint16_t, h);
+      b[e] = __builtin_bit_cast(uint16_t, (f16)(t - (float)h));
+    }
+    const size_t o = i * dp + c;
+    *reinterpret_cast<uint2*>(hi + o) =
+        make_uint2(a[0] | (uint32_t)a[1] << 16, a[2] | (uint32_t)a[3] << 16);
+    *reinterpret_cast<uint2*>(lo + o) =
+        make_uint2(b[0] | (uint32_t)b[1] << 16, b[2] | (uint32_t)b[3] << 16);
+  }
+  if (lane != 0) return;
+  ex[i] = e0;
+  if (!st) return;
+  if (!labels) {
+    atomicMax(&st->ewmax, e0 + XENT_BIAS);
+    return;
+  }
+  if (zero) {
+    if (lab != NO_LABEL) small[SW_BAD_CLASS] = 1u;
+    return;
+  }
+  atomicAdd(&st->count, 1u);
+  const float g = gloss ? fabsf(gloss[i]) : 1.f;
+  if (g > 0.f && g < INFINITY) atomicMax(&st->uexp, ilogbf(g) + e0 + XENT_BIAS);
+}
+
+// The same facts for 16-bit rows: a thread a row, a wave at a time over the
+// rows without a label, whose values have to be finite to be multiplied by zero.
+template <class T>
+__global__ __launch_bounds__(256) void k_survey(const T* x, size_t ld, size_t n, uint32_t d,
+                                                const uint32_t* labels, uint32_t k,
+                                                const float* gloss, XentState* st,
+                                                uint32_t* small) {
+  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+  const uint32_t lane = threadIdx.x & 63;
+  const uint32_t lab = i < n ? labels[i] : NO_LABEL;
+  const bool has = lab < k;
+  const float g = has ? gloss ? fabsf(gloss[i]) : 1.f : 0.f;
+  const int e = g > 0.f && g < INFINITY ? ilogbf(g) + XENT_BIAS : 0;
+  if (!has && lab != NO_LABEL) small[SW_BAD_CLASS] = 1u;
+  const unsigned long long some = __ballot(has);
+  int top = e;
+  for (int o = 32; o > 0; o >>= 1) top = max(top, __shfl_xor(top, o, 64));
+  if (lane == 0) {
+    if (some) atomicAdd(&st->count, (uint32_t)__popcll(some));
+    if (top) atomicMax(&st->uexp, top);
+  }
+  unsigned long long none = __ballot(i < n && !has);
+  const size_t first = i - lane;
+  bool odd = false;
+  while (none) {
+    const int r = __ffsll((long long)none) - 1;
+    none &= none - 1;
+    const T* row = x + (first + r) * ld;
+    for (uint32_t c = lane * 8; c < d; c += 512) {
+      const Vec<T> v = c + 8 <= d ? load_vec(row + c) : load_some(row + c, (int)(d - c));
+#pragma unroll
+      for (int q = 0; q < 8; q++) odd = odd || !(fabsf(v.get(q)) < INFINITY);
+    }
+  }
+  if (__ballot(odd) != 0ull && lane == 0) st->odd = 1u;
+}
+
+// The parts' maxima and sums joined: 64 rows a workgroup, 16 shares of the parts.
+__global__ __launch_bounds__(1024) void k_join(const float2* __restrict__ part, uint32_t nparts,
+                                               uint32_t n, const uint32_t* labels, uint32_t k,
+                                               const float* zlabel, float* loss, float* lse,
+                                               uint32_t* small) {
+  __shared__ float2 sh[16][64];
+  const uint32_t c = threadIdx.x & 63, g = threadIdx.x >> 6;
+  const uint32_t i = blockIdx.x * 64 + c;
+  float m = -INFINITY, s = 0.f;
+  auto join = [&](float2 p) __attribute__((always_inline)) {
+    const float b = fmaxf(m, p.x), bb = b == -INFINITY ? 0.f : b;
+    s = s * __builtin_amdgcn_exp2f(m - bb) + p.y * __builtin_amdgcn_exp2f(p.x - bb);
+    m = b;
+  };
+  if (i < n) {
+    uint32_t t = g;
+    for (; t + 48 < nparts; t += 64) {  // four loads in flight
+      const float2 p0 = part[(size_t)t * n + i], p1 = part[(size_t)(t + 16) * n + i],
+                   p2 = part[(size_t)(t + 32) * n + i], p3 = part[(size_t)(t + 48) * n + i];
+      join(p0), join(p1), join(p2), join(p3);
+    }
+    for (; t < nparts; t += 16) join(part[(size_t)t * n + i]);
+  }
+  sh[g][c] = make_float2(m, s);
+  __syncthreads();
+  if (g != 0 || i >= n) return;
+  m = -INFINITY, s = 0.f;
+#pragma unroll
+  for (int t = 0; t < 16; t++) join(sh[t][c]);
   const float l2 = (m == -INFINITY ? 0.f : m) + log2f(s);
   const uint32_t lab = labels[i];
   if (lse) lse[i] = l2 * LN2;
@@ -127,124 +163,279 @@ __global__ __launch_bounds__(256) void k_xent_join(const float2* part, size_t np
   if (lab >= k && lab != NO_LABEL) small[SW_BAD_CLASS] = 1u;
 }
 
-// 1 / (rows with a label), 0 when there is none.
-__global__ __launch_bounds__(1024) void k_xent_count(const uint32_t* labels, size_t n, size_t k,
-                                                     float* out) {
-  __shared__ uint32_t c;
-  if (threadIdx.x == 0) c = 0;
-  __syncthreads();
-  uint32_t mine = 0;
-  for (size_t i = threadIdx.x; i < n; i += 1024) mine += labels[i] < k ? 1u : 0u;
-  atomicAdd(&c, mine);
-  __syncthreads();
-  if (threadIdx.x == 0) *out = c ? 1.f / (float)c : 0.f;
-}
-// labels with those out of range as NONE; rows without one zeroed (f32 copies).
-__global__ __launch_bounds__(256) void k_xent_rows(const void* x, int kind, size_t ldx, size_t n,
-                                                   size_t d, const uint32_t* labels, size_t k,
-                                                   uint32_t* lab, float* out, uint32_t* small) {
-  const size_t i = blockIdx.x;
-  const uint32_t l = labels[i];
-  const bool has = l < k;
-  if (threadIdx.x == 0) {
-    lab[i] = has ? l : NO_LABEL;
-    if (!has && l != NO_LABEL) small[SW_BAD_CLASS] = 1u;
-  }
-  for (size_t j = threadIdx.x; j < d; j += 256)
-    out[i * d + j] = has ? load_kind(x, kind, i * ldx + j) : 0.f;
-}
-__global__ __launch_bounds__(256) void k_xent_out(const float* acc, size_t n, size_t d, void* out,
-                                                  int kind, size_t ld) {
+// out = the splits' sums added, in their order.
+template <class T>
+__global__ __launch_bounds__(256) void k_splits(const float* __restrict__ part, uint32_t splits,
+                                                size_t rows, uint32_t cols, size_t ldp, T* out,
+                                                size_t ldo) {
   const size_t t = (size_t)blockIdx.x * 256 + threadIdx.x;
-  if (t >= n * d) return;
-  store_kind(out, kind, t / d * ld + t % d, acc[t]);
+  const size_t per = ldp / 4, i = t / per;
+  if (i >= rows) return;
+  const uint32_t j = (uint32_t)(t % per) * 4;
+  if (j >= cols) return;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (uint32_t s = 0; s < splits; s++) {
+    const float4 p = *reinterpret_cast<const float4*>(part + (s * rows + i) * ldp + j);
+    v[0] += p.x, v[1] += p.y, v[2] += p.z, v[3] += p.w;
+  }
+  T* o = out + i * ldo + j;
+#pragma unroll
+  for (int e = 0; e < 4; e++)
+    if (j + e < cols) o[e] = from_f32<T>(v[e]);
 }
 
-void prod(emh_ctx* c, const ProdArgs& g) {
-  k_prod<<<dim3((unsigned)((g.b.rows + 63) / 64), (unsigned)((g.a.rows + 63) / 64)), 256, 0,
-           c->stream>>>(g);
+// Scratch of one call, 256-byte aligned pieces (first sized, then taken).
+struct Carve {
+  char* base = nullptr;
+  size_t used = 0;
+  template <class T>
+  T* take(size_t count) {
+    const size_t at = used;
+    used = (at + count * sizeof(T) + 255) & ~(size_t)255;
+    return reinterpret_cast<T*>(base + at);
+  }
+};
+
+uint32_t up(size_t v, size_t to) { return (uint32_t)((v + to - 1) / to * to); }
+
+// Whether rows can be the tiles' operand where they lie: every row at a 16-byte
+// address, whole 16-byte chunks (whole: whole slabs, for products along the row),
+// and offsets in a tile that stay below 2^31.
+bool direct(const MatIn& m, size_t d, bool whole) {
+  return m.kind != EMH_F32 && (uintptr_t)m.p % 16 == 0 && m.ld % 8 == 0 &&
+         m.ld < (size_t(1) << 22) && d % (whole ? SLAB : 8) == 0;
+}
+
+// An operand of the products: as it lies, or laid out in the call's scratch.
+struct Laid {
+  bool packed = false;
+  uint32_t dp = 0;  // elements of a laid-out row
+  char* p[2] = {nullptr, nullptr};
+  int* ex = nullptr;
+  void size(Carve& w, const MatIn& m, size_t rows, size_t d, bool need) {
+    packed = need;
+    dp = up(d, SLAB);
+    if (!need) return;
+    p[0] = w.take<char>(rows * dp * 2);
+    if (m.kind == EMH_F32) {
+      p[1] = w.take<char>(rows * dp * 2);
+      ex = w.take<int>(up(rows, 256));
+    }
+  }
+  Operand deep(const MatIn& m, size_t first, size_t rows) const {
+    Operand o{};
+    o.ld = packed ? dp * 2 : (uint32_t)(m.ld * 2);
+    for (int i = 0; i < 2; i++)
+      o.p[i] = (packed ? p[i] : (char*)m.p) + (p[1] || i == 0 ? first * o.ld : 0);
+    o.rows = (uint32_t)rows;
+    o.wide = packed ? dp : 0;
+    return o;
+  }
+};
+
+void pack(emh_ctx* c, const MatIn& m, size_t rows, size_t d, const Laid& l, const uint32_t* labels,
+          size_t k, const float* gloss, XentState* st, const uint32_t* when) {
+  const dim3 grid = grid1(rows, 4);
+  if (m.kind == EMH_F32)
+    k_pack32<<<grid, 256, 0, c->stream>>>((const float*)m.p, m.ld, rows, (uint32_t)d, l.dp, labels,
+                                          (uint32_t)k, gloss, (f16*)l.p[0], (f16*)l.p[1], l.ex, st,
+                                          c->small);
+  else  // (16-bit words, whatever they stand for)
+    k_pack16<f16><<<grid, 256, 0, c->stream>>>((const f16*)m.p, m.ld, rows, (uint32_t)d, l.dp, labels,
+                                               (uint32_t)k, (f16*)l.p[0], when);
+}
+
+// The shape and splits of a product of rows x cols over `steps` slabs: the
+// fewest rounds of workgroups times a workgroup's time, with the cost of
+// writing and adding the splits' sums.
+struct Plan {
+  bool large = true;
+  uint32_t rtiles = 1, ctiles = 1, splits = 1;
+};
+Plan plan_of(size_t rows, size_t cols, size_t steps, int cus, bool may_split) {
+  Plan best;
+  double least = 1e300;
+  for (int large = 1; large >= 0; large--) {
+    const size_t t = large ? TileL::TR : TileS::TR;
+    const size_t rt = (rows + t - 1) / t, ct = (cols + t - 1) / t;
+    const double at_once = large ? cus : 2.0 * cus;   // workgroups
+    const double step = large ? 1.0 : 0.6;            // us a slab, when the card is full
+    for (size_t s = 1; s <= (may_split ? 32 : 1); s++) {
+      if (s > 1 && steps < 4 * s) break;
+      const double rounds = std::ceil((double)(rt * ct * s) / at_once);
+      double us = rounds * ((double)((steps + s - 1) / s) + 4.0) * step;
+      if (s > 1) us += 3.0 + 8e-6 * (double)s * (double)rows * (double)cols / 4.0;
+      if (us < least) {
+        least = us;
+        best.large = large != 0;
+        best.rtiles = (uint32_t)rt, best.ctiles = (uint32_t)ct, best.splits = (uint32_t)s;
+      }
+    }
+  }
+  return best;
+}
+
+void join_splits(emh_ctx* c, const float* part, uint32_t splits, size_t rows, size_t cols, size_t ldp,
+                 void* out, size_t ldo, int kind) {
+  const dim3 grid = grid1(rows * (ldp / 4), 256);
+  if (kind == EMH_F32)
+    k_splits<float><<<grid, 256, 0, c->stream>>>(part, splits, rows, (uint32_t)cols, ldp, (float*)out, ldo);
+  else if (kind == EMH_F16)
+    k_splits<f16><<<grid, 256, 0, c->stream>>>(part, splits, rows, (uint32_t)cols, ldp, (f16*)out, ldo);
+  else
+    k_splits<bf16><<<grid, 256, 0, c->stream>>>(part, splits, rows, (uint32_t)cols, ldp, (bf16*)out, ldo);
 }
 
 }  // namespace
 
 void launch_cross_entropy(emh_ctx* c, const XentIn& in, float* loss, float* lse) {
-  const size_t parts = (in.k + 63) / 64;
-  char* ws = (char*)c->xent.get(parts * in.n * 8 + in.n * 4);
-  ProdArgs g{};
-  g.a = {in.x.p, in.x.kind, in.x.ld, 1, in.n};
-  g.b = {in.w.p, in.w.kind, in.w.ld, 1, in.k};
-  g.depth = in.d;
-  g.labels = in.labels;
-  g.s2 = in.scale * LOG2E;
-  g.part = (float2*)ws;
-  g.zlabel = (float*)(ws + parts * in.n * 8);
-  prod(c, g);
-  k_xent_join<<<grid1(in.n, 256), 256, 0, c->stream>>>(g.part, parts, in.n, in.labels, in.k,
-                                                       g.zlabel, loss, lse, c->small);
-  EMH_HIP(hipGetLastError());
+  const size_t n = in.n, d = in.d, k = in.k;
+  const bool f32 = in.x.kind == EMH_F32;
+  const size_t slabs = up(d, SLAB) / SLAB, passes = f32 ? 3 : 1;
+  // Rows at a time: what bounds them is the parts' maxima and sums (512 MB).
+  const size_t all = (k + 127) / 128 * 2;
+  const size_t rows = std::min(n, std::max<size_t>(256, ((size_t(64) << 20) / all) & ~(size_t)255));
+  Carve w;
+  Laid lx, lw;
+  float2* part = nullptr;
+  float* zlabel = nullptr;
+  for (int pass = 0; pass < 2; pass++) {
+    w.used = 0;
+    lx.size(w, in.x, n, d, !direct(in.x, d, true));
+    lw.size(w, in.w, k, d, !direct(in.w, d, true));
+    part = w.take<float2>(all * rows);
+    zlabel = w.take<float>(rows);
+    if (pass == 0) w.base = (char*)c->xent.get(w.used);
+  }
+  if (lx.packed) pack(c, in.x, n, d, lx, nullptr, 0, nullptr, nullptr, nullptr);
+  if (lw.packed) pack(c, in.w, k, d, lw, nullptr, 0, nullptr, nullptr, nullptr);
+  for (size_t r0 = 0; r0 < n; r0 += rows) {
+    const size_t m = std::min(rows, n - r0);
+    const Plan p = plan_of(m, k, slabs * passes, c->cus, false);
+    LogitArgs a{};
+    a.t.r = lx.deep(in.x, r0, m);
+    a.t.c = lw.deep(in.w, 0, k);
+    a.t.slabs = (uint32_t)slabs, a.t.passes = (uint32_t)passes;
+    a.t.rtiles = p.rtiles, a.t.ctiles = p.ctiles, a.t.splits = 1;
+    a.n = (uint32_t)m, a.m = a.k = (uint32_t)k;
+    a.labels = in.labels + r0;
+    a.s2 = in.scale * 1.44269504f;
+    a.ex = f32 ? lx.ex + r0 : nullptr;
+    a.ew = lw.ex;
+    a.part = part, a.zlabel = zlabel;
+    launch_logits(c->stream, a, in.x.kind, p.large, false);
+    k_join<<<grid1(m, 64), 1024, 0, c->stream>>>(part, p.ctiles * 2, (uint32_t)m, in.labels + r0,
+                                                 (uint32_t)k, zlabel, loss + r0,
+                                                 lse ? lse + r0 : nullptr, c->small);
+    EMH_HIP(hipGetLastError());
+  }
 }
 
 void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, const float* gloss,
                                const MatOut& dx, const MatOut& dw) {
   const size_t n = in.n, d = in.d, k = in.k;
-  // Classes a piece: 256 MB of their gradients.
-  const size_t piece = std::min(k, std::max<size_t>(64, (size_t(64) << 20) / std::max<size_t>(n, 1)));
-  char* ws = (char*)c->xent.get((n * piece + 2 * n * d + n + 1) * 4);
-  float* G = (float*)ws;
-  float* xs = G + n * piece;
-  float* acc = xs + n * d;
-  uint32_t* lab = (uint32_t*)(acc + n * d);
-  float* mean = (float*)(lab + n);
-  if (n > 0) {
-    k_xent_rows<<<dim3((unsigned)n), 256, 0, c->stream>>>(in.x.p, in.x.kind, in.x.ld, n, d,
-                                                          in.labels, k, lab, xs, c->small);
-    if (!gloss) k_xent_count<<<1, 1024, 0, c->stream>>>(in.labels, n, k, mean);
+  const bool f32 = in.x.kind == EMH_F32;
+  if (n == 0) {  // no row, no gradient
+    if (dw.p) join_splits(c, nullptr, 0, k, d, up(d, 4), dw.p, dw.ld, dw.kind);
+    EMH_HIP(hipGetLastError());
+    return;
   }
+  const size_t slabs = up(d, SLAB) / SLAB, passes = f32 ? 3 : 1, planes = f32 ? 4 : 1;
+  // Classes a piece: 1 GB of G.
+  const size_t np = up(n, 256);
+  const size_t piece =
+      std::min<size_t>(up(k, 256), std::max<size_t>(256, ((size_t(512) << 20) / (np * planes)) & ~(size_t)255));
+  const size_t ldg = piece * 2, pieces = (k + piece - 1) / piece, ldp = up(d, 4);
+  const Plan px = plan_of(n, d, passes * ((std::min(piece, k) + SLAB - 1) / SLAB), c->cus, true);
+  const Plan pw = plan_of(std::min(piece, k), d, passes * ((n + SLAB - 1) / SLAB), c->cus, true);
+  const bool px_part = px.splits > 1 || pieces > 1, pw_part = pw.splits > 1;
+  // Rows without a label are zeroed where x is laid out. Where the tiles can read
+  // it as it lies, a copy is made only if such a row holds a value that is not
+  // finite (which zero would not silence): the survey finds out, the copy and the product follow it.
+  const bool x_as_is = direct(in.x, d, true);
+  Carve w;
+  Laid lx, lw;
+  XentState* st = nullptr;
+  char* G[4] = {};
+  float *partx = nullptr, *partw = nullptr;
+  for (int pass = 0; pass < 2; pass++) {
+    w.used = 0;
+    st = w.take<XentState>(1);
+    lx.size(w, in.x, n, d, true);
+    lw.size(w, in.w, k, d, !direct(in.w, d, true));
+    for (size_t i = 0; i < planes; i++) G[i] = w.take<char>(np * ldg);
+    if (dx.p && px_part) partx = w.take<float>(px.splits * n * ldp);
+    if (dw.p && pw_part) partw = w.take<float>((size_t)pw.splits * std::min(piece, k) * ldp);
+    if (pass == 0) w.base = (char*)c->xent.get(w.used);
+  }
+  launch_fill_u32(c, (uint32_t*)st, sizeof(XentState) / 4, 0);
+  if (!f32) {
+    const dim3 grid = grid1(n, 256);
+    if (in.x.kind == EMH_F16)
+      k_survey<f16><<<grid, 256, 0, c->stream>>>((const f16*)in.x.p, in.x.ld, n, (uint32_t)d, in.labels,
+                                                 (uint32_t)k, gloss, st, c->small);
+    else
+      k_survey<bf16><<<grid, 256, 0, c->stream>>>((const bf16*)in.x.p, in.x.ld, n, (uint32_t)d,
+                                                  in.labels, (uint32_t)k, gloss, st, c->small);
+  }
+  pack(c, in.x, n, d, lx, in.labels, k, gloss, st, x_as_is ? &st->odd : nullptr);
+  if (lw.packed) pack(c, in.w, k, d, lw, nullptr, 0, nullptr, f32 ? st : nullptr, nullptr);
+  Laid as_is;
+  const Laid& xl = x_as_is ? as_is : lx;
   for (size_t v0 = 0; v0 < k; v0 += piece) {
     const size_t m = std::min(piece, k - v0);
-    const char* wp = (const char*)in.w.p + v0 * in.w.ld * kind_bytes(in.w.kind);
-    if (n > 0) {
-      ProdArgs g{};
-      g.a = {xs, EMH_F32, d, 1, n};
-      g.b = {wp, in.w.kind, in.w.ld, 1, m};
-      g.depth = d;
-      g.mode = 1;
-      g.labels = lab;
-      g.s2 = in.scale * LOG2E;
-      g.col0 = v0;
-      g.lse = lse;
-      g.up = gloss ? gloss : mean;
-      g.up_each = gloss != nullptr;
-      g.scale = in.scale;
-      g.out = G;
-      g.ldo = m;
-      prod(c, g);
-    }
-    if (dx.p && n > 0) {
-      ProdArgs g{};
-      g.a = {G, EMH_F32, m, 1, n};
-      g.b = {wp, in.w.kind, 1, in.w.ld, d};
-      g.depth = m;
-      g.mode = 2;
-      g.out = acc;
-      g.ldo = d;
-      g.add = v0 > 0;
-      prod(c, g);
+    const Plan pg = plan_of(n, m, slabs * passes, c->cus, false);
+    LogitArgs a{};
+    a.t.r = xl.deep(in.x, 0, n);
+    a.t.c = lw.deep(in.w, v0, m);
+    a.t.slabs = (uint32_t)slabs, a.t.passes = (uint32_t)passes;
+    a.t.rtiles = pg.rtiles, a.t.ctiles = pg.ctiles, a.t.splits = 1;
+    a.n = (uint32_t)n, a.m = (uint32_t)m, a.col0 = (uint32_t)v0, a.k = (uint32_t)k;
+    a.labels = in.labels;
+    a.s2 = in.scale * 1.44269504f;
+    a.ex = lx.ex, a.ew = f32 ? lw.ex + v0 : nullptr;
+    a.lse = lse, a.gloss = gloss, a.st = st, a.scale = in.scale;
+    for (int i = 0; i < 4; i++) a.g[i] = G[i];
+    a.ldg = ldg;
+    launch_logits(c->stream, a, in.x.kind, pg.large, true);
+    ProdArgs p{};
+    p.labels = in.labels, p.k = (uint32_t)k;
+    p.gloss = gloss, p.st = st, p.scale = in.scale;
+    p.t.passes = (uint32_t)passes;
+    p.cols = (uint32_t)d, p.ldp = ldp;
+    if (dx.p) {
+      p.t.r = {{G[0], G[1]}, (uint32_t)ldg, (uint32_t)n, 0};
+      p.t.c = lw.deep(in.w, v0, m);
+      p.t.c.wide = lw.packed ? lw.dp : (uint32_t)d;
+      p.t.slabs = (uint32_t)((m + SLAB - 1) / SLAB);
+      p.t.rtiles = px.rtiles, p.t.ctiles = px.ctiles, p.t.splits = px.splits;
+      p.rows = (uint32_t)n, p.dw = false;
+      p.out = dx.p, p.ldo = dx.ld;
+      p.part = px_part ? partx : nullptr;
+      p.add = v0 > 0;
+      launch_prod(c->stream, p, in.x.kind, px.large);
     }
     if (dw.p) {
-      ProdArgs g{};
-      g.a = {G, EMH_F32, 1, m, m};
-      g.b = {xs, EMH_F32, 1, d, d};
-      g.depth = n;
-      g.mode = 3;
-      g.out = (char*)dw.p + v0 * dw.ld * kind_bytes(dw.kind);
-      g.okind = dw.kind;
-      g.ldo = dw.ld;
-      prod(c, g);
+      p.t.r = {{f32 ? G[2] : G[0], G[3]}, (uint32_t)ldg, up(n, SLAB), (uint32_t)piece};
+      p.t.c = xl.deep(in.x, 0, n);
+      p.t.c.wide = xl.packed ? xl.dp : (uint32_t)d;
+      p.t.slabs = (uint32_t)((n + SLAB - 1) / SLAB);
+      p.t.rtiles = (uint32_t)((m + (pw.large ? TileL::TR : TileS::TR) - 1) / (pw.large ? TileL::TR : TileS::TR));
+      p.t.ctiles = pw.ctiles, p.t.splits = pw.splits;
+      p.rows = (uint32_t)m, p.dw = true;
+      p.out = (char*)dw.p + v0 * dw.ld * kind_bytes(dw.kind), p.ldo = dw.ld;
+      p.part = pw_part ? partw : nullptr;
+      p.add = false;
+      if (x_as_is) {
+        p.when = &st->odd;
+        p.alt = lx.deep(in.x, 0, n);
+      }
+      launch_prod(c->stream, p, in.x.kind, pw.large);
+      if (pw_part) join_splits(c, partw, pw.splits, m, d, ldp, p.out, dw.ld, dw.kind);
     }
   }
-  if (dx.p && n > 0)
-    k_xent_out<<<grid1(n * d, 256), 256, 0, c->stream>>>(acc, n, d, dx.p, dx.kind, dx.ld);
+  if (dx.p && px_part) join_splits(c, partx, px.splits, n, d, ldp, dx.p, dx.ld, dx.kind);
   EMH_HIP(hipGetLastError());
 }
 

@@ -1,0 +1,99 @@
+// The cross entropy's gradient products: dx = G w and dw = G^T x (emh_xent.h).
+#include "emh_xent.h"
+
+namespace emh {
+namespace {
+
+template <class T, class S, bool F32, bool DW, class O>
+__global__ __launch_bounds__(S::THREADS, 2) void k_grads(const ProdArgs a) {
+  __shared__ __attribute__((aligned(1024))) char ring[2 * S::STAGE];
+  const TileAt at = tile_at(a.t);
+  v16f acc[S::WA][S::WB];
+  TileIn t = a.t;
+  if (DW && a.when && *a.when != 0u) t.c = a.alt;
+  tile_sums<T, S, !DW, false>(t, at, ring, acc);
+
+  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, li = lane & 31, h = lane >> 5;
+  const int wr = w % S::NWR, wc = w / S::NWR;
+  const uint32_t i0 = at.rt * S::TR + wr * S::WB * 32 + li;
+  const uint32_t j0 = at.ct * S::TC + wc * S::WA * 32;
+  RowScale rs;
+  rs.init(a.st, a.gloss, a.scale);
+#pragma unroll
+  for (int y = 0; y < S::WB; y++) {
+    const uint32_t i = i0 + y * 32;
+    if (i >= a.rows) continue;
+    const bool zero = !DW && a.labels[i] >= a.k;
+    int by = 0;
+    if constexpr (F32)
+      by = DW ? -rs.gexp : a.st->ewmax - XENT_BIAS - row_exp(a.gloss, i);
+    else if constexpr (__is_same(T, f16))
+      by = -rs.gexp;
+#pragma unroll
+    for (int b = 0; b < S::WA; b++)
+#pragma unroll
+      for (int p = 0; p < 2; p++) {
+        float v[2][4], g[8];
+#pragma unroll
+        for (int f = 0; f < 2; f++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const float t = acc[b][y][4 * (2 * p + f) + e];
+            v[f][e] = zero ? 0.f : (__is_same(T, f16) ? ldexpf(t, by) : t) * rs.by;
+          }
+        if (a.part) {
+          // Whole fours: ldp is a multiple of 4.
+#pragma unroll
+          for (int f = 0; f < 2; f++) {
+            const uint32_t j = j0 + b * 32 + 8 * (2 * p + f) + 4 * h;
+            if (j >= a.cols) continue;
+            float4* o = reinterpret_cast<float4*>(
+                a.part + ((size_t)at.split * a.rows + i) * a.ldp + j);
+            float4 s = make_float4(v[f][0], v[f][1], v[f][2], v[f][3]);
+            if (a.add) {
+              const float4 had = *o;
+              s = make_float4(had.x + s.x, had.y + s.y, had.z + s.z, had.w + s.w);
+            }
+            *o = s;
+          }
+          continue;
+        }
+        eight(v[0], v[1], g);
+        const uint32_t j = j0 + b * 32 + 16 * p + 8 * h;
+        O* o = reinterpret_cast<O*>(a.out) + (size_t)i * a.ldo + j;
+        if (j + 8 <= a.cols) {
+          store_vec(o, g);
+          if constexpr (sizeof(O) == 4) store_vec(o + 4, g + 4);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; e++)
+            if (j + e < a.cols) o[e] = from_f32<O>(g[e]);
+        }
+      }
+  }
+}
+
+template <class T, bool F32, class O>
+void launch(hipStream_t s, const ProdArgs& a, bool large) {
+  const unsigned blocks = a.t.rtiles * a.t.ctiles * a.t.splits;
+  if (large)
+    a.dw ? k_grads<T, TileL, F32, true, O><<<blocks, TileL::THREADS, 0, s>>>(a)
+         : k_grads<T, TileL, F32, false, O><<<blocks, TileL::THREADS, 0, s>>>(a);
+  else
+    a.dw ? k_grads<T, TileS, F32, true, O><<<blocks, TileS::THREADS, 0, s>>>(a)
+         : k_grads<T, TileS, F32, false, O><<<blocks, TileS::THREADS, 0, s>>>(a);
+}
+
+}  // namespace
+
+void launch_prod(hipStream_t s, const ProdArgs& a, int kind, bool large) {
+  if (kind == EMH_F32)
+    launch<f16, true, float>(s, a, large);
+  else if (kind == EMH_F16)
+    launch<f16, false, f16>(s, a, large);
+  else
+    launch<bf16, false, bf16>(s, a, large);
+  EMH_HIP(hipGetLastError());
+}
+
+}  // namespace emh

@@ -1,0 +1,177 @@
+// The cross entropy's logits in tiles: every row's maximum and sum over each tile's
+// columns, or the gradients of a piece of the classes (emh_xent.h).
+#include "emh_xent.h"
+
+namespace emh {
+namespace {
+
+constexpr float LOG2E = 1.44269504f;
+
+// F32: operands are planes of f16 with exponents.
+template <class T, class S, bool F32, bool GRAD>
+__global__ __launch_bounds__(S::THREADS, 2) void k_logits(const LogitArgs a) {
+  __shared__ __attribute__((aligned(1024))) char ring[2 * S::STAGE];
+  const TileAt at = tile_at(a.t);
+  v16f acc[S::WA][S::WB];
+  tile_sums<T, S, true, true>(a.t, at, ring, acc);
+
+  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, li = lane & 31, h = lane >> 5;
+  const int wr = w % S::NWR, wc = w / S::NWR;
+  const uint32_t i0 = at.rt * S::TR + wr * S::WB * 32 + li;
+  const uint32_t j0 = at.ct * S::TC + wc * S::WA * 32;
+
+  // To logits times log2(e).
+  int ex[S::WB];
+#pragma unroll
+  for (int y = 0; y < S::WB; y++) ex[y] = F32 ? a.ex[min(i0 + y * 32, a.n - 1)] : 0;
+#pragma unroll
+  for (int b = 0; b < S::WA; b++)
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      int ew[4] = {0, 0, 0, 0};
+      if constexpr (F32) {  // (the exponents' buffer is a whole number of tiles long)
+        const int4 v = *reinterpret_cast<const int4*>(a.ew + j0 + b * 32 + 8 * q + 4 * h);
+        ew[0] = v.x, ew[1] = v.y, ew[2] = v.z, ew[3] = v.w;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+#pragma unroll
+        for (int y = 0; y < S::WB; y++) {
+          const float z = acc[b][y][4 * q + e];
+          acc[b][y][4 * q + e] = (F32 ? ldexpf(z, ex[y] + ew[e]) : z) * a.s2;
+        }
+    }
+
+  // Columns of the wave that there are; all of them but in the last tile.
+  const int left = (int)min(a.m - min(a.m, j0), (uint32_t)(S::WA * 32));
+  const bool full = left == S::WA * 32;
+  if constexpr (!GRAD) {
+    const uint32_t pi = at.ct * S::NWC + wc;
+    if (!full) {
+      int have = left - 4 * h;
+      asm volatile("" : "+v"(have));  // (the comparisons are made here, not kept)
+#pragma unroll
+      for (int b = 0; b < S::WA; b++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          const bool in = b * 32 + 8 * (r >> 2) + (r & 3) < have;
+#pragma unroll
+          for (int y = 0; y < S::WB; y++) acc[b][y][r] = in ? acc[b][y][r] : -INFINITY;
+        }
+    }
+#pragma unroll
+    for (int y = 0; y < S::WB; y++) {
+      const uint32_t i = i0 + y * 32;
+      const uint32_t lab = i < a.n ? a.labels[i] : NO_LABEL;
+      uint32_t own = lab - j0 - 4 * h;  // the label's column of the lane's, if it has it
+      asm volatile("" : "+v"(own));
+      float m = -INFINITY, z = 0.f;
+      bool mine = false;
+#pragma unroll
+      for (int b = 0; b < S::WA; b++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          const bool is = own == (uint32_t)(b * 32 + 8 * (r >> 2) + (r & 3));
+          z = is ? acc[b][y][r] : z;
+          mine = mine || is;
+          m = fmaxf(m, acc[b][y][r]);  // (passes over NaN: the sum keeps it)
+        }
+      if (mine && lab < a.k) a.zlabel[i] = z;
+      m = fmaxf(m, __shfl_xor(m, 32, 64));
+      const float mm = m == -INFINITY ? 0.f : m;
+      float s = 0.f;
+#pragma unroll
+      for (int b = 0; b < S::WA; b++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) s += __builtin_amdgcn_exp2f(acc[b][y][r] - mm);
+      s += __shfl_xor(s, 32, 64);
+      if (h == 0 && i < a.n) a.part[(size_t)pi * a.n + i] = make_float2(m, s);
+    }
+  } else {
+    RowScale rs;
+    rs.init(a.st, a.gloss, a.scale);
+    int ewmax = 0;
+    if constexpr (F32) ewmax = a.st->ewmax - XENT_BIAS;
+#pragma unroll
+    for (int y = 0; y < S::WB; y++) {
+      const uint32_t i = i0 + y * 32;
+      const uint32_t ic = min(i, a.n - 1);
+      const uint32_t lab = i < a.n ? a.labels[ic] : NO_LABEL;
+      const bool has = lab < a.k;
+      const float l2 = a.lse[ic] * LOG2E;
+      const float u = a.gloss ? a.gloss[ic] : 1.f;
+      const int ga = F32 ? row_exp(a.gloss, ic) : 0;
+      // The label's column (another piece's: none of this one), and the columns
+      // there are, none in a row without a label, from the lane's first.
+      uint32_t own = lab - a.col0 - j0 - 4 * h;
+      int have = (has ? left : 0) - 4 * h;
+      asm volatile("" : "+v"(own), "+v"(have));
+#pragma unroll
+      for (int b = 0; b < S::WA; b++)
+#pragma unroll
+        for (int p = 0; p < 2; p++) {
+          float v[2][4];
+#pragma unroll
+          for (int f = 0; f < 2; f++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const int c = b * 32 + 8 * (2 * p + f) + e;
+              const float soft = __builtin_amdgcn_exp2f(acc[b][y][4 * (2 * p + f) + e] - l2);
+              const float g = (soft - (own == (uint32_t)c ? 1.f : 0.f)) * u;
+              v[f][e] = c < have ? g : 0.f;
+            }
+          float g[8];
+          eight(v[0], v[1], g);
+          const uint32_t j = j0 + b * 32 + 16 * p + 8 * h;
+          const size_t o = (size_t)i * a.ldg + (size_t)j * 2;
+          if constexpr (!F32) {
+            if constexpr (__is_same(T, f16)) {
+#pragma unroll
+              for (int e = 0; e < 8; e++) g[e] = ldexpf(g[e], rs.gexp);
+            }
+            store_vec(reinterpret_cast<T*>(a.g[0] + o), g);
+          } else {
+            float hi[8], lo[8];
+            const int4 w0 = *reinterpret_cast<const int4*>(a.ew + j);
+            const int4 w1 = *reinterpret_cast<const int4*>(a.ew + j + 4);
+            const int ew[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+            for (int which = 0; which < 2; which++) {
+#pragma unroll
+              for (int e = 0; e < 8; e++) {
+                const int by = which ? ex[y] + rs.gexp : ew[e] - ewmax + ga;
+                const float t = ldexpf(g[e], by);
+                hi[e] = (float)(f16)t;
+                lo[e] = t - hi[e];
+              }
+              store_vec(reinterpret_cast<f16*>(a.g[2 * which] + o), hi);
+              store_vec(reinterpret_cast<f16*>(a.g[2 * which + 1] + o), lo);
+            }
+          }
+        }
+    }
+  }
+}
+
+template <class T, bool F32, bool GRAD>
+void launch(hipStream_t s, const LogitArgs& a, bool large) {
+  const unsigned blocks = a.t.rtiles * a.t.ctiles;
+  if (large)
+    k_logits<T, TileL, F32, GRAD><<<blocks, TileL::THREADS, 0, s>>>(a);
+  else
+    k_logits<T, TileS, F32, GRAD><<<blocks, TileS::THREADS, 0, s>>>(a);
+}
+
+}  // namespace
+
+void launch_logits(hipStream_t s, const LogitArgs& a, int kind, bool large, bool grads) {
+  if (kind == EMH_F32)
+    grads ? launch<f16, true, true>(s, a, large) : launch<f16, true, false>(s, a, large);
+  else if (kind == EMH_F16)
+    grads ? launch<f16, false, true>(s, a, large) : launch<f16, false, false>(s, a, large);
+  else
+    grads ? launch<bf16, false, true>(s, a, large) : launch<bf16, false, false>(s, a, large);
+  EMH_HIP(hipGetLastError());
+}
+
+}  // namespace emh
