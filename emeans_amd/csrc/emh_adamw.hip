@@ -102,12 +102,14 @@ __device__ __forceinline__ uint32_t encode4(const float* v, float& scale) {
     const float m = fabsf(v[e]);
     top = fmaxf(top, m <= 3.4028235e38f ? m : 0.f);
   }
-  scale = lanes_max<64>(top) / F8_TOP;
-  const float by = scale > 0.f ? scale : 1.f;
+  scale = lanes_max<64>(top) * (1.f / F8_TOP);
+  // (One reciprocal a block: a code near a tie may be its neighbour. Finite, or a
+  // zero in a block of the least numbers would become a NaN.)
+  const float by = fminf(__builtin_amdgcn_rcpf(scale), 3.4028235e38f);
   float q[4];
 #pragma unroll
   for (int e = 0; e < 4; e++) {
-    q[e] = v[e] / by;
+    q[e] = v[e] * by;
     if (LEAST && v[e] > 0.f && q[e] < F8_LEAST) q[e] = F8_LEAST;
     // (A quotient that rounded past the top; infinities and NaN become the NaN code.)
     if (fabsf(v[e]) <= 3.4028235e38f)
@@ -119,25 +121,32 @@ __device__ __forceinline__ uint32_t encode4(const float* v, float& scale) {
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], (int)w, true);
 }
 
-constexpr int ADAM_U = (int)(ADAM_CHUNK / 1024);  // a thread's fours
+// sqrt(v) within a unit in the last place, below the normal range too (where
+// the instruction takes zero for v).
+__device__ __forceinline__ float root(float v) {
+  const bool small = v < 1.17549435e-38f;
+  const float t = __builtin_amdgcn_sqrtf(small ? v * 18446744073709551616.f : v);  // 2^64
+  return small ? t * 2.3283064365386963e-10f : t;                                  // 2^-32
+}
 
+template <int U>  // a chunk: 1024 U elements
 __global__ __launch_bounds__(256) void k_adamw(const AdamTensor* __restrict__ tensors,
                                                const uint2* __restrict__ chunks,
                                                const AdamScalars s) {
   const uint2 at = chunks[blockIdx.x];
   const AdamTensor t = tensors[at.x];
-  const size_t base = (size_t)at.y * ADAM_CHUNK;
+  const size_t base = (size_t)at.y * (1024 * U);
   const size_t here = t.len - base;  // > 0
   const int lane4 = (int)threadIdx.x * 4;
   const bool eight = t.m_scale != nullptr;
   const float keep = (float)(1.0 - s.lr * t.weight_decay);
-  float p[ADAM_U][4], g[ADAM_U][4], m[ADAM_U][4], v[ADAM_U][4];
-  uint32_t mc[ADAM_U], vc[ADAM_U];
-  float msc[ADAM_U], vsc[ADAM_U];
+  float p[U][4], g[U][4], m[U][4], v[U][4];
+  uint32_t mc[U], vc[U];
+  float msc[U], vsc[U];
 #pragma unroll
-  for (int u = 0; u < ADAM_U; u++) {
+  for (int u = 0; u < U; u++) {
     const int o = u * 1024 + lane4;
-    const int left = (int)min((size_t)ADAM_CHUNK, here) - o;
+    const int left = (int)min((size_t)(1024 * U), here) - o;
     const size_t i = base + o;
     load4_kind(t.param, t.param_kind, i, left, p[u]);
     load4_kind(t.grad, t.grad_kind, i, left, g[u]);
@@ -152,9 +161,9 @@ __global__ __launch_bounds__(256) void k_adamw(const AdamTensor* __restrict__ te
     }
   }
 #pragma unroll
-  for (int u = 0; u < ADAM_U; u++) {
+  for (int u = 0; u < U; u++) {
     const int o = u * 1024 + lane4;
-    const int left = (int)min((size_t)ADAM_CHUNK, here) - o;
+    const int left = (int)min((size_t)(1024 * U), here) - o;
     const size_t i = base + o;
     if (eight) {
       decode4(mc[u], msc[u], m[u]);
@@ -168,7 +177,11 @@ __global__ __launch_bounds__(256) void k_adamw(const AdamTensor* __restrict__ te
       const float ge = g[u][e] * s.gscale;
       m[u][e] = s.beta1 * m[u][e] + s.new1 * ge;
       v[u][e] = s.beta2 * v[u][e] + s.new2 * ge * ge;
-      const float by = m[u][e] / (sqrtf(v[u][e] * s.inv2) + s.eps);
+      // The root and the quotient within two units of the last place (the correctly
+      // rounded ones are twenty instructions each, which bounded the step: 595 us at
+      // 134 million elements).
+      r[e] = root(v[u][e]);
+      const float by = m[u][e] * __builtin_amdgcn_rcpf(r[e] * s.root2 + s.eps);
       p[u][e] = p[u][e] * keep - s.rate * by;
     }
     store4_kind(t.param, t.param_kind, i, left, p[u]);
@@ -177,7 +190,7 @@ __global__ __launch_bounds__(256) void k_adamw(const AdamTensor* __restrict__ te
       // (Elements past the tensor's end are zeros here and have no part in the scale.)
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        r[e] = e < left ? sqrtf(v[u][e]) : 0.f;
+        r[e] = e < left ? r[e] : 0.f;
         m[u][e] = e < left ? m[u][e] : 0.f;
       }
       float ms, vs;
@@ -198,9 +211,13 @@ __global__ __launch_bounds__(256) void k_adamw(const AdamTensor* __restrict__ te
 }  // namespace
 
 void launch_adamw(emh_ctx* c, const AdamTensor* tensors, const uint2* chunks, size_t nchunks,
-                  const AdamScalars& s) {
+                  size_t chunk, const AdamScalars& s) {
   if (nchunks == 0) return;
-  k_adamw<<<dim3((unsigned)nchunks), 256, 0, c->stream>>>(tensors, chunks, s);
+  const dim3 grid((unsigned)nchunks);
+  if (chunk == ADAM_CHUNK)
+    k_adamw<(int)(ADAM_CHUNK / 1024)><<<grid, 256, 0, c->stream>>>(tensors, chunks, s);
+  else
+    k_adamw<(int)(ADAM_CHUNK_FEW / 1024)><<<grid, 256, 0, c->stream>>>(tensors, chunks, s);
   EMH_HIP(hipGetLastError());
 }
 

@@ -163,6 +163,7 @@ enum SmallWord : int {
   SW_TICKET = 6,          // blocks of the scatter count kernel that have finished (reset by the last)
   SW_NBIG = 7,            // clusters of the current scatter with more rows than the per-column path takes
   SW_BAD_INIT = 8,        // set when a training run's initial centroids are not finite
+  SW_ODD_ROW = 10,        // number of the last cross entropy gradient whose rows without a label had values that are not finite
   SW_BAD_CLASS = 9,       // set when the cross entropy saw a label >= k that is not NONE
   SW_WORDS = 16,
 };
@@ -251,6 +252,7 @@ struct emh_ctx {
   // carved from a block kept between calls, since hipFree waits for the
   // whole device, the other contexts' streams included.
   emh::Scratch trun, kpp, iscore, cnorm;
+  uint32_t xent_calls = 0;  // gradients of the cross entropy so far (see SW_ODD_ROW)
   emh::Scratch norm_part;  // layer_norm_grad: the blocks' sums of dweight and dbias
   emh::Scratch xent;       // cross_entropy's parts, gradients of a piece and laid-out operands
   emh::Scratch preview_ticket;  // k_mass_preview's last-block ticket (left at zero)

@@ -13,7 +13,7 @@ struct emh_adamw {
   emh_ctx* ctx = nullptr;
   emh::AdamTensor* tensors = nullptr;  // on the device
   uint2* chunks = nullptr;
-  size_t nchunks = 0;
+  size_t nchunks = 0, chunk = emh::ADAM_CHUNK;
   std::vector<emh_buf*> written;
 };
 
@@ -283,6 +283,9 @@ int emh_adamw_create(emh_ctx* c, const emh_adamw_tensor* tensors, size_t count, 
     std::vector<Written> read;
     auto plan = std::make_unique<emh_adamw>();
     plan->ctx = c;
+    size_t total = 0;
+    for (size_t i = 0; i < count; i++) total += tensors[i].param ? tensors[i].param->len : 0;
+    if (total <= emh::ADAM_FEW) plan->chunk = emh::ADAM_CHUNK_FEW;
     for (size_t i = 0; i < count; i++) {
       const emh_adamw_tensor& t = tensors[i];
       EMH_ENSURE(t.param && real_kind(t.param->kind), "tensor %zu: param must be f32, f16 or bf16", i);
@@ -326,8 +329,8 @@ int emh_adamw_create(emh_ctx* c, const emh_adamw_tensor* tensors, size_t count, 
       }
       a.len = len;
       a.weight_decay = t.weight_decay;
-      EMH_ENSURE(len < (size_t(1) << 43), "tensor %zu is too long", i);
-      for (size_t k = 0; k * emh::ADAM_CHUNK < len; k++)
+      EMH_ENSURE(len < (size_t(1) << 41), "tensor %zu is too long", i);
+      for (size_t k = 0; k * plan->chunk < len; k++)
         chunks.push_back(make_uint2((unsigned)table.size(), (unsigned)k));
       table.push_back(a);
     }
@@ -385,13 +388,13 @@ int emh_adamw_step(emh_adamw* plan, const emh_adamw_config* cfg) {
     s.new1 = (float)(1.0 - cfg->beta1);
     s.new2 = (float)(1.0 - cfg->beta2);
     s.rate = (float)(cfg->lr / (1.0 - std::pow(cfg->beta1, (double)cfg->step)));
-    s.inv2 = (float)(1.0 / (1.0 - std::pow(cfg->beta2, (double)cfg->step)));
+    s.root2 = (float)(1.0 / std::sqrt(1.0 - std::pow(cfg->beta2, (double)cfg->step)));
     s.eps = (float)cfg->eps;
     s.gscale = (float)cfg->grad_scale;
     s.lr = cfg->lr;
     use_device(plan->ctx);
     for (emh_buf* b : plan->written) ++b->gen;
-    emh::launch_adamw(plan->ctx, plan->tensors, plan->chunks, plan->nchunks, s);
+    emh::launch_adamw(plan->ctx, plan->tensors, plan->chunks, plan->nchunks, plan->chunk, s);
   });
 }
 

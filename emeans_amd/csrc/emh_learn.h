@@ -55,12 +55,15 @@ struct AdamTensor {  // as the kernel reads it
 };
 struct AdamScalars {
   float beta1, beta2, new1, new2;  // new = 1 - beta
-  float rate, inv2, eps, gscale;   // lr / (1 - beta1^t), 1 / (1 - beta2^t)
+  float rate, root2, eps, gscale;  // lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t)
   double lr;
 };
-constexpr size_t ADAM_CHUNK = 4096;  // elements of a workgroup's share of one tensor
+// Elements of a workgroup's share of one tensor: four loads of each array in
+// flight a thread, or, in a plan of few elements, one, and four times the workgroups.
+constexpr size_t ADAM_CHUNK = 4096, ADAM_CHUNK_FEW = 1024;
+constexpr size_t ADAM_FEW = size_t(2) << 20;
 // chunks[i]: the tensor and the chunk in it that workgroup i takes.
 void launch_adamw(emh_ctx* c, const AdamTensor* tensors, const uint2* chunks, size_t nchunks,
-                  const AdamScalars& s);
+                  size_t chunk, const AdamScalars& s);
 
 }  // namespace emh

@@ -73,6 +73,28 @@ __device__ __forceinline__ void store_cols(T* row, int col, int d, const float* 
     store_some(row + min(col, d), v, d - col);
 }
 
+// A vector's columns of a norm's weight or bias (T or f32), `fill` without one.
+template <class T>
+__device__ __forceinline__ void load_affine(const void* p, int kind, int col, int d, float fill,
+                                            float* out) {
+  constexpr int N = VecOf<T>::N;
+  if (!p) {
+#pragma unroll
+    for (int e = 0; e < N; e++) out[e] = fill;
+  } else if (kind == EMH_F32) {
+#pragma unroll
+    for (int q = 0; q < N; q += 4) {
+      const Vec<float> v = load_cols(reinterpret_cast<const float*>(p), col + q, d);
+#pragma unroll
+      for (int e = 0; e < 4; e++) out[q + e] = v.get(e);
+    }
+  } else {
+    const Vec<T> v = load_cols(reinterpret_cast<const T*>(p), col, d);
+#pragma unroll
+    for (int e = 0; e < N; e++) out[e] = v.get(e);
+  }
+}
+
 // Forward: LPR threads a row, NV vectors of 16 bytes a thread.
 template <class T, int LPR, int NV>
 __global__ __launch_bounds__(256) void k_norm(const NormArgs a) {
@@ -82,13 +104,10 @@ __global__ __launch_bounds__(256) void k_norm(const NormArgs a) {
   const int d = a.d;
   float w[NV * N], b[NV * N];
 #pragma unroll
-  for (int j = 0; j < NV; j++)
-#pragma unroll
-    for (int e = 0; e < N; e++) {
-      const int col = (l + LPR * j) * N + e;
-      w[j * N + e] = a.w && col < d ? load_kind(a.w, a.wkind, col) : 1.f;
-      b[j * N + e] = a.b && col < d ? load_kind(a.b, a.bkind, col) : 0.f;
-    }
+  for (int j = 0; j < NV; j++) {
+    load_affine<T>(a.w, a.wkind, (l + LPR * j) * N, d, 1.f, w + j * N);
+    load_affine<T>(a.b, a.bkind, (l + LPR * j) * N, d, 0.f, b + j * N);
+  }
   const float inv = 1.0f / (float)d;
   int slot = 0;
   // (The bound is the workgroup's: all its threads meet at row_sum's barriers.)
@@ -130,65 +149,54 @@ __global__ __launch_bounds__(256) void k_norm(const NormArgs a) {
   }
 }
 
-// Backward, TB threads: the next row's loads are in flight while a row's sums
-// are formed.
+// Backward, TB threads. (The row's elements stay packed and are unpacked again for
+// the result: what that takes is fewer registers, so twice the waves, whose rows are
+// in flight together.)
 template <class T, int LPR, int NV, int TB>
-__global__ __launch_bounds__(TB) void k_norm_grad(const NormArgs a) {
+__global__ __launch_bounds__(TB, NV * VecOf<T>::N <= 16 ? 4 : 2) void k_norm_grad(const NormArgs a) {
   constexpr int N = VecOf<T>::N, G = TB / LPR;
   __shared__ float red[4][TB / 64];
-  __shared__ float fold[G > 1 ? TB * NV * N : 1];
+  __shared__ float fold[TB * NV * N];
   const int l = threadIdx.x % LPR, g = threadIdx.x / LPR;
   const int d = a.d;
   float w[NV * N], aw[NV * N], ab[NV * N];
 #pragma unroll
-  for (int j = 0; j < NV; j++)
+  for (int j = 0; j < NV; j++) {
+    load_affine<T>(a.w, a.wkind, (l + LPR * j) * N, d, 1.f, w + j * N);
 #pragma unroll
-    for (int e = 0; e < N; e++) {
-      const int col = (l + LPR * j) * N + e;
-      w[j * N + e] = a.w && col < d ? load_kind(a.w, a.wkind, col) : 1.f;
-      aw[j * N + e] = ab[j * N + e] = 0.f;
-    }
+    for (int e = 0; e < N; e++) aw[j * N + e] = ab[j * N + e] = 0.f;
+  }
   const float inv = 1.0f / (float)d;
-  Vec<T> x[NV], dy[NV];
-  float mean, rstd;
-  auto fetch = [&](size_t row) __attribute__((always_inline)) {
+  const size_t step = (size_t)gridDim.x * G;
+  int slot = 0;
+  for (size_t r0 = (size_t)blockIdx.x * G; r0 < a.rows; r0 += step) {
+    const size_t row = r0 + g;
     const bool live = row < a.rows;
     const size_t r = live ? row : 0;
     const T* xp = reinterpret_cast<const T*>(a.x) + r * a.ldx;
     const T* dp = reinterpret_cast<const T*>(a.dy) + r * a.lddy;
+    const int have = live ? d : 0;
+    Vec<T> x[NV], dy[NV];
 #pragma unroll
     for (int j = 0; j < NV; j++) {
-      x[j] = load_cols(xp, (l + LPR * j) * N, d);
-      dy[j] = load_cols(dp, (l + LPR * j) * N, d);
+      x[j] = load_cols(xp, (l + LPR * j) * N, have);
+      dy[j] = load_cols(dp, (l + LPR * j) * N, have);
     }
-    mean = a.mean[r];
-    rstd = a.rstd[r];
-  };
-  const size_t step = (size_t)gridDim.x * G;
-  int slot = 0;
-  size_t r0 = (size_t)blockIdx.x * G;
-  if (r0 < a.rows) fetch(r0 + g);
-  for (; r0 < a.rows; r0 += step) {
-    const size_t row = r0 + g;
-    const bool live = row < a.rows;
-    float h[NV * N], u[NV * N];
+    const float mean = a.mean[r], rstd = a.rstd[r];
     float c1 = 0.f, c2 = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; j++)
 #pragma unroll
       for (int e = 0; e < N; e++) {
+        // Past the row (and in no row) dy is zero, and x is made the mean.
         const int i = j * N + e;
-        const bool in = live && (l + LPR * j) * N + e < d;
-        h[i] = in ? (x[j].get(e) - mean) * rstd : 0.f;
-        const float t = in ? dy[j].get(e) : 0.f;
+        const float h = (l + LPR * j) * N + e < have ? (x[j].get(e) - mean) * rstd : 0.f;
+        const float t = dy[j].get(e);
         ab[i] += t;
-        aw[i] = fmaf(t, h[i], aw[i]);
-        u[i] = t * w[i];
-        c1 += u[i];
-        c2 = fmaf(u[i], h[i], c2);
+        aw[i] = fmaf(t, h, aw[i]);
+        c1 = fmaf(t, w[i], c1);
+        c2 = fmaf(t * w[i], h, c2);
       }
-    const float rs = rstd;
-    if (r0 + step < a.rows) fetch(r0 + step + g);
     c1 = row_sum<LPR, TB>(c1, red, slot) * inv;
     c2 = row_sum<LPR, TB>(c2, red, slot ^ 1) * inv;
     slot ^= 2;
@@ -199,41 +207,30 @@ __global__ __launch_bounds__(TB) void k_norm_grad(const NormArgs a) {
         float t[N];
 #pragma unroll
         for (int e = 0; e < N; e++)
-          t[e] = rs * (u[j * N + e] - c1 - h[j * N + e] * c2);
+          t[e] = rstd * (dy[j].get(e) * w[j * N + e] - c1 - (x[j].get(e) - mean) * rstd * c2);
         store_cols(o, (l + LPR * j) * N, d, t);
       }
     }
   }
   if (!a.part) return;
-  // The groups' sums of a column, added by the first group: dweight, then dbias.
+  // The groups' sums of a column added through LDS: dweight, then dbias.
+  static_assert(G > 1, "groups to add");
 #pragma unroll
   for (int which = 0; which < 2; which++) {
-    float* v = which ? ab : aw;
-    if constexpr (G > 1) {
-      if (which) __syncthreads();
+    if (which) __syncthreads();
 #pragma unroll
-      for (int i = 0; i < NV * N; i++) fold[i * TB + threadIdx.x] = v[i];
-      __syncthreads();
-    }
-    if (g == 0) {
-      float* out = a.part + ((size_t)blockIdx.x * 2 + which) * d;
+    for (int i = 0; i < NV * N; i++) fold[i * TB + threadIdx.x] = which ? ab[i] : aw[i];
+    __syncthreads();
+    float* out = a.part + ((size_t)blockIdx.x * 2 + which) * d;
 #pragma unroll
-      for (int j = 0; j < NV; j++) {
-        float s[N];
-#pragma unroll
-        for (int e = 0; e < N; e++) {
-          if constexpr (G > 1) {
-            s[e] = 0.f;
-            for (int k = 0; k < G; k++) s[e] += fold[(j * N + e) * TB + k * LPR + l];
-          } else {
-            s[e] = v[j * N + e];
-          }
-        }
-        const int col = (l + LPR * j) * N;
-#pragma unroll
-        for (int e = 0; e < N; e++)
-          if (col + e < d) out[col + e] = s[e];
-      }
+    for (int i0 = 0; i0 < NV * N; i0 += G) {
+      const int i = i0 + g;
+      const int col = (l + LPR * (i / N)) * N + i % N;
+      if (i >= NV * N || col >= d) continue;
+      float s = 0.f;
+#pragma unroll 8
+      for (int k = 0; k < G; k++) s += fold[i * TB + k * LPR + l];
+      out[col] = s;
     }
   }
 }
@@ -414,11 +411,11 @@ void launch_layer_norm_grad(emh_ctx* c, const MatIn& dy, const MatIn& x, size_t 
     using T = decltype(t);
     const bool held = by_shape<T>(d, [&](auto s) {
       using S = decltype(s);
-      // A workgroup a CU: as many waves as its registers allow, and the fewest
-      // rows of sums to write and add.
-      constexpr int TB = S::NV * VecOf<T>::N <= 16 ? 1024 : 512;
+      // As many waves a CU as the registers allow (two workgroups of at most 16
+      // columns a thread, else one): few rows of sums to write and add.
+      constexpr int TB = 512;
       constexpr size_t G = TB / S::LPR;
-      parts = std::min((rows + G - 1) / G, (size_t)c->cus * (1024 / TB));
+      parts = std::min((rows + G - 1) / G, (size_t)c->cus * (S::NV * VecOf<T>::N <= 16 ? 2 : 1));
       if (sums) a.part = (float*)c->norm_part.get(parts * 2 * d * 4);
       k_norm_grad<T, S::LPR, S::NV, TB><<<dim3((unsigned)parts), TB, 0, c->stream>>>(a);
     });

@@ -104,19 +104,39 @@ __device__ __forceinline__ void store_kind(void* p, int kind, size_t i, float v)
     reinterpret_cast<bf16*>(p)[i] = (bf16)v;
 }
 
-// Sums over groups of W consecutive lanes (W a power of two, at most 64), in
-// every lane.
-template <int W>
-__device__ __forceinline__ float lanes_sum(float v) {
-#pragma unroll
-  for (int o = W / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+// Reductions over groups of W consecutive lanes (16, 32 or 64), the result in
+// every lane, without LDS: lane permutations within rows of 16 (neighbours, pairs,
+// then mirrored halves and rows, whose lanes agree by then), and the swaps of rows
+// and halves between two registers.
+template <int CTRL>
+__device__ __forceinline__ float lane_perm(float v) {
+  return __int_as_float(
+      __builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, false));
+}
+template <int W, class F>
+__device__ __forceinline__ float lanes_reduce(float v, F&& f) {
+  static_assert(W == 16 || W == 32 || W == 64, "group of lanes");
+  v = f(v, lane_perm<0xB1>(v));   // quad_perm 1 0 3 2
+  v = f(v, lane_perm<0x4E>(v));   // quad_perm 2 3 0 1
+  v = f(v, lane_perm<0x141>(v));  // row_half_mirror
+  v = f(v, lane_perm<0x140>(v));  // row_mirror
+  if constexpr (W >= 32) {
+    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = f(__uint_as_float(s[0]), __uint_as_float(s[1]));
+  }
+  if constexpr (W == 64) {
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = f(__uint_as_float(s[0]), __uint_as_float(s[1]));
+  }
   return v;
 }
 template <int W>
+__device__ __forceinline__ float lanes_sum(float v) {
+  return lanes_reduce<W>(v, [](float a, float b) { return a + b; });
+}
+template <int W>
 __device__ __forceinline__ float lanes_max(float v) {
-#pragma unroll
-  for (int o = W / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-  return v;
+  return lanes_reduce<W>(v, [](float a, float b) { return fmaxf(a, b); });
 }
 
 }  // namespace emh

@@ -35,7 +35,20 @@ struct XentState {
   uint32_t count;  // rows with a label
   int uexp;        // largest exponent of |gloss_i| 2^ex_i over them (no gloss: of 2^ex_i), + BIAS
   int ewmax;       // largest ew_v, + BIAS
-  uint32_t odd;    // a row without a label holds a value that is not finite
+};
+// Rows without a label have zeros in G, which silence any finite value of x in dw.
+// f32 rows are laid out for the call anyway, and are made zeros there. 16-bit rows
+// that the tiles can read as they lie are looked at (k_survey): only when one
+// without a label holds a value that is not finite, which the call's number in
+// `flag` then says, the kernel of the logits makes the copy `rows` of x with
+// zeros in their place, and dw reads that.
+struct OddRows {
+  const uint32_t* flag;  // null: nothing to do
+  uint32_t call;
+  char* rows;
+  uint32_t dp;           // elements of a row there
+  const char* x;
+  size_t ld, d;
 };
 constexpr int XENT_BIAS = 4096;  // (so that zero is less than any)
 
@@ -53,6 +66,7 @@ struct LogitArgs {
   const float* gloss;
   const XentState* st;
   float scale;
+  OddRows odd;
   char* g[4];       // G; f32: Ga's planes, Gb's planes
   size_t ldg;       // bytes (rows and columns to full tiles)
 };
@@ -73,7 +87,8 @@ struct ProdArgs {
   float* part;          // one split's sums: [split][row][ldp] in f32
   size_t ldp;
   bool add;             // into what an earlier piece left
-  const uint32_t* when; // dw: where it is not zero, x is read from here
+  const uint32_t* flag; // dw: where it is `call`, x is read from alt
+  uint32_t call;
   Operand alt;
 };
 void launch_prod(hipStream_t s, const ProdArgs& a, int kind, bool large);

@@ -12,13 +12,11 @@ namespace {
 constexpr float LN2 = 0.693147181f;
 
 // Rows to 16-byte aligned rows of dp elements, the rest zero (dp a multiple of
-// SLAB). labels: rows without one become zeros. when: only if it is not zero.
-// A wave a row.
+// SLAB). labels: rows without one become zeros. A wave a row.
 template <class T>
 __global__ __launch_bounds__(256) void k_pack16(const T* x, size_t ld, size_t n, uint32_t d,
                                                 uint32_t dp, const uint32_t* labels, uint32_t k,
-                                                T* out, const uint32_t* when) {
-  if (when && *when == 0u) return;
+                                                T* out) {
   const size_t i = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (i >= n) return;
   const uint32_t lane = threadIdx.x & 63;
@@ -31,35 +29,42 @@ __global__ __launch_bounds__(256) void k_pack16(const T* x, size_t ld, size_t n,
   }
 }
 
-// f32 rows to planes of f16 (see emh_xent.h) and their exponents e (x = plane
-// 2^e). With st, what the gradients need to know: rows (labels given) their count
-// and the largest exponent of |gloss| 2^e, rows without a label become zeros;
-// classes the largest exponent. A wave a row.
+// f32 rows to planes of f16 (emh_xent.h) and their exponents e (x = plane 2^e);
+// labels: rows without one become zeros. A wave a row, which it holds where it
+// has at most 1,024 elements, and reads twice beyond.
 __global__ __launch_bounds__(256) void k_pack32(const float* x, size_t ld, size_t n, uint32_t d,
                                                 uint32_t dp, const uint32_t* labels, uint32_t k,
-                                                const float* gloss, f16* hi, f16* lo, int* ex,
-                                                XentState* st, uint32_t* small) {
+                                                f16* hi, f16* lo, int* ex) {
   const size_t i = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (i >= n) return;
   const uint32_t lane = threadIdx.x & 63;
   const float* row = x + i * ld;
-  const uint32_t lab = labels ? labels[i] : 0u;
-  const bool zero = labels && lab >= k;
-  float top = 0.f;
-  for (uint32_t c = lane * 4; c < d; c += 256) {
-    const Vec<float> v = c + 4 <= d ? load_vec(row + c) : load_some(row + c, (int)(d - c));
+  const bool zero = labels && labels[i] >= k;
+  constexpr uint32_t HELD = 4;  // vectors of four a lane
+  auto get = [&](uint32_t c) __attribute__((always_inline)) {
+    Vec<float> v{make_uint4(0u, 0u, 0u, 0u)};
+    if (!zero && c < d) v = c + 4 <= d ? load_vec(row + c) : load_some(row + c, (int)(d - c));
+    return v;
+  };
+  auto largest = [](const Vec<float>& v, float top) __attribute__((always_inline)) {
 #pragma unroll
     for (int e = 0; e < 4; e++) {
       const float m = fabsf(v.get(e));
       top = fmaxf(top, m < INFINITY ? m : 0.f);
     }
-  }
+    return top;
+  };
+  Vec<float> held[HELD];
+  float top = 0.f;
+#pragma unroll
+  for (uint32_t q = 0; q < HELD; q++) held[q] = get(lane * 4 + q * 256);
+#pragma unroll
+  for (uint32_t q = 0; q < HELD; q++) top = largest(held[q], top);
+  for (uint32_t c = lane * 4 + HELD * 256; c < d; c += 256) top = largest(get(c), top);
   top = lanes_max<64>(top);
-  const int e0 = !zero && top > 0.f ? max(ilogbf(top) - 13, -120) : 0;
+  const int e0 = top > 0.f ? max(ilogbf(top) - 13, -120) : 0;
   const float by = ldexpf(1.f, -e0);
-  for (uint32_t c = lane * 4; c < dp; c += 256) {
-    Vec<float> v{make_uint4(0u, 0u, 0u, 0u)};
-    if (!zero && c < d) v = c + 4 <= d ? load_vec(row + c) : load_some(row + c, (int)(d - c));
+  auto put = [&](uint32_t c, const Vec<float>& v) __attribute__((always_inline)) {
     uint16_t a[4], b[4];
 #pragma unroll
     for (int e = 0; e < 4; e++) {
@@ -73,58 +78,192 @@ __global__ __launch_bounds__(256) void k_pack32(const float* x, size_t ld, size_
         make_uint2(a[0] | (uint32_t)a[1] << 16, a[2] | (uint32_t)a[3] << 16);
     *reinterpret_cast<uint2*>(lo + o) =
         make_uint2(b[0] | (uint32_t)b[1] << 16, b[2] | (uint32_t)b[3] << 16);
-  }
-  if (lane != 0) return;
-  ex[i] = e0;
-  if (!st) return;
-  if (!labels) {
-    atomicMax(&st->ewmax, e0 + XENT_BIAS);
-    return;
-  }
-  if (zero) {
-    if (lab != NO_LABEL) small[SW_BAD_CLASS] = 1u;
-    return;
-  }
-  atomicAdd(&st->count, 1u);
-  const float g = gloss ? fabsf(gloss[i]) : 1.f;
-  if (g > 0.f && g < INFINITY) atomicMax(&st->uexp, ilogbf(g) + e0 + XENT_BIAS);
+  };
+#pragma unroll
+  for (uint32_t q = 0; q < HELD; q++)
+    if (lane * 4 + q * 256 < dp) put(lane * 4 + q * 256, held[q]);
+  for (uint32_t c = lane * 4 + HELD * 256; c < dp; c += 256) put(c, get(c));
+  if (lane == 0) ex[i] = e0;
 }
 
-// The same facts for 16-bit rows: a thread a row, a wave at a time over the
-// rows without a label, whose values have to be finite to be multiplied by zero.
+// The call's state, by workgroup 0 alone (a pass over the labels, and of f32
+// operands over the exponents); the others, for 16-bit rows that are read as they
+// lie (OddRows), look at the rows without a label, a wave at sixteen labels.
 template <class T>
-__global__ __launch_bounds__(256) void k_survey(const T* x, size_t ld, size_t n, uint32_t d,
-                                                const uint32_t* labels, uint32_t k,
-                                                const float* gloss, XentState* st,
-                                                uint32_t* small) {
-  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-  const uint32_t lane = threadIdx.x & 63;
-  const uint32_t lab = i < n ? labels[i] : NO_LABEL;
-  const bool has = lab < k;
-  const float g = has ? gloss ? fabsf(gloss[i]) : 1.f : 0.f;
-  const int e = g > 0.f && g < INFINITY ? ilogbf(g) + XENT_BIAS : 0;
-  if (!has && lab != NO_LABEL) small[SW_BAD_CLASS] = 1u;
-  const unsigned long long some = __ballot(has);
-  int top = e;
-  for (int o = 32; o > 0; o >>= 1) top = max(top, __shfl_xor(top, o, 64));
-  if (lane == 0) {
-    if (some) atomicAdd(&st->count, (uint32_t)__popcll(some));
-    if (top) atomicMax(&st->uexp, top);
-  }
-  unsigned long long none = __ballot(i < n && !has);
-  const size_t first = i - lane;
-  bool odd = false;
-  while (none) {
-    const int r = __ffsll((long long)none) - 1;
-    none &= none - 1;
-    const T* row = x + (first + r) * ld;
-    for (uint32_t c = lane * 8; c < d; c += 512) {
-      const Vec<T> v = c + 8 <= d ? load_vec(row + c) : load_some(row + c, (int)(d - c));
+__global__ __launch_bounds__(1024) void k_survey(const T* x, size_t ld, uint32_t n, uint32_t d,
+                                                 const uint32_t* __restrict__ labels, uint32_t k,
+                                                 const float* __restrict__ gloss,
+                                                 const int* __restrict__ ex,
+                                                 const int* __restrict__ ew, XentState* st,
+                                                 uint32_t* small, uint32_t call) {
+  const uint32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  if (blockIdx.x > 0) {
+    const uint32_t first = (blockIdx.x - 1) * 256 + w * 16;
+    const bool none = lane < 16 && first + lane < n && labels[first + lane] >= k;
+    unsigned long long left = __ballot(none);
+    bool odd = false;
+    while (left) {
+      const int r = __ffsll((long long)left) - 1;
+      left &= left - 1;
+      const T* row = x + (size_t)(first + r) * ld;
+#pragma unroll 4
+      for (uint32_t c = lane * 8; c < d; c += 512) {
+        const Vec<T> v = c + 8 <= d ? load_vec(row + c) : load_some(row + c, (int)(d - c));
 #pragma unroll
-      for (int q = 0; q < 8; q++) odd = odd || !(fabsf(v.get(q)) < INFINITY);
+        for (int q = 0; q < 8; q++) odd = odd || !(fabsf(v.get(q)) < INFINITY);
+      }
     }
+    if (__ballot(odd) != 0ull && lane == 0) small[SW_ODD_ROW] = call;
+    return;
   }
-  if (__ballot(odd) != 0ull && lane == 0) st->odd = 1u;
+  __shared__ int sh[3][16];
+  int count = 0, uexp = 0, ewmax = 0;
+  bool bad = false;
+#pragma unroll 4
+  for (uint32_t i = threadIdx.x; i < n; i += 1024) {
+    const uint32_t lab = labels[i];
+    const bool has = lab < k;
+    bad = bad || (!has && lab != NO_LABEL);
+    count += has ? 1 : 0;
+    const float g = gloss ? fabsf(gloss[i]) : 1.f;
+    const int e = (ex ? ex[i] : 0) + XENT_BIAS + (gloss ? ilogbf(g) : 0);
+    if (has && g > 0.f && g < INFINITY) uexp = max(uexp, e);
+  }
+  if (ew) {
+#pragma unroll 8
+    for (uint32_t j = threadIdx.x; j < k; j += 1024) ewmax = max(ewmax, ew[j] + XENT_BIAS);
+  }
+  if (bad) small[SW_BAD_CLASS] = 1u;
+  for (int o = 32; o > 0; o >>= 1) {
+    count += __shfl_xor(count, o, 64);
+    uexp = max(uexp, __shfl_xor(uexp, o, 64));
+    ewmax = max(ewmax, __shfl_xor(ewmax, o, 64));
+  }
+  if (lane == 0) sh[0][w] = count, sh[1][w] = uexp, sh[2][w] = ewmax;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int i = 1; i < 16; i++) {
+    count += sh[0][i];
+    uexp = max(uexp, sh[1][i]);
+    ewmax = max(ewmax, sh[2][i]);
+  }
+  *st = XentState{(uint32_t)count, uexp, ewmax};
+}
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+
+// Few rows (at most 16 R) against all classes, the operands read as they lie, once:
+// a workgroup takes 16 classes at a time, its four waves a quarter of the depth
+// each (every fourth 64 bytes of a row), with 16 x 16 MFMAs, the classes as their A: a
+// lane then holds four classes of one row. f32 in f32 MFMAs. The workgroup's maximum
+// and sum of its classes go to part[row][workgroup].
+// Bound by the classes' bytes from HBM, or by latency: 16 rows of 384 against
+// 256 classes are 25 KB a CU.
+template <class T, int R>
+__global__ __launch_bounds__(256) void k_few(const T* __restrict__ x, size_t ldx, uint32_t n,
+                                             uint32_t d, const T* __restrict__ w, size_t ldw,
+                                             uint32_t k, const uint32_t* __restrict__ labels,
+                                             float s2, float2* part, float* zlabel) {
+  constexpr int N = VecOf<T>::N, DEEP = 4 * N;  // a chunk: DEEP of the depth, N a lane
+  constexpr int U = R == 4 ? 4 : 8;             // chunks in flight
+  __shared__ v4f sum[4][R][64];
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t l = lane & 15, q = lane >> 4;
+  const uint32_t groups = (k + 15) / 16, chunks = (d + DEEP - 1) / DEEP;
+  float m = -INFINITY, s = 0.f;  // of the row that this lane keeps (wave r: rows 16 r ..)
+  const uint32_t mine = wave * 16 + l;
+  const uint32_t lab = wave < R && mine < n ? labels[mine] : NO_LABEL;
+  auto fetch = [&](const T* p, size_t ld, uint32_t row, uint32_t rows, uint32_t c) __attribute__((always_inline)) {
+    const T* at = p + (size_t)min(row, rows - 1) * ld;
+    const uint32_t col = c * DEEP + q * N;
+    if (col + N <= d) return load_vec(at + col);
+    return load_some(at + min(col, d), (int)d - (int)col);
+  };
+  for (uint32_t g = blockIdx.x; g < groups; g += gridDim.x) {
+    v4f acc[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) acc[r] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (uint32_t c0 = wave; c0 < chunks; c0 += 4 * U) {
+      Vec<T> a[U];
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        if (c0 + 4 * u < chunks) a[u] = fetch(w, ldw, g * 16 + l, k, c0 + 4 * u);
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        if (c0 + 4 * u >= chunks) continue;
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+          const Vec<T> b = fetch(x, ldx, r * 16 + l, n, c0 + 4 * u);
+          if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              acc[r] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[u].get(e), b.get(e), acc[r], 0, 0, 0);
+          } else if constexpr (__is_same(T, f16)) {
+            acc[r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a[u].raw),
+                                                            __builtin_bit_cast(v8h, b.raw), acc[r], 0, 0, 0);
+          } else {
+            acc[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a[u].raw),
+                                                             __builtin_bit_cast(v8bf, b.raw), acc[r], 0, 0, 0);
+          }
+        }
+      }
+    }
+    __syncthreads();  // the last group's sums have been read
+#pragma unroll
+    for (int r = 0; r < R; r++) sum[wave][r][lane] = acc[r];
+    __syncthreads();
+    if (wave >= R) continue;
+    v4f z = sum[0][wave][lane];
+#pragma unroll
+    for (int i = 1; i < 4; i++) z += sum[i][wave][lane];
+    float top = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const uint32_t j = g * 16 + q * 4 + e;
+      z[e] = j < k ? z[e] * s2 : -INFINITY;
+      if (j == lab && j < k) zlabel[mine] = z[e];
+      top = fmaxf(top, z[e]);  // (passes over NaN: the sum keeps it)
+    }
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    const float b = fmaxf(m, top), bb = b == -INFINITY ? 0.f : b;
+    s *= __builtin_amdgcn_exp2f(m - bb);
+#pragma unroll
+    for (int e = 0; e < 4; e++) s += __builtin_amdgcn_exp2f(z[e] - bb);
+    m = b;
+  }
+  if (wave >= R) return;
+  s += __shfl_xor(s, 16, 64);  // (the four lanes of a row share m)
+  s += __shfl_xor(s, 32, 64);
+  if (q == 0 && mine < n) part[(size_t)mine * gridDim.x + blockIdx.x] = make_float2(m, s);
+}
+
+// Its parts joined, a workgroup a row.
+__global__ __launch_bounds__(256) void k_join_few(const float2* __restrict__ part, uint32_t nparts,
+                                                  const uint32_t* labels, uint32_t k,
+                                                  const float* zlabel, float* loss, float* lse,
+                                                  uint32_t* small) {
+  __shared__ float2 sh[4];
+  const uint32_t i = blockIdx.x;
+  float m = -INFINITY, s = 0.f;
+  auto join = [&](float2 p) __attribute__((always_inline)) {
+    const float b = fmaxf(m, p.x), bb = b == -INFINITY ? 0.f : b;
+    s = s * __builtin_amdgcn_exp2f(m - bb) + p.y * __builtin_amdgcn_exp2f(p.x - bb);
+    m = b;
+  };
+#pragma unroll 4
+  for (uint32_t t = threadIdx.x; t < nparts; t += 256) join(part[(size_t)i * nparts + t]);
+  for (int o = 32; o > 0; o >>= 1) join(make_float2(__shfl_xor(m, o, 64), __shfl_xor(s, o, 64)));
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = make_float2(m, s);
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  m = sh[0].x, s = sh[0].y;
+  for (int t = 1; t < 4; t++) join(sh[t]);
+  const float l2 = (m == -INFINITY ? 0.f : m) + log2f(s);
+  const uint32_t lab = labels[i];
+  if (lse) lse[i] = l2 * LN2;
+  loss[i] = lab < k ? (l2 - zlabel[i]) * LN2 : 0.f;
+  if (lab >= k && lab != NO_LABEL) small[SW_BAD_CLASS] = 1u;
 }
 
 // The parts' maxima and sums joined: 64 rows a workgroup, 16 shares of the parts.
@@ -235,15 +374,39 @@ struct Laid {
 };
 
 void pack(emh_ctx* c, const MatIn& m, size_t rows, size_t d, const Laid& l, const uint32_t* labels,
-          size_t k, const float* gloss, XentState* st, const uint32_t* when) {
+          size_t k) {
   const dim3 grid = grid1(rows, 4);
   if (m.kind == EMH_F32)
     k_pack32<<<grid, 256, 0, c->stream>>>((const float*)m.p, m.ld, rows, (uint32_t)d, l.dp, labels,
-                                          (uint32_t)k, gloss, (f16*)l.p[0], (f16*)l.p[1], l.ex, st,
-                                          c->small);
+                                          (uint32_t)k, (f16*)l.p[0], (f16*)l.p[1], l.ex);
   else  // (16-bit words, whatever they stand for)
     k_pack16<f16><<<grid, 256, 0, c->stream>>>((const f16*)m.p, m.ld, rows, (uint32_t)d, l.dp, labels,
-                                               (uint32_t)k, (f16*)l.p[0], when);
+                                               (uint32_t)k, (f16*)l.p[0]);
+}
+
+// At most this many rows take the kernel that reads the classes once, as they lie.
+constexpr size_t FEW_ROWS = 64;
+constexpr uint32_t FEW_BLOCKS = 2048;
+template <class T>
+void few(emh_ctx* c, const XentIn& in, float* loss, float* lse) {
+  const uint32_t n = (uint32_t)in.n, k = (uint32_t)in.k;
+  const uint32_t blocks = std::min((k + 15) / 16, FEW_BLOCKS);
+  char* ws = (char*)c->xent.get((size_t)blocks * n * sizeof(float2) + n * 4);
+  float2* part = (float2*)ws;
+  float* zlabel = (float*)(part + (size_t)blocks * n);
+  auto run = [&](auto kernel) {
+    kernel<<<dim3(blocks), 256, 0, c->stream>>>((const T*)in.x.p, in.x.ld, n, (uint32_t)in.d,
+                                                (const T*)in.w.p, in.w.ld, k, in.labels,
+                                                in.scale * 1.44269504f, part, zlabel);
+  };
+  if (n <= 16)
+    run(k_few<T, 1>);
+  else if (n <= 32)
+    run(k_few<T, 2>);
+  else
+    run(k_few<T, 4>);
+  k_join_few<<<dim3(n), 256, 0, c->stream>>>(part, blocks, in.labels, k, zlabel, loss, lse, c->small);
+  EMH_HIP(hipGetLastError());
 }
 
 // The shape and splits of a product of rows x cols over `steps` slabs: the
@@ -260,12 +423,12 @@ Plan plan_of(size_t rows, size_t cols, size_t steps, int cus, bool may_split) {
     const size_t t = large ? TileL::TR : TileS::TR;
     const size_t rt = (rows + t - 1) / t, ct = (cols + t - 1) / t;
     const double at_once = large ? cus : 2.0 * cus;   // workgroups
-    const double step = large ? 1.0 : 0.6;            // us a slab, when the card is full
+    const double step = large ? 1.8 : 1.2;            // us a slab, when the card is full
     for (size_t s = 1; s <= (may_split ? 32 : 1); s++) {
       if (s > 1 && steps < 4 * s) break;
       const double rounds = std::ceil((double)(rt * ct * s) / at_once);
-      double us = rounds * ((double)((steps + s - 1) / s) + 4.0) * step;
-      if (s > 1) us += 3.0 + 8e-6 * (double)s * (double)rows * (double)cols / 4.0;
+      double us = rounds * ((double)((steps + s - 1) / s) * step + 4.0);
+      if (s > 1) us += 3.0 + 1.8e-6 * (double)s * (double)rows * (double)cols;
       if (us < least) {
         least = us;
         best.large = large != 0;
@@ -292,6 +455,15 @@ void join_splits(emh_ctx* c, const float* part, uint32_t splits, size_t rows, si
 void launch_cross_entropy(emh_ctx* c, const XentIn& in, float* loss, float* lse) {
   const size_t n = in.n, d = in.d, k = in.k;
   const bool f32 = in.x.kind == EMH_F32;
+  if (n <= FEW_ROWS) {
+    if (f32)
+      few<float>(c, in, loss, lse);
+    else if (in.x.kind == EMH_F16)
+      few<f16>(c, in, loss, lse);
+    else
+      few<bf16>(c, in, loss, lse);
+    return;
+  }
   const size_t slabs = up(d, SLAB) / SLAB, passes = f32 ? 3 : 1;
   // Rows at a time: what bounds them is the parts' maxima and sums (512 MB).
   const size_t all = (k + 127) / 128 * 2;
@@ -308,8 +480,8 @@ void launch_cross_entropy(emh_ctx* c, const XentIn& in, float* loss, float* lse)
     zlabel = w.take<float>(rows);
     if (pass == 0) w.base = (char*)c->xent.get(w.used);
   }
-  if (lx.packed) pack(c, in.x, n, d, lx, nullptr, 0, nullptr, nullptr, nullptr);
-  if (lw.packed) pack(c, in.w, k, d, lw, nullptr, 0, nullptr, nullptr, nullptr);
+  if (lx.packed) pack(c, in.x, n, d, lx, nullptr, 0);
+  if (lw.packed) pack(c, in.w, k, d, lw, nullptr, 0);
   for (size_t r0 = 0; r0 < n; r0 += rows) {
     const size_t m = std::min(rows, n - r0);
     const Plan p = plan_of(m, k, slabs * passes, c->cus, false);
@@ -350,9 +522,7 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
   const Plan px = plan_of(n, d, passes * ((std::min(piece, k) + SLAB - 1) / SLAB), c->cus, true);
   const Plan pw = plan_of(std::min(piece, k), d, passes * ((n + SLAB - 1) / SLAB), c->cus, true);
   const bool px_part = px.splits > 1 || pieces > 1, pw_part = pw.splits > 1;
-  // Rows without a label are zeroed where x is laid out. Where the tiles can read
-  // it as it lies, a copy is made only if such a row holds a value that is not
-  // finite (which zero would not silence): the survey finds out, the copy and the product follow it.
+  // Rows without a label: see OddRows.
   const bool x_as_is = direct(in.x, d, true);
   Carve w;
   Laid lx, lw;
@@ -369,18 +539,22 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
     if (dw.p && pw_part) partw = w.take<float>((size_t)pw.splits * std::min(piece, k) * ldp);
     if (pass == 0) w.base = (char*)c->xent.get(w.used);
   }
-  launch_fill_u32(c, (uint32_t*)st, sizeof(XentState) / 4, 0);
-  if (!f32) {
-    const dim3 grid = grid1(n, 256);
-    if (in.x.kind == EMH_F16)
-      k_survey<f16><<<grid, 256, 0, c->stream>>>((const f16*)in.x.p, in.x.ld, n, (uint32_t)d, in.labels,
-                                                 (uint32_t)k, gloss, st, c->small);
+  const uint32_t call = ++c->xent_calls;
+  if (!x_as_is) pack(c, in.x, n, d, lx, in.labels, k);
+  if (lw.packed) pack(c, in.w, k, d, lw, nullptr, 0);
+  {
+    const dim3 grid(x_as_is ? 1 + (unsigned)((n + 255) / 256) : 1);
+    auto run = [&](auto t) {
+      using T = decltype(t);
+      k_survey<T><<<grid, 1024, 0, c->stream>>>((const T*)in.x.p, in.x.ld, (uint32_t)n, (uint32_t)d,
+                                                in.labels, (uint32_t)k, gloss, lx.ex, lw.ex, st,
+                                                c->small, call);
+    };
+    if (in.x.kind == EMH_BF16)
+      run(bf16{});
     else
-      k_survey<bf16><<<grid, 256, 0, c->stream>>>((const bf16*)in.x.p, in.x.ld, n, (uint32_t)d,
-                                                  in.labels, (uint32_t)k, gloss, st, c->small);
+      run(f16{});  // (f32 rows are laid out: none is looked at)
   }
-  pack(c, in.x, n, d, lx, in.labels, k, gloss, st, x_as_is ? &st->odd : nullptr);
-  if (lw.packed) pack(c, in.w, k, d, lw, nullptr, 0, nullptr, f32 ? st : nullptr, nullptr);
   Laid as_is;
   const Laid& xl = x_as_is ? as_is : lx;
   for (size_t v0 = 0; v0 < k; v0 += piece) {
@@ -396,6 +570,8 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
     a.s2 = in.scale * 1.44269504f;
     a.ex = lx.ex, a.ew = f32 ? lw.ex + v0 : nullptr;
     a.lse = lse, a.gloss = gloss, a.st = st, a.scale = in.scale;
+    if (x_as_is && v0 == 0)
+      a.odd = {c->small + SW_ODD_ROW, call, lx.p[0], lx.dp, (const char*)in.x.p, in.x.ld, d};
     for (int i = 0; i < 4; i++) a.g[i] = G[i];
     a.ldg = ldg;
     launch_logits(c->stream, a, in.x.kind, pg.large, true);
@@ -428,7 +604,8 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
       p.part = pw_part ? partw : nullptr;
       p.add = false;
       if (x_as_is) {
-        p.when = &st->odd;
+        p.flag = c->small + SW_ODD_ROW;
+        p.call = call;
         p.alt = lx.deep(in.x, 0, n);
       }
       launch_prod(c->stream, p, in.x.kind, pw.large);

@@ -10,7 +10,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_grads(const ProdArgs a) {
   const TileAt at = tile_at(a.t);
   v16f acc[S::WA][S::WB];
   TileIn t = a.t;
-  if (DW && a.when && *a.when != 0u) t.c = a.alt;
+  if (DW && a.flag && *a.flag == a.call) t.c = a.alt;
   tile_sums<T, S, !DW, false>(t, at, ring, acc);
 
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, li = lane & 31, h = lane >> 5;

@@ -7,10 +7,29 @@ namespace {
 
 constexpr float LOG2E = 1.44269504f;
 
+// x with zeros in rows without a label (OddRows): every workgroup its share.
+template <class T>
+__device__ __forceinline__ void copy_rows(const LogitArgs& a) {
+  const OddRows& o = a.odd;
+  for (uint32_t i = blockIdx.x; i < a.n; i += gridDim.x) {
+    const T* row = reinterpret_cast<const T*>(o.x) + i * o.ld;
+    const bool has = a.labels[i] < a.k;
+    for (uint32_t c = threadIdx.x * 8; c < o.dp; c += blockDim.x * 8) {
+      Vec<T> v{make_uint4(0u, 0u, 0u, 0u)};
+      if (has && c < o.d)
+        v = c + 8 <= o.d ? load_vec(row + c) : load_some(row + c, (int)(o.d - c));
+      *reinterpret_cast<uint4*>(o.rows + ((size_t)i * o.dp + c) * 2) = v.raw;
+    }
+  }
+}
+
 // F32: operands are planes of f16 with exponents.
 template <class T, class S, bool F32, bool GRAD>
 __global__ __launch_bounds__(S::THREADS, 2) void k_logits(const LogitArgs a) {
   __shared__ __attribute__((aligned(1024))) char ring[2 * S::STAGE];
+  if constexpr (GRAD && !F32) {
+    if (a.odd.flag && *a.odd.flag == a.odd.call) copy_rows<T>(a);
+  }
   const TileAt at = tile_at(a.t);
   v16f acc[S::WA][S::WB];
   tile_sums<T, S, true, true>(a.t, at, ring, acc);
@@ -88,10 +107,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_logits(const LogitArgs a) {
       if (h == 0 && i < a.n) a.part[(size_t)pi * a.n + i] = make_float2(m, s);
     }
   } else {
-    RowScale rs;
-    rs.init(a.st, a.gloss, a.scale);
-    int ewmax = 0;
-    if constexpr (F32) ewmax = a.st->ewmax - XENT_BIAS;
+    // G in place of the logits.
 #pragma unroll
     for (int y = 0; y < S::WB; y++) {
       const uint32_t i = i0 + y * 32;
@@ -100,7 +116,6 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_logits(const LogitArgs a) {
       const bool has = lab < a.k;
       const float l2 = a.lse[ic] * LOG2E;
       const float u = a.gloss ? a.gloss[ic] : 1.f;
-      const int ga = F32 ? row_exp(a.gloss, ic) : 0;
       // The label's column (another piece's: none of this one), and the columns
       // there are, none in a row without a label, from the lane's first.
       uint32_t own = lab - a.col0 - j0 - 4 * h;
@@ -109,46 +124,75 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_logits(const LogitArgs a) {
 #pragma unroll
       for (int b = 0; b < S::WA; b++)
 #pragma unroll
-        for (int p = 0; p < 2; p++) {
-          float v[2][4];
+        for (int r = 0; r < 16; r++) {
+          const int c = b * 32 + 8 * (r >> 2) + (r & 3);
+          const float soft = __builtin_amdgcn_exp2f(acc[b][y][r] - l2);
+          const float g = (soft - (own == (uint32_t)c ? 1.f : 0.f)) * u;
+          acc[b][y][r] = c < have ? g : 0.f;
+        }
+    }
+    // Through LDS (the ring is free once every wave is here), so that a row's
+    // 2 TC bytes go to memory together: eight columns a lane are one 16-byte chunk,
+    // XOR-swizzled by the row.
+    RowScale rs;
+    rs.init(a.st, a.gloss, a.scale);
+    int ewmax = 0;
+    if constexpr (F32) ewmax = a.st->ewmax - XENT_BIAS;
+    constexpr int CH = S::TC / 8;
+    const uint32_t r0 = wr * S::WB * 32 + li;
 #pragma unroll
-          for (int f = 0; f < 2; f++)
+    for (int plane = 0; plane < (F32 ? 4 : 1); plane++) {
+      __syncthreads();
+#pragma unroll
+      for (int y = 0; y < S::WB; y++) {
+        const int ga = F32 ? row_exp(a.gloss, min(i0 + y * 32, a.n - 1)) : 0;
+        const uint32_t row = r0 + y * 32;
+#pragma unroll
+        for (int b = 0; b < S::WA; b++)
+#pragma unroll
+          for (int p = 0; p < 2; p++) {
+            float lo[4], hi[4], g[8];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-              const int c = b * 32 + 8 * (2 * p + f) + e;
-              const float soft = __builtin_amdgcn_exp2f(acc[b][y][4 * (2 * p + f) + e] - l2);
-              const float g = (soft - (own == (uint32_t)c ? 1.f : 0.f)) * u;
-              v[f][e] = c < have ? g : 0.f;
+              lo[e] = acc[b][y][8 * p + e];
+              hi[e] = acc[b][y][8 * p + 4 + e];
             }
-          float g[8];
-          eight(v[0], v[1], g);
-          const uint32_t j = j0 + b * 32 + 16 * p + 8 * h;
-          const size_t o = (size_t)i * a.ldg + (size_t)j * 2;
-          if constexpr (!F32) {
-            if constexpr (__is_same(T, f16)) {
+            eight(lo, hi, g);
+            if constexpr (F32) {
+              int by[8];
+              if (plane < 2) {
+                const uint32_t j = j0 + b * 32 + 16 * p + 8 * h;
+                const int4 w0 = *reinterpret_cast<const int4*>(a.ew + j);
+                const int4 w1 = *reinterpret_cast<const int4*>(a.ew + j + 4);
+                const int ew[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+                for (int e = 0; e < 8; e++) by[e] = ew[e] - ewmax + ga;
+              } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++) by[e] = ex[y] + rs.gexp;
+              }
+#pragma unroll
+              for (int e = 0; e < 8; e++) {
+                const float t = ldexpf(g[e], by[e]);
+                g[e] = plane & 1 ? t - (float)(f16)t : t;
+              }
+            } else if constexpr (__is_same(T, f16)) {
 #pragma unroll
               for (int e = 0; e < 8; e++) g[e] = ldexpf(g[e], rs.gexp);
             }
-            store_vec(reinterpret_cast<T*>(a.g[0] + o), g);
-          } else {
-            float hi[8], lo[8];
-            const int4 w0 = *reinterpret_cast<const int4*>(a.ew + j);
-            const int4 w1 = *reinterpret_cast<const int4*>(a.ew + j + 4);
-            const int ew[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-#pragma unroll
-            for (int which = 0; which < 2; which++) {
-#pragma unroll
-              for (int e = 0; e < 8; e++) {
-                const int by = which ? ex[y] + rs.gexp : ew[e] - ewmax + ga;
-                const float t = ldexpf(g[e], by);
-                hi[e] = (float)(f16)t;
-                lo[e] = t - hi[e];
-              }
-              store_vec(reinterpret_cast<f16*>(a.g[2 * which] + o), hi);
-              store_vec(reinterpret_cast<f16*>(a.g[2 * which + 1] + o), lo);
-            }
+            const uint32_t chunk = (wc * S::WA + b) * 4 + 2 * p + h;
+            store_vec(reinterpret_cast<T*>(ring + row * S::TC * 2 + ((chunk ^ (row & (CH - 1))) << 4)), g);
           }
-        }
+      }
+      __syncthreads();
+      char* const out = a.g[plane] + (size_t)at.rt * S::TR * a.ldg + (size_t)at.ct * S::TC * 2;
+#pragma unroll 4
+      for (int t = threadIdx.x; t < S::TR * CH; t += S::THREADS) {
+        const uint32_t row = t / CH, chunk = t % CH;
+        const uint4 v = *reinterpret_cast<const uint4*>(ring + row * S::TC * 2 +
+                                                        ((chunk ^ (row & (CH - 1))) << 4));
+        *reinterpret_cast<uint4*>(out + row * a.ldg + chunk * 16) = v;
+      }
     }
   }
 }
