@@ -129,6 +129,183 @@ __device__ __forceinline__ float root(float v) {
   return small ? t * 2.3283064365386963e-10f : t;                                  // 2^-32
 }
 
+// One element's step; r: the root of the new v.
+__device__ __forceinline__ void step1(const AdamScalars& s, float keep, float& p, float g, float& m,
+                                      float& v, float& r) {
+  const float ge = g * s.gscale;
+  m = s.beta1 * m + s.new1 * ge;
+  v = s.beta2 * v + s.new2 * ge * ge;
+  // The root and the quotient within two units of the last place (the correctly
+  // rounded ones are twenty instructions each).
+  r = root(v);
+  p = p * keep - s.rate * (m * __builtin_amdgcn_rcpf(r * s.root2 + s.eps));
+}
+
+// Vectors in global memory (a pointer that comes from a table is otherwise taken to be
+// of any address space) at any element's address.
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t u32_any __attribute__((aligned(1)));
+#define EMH_GLOBAL __attribute__((address_space(1)))
+template <class V>
+__device__ __forceinline__ V gload(const void* p, size_t byte) {
+  return *(const EMH_GLOBAL V*)((const EMH_GLOBAL char*)p + byte);
+}
+template <class V>
+__device__ __forceinline__ void gstore(void* p, size_t byte, V v) {
+  *(EMH_GLOBAL V*)((EMH_GLOBAL char*)p + byte) = v;
+}
+__device__ __forceinline__ void unpack16(u32x2_any w, int kind, float* v) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const uint16_t b = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+    v[e] = kind == EMH_F16 ? (float)__builtin_bit_cast(f16, b) : __uint_as_float((uint32_t)b << 16);
+  }
+}
+template <class T>
+__device__ __forceinline__ u32x2_any pack16_of(const float* v) {
+  u32x2_any w;
+#pragma unroll
+  for (int e = 0; e < 2; e++)
+    w[e] = (uint32_t)__builtin_bit_cast(uint16_t, (T)v[2 * e]) |
+           (uint32_t)__builtin_bit_cast(uint16_t, (T)v[2 * e + 1]) << 16;
+  return w;
+}
+__device__ __forceinline__ u32x2_any pack16(const float* v, int kind) {
+  return kind == EMH_F16 ? pack16_of<f16>(v) : pack16_of<bf16>(v);
+}
+__device__ __forceinline__ void unpack32(u32x4_any w, float* v) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) v[e] = __uint_as_float(w[e]);
+}
+__device__ __forceinline__ u32x4_any pack32(const float* v) {
+  u32x4_any w;
+#pragma unroll
+  for (int e = 0; e < 4; e++) w[e] = __float_as_uint(v[e]);
+  return w;
+}
+
+// A whole chunk: every load goes out before the first is used.
+template <int U, bool P16, bool G16, bool EIGHT>
+__device__ __forceinline__ void whole_chunk(const AdamTensor& t, const AdamScalars& s, size_t base) {
+  const float keep = (float)(1.0 - s.lr * t.weight_decay);
+  const size_t i0 = base + threadIdx.x * 4;
+  u32x4_any p4[P16 ? 1 : U], g4[G16 ? 1 : U], m4[EIGHT ? 1 : U], v4[EIGHT ? 1 : U];
+  u32x2_any p2[P16 ? U : 1], g2[G16 ? U : 1];
+  uint32_t mc[U], vc[U];
+  float msc[U], vsc[U];
+#pragma unroll
+  for (int u = 0; u < U; u++) {
+    const size_t i = i0 + u * 1024;
+    if constexpr (P16)
+      p2[u] = gload<u32x2_any>(t.param, i * 2);
+    else
+      p4[u] = gload<u32x4_any>(t.param, i * 4);
+    if constexpr (G16)
+      g2[u] = gload<u32x2_any>(t.grad, i * 2);
+    else
+      g4[u] = gload<u32x4_any>(t.grad, i * 4);
+    if constexpr (EIGHT) {
+      mc[u] = gload<u32_any>(t.m, i);
+      vc[u] = gload<u32_any>(t.v, i);
+      const size_t block = i / EMH_ADAMW_BLOCK;  // (a wave's)
+      msc[u] = gload<float>(t.m_scale, block * 4);
+      vsc[u] = gload<float>(t.v_scale, block * 4);
+    } else {
+      m4[u] = gload<u32x4_any>(t.m, i * 4);
+      v4[u] = gload<u32x4_any>(t.v, i * 4);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; u++) {
+    const size_t i = i0 + u * 1024;
+    float p[4], g[4], m[4], v[4], r[4];
+    if constexpr (P16)
+      unpack16(p2[u], t.param_kind, p);
+    else
+      unpack32(p4[u], p);
+    if constexpr (G16)
+      unpack16(g2[u], t.grad_kind, g);
+    else
+      unpack32(g4[u], g);
+    if constexpr (EIGHT) {
+      decode4(mc[u], msc[u], m);
+      decode4(vc[u], vsc[u], v);
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[e] *= v[e];
+    } else {
+      unpack32(m4[u], m);
+      unpack32(v4[u], v);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) step1(s, keep, p[e], g[e], m[e], v[e], r[e]);
+    if constexpr (P16)
+      gstore(t.param, i * 2, pack16(p, t.param_kind));
+    else
+      gstore(t.param, i * 4, pack32(p));
+    if (t.copy) gstore(t.copy, i * 2, pack16(p, t.copy_kind));
+    if constexpr (EIGHT) {
+      float ms, vs;
+      const uint32_t a = encode4<false>(m, ms), b = encode4<true>(r, vs);
+      gstore<u32_any>(t.m, i, a);
+      gstore<u32_any>(t.v, i, b);
+      if ((threadIdx.x & 63) == 0) {
+        gstore(t.m_scale, i / EMH_ADAMW_BLOCK * 4, ms);
+        gstore(t.v_scale, i / EMH_ADAMW_BLOCK * 4, vs);
+      }
+    } else {
+      gstore(t.m, i * 4, pack32(m));
+      gstore(t.v, i * 4, pack32(v));
+    }
+  }
+}
+
+// A tensor's last chunk: fours that may be cut short.
+__device__ __forceinline__ void last_chunk(const AdamTensor& t, const AdamScalars& s, size_t base,
+                                           int count) {
+  const float keep = (float)(1.0 - s.lr * t.weight_decay);
+  for (int o = (int)threadIdx.x * 4; o < ((count + 255) & ~255); o += 1024) {
+    const int left = count - o;  // (whole waves come here together: a block's scale is theirs)
+    const size_t i = base + o;
+    float p[4], g[4], m[4], v[4], r[4];
+    load4_kind(t.param, t.param_kind, i, left, p);
+    load4_kind(t.grad, t.grad_kind, i, left, g);
+    if (t.m_scale) {
+      const size_t block = i / EMH_ADAMW_BLOCK;
+      decode4(load4_codes(t.m, i, left), t.m_scale[block], m);
+      decode4(load4_codes(t.v, i, left), t.v_scale[block], v);
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[e] *= v[e];
+    } else {
+      load4_kind(t.m, EMH_F32, i, left, m);
+      load4_kind(t.v, EMH_F32, i, left, v);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) step1(s, keep, p[e], g[e], m[e], v[e], r[e]);
+    store4_kind(t.param, t.param_kind, i, left, p);
+    if (t.copy) store4_kind(t.copy, t.copy_kind, i, left, p);
+    if (t.m_scale) {
+      // (Elements past the tensor's end are zeros here and have no part in the scale.)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        r[e] = e < left ? r[e] : 0.f;
+        m[e] = e < left ? m[e] : 0.f;
+      }
+      float ms, vs;
+      const uint32_t a = encode4<false>(m, ms), b = encode4<true>(r, vs);
+      store4_codes(t.m, i, left, a);
+      store4_codes(t.v, i, left, b);
+      if ((threadIdx.x & 63) == 0) {
+        t.m_scale[i / EMH_ADAMW_BLOCK] = ms;
+        t.v_scale[i / EMH_ADAMW_BLOCK] = vs;
+      }
+    } else {
+      store4_kind(t.m, EMH_F32, i, left, m);
+      store4_kind(t.v, EMH_F32, i, left, v);
+    }
+  }
+}
+
 template <int U>  // a chunk: 1024 U elements
 __global__ __launch_bounds__(256) void k_adamw(const AdamTensor* __restrict__ tensors,
                                                const uint2* __restrict__ chunks,
@@ -137,74 +314,21 @@ __global__ __launch_bounds__(256) void k_adamw(const AdamTensor* __restrict__ te
   const AdamTensor t = tensors[at.x];
   const size_t base = (size_t)at.y * (1024 * U);
   const size_t here = t.len - base;  // > 0
-  const int lane4 = (int)threadIdx.x * 4;
-  const bool eight = t.m_scale != nullptr;
-  const float keep = (float)(1.0 - s.lr * t.weight_decay);
-  float p[U][4], g[U][4], m[U][4], v[U][4];
-  uint32_t mc[U], vc[U];
-  float msc[U], vsc[U];
-#pragma unroll
-  for (int u = 0; u < U; u++) {
-    const int o = u * 1024 + lane4;
-    const int left = (int)min((size_t)(1024 * U), here) - o;
-    const size_t i = base + o;
-    load4_kind(t.param, t.param_kind, i, left, p[u]);
-    load4_kind(t.grad, t.grad_kind, i, left, g[u]);
-    if (eight) {
-      mc[u] = load4_codes(t.m, i, left);
-      vc[u] = load4_codes(t.v, i, left);
-      msc[u] = left > 0 ? t.m_scale[i / EMH_ADAMW_BLOCK] : 0.f;
-      vsc[u] = left > 0 ? t.v_scale[i / EMH_ADAMW_BLOCK] : 0.f;
-    } else {
-      load4_kind(t.m, EMH_F32, i, left, m[u]);
-      load4_kind(t.v, EMH_F32, i, left, v[u]);
-    }
+  if (here < (size_t)(1024 * U)) {
+    last_chunk(t, s, base, (int)here);
+    return;
   }
-#pragma unroll
-  for (int u = 0; u < U; u++) {
-    const int o = u * 1024 + lane4;
-    const int left = (int)min((size_t)(1024 * U), here) - o;
-    const size_t i = base + o;
-    if (eight) {
-      decode4(mc[u], msc[u], m[u]);
-      decode4(vc[u], vsc[u], v[u]);
-#pragma unroll
-      for (int e = 0; e < 4; e++) v[u][e] *= v[u][e];
-    }
-    float r[4];
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const float ge = g[u][e] * s.gscale;
-      m[u][e] = s.beta1 * m[u][e] + s.new1 * ge;
-      v[u][e] = s.beta2 * v[u][e] + s.new2 * ge * ge;
-      // The root and the quotient within two units of the last place (the correctly
-      // rounded ones are twenty instructions each, which bounded the step: 595 us at
-      // 134 million elements).
-      r[e] = root(v[u][e]);
-      const float by = m[u][e] * __builtin_amdgcn_rcpf(r[e] * s.root2 + s.eps);
-      p[u][e] = p[u][e] * keep - s.rate * by;
-    }
-    store4_kind(t.param, t.param_kind, i, left, p[u]);
-    if (t.copy) store4_kind(t.copy, t.copy_kind, i, left, p[u]);
-    if (eight) {
-      // (Elements past the tensor's end are zeros here and have no part in the scale.)
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        r[e] = e < left ? r[e] : 0.f;
-        m[u][e] = e < left ? m[u][e] : 0.f;
-      }
-      float ms, vs;
-      const uint32_t a = encode4<false>(m[u], ms), b = encode4<true>(r, vs);
-      store4_codes(t.m, i, left, a);
-      store4_codes(t.v, i, left, b);
-      if ((threadIdx.x & 63) == 0 && left > 0) {
-        t.m_scale[i / EMH_ADAMW_BLOCK] = ms;
-        t.v_scale[i / EMH_ADAMW_BLOCK] = vs;
-      }
-    } else {
-      store4_kind(t.m, EMH_F32, i, left, m[u]);
-      store4_kind(t.v, EMH_F32, i, left, v[u]);
-    }
+  const bool p16 = t.param_kind != EMH_F32, g16 = t.grad_kind != EMH_F32;
+  if (t.m_scale) {
+    if (p16)
+      g16 ? whole_chunk<U, true, true, true>(t, s, base) : whole_chunk<U, true, false, true>(t, s, base);
+    else
+      g16 ? whole_chunk<U, false, true, true>(t, s, base) : whole_chunk<U, false, false, true>(t, s, base);
+  } else {
+    if (p16)
+      g16 ? whole_chunk<U, true, true, false>(t, s, base) : whole_chunk<U, true, false, false>(t, s, base);
+    else
+      g16 ? whole_chunk<U, false, true, false>(t, s, base) : whole_chunk<U, false, false, false>(t, s, base);
   }
 }
 

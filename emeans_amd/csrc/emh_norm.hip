@@ -58,25 +58,22 @@ __device__ __forceinline__ float row_sum(float v, float (*red)[TB / 64], int slo
   return v;
 }
 
-template <class T>
-__device__ __forceinline__ Vec<T> load_cols(const T* row, int col, int d) {
-  constexpr int N = VecOf<T>::N;
-  if (col + N <= d) return load_vec(row + col);
-  return load_some(row + min(col, d), d - col);
-}
-template <class T>
-__device__ __forceinline__ void store_cols(T* row, int col, int d, const float* v) {
-  constexpr int N = VecOf<T>::N;
-  if (col + N <= d)
-    store_vec(row + col, v);
-  else
-    store_some(row + min(col, d), v, d - col);
-}
+// A thread's vectors begin at columns `col`, d >= N. Where one would pass the row's end
+// it is the row's last N columns instead (at): those before col are another thread's
+// too, and count there (in); both store the same value. One load and one store a
+// vector, whatever d is. (Element by element the last vector of 300 f16 took half of
+// the forward pass.)
+template <int N>
+struct Cols {
+  int at, from;  // in(e): at + e >= from
+  __device__ __forceinline__ Cols(int col, int d) : at(min(col, d - N)), from(col) {}
+  __device__ __forceinline__ bool in(int e) const { return at + e >= from; }
+  __device__ __forceinline__ bool any() const { return at + N > from; }
+};
 
-// A vector's columns of a norm's weight or bias (T or f32), `fill` without one.
+// A vector of a norm's weight or bias (T or f32), `fill` without one.
 template <class T>
-__device__ __forceinline__ void load_affine(const void* p, int kind, int col, int d, float fill,
-                                            float* out) {
+__device__ __forceinline__ void load_affine(const void* p, int kind, int at, float fill, float* out) {
   constexpr int N = VecOf<T>::N;
   if (!p) {
 #pragma unroll
@@ -84,53 +81,63 @@ __device__ __forceinline__ void load_affine(const void* p, int kind, int col, in
   } else if (kind == EMH_F32) {
 #pragma unroll
     for (int q = 0; q < N; q += 4) {
-      const Vec<float> v = load_cols(reinterpret_cast<const float*>(p), col + q, d);
+      const Vec<float> v = load_vec(reinterpret_cast<const float*>(p) + at + q);
 #pragma unroll
       for (int e = 0; e < 4; e++) out[q + e] = v.get(e);
     }
   } else {
-    const Vec<T> v = load_cols(reinterpret_cast<const T*>(p), col, d);
+    const Vec<T> v = load_vec(reinterpret_cast<const T*>(p) + at);
 #pragma unroll
     for (int e = 0; e < N; e++) out[e] = v.get(e);
   }
 }
 
-// Forward: LPR threads a row, NV vectors of 16 bytes a thread.
+// Forward: LPR threads a row, NV vectors of 16 bytes a thread. The next row is on
+// its way while a row's sums are formed.
 template <class T, int LPR, int NV>
 __global__ __launch_bounds__(256) void k_norm(const NormArgs a) {
   constexpr int N = VecOf<T>::N, TB = 256, G = TB / LPR;
   __shared__ float red[4][TB / 64];
   const int l = threadIdx.x % LPR, g = threadIdx.x / LPR;
   const int d = a.d;
+  auto cols = [&](int j) __attribute__((always_inline)) { return Cols<N>((l + LPR * j) * N, d); };
+  Vec<T> next[NV];
+  auto fetch = [&](size_t row) __attribute__((always_inline)) {
+    const T* x = reinterpret_cast<const T*>(a.x) + (row < a.rows ? row : 0) * a.ldx;
+#pragma unroll
+    for (int j = 0; j < NV; j++) next[j] = load_vec(x + cols(j).at);
+  };
+  fetch((size_t)blockIdx.x * G + g);
   float w[NV * N], b[NV * N];
 #pragma unroll
   for (int j = 0; j < NV; j++) {
-    load_affine<T>(a.w, a.wkind, (l + LPR * j) * N, d, 1.f, w + j * N);
-    load_affine<T>(a.b, a.bkind, (l + LPR * j) * N, d, 0.f, b + j * N);
+    load_affine<T>(a.w, a.wkind, cols(j).at, 1.f, w + j * N);
+    load_affine<T>(a.b, a.bkind, cols(j).at, 0.f, b + j * N);
   }
   const float inv = 1.0f / (float)d;
   int slot = 0;
+  const size_t step = (size_t)gridDim.x * G;
   // (The bound is the workgroup's: all its threads meet at row_sum's barriers.)
-  for (size_t r0 = (size_t)blockIdx.x * G; r0 < a.rows; r0 += (size_t)gridDim.x * G) {
+  for (size_t r0 = (size_t)blockIdx.x * G; r0 < a.rows; r0 += step) {
     const size_t row = r0 + g;
     const bool live = row < a.rows;
-    const T* x = reinterpret_cast<const T*>(a.x) + (live ? row : 0) * a.ldx;
     Vec<T> v[NV];
 #pragma unroll
-    for (int j = 0; j < NV; j++) v[j] = load_cols(x, (l + LPR * j) * N, d);
+    for (int j = 0; j < NV; j++) v[j] = next[j];
+    if (r0 + step < a.rows) fetch(r0 + step + g);
     float s = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; j++)
 #pragma unroll
-      for (int e = 0; e < N; e++) s += v[j].get(e);  // zeros past d
+      for (int e = 0; e < N; e++) s += cols(j).in(e) ? v[j].get(e) : 0.f;
     const float mean = row_sum<LPR, TB>(s, red, slot) * inv;
     float q = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; j++)
 #pragma unroll
       for (int e = 0; e < N; e++) {
-        const float o = v[j].get(e) - mean;
-        q = fmaf(o, (l + LPR * j) * N + e < d ? o : 0.f, q);
+        const float o = cols(j).in(e) ? v[j].get(e) - mean : 0.f;
+        q = fmaf(o, o, q);
       }
     const float rstd = 1.0f / sqrtf(row_sum<LPR, TB>(q, red, slot ^ 1) * inv + a.eps);
     slot ^= 2;
@@ -142,74 +149,96 @@ __global__ __launch_bounds__(256) void k_norm(const NormArgs a) {
 #pragma unroll
       for (int e = 0; e < N; e++)
         o[e] = fmaf((v[j].get(e) - mean) * rstd, w[j * N + e], b[j * N + e]);
-      store_cols(y, (l + LPR * j) * N, d, o);
+      if (cols(j).any()) store_vec(y + cols(j).at, o);
     }
     if (l == 0 && a.mean) a.mean[row] = mean;
     if (l == 0 && a.rstd) a.rstd[row] = rstd;
   }
 }
 
-// Backward, TB threads. (The row's elements stay packed and are unpacked again for
-// the result: what that takes is fewer registers, so twice the waves, whose rows are
-// in flight together.)
+// Backward, TB threads. The row's elements stay packed and are unpacked again for
+// the result: what that takes is fewer registers, so more waves, whose rows are in
+// flight together. AHEAD: the next row is on its way, too, where there are registers.
 template <class T, int LPR, int NV, int TB>
-__global__ __launch_bounds__(TB, NV * VecOf<T>::N <= 16 ? 4 : 2) void k_norm_grad(const NormArgs a) {
+__global__ __launch_bounds__(TB, TB / 256) void k_norm_grad(const NormArgs a) {
   constexpr int N = VecOf<T>::N, G = TB / LPR;
+  constexpr bool AHEAD = NV * N <= 12;
   __shared__ float red[4][TB / 64];
   __shared__ float fold[TB * NV * N];
   const int l = threadIdx.x % LPR, g = threadIdx.x / LPR;
   const int d = a.d;
+  auto cols = [&](int j) __attribute__((always_inline)) { return Cols<N>((l + LPR * j) * N, d); };
   float w[NV * N], aw[NV * N], ab[NV * N];
 #pragma unroll
   for (int j = 0; j < NV; j++) {
-    load_affine<T>(a.w, a.wkind, (l + LPR * j) * N, d, 1.f, w + j * N);
+    load_affine<T>(a.w, a.wkind, cols(j).at, 1.f, w + j * N);
 #pragma unroll
     for (int e = 0; e < N; e++) aw[j * N + e] = ab[j * N + e] = 0.f;
   }
   const float inv = 1.0f / (float)d;
   const size_t step = (size_t)gridDim.x * G;
   int slot = 0;
-  for (size_t r0 = (size_t)blockIdx.x * G; r0 < a.rows; r0 += step) {
-    const size_t row = r0 + g;
-    const bool live = row < a.rows;
-    const size_t r = live ? row : 0;
+  struct Row {
+    Vec<T> x[NV], dy[NV];
+    float mean, rstd;
+  };
+  auto fetch = [&](size_t row, Row& o) __attribute__((always_inline)) {
+    const size_t r = row < a.rows ? row : 0;
     const T* xp = reinterpret_cast<const T*>(a.x) + r * a.ldx;
     const T* dp = reinterpret_cast<const T*>(a.dy) + r * a.lddy;
-    const int have = live ? d : 0;
-    Vec<T> x[NV], dy[NV];
 #pragma unroll
     for (int j = 0; j < NV; j++) {
-      x[j] = load_cols(xp, (l + LPR * j) * N, have);
-      dy[j] = load_cols(dp, (l + LPR * j) * N, have);
+      o.x[j] = load_vec(xp + cols(j).at);
+      o.dy[j] = load_vec(dp + cols(j).at);
     }
-    const float mean = a.mean[r], rstd = a.rstd[r];
+    o.mean = a.mean[r];
+    o.rstd = a.rstd[r];
+  };
+  auto one = [&](const Row& o, size_t row) __attribute__((always_inline)) {
+    const bool live = row < a.rows;
     float c1 = 0.f, c2 = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; j++)
 #pragma unroll
       for (int e = 0; e < N; e++) {
-        // Past the row (and in no row) dy is zero, and x is made the mean.
         const int i = j * N + e;
-        const float h = (l + LPR * j) * N + e < have ? (x[j].get(e) - mean) * rstd : 0.f;
-        const float t = dy[j].get(e);
+        const float h = live ? (o.x[j].get(e) - o.mean) * o.rstd : 0.f;
+        const float t = live ? o.dy[j].get(e) : 0.f;
         ab[i] += t;
         aw[i] = fmaf(t, h, aw[i]);
-        c1 = fmaf(t, w[i], c1);
-        c2 = fmaf(t * w[i], h, c2);
+        const float u = cols(j).in(e) ? t * w[i] : 0.f;
+        c1 += u;
+        c2 = fmaf(u, cols(j).in(e) ? h : 0.f, c2);
       }
     c1 = row_sum<LPR, TB>(c1, red, slot) * inv;
     c2 = row_sum<LPR, TB>(c2, red, slot ^ 1) * inv;
     slot ^= 2;
     if (live && a.y) {
-      T* o = reinterpret_cast<T*>(a.y) + row * a.ldy;
+      T* y = reinterpret_cast<T*>(a.y) + row * a.ldy;
 #pragma unroll
       for (int j = 0; j < NV; j++) {
         float t[N];
 #pragma unroll
         for (int e = 0; e < N; e++)
-          t[e] = rstd * (dy[j].get(e) * w[j * N + e] - c1 - (x[j].get(e) - mean) * rstd * c2);
-        store_cols(o, (l + LPR * j) * N, d, t);
+          t[e] = o.rstd * (o.dy[j].get(e) * w[j * N + e] - c1 - (o.x[j].get(e) - o.mean) * o.rstd * c2);
+        if (cols(j).any()) store_vec(y + cols(j).at, t);
       }
+    }
+  };
+  size_t r0 = (size_t)blockIdx.x * G;
+  if constexpr (AHEAD) {
+    Row next;
+    fetch(r0 + g, next);
+    for (; r0 < a.rows; r0 += step) {
+      const Row now = next;
+      if (r0 + step < a.rows) fetch(r0 + step + g, next);
+      one(now, r0 + g);
+    }
+  } else {
+    for (; r0 < a.rows; r0 += step) {
+      Row now;
+      fetch(r0 + g, now);
+      one(now, r0 + g);
     }
   }
   if (!a.part) return;
@@ -225,8 +254,10 @@ __global__ __launch_bounds__(TB, NV * VecOf<T>::N <= 16 ? 4 : 2) void k_norm_gra
 #pragma unroll
     for (int i0 = 0; i0 < NV * N; i0 += G) {
       const int i = i0 + g;
-      const int col = (l + LPR * (i / N)) * N + i % N;
-      if (i >= NV * N || col >= d) continue;
+      if (i >= NV * N) continue;
+      const Cols<N> c = cols(i / N);
+      const int col = c.at + i % N;
+      if (!c.in(i % N)) continue;
       float s = 0.f;
 #pragma unroll 8
       for (int k = 0; k < G; k++) s += fold[i * TB + k * LPR + l];
@@ -235,7 +266,8 @@ __global__ __launch_bounds__(TB, NV * VecOf<T>::N <= 16 ? 4 : 2) void k_norm_gra
   }
 }
 
-// Rows too long for the registers of a workgroup: one workgroup a row, read
+// Rows too long for the registers of a workgroup (or shorter than a vector): one
+// workgroup a row, read
 // again for every step (from L2, mostly).
 template <class T>
 __global__ __launch_bounds__(256) void k_norm_wide(const NormArgs a) {
@@ -298,25 +330,25 @@ __global__ __launch_bounds__(256) void k_norm_cols(const NormArgs a) {
   a.part[((size_t)blockIdx.y * 2 + 1) * a.d + col] = sb;
 }
 
-// out = the nparts rows of sums added: 64 columns a workgroup, 16 shares of the
+// out = the nparts rows of sums added: 16 columns a workgroup, 64 shares of the
 // rows in step and then one after another.
 __global__ __launch_bounds__(1024) void k_norm_sums(const float* __restrict__ part, int nparts,
                                                     int d, void* dw, int dwkind, void* db,
                                                     int dbkind) {
-  __shared__ float s[16][64];
-  const int c = threadIdx.x & 63, g = threadIdx.x >> 6;
-  const int col = blockIdx.x * 64 + c;
+  __shared__ float s[64][17];
+  const int c = threadIdx.x & 15, g = threadIdx.x >> 4;
+  const int col = blockIdx.x * 16 + c;
   float v = 0.f;
   if (col < 2 * d) {
 #pragma unroll 8
-    for (int i = g; i < nparts; i += 16) v += part[(size_t)i * 2 * d + col];
+    for (int i = g; i < nparts; i += 64) v += part[(size_t)i * 2 * d + col];
   }
   s[g][c] = v;
   __syncthreads();
   if (g != 0 || col >= 2 * d) return;
   v = 0.f;
 #pragma unroll
-  for (int i = 0; i < 16; i++) v += s[i][c];
+  for (int i = 0; i < 64; i++) v += s[i][c];
   if (col < d) {
     if (dw) store_kind(dw, dwkind, col, v);
   } else if (db) {
@@ -345,12 +377,15 @@ template <int L, int V>
 struct Shape {
   static constexpr int LPR = L, NV = V;
 };
-// The threads that share a row and the vectors each holds: the fewest that hold
-// the row. False: none does.
+// The threads that share a row and the vectors each holds: the fewest vectors
+// that hold the row. False: none does. (Rows of 300 f16 on 16 or 32 lanes with
+// fewer idle ones took 8.7 us forward and 15.5 back; on 64, 8.0 and 12.6.)
 template <class T, class F>
 bool by_shape(size_t d, F&& f) {
   const size_t v = (d + VecOf<T>::N - 1) / VecOf<T>::N;
-  if (v <= 16)
+  if (d < (size_t)VecOf<T>::N)
+    return false;
+  else if (v <= 16)
     f(Shape<16, 1>{});
   else if (v <= 64)
     f(Shape<64, 1>{});
@@ -411,11 +446,11 @@ void launch_layer_norm_grad(emh_ctx* c, const MatIn& dy, const MatIn& x, size_t 
     using T = decltype(t);
     const bool held = by_shape<T>(d, [&](auto s) {
       using S = decltype(s);
-      // As many waves a CU as the registers allow (two workgroups of at most 16
-      // columns a thread, else one): few rows of sums to write and add.
-      constexpr int TB = 512;
+      // A workgroup a CU, of as many waves as the registers allow: few rows of
+      // sums to write and add.
+      constexpr int TB = S::NV * VecOf<T>::N < 16 ? 1024 : S::NV * VecOf<T>::N == 16 ? 768 : 512;
       constexpr size_t G = TB / S::LPR;
-      parts = std::min((rows + G - 1) / G, (size_t)c->cus * (S::NV * VecOf<T>::N <= 16 ? 2 : 1));
+      parts = std::min((rows + G - 1) / G, (size_t)c->cus);
       if (sums) a.part = (float*)c->norm_part.get(parts * 2 * d * 4);
       k_norm_grad<T, S::LPR, S::NV, TB><<<dim3((unsigned)parts), TB, 0, c->stream>>>(a);
     });
@@ -428,7 +463,7 @@ void launch_layer_norm_grad(emh_ctx* c, const MatIn& dy, const MatIn& x, size_t 
     if (dx.p) k_norm_grad_wide<T><<<dim3((unsigned)rows), 256, 0, c->stream>>>(a);
   });
   if (sums)
-    k_norm_sums<<<grid1(2 * d, 64), 1024, 0, c->stream>>>(a.part, (int)parts, (int)d, dweight.p,
+    k_norm_sums<<<grid1(2 * d, 16), 1024, 0, c->stream>>>(a.part, (int)parts, (int)d, dweight.p,
                                                           dweight.kind, dbias.p, dbias.kind);
   EMH_HIP(hipGetLastError());
 }

@@ -13,7 +13,8 @@
 // In LDS the 16-byte chunks of a row are XOR-swizzled so that neither kind of
 // read meets a bank twice: a DEEP row r's chunks by (r / 2) % 8 (two rows fill the
 // 64 banks: sixteen rows' equal chunks are sixteen different ones), a WIDE row's
-// by 4 (r % 4) (a transposing read takes 64 bytes of each of four rows).
+// by 4 (r % 4) (a transposing read takes 64 bytes of each of four rows; rows of
+// 384 bytes lie half the banks apart already: by 4 (r / 2 % 2)).
 //
 // The columns are the MFMA's A and the rows its B, so that a lane holds one
 // row of each 32 x 32 block and four consecutive columns at a time.
@@ -43,6 +44,8 @@ __device__ __forceinline__ v16f mfma16(bf16, v8s a, v8s b, v16f c) {
                                                  __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
 }
 
+}  // namespace
+
 constexpr int SLAB = 64;  // depth of a slab
 
 // A workgroup's shape: waves of NWR x NWC, each WB x WA blocks of 32 x 32.
@@ -52,11 +55,27 @@ struct TileShape {
   static constexpr int NW = NWR * NWC, THREADS = 64 * NW;
   static constexpr int TR = NWR * WB * 32, TC = NWC * WA * 32;
   static constexpr int RBYTES = TR * SLAB * 2, CBYTES = TC * SLAB * 2;
-  static constexpr int STAGE = RBYTES + CBYTES;
+  // (A power of two: the stages are toggled by XOR.)
+  static constexpr int STAGE = RBYTES + CBYTES <= 32768 ? 32768 : 65536;
+  static constexpr int RING = STAGE + RBYTES + CBYTES;
   static constexpr int RD = RBYTES / (1024 * NW), CD = CBYTES / (1024 * NW);  // DMAs a wave
 };
 typedef TileShape<4, 2, 2, 4> TileL;  // 256 x 256, 8 waves
-typedef TileShape<2, 2, 2, 2> TileS;  // 128 x 128, 4 waves
+typedef TileShape<4, 2, 2, 3> TileM;  // 256 x 192, 8 waves
+typedef TileShape<2, 2, 2, 2> TileS;  // 128 x 128, 4 waves (two workgroups a CU)
+enum Tile : int { TILE_L, TILE_M, TILE_S, TILES };
+constexpr uint32_t TILE_ROWS[TILES] = {TileL::TR, TileM::TR, TileS::TR};
+constexpr uint32_t TILE_COLS[TILES] = {TileL::TC, TileM::TC, TileS::TC};
+// Runs f with the shape as a type.
+template <class F>
+void by_tile(Tile t, F&& f) {
+  if (t == TILE_L)
+    f(TileL{});
+  else if (t == TILE_M)
+    f(TileM{});
+  else
+    f(TileS{});
+}
 
 // One operand. f32 matrices come as two planes of fp16 (emh_xent.h).
 struct Operand {
@@ -73,6 +92,8 @@ struct TileIn {
   uint32_t passes;  // 1, or 3: planes (0, 0), (0, 1), (1, 0)
   uint32_t rtiles, ctiles, splits;  // workgroups: rtiles ctiles splits
 };
+
+namespace {
 
 // Which tile, and which steps (pass, slab) of it, a workgroup takes.
 struct TileAt {
@@ -108,7 +129,10 @@ __device__ __forceinline__ uint32_t deep_swz(uint32_t row) { return (row >> 1) &
 template <bool DEEP, int T, int ND, int NW>
 struct Side16 {
   static constexpr uint32_t RB = 2 * T;         // WIDE: bytes of a row in LDS
-  static constexpr uint32_t LPR = RB / 16;      // ... lanes of a DMA that share it
+  static constexpr uint32_t LPR = RB / 16;      // ... its chunks
+  static __device__ __forceinline__ uint32_t wide_swz(uint32_t krow) {
+    return RB % 256 == 0 ? (krow & 3) << 2 : ((krow >> 1) & 1) << 2;
+  }
   uint32_t off[ND];                             // DEEP: row and chunk; WIDE: chunk
   uint32_t krow[ND];                            // WIDE: row in the slab
   uint32_t at[DEEP ? 1 : 4];                    // LDS reads (WIDE: by block)
@@ -124,8 +148,8 @@ struct Side16 {
         const uint32_t r = min(t0 + row, o.rows - 1) - t0;
         off[j] = r * o.ld + (((lane & 7) ^ deep_swz(row)) << 4);
       } else {
-        krow[j] = d * (64 / LPR) + lane / LPR;
-        const uint32_t chunk = (lane % LPR) ^ ((krow[j] & 3) << 2);
+        krow[j] = (d * 64 + lane) / LPR;
+        const uint32_t chunk = ((d * 64 + lane) % LPR) ^ wide_swz(krow[j]);
         const uint32_t col = t0 + chunk * 8;
         off[j] = (col < o.wide ? col : 0u) * 2;
       }
@@ -142,7 +166,7 @@ struct Side16 {
 #pragma unroll
       for (int a = 0; a < 4; a++) {
         const uint32_t chunk = (uint32_t)(b0 + a) * 4 + (g & 1) * 2 + ((l & 3) >> 1);
-        at[a] = lds + (8 * (g >> 1) + (l >> 2)) * RB + (((chunk ^ ((l >> 2) << 2))) << 4) + (l & 1) * 8;
+        at[a] = lds + (8 * (g >> 1) + (l >> 2)) * RB + ((chunk ^ wide_swz(l >> 2)) << 4) + (l & 1) * 8;
       }
     }
   }
@@ -213,8 +237,6 @@ __device__ __forceinline__ void tile_sums(const TileIn& t, const TileAt& at, cha
       }
     }
   };
-  static_assert((S::STAGE & (S::STAGE - 1)) == 0, "stages are toggled by XOR");
-
 #pragma unroll
   for (int a = 0; a < S::WA; a++)
 #pragma unroll

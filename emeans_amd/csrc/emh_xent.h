@@ -70,8 +70,7 @@ struct LogitArgs {
   char* g[4];       // G; f32: Ga's planes, Gb's planes
   size_t ldg;       // bytes (rows and columns to full tiles)
 };
-// Bits of what a call is: which instantiation runs.
-void launch_logits(hipStream_t s, const LogitArgs& a, int kind, bool large, bool grads);
+void launch_logits(hipStream_t s, const LogitArgs& a, int kind, Tile tile, bool grads);
 
 struct ProdArgs {
   TileIn t;
@@ -91,7 +90,7 @@ struct ProdArgs {
   uint32_t call;
   Operand alt;
 };
-void launch_prod(hipStream_t s, const ProdArgs& a, int kind, bool large);
+void launch_prod(hipStream_t s, const ProdArgs& a, int kind, Tile tile);
 
 // A row's weight in G, the powers of two of G (see above) and the factor left for the
 // results: all from the call's state.

@@ -245,6 +245,8 @@ __global__ __launch_bounds__(256) void k_join_few(const float2* __restrict__ par
                                                   uint32_t* small) {
   __shared__ float2 sh[4];
   const uint32_t i = blockIdx.x;
+  const uint32_t lab = labels[i];
+  const float zl = zlabel[i];
   float m = -INFINITY, s = 0.f;
   auto join = [&](float2 p) __attribute__((always_inline)) {
     const float b = fmaxf(m, p.x), bb = b == -INFINITY ? 0.f : b;
@@ -260,9 +262,8 @@ __global__ __launch_bounds__(256) void k_join_few(const float2* __restrict__ par
   m = sh[0].x, s = sh[0].y;
   for (int t = 1; t < 4; t++) join(sh[t]);
   const float l2 = (m == -INFINITY ? 0.f : m) + log2f(s);
-  const uint32_t lab = labels[i];
   if (lse) lse[i] = l2 * LN2;
-  loss[i] = lab < k ? (l2 - zlabel[i]) * LN2 : 0.f;
+  loss[i] = lab < k ? (l2 - zl) * LN2 : 0.f;
   if (lab >= k && lab != NO_LABEL) small[SW_BAD_CLASS] = 1u;
 }
 
@@ -405,6 +406,8 @@ void few(emh_ctx* c, const XentIn& in, float* loss, float* lse) {
     run(k_few<T, 2>);
   else
     run(k_few<T, 4>);
+  // (A launch of its own: the fence and the ticket that let the last workgroup join
+  // the parts cost 70 us with 1,024 workgroups, 6 with 16.)
   k_join_few<<<dim3(n), 256, 0, c->stream>>>(part, blocks, in.labels, k, zlabel, loss, lse, c->small);
   EMH_HIP(hipGetLastError());
 }
@@ -413,26 +416,26 @@ void few(emh_ctx* c, const XentIn& in, float* loss, float* lse) {
 // fewest rounds of workgroups times a workgroup's time, with the cost of
 // writing and adding the splits' sums.
 struct Plan {
-  bool large = true;
+  Tile tile = TILE_L;
   uint32_t rtiles = 1, ctiles = 1, splits = 1;
 };
 Plan plan_of(size_t rows, size_t cols, size_t steps, int cus, bool may_split) {
+  // us a slab on a full card (256 x 256: 1.18 PFLOP/s), workgroups a CU.
+  constexpr double STEP[TILES] = {1.8, 1.4, 1.2};
+  constexpr int PER_CU[TILES] = {1, 1, 2};
   Plan best;
   double least = 1e300;
-  for (int large = 1; large >= 0; large--) {
-    const size_t t = large ? TileL::TR : TileS::TR;
-    const size_t rt = (rows + t - 1) / t, ct = (cols + t - 1) / t;
-    const double at_once = large ? cus : 2.0 * cus;   // workgroups
-    const double step = large ? 1.8 : 1.2;            // us a slab, when the card is full
+  for (int tile = 0; tile < TILES; tile++) {
+    const size_t rt = (rows + TILE_ROWS[tile] - 1) / TILE_ROWS[tile];
+    const size_t ct = (cols + TILE_COLS[tile] - 1) / TILE_COLS[tile];
     for (size_t s = 1; s <= (may_split ? 32 : 1); s++) {
       if (s > 1 && steps < 4 * s) break;
-      const double rounds = std::ceil((double)(rt * ct * s) / at_once);
-      double us = rounds * ((double)((steps + s - 1) / s) * step + 4.0);
-      if (s > 1) us += 3.0 + 1.8e-6 * (double)s * (double)rows * (double)cols;
+      const double rounds = std::ceil((double)(rt * ct * s) / ((double)cus * PER_CU[tile]));
+      double us = rounds * ((double)((steps + s - 1) / s) * STEP[tile] + 4.0);
+      if (s > 1) us += 3.0 + 1.2e-6 * (double)s * (double)rows * (double)cols;
       if (us < least) {
         least = us;
-        best.large = large != 0;
-        best.rtiles = (uint32_t)rt, best.ctiles = (uint32_t)ct, best.splits = (uint32_t)s;
+        best = {(Tile)tile, (uint32_t)rt, (uint32_t)ct, (uint32_t)s};
       }
     }
   }
@@ -496,7 +499,7 @@ void launch_cross_entropy(emh_ctx* c, const XentIn& in, float* loss, float* lse)
     a.ex = f32 ? lx.ex + r0 : nullptr;
     a.ew = lw.ex;
     a.part = part, a.zlabel = zlabel;
-    launch_logits(c->stream, a, in.x.kind, p.large, false);
+    launch_logits(c->stream, a, in.x.kind, p.tile, false);
     k_join<<<grid1(m, 64), 1024, 0, c->stream>>>(part, p.ctiles * 2, (uint32_t)m, in.labels + r0,
                                                  (uint32_t)k, zlabel, loss + r0,
                                                  lse ? lse + r0 : nullptr, c->small);
@@ -574,7 +577,7 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
       a.odd = {c->small + SW_ODD_ROW, call, lx.p[0], lx.dp, (const char*)in.x.p, in.x.ld, d};
     for (int i = 0; i < 4; i++) a.g[i] = G[i];
     a.ldg = ldg;
-    launch_logits(c->stream, a, in.x.kind, pg.large, true);
+    launch_logits(c->stream, a, in.x.kind, pg.tile, true);
     ProdArgs p{};
     p.labels = in.labels, p.k = (uint32_t)k;
     p.gloss = gloss, p.st = st, p.scale = in.scale;
@@ -590,14 +593,14 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
       p.out = dx.p, p.ldo = dx.ld;
       p.part = px_part ? partx : nullptr;
       p.add = v0 > 0;
-      launch_prod(c->stream, p, in.x.kind, px.large);
+      launch_prod(c->stream, p, in.x.kind, px.tile);
     }
     if (dw.p) {
       p.t.r = {{f32 ? G[2] : G[0], G[3]}, (uint32_t)ldg, up(n, SLAB), (uint32_t)piece};
       p.t.c = xl.deep(in.x, 0, n);
       p.t.c.wide = xl.packed ? xl.dp : (uint32_t)d;
       p.t.slabs = (uint32_t)((n + SLAB - 1) / SLAB);
-      p.t.rtiles = (uint32_t)((m + (pw.large ? TileL::TR : TileS::TR) - 1) / (pw.large ? TileL::TR : TileS::TR));
+      p.t.rtiles = ((uint32_t)m + TILE_ROWS[pw.tile] - 1) / TILE_ROWS[pw.tile];
       p.t.ctiles = pw.ctiles, p.t.splits = pw.splits;
       p.rows = (uint32_t)m, p.dw = true;
       p.out = (char*)dw.p + v0 * dw.ld * kind_bytes(dw.kind), p.ldo = dw.ld;
@@ -608,7 +611,7 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
         p.call = call;
         p.alt = lx.deep(in.x, 0, n);
       }
-      launch_prod(c->stream, p, in.x.kind, pw.large);
+      launch_prod(c->stream, p, in.x.kind, pw.tile);
       if (pw_part) join_splits(c, partw, pw.splits, m, d, ldp, p.out, dw.ld, dw.kind);
     }
   }

@@ -6,7 +6,7 @@ namespace {
 
 template <class T, class S, bool F32, bool DW, class O>
 __global__ __launch_bounds__(S::THREADS, 2) void k_grads(const ProdArgs a) {
-  __shared__ __attribute__((aligned(1024))) char ring[2 * S::STAGE];
+  __shared__ __attribute__((aligned(1024))) char ring[S::RING];
   const TileAt at = tile_at(a.t);
   v16f acc[S::WA][S::WB];
   TileIn t = a.t;
@@ -74,25 +74,26 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_grads(const ProdArgs a) {
 }
 
 template <class T, bool F32, class O>
-void launch(hipStream_t s, const ProdArgs& a, bool large) {
-  const unsigned blocks = a.t.rtiles * a.t.ctiles * a.t.splits;
-  if (large)
-    a.dw ? k_grads<T, TileL, F32, true, O><<<blocks, TileL::THREADS, 0, s>>>(a)
-         : k_grads<T, TileL, F32, false, O><<<blocks, TileL::THREADS, 0, s>>>(a);
-  else
-    a.dw ? k_grads<T, TileS, F32, true, O><<<blocks, TileS::THREADS, 0, s>>>(a)
-         : k_grads<T, TileS, F32, false, O><<<blocks, TileS::THREADS, 0, s>>>(a);
+void launch(hipStream_t s, const ProdArgs& a, Tile tile) {
+  by_tile(tile, [&](auto shape) {
+    using S = decltype(shape);
+    const unsigned blocks = a.t.rtiles * a.t.ctiles * a.t.splits;
+    if (a.dw)
+      k_grads<T, S, F32, true, O><<<blocks, S::THREADS, 0, s>>>(a);
+    else
+      k_grads<T, S, F32, false, O><<<blocks, S::THREADS, 0, s>>>(a);
+  });
 }
 
 }  // namespace
 
-void launch_prod(hipStream_t s, const ProdArgs& a, int kind, bool large) {
+void launch_prod(hipStream_t s, const ProdArgs& a, int kind, Tile tile) {
   if (kind == EMH_F32)
-    launch<f16, true, float>(s, a, large);
+    launch<f16, true, float>(s, a, tile);
   else if (kind == EMH_F16)
-    launch<f16, false, f16>(s, a, large);
+    launch<f16, false, f16>(s, a, tile);
   else
-    launch<bf16, false, bf16>(s, a, large);
+    launch<bf16, false, bf16>(s, a, tile);
   EMH_HIP(hipGetLastError());
 }
 

@@ -26,7 +26,7 @@ __device__ __forceinline__ void copy_rows(const LogitArgs& a) {
 // F32: operands are planes of f16 with exponents.
 template <class T, class S, bool F32, bool GRAD>
 __global__ __launch_bounds__(S::THREADS, 2) void k_logits(const LogitArgs a) {
-  __shared__ __attribute__((aligned(1024))) char ring[2 * S::STAGE];
+  __shared__ __attribute__((aligned(1024))) char ring[S::RING];
   if constexpr (GRAD && !F32) {
     if (a.odd.flag && *a.odd.flag == a.odd.call) copy_rows<T>(a);
   }
@@ -181,7 +181,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_logits(const LogitArgs a) {
               for (int e = 0; e < 8; e++) g[e] = ldexpf(g[e], rs.gexp);
             }
             const uint32_t chunk = (wc * S::WA + b) * 4 + 2 * p + h;
-            store_vec(reinterpret_cast<T*>(ring + row * S::TC * 2 + ((chunk ^ (row & (CH - 1))) << 4)), g);
+            store_vec(reinterpret_cast<T*>(ring + row * S::TC * 2 + ((chunk ^ (row & 7)) << 4)), g);
           }
       }
       __syncthreads();
@@ -190,7 +190,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_logits(const LogitArgs a) {
       for (int t = threadIdx.x; t < S::TR * CH; t += S::THREADS) {
         const uint32_t row = t / CH, chunk = t % CH;
         const uint4 v = *reinterpret_cast<const uint4*>(ring + row * S::TC * 2 +
-                                                        ((chunk ^ (row & (CH - 1))) << 4));
+                                                        ((chunk ^ (row & 7)) << 4));
         *reinterpret_cast<uint4*>(out + row * a.ldg + chunk * 16) = v;
       }
     }
@@ -198,23 +198,22 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_logits(const LogitArgs a) {
 }
 
 template <class T, bool F32, bool GRAD>
-void launch(hipStream_t s, const LogitArgs& a, bool large) {
-  const unsigned blocks = a.t.rtiles * a.t.ctiles;
-  if (large)
-    k_logits<T, TileL, F32, GRAD><<<blocks, TileL::THREADS, 0, s>>>(a);
-  else
-    k_logits<T, TileS, F32, GRAD><<<blocks, TileS::THREADS, 0, s>>>(a);
+void launch(hipStream_t s, const LogitArgs& a, Tile tile) {
+  by_tile(tile, [&](auto shape) {
+    using S = decltype(shape);
+    k_logits<T, S, F32, GRAD><<<a.t.rtiles * a.t.ctiles, S::THREADS, 0, s>>>(a);
+  });
 }
 
 }  // namespace
 
-void launch_logits(hipStream_t s, const LogitArgs& a, int kind, bool large, bool grads) {
+void launch_logits(hipStream_t s, const LogitArgs& a, int kind, Tile tile, bool grads) {
   if (kind == EMH_F32)
-    grads ? launch<f16, true, true>(s, a, large) : launch<f16, true, false>(s, a, large);
+    grads ? launch<f16, true, true>(s, a, tile) : launch<f16, true, false>(s, a, tile);
   else if (kind == EMH_F16)
-    grads ? launch<f16, false, true>(s, a, large) : launch<f16, false, false>(s, a, large);
+    grads ? launch<f16, false, true>(s, a, tile) : launch<f16, false, false>(s, a, tile);
   else
-    grads ? launch<bf16, false, true>(s, a, large) : launch<bf16, false, false>(s, a, large);
+    grads ? launch<bf16, false, true>(s, a, tile) : launch<bf16, false, false>(s, a, tile);
   EMH_HIP(hipGetLastError());
 }
 
