@@ -93,40 +93,41 @@ __device__ __forceinline__ void decode4(uint32_t w, float scale, float* v) {
   const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
   v[0] = lo[0] * scale, v[1] = lo[1] * scale, v[2] = hi[0] * scale, v[3] = hi[1] * scale;
 }
-// The codes of v in a block whose scale this finds (a wave's 256 values).
+// The codes of v in a block whose scale this finds (a wave's 256 values). The
+// quotients are correctly rounded (one reciprocal a block, refined, then a product
+// and its remainder): a code one step off changes a small root by up to half, and
+// the parameter's step with it. A quotient is at most 448 (1 + 2^-23), which rounds to
+// 448; infinities and NaN become the NaN code.
 template <bool LEAST>
 __device__ __forceinline__ uint32_t encode4(const float* v, float& scale) {
-  float top = 0.f;
+  float top = lanes_max<64>(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))));
+  top = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(top)));  // (the wave's)
+  if (!(top < INFINITY)) {  // without the infinite ones (the maximum passes over NaN)
+    top = 0.f;
 #pragma unroll
-  for (int e = 0; e < 4; e++) {
-    const float m = fabsf(v[e]);
-    top = fmaxf(top, m <= 3.4028235e38f ? m : 0.f);
+    for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.f);
+    top = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(lanes_max<64>(top))));
   }
-  scale = lanes_max<64>(top) * (1.f / F8_TOP);
-  // (One reciprocal a block: a code near a tie may be its neighbour. Finite, or a
-  // zero in a block of the least numbers would become a NaN.)
-  const float by = fminf(__builtin_amdgcn_rcpf(scale), 3.4028235e38f);
+  scale = top * (1.f / F8_TOP);
   float q[4];
+  if (scale > 1e-30f && scale < 1e30f) {
+    const float r0 = __builtin_amdgcn_rcpf(scale);
+    const float by = fmaf(r0, fmaf(-scale, r0, 1.f), r0);
 #pragma unroll
-  for (int e = 0; e < 4; e++) {
-    q[e] = v[e] * by;
-    if (LEAST && v[e] > 0.f && q[e] < F8_LEAST) q[e] = F8_LEAST;
-    // (A quotient that rounded past the top; infinities and NaN become the NaN code.)
-    if (fabsf(v[e]) <= 3.4028235e38f)
-      q[e] = fminf(fmaxf(q[e], -F8_TOP), F8_TOP);
-    else
-      q[e] = __builtin_nanf("");
+    for (int e = 0; e < 4; e++) {
+      const float q0 = v[e] * by;
+      q[e] = fmaf(fmaf(-scale, q0, v[e]), by, q0);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; e++) q[e] = scale > 0.f ? v[e] / scale : v[e];
   }
-  uint32_t w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
+  if (LEAST) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) q[e] = v[e] > 0.f && q[e] < F8_LEAST ? F8_LEAST : q[e];
+  }
+  const uint32_t w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], (int)w, true);
-}
-
-// sqrt(v) within a unit in the last place, below the normal range too (where
-// the instruction takes zero for v).
-__device__ __forceinline__ float root(float v) {
-  const bool small = v < 1.17549435e-38f;
-  const float t = __builtin_amdgcn_sqrtf(small ? v * 18446744073709551616.f : v);  // 2^64
-  return small ? t * 2.3283064365386963e-10f : t;                                  // 2^-32
 }
 
 // One element's step; r: the root of the new v.
@@ -135,9 +136,9 @@ __device__ __forceinline__ void step1(const AdamScalars& s, float keep, float& p
   const float ge = g * s.gscale;
   m = s.beta1 * m + s.new1 * ge;
   v = s.beta2 * v + s.new2 * ge * ge;
-  // The root and the quotient within two units of the last place (the correctly
-  // rounded ones are twenty instructions each).
-  r = root(v);
+  r = sqrtf(v);
+  // The quotient within two units of the last place (the correctly rounded one is
+  // twenty instructions).
   p = p * keep - s.rate * (m * __builtin_amdgcn_rcpf(r * s.root2 + s.eps));
 }
 

@@ -55,9 +55,7 @@ struct TileShape {
   static constexpr int NW = NWR * NWC, THREADS = 64 * NW;
   static constexpr int TR = NWR * WB * 32, TC = NWC * WA * 32;
   static constexpr int RBYTES = TR * SLAB * 2, CBYTES = TC * SLAB * 2;
-  // (A power of two: the stages are toggled by XOR.)
-  static constexpr int STAGE = RBYTES + CBYTES <= 32768 ? 32768 : 65536;
-  static constexpr int RING = STAGE + RBYTES + CBYTES;
+  static constexpr int STAGE = RBYTES + CBYTES, RING = 2 * STAGE;
   static constexpr int RD = RBYTES / (1024 * NW), CD = CBYTES / (1024 * NW);  // DMAs a wave
 };
 typedef TileShape<4, 2, 2, 4> TileL;  // 256 x 256, 8 waves
@@ -66,6 +64,11 @@ typedef TileShape<2, 2, 2, 2> TileS;  // 128 x 128, 4 waves (two workgroups a CU
 enum Tile : int { TILE_L, TILE_M, TILE_S, TILES };
 constexpr uint32_t TILE_ROWS[TILES] = {TileL::TR, TileM::TR, TileS::TR};
 constexpr uint32_t TILE_COLS[TILES] = {TileL::TC, TileM::TC, TileS::TC};
+// Rows and columns of whole tiles of any shape.
+constexpr uint32_t ALL_ROWS = 256, ALL_COLS = 768;
+static_assert(ALL_ROWS % TileL::TR == 0 && ALL_ROWS % TileM::TR == 0 && ALL_ROWS % TileS::TR == 0 &&
+                  ALL_COLS % TileL::TC == 0 && ALL_COLS % TileM::TC == 0 && ALL_COLS % TileS::TC == 0,
+              "whole tiles");
 // Runs f with the shape as a type.
 template <class F>
 void by_tile(Tile t, F&& f) {
@@ -228,7 +231,7 @@ __device__ __forceinline__ void tile_sums(const TileIn& t, const TileAt& at, cha
             ldst + lst + S::RBYTES + (uint32_t)(q - S::RD) * S::NW * 1024);
   };
   auto advance = [&]() __attribute__((always_inline)) {
-    lst ^= S::STAGE;
+    lst = S::STAGE - lst;
     if (lleft > 1) {
       lleft--;
       if (++lslab == t.slabs) {
@@ -271,7 +274,7 @@ __device__ __forceinline__ void tile_sums(const TileIn& t, const TileAt& at, cha
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
       }
-      const uint32_t from = ks == 3 ? st ^ S::STAGE : st;
+      const uint32_t from = ks == 3 ? S::STAGE - st : st;
 #pragma unroll
       for (int a = 0; a < S::WA; a++) {
 #pragma unroll
@@ -291,7 +294,7 @@ __device__ __forceinline__ void tile_sums(const TileIn& t, const TileAt& at, cha
       }
     }
     advance();
-    st ^= S::STAGE;
+    st = S::STAGE - st;
   }
   wait_vm<0>();  // the DMAs past the last step have landed
   asm volatile("" ::: "memory");

@@ -30,6 +30,19 @@
 
 namespace emh {
 
+// exp(z - of) as the softmax takes it: the difference first, in z's own units, which is
+// exact where it matters (z near of); a logit in units of log 2 would be rounded by
+// a unit in its last place beforehand, a relative error of |z| 2^-24 in every term.
+__device__ __forceinline__ float exp_of(float z, float of) {
+  return __builtin_amdgcn_exp2f((z - of) * 1.44269504f);
+}
+// A row's maximum and sum of exponentials, joined with another's.
+__device__ __forceinline__ void join_sums(float& m, float& s, float2 p) {
+  const float b = fmaxf(m, p.x), bb = b == -INFINITY ? 0.f : b;
+  s = s * exp_of(m, bb) + p.y * exp_of(p.x, bb);
+  m = b;
+}
+
 // What a gradient call finds out about its rows, on the device.
 struct XentState {
   uint32_t count;  // rows with a label
@@ -57,15 +70,14 @@ struct LogitArgs {
   uint32_t n, m;    // rows, classes of the piece
   uint32_t col0, k; // its first class, all classes
   const uint32_t* labels;
-  float s2;         // scale log2(e)
+  float scale;
   const int* ex;    // f32: exponents of the rows, and of the piece's classes
   const int* ew;
-  float2* part;     // statistics: [part][row] (max, sum) of z log2(e)
+  float2* part;     // statistics: [part][row] (max, sum) of z
   float* zlabel;
   const float* lse; // gradients
   const float* gloss;
   const XentState* st;
-  float scale;
   OddRows odd;
   char* g[4];       // G; f32: Ga's planes, Gb's planes
   size_t ldg;       // bytes (rows and columns to full tiles)

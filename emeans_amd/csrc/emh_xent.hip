@@ -11,6 +11,15 @@ namespace {
 
 constexpr float LN2 = 0.693147181f;
 
+// A row's lse and loss from the maximum and sum of all its classes.
+__device__ __forceinline__ void finish_row(uint32_t i, float m, float s, uint32_t lab, uint32_t k,
+                                           float zlabel, float* loss, float* lse, uint32_t* small) {
+  const float top = m == -INFINITY ? 0.f : m, ls = log2f(s) * LN2;
+  if (lse) lse[i] = top + ls;
+  loss[i] = lab < k ? (top - zlabel) + ls : 0.f;
+  if (lab >= k && lab != NO_LABEL) small[SW_BAD_CLASS] = 1u;
+}
+
 // Rows to 16-byte aligned rows of dp elements, the rest zero (dp a multiple of
 // SLAB). labels: rows without one become zeros. A wave a row.
 template <class T>
@@ -163,7 +172,7 @@ template <class T, int R>
 __global__ __launch_bounds__(256) void k_few(const T* __restrict__ x, size_t ldx, uint32_t n,
                                              uint32_t d, const T* __restrict__ w, size_t ldw,
                                              uint32_t k, const uint32_t* __restrict__ labels,
-                                             float s2, float2* part, float* zlabel) {
+                                             float scale, float2* part, float* zlabel) {
   constexpr int N = VecOf<T>::N, DEEP = 4 * N;  // a chunk: DEEP of the depth, N a lane
   constexpr int U = R == 4 ? 4 : 8;             // chunks in flight
   __shared__ v4f sum[4][R][64];
@@ -184,16 +193,20 @@ __global__ __launch_bounds__(256) void k_few(const T* __restrict__ x, size_t ldx
 #pragma unroll
     for (int r = 0; r < R; r++) acc[r] = v4f{0.f, 0.f, 0.f, 0.f};
     for (uint32_t c0 = wave; c0 < chunks; c0 += 4 * U) {
-      Vec<T> a[U];
+      // (Past the last chunk it is read again, and not used: no load waits for a branch.)
+      Vec<T> a[U], b0[U];
 #pragma unroll
-      for (int u = 0; u < U; u++)
-        if (c0 + 4 * u < chunks) a[u] = fetch(w, ldw, g * 16 + l, k, c0 + 4 * u);
+      for (int u = 0; u < U; u++) {
+        const uint32_t c = min(c0 + 4 * u, chunks - 1);
+        a[u] = fetch(w, ldw, g * 16 + l, k, c);
+        b0[u] = fetch(x, ldx, l, n, c);
+      }
 #pragma unroll
       for (int u = 0; u < U; u++) {
         if (c0 + 4 * u >= chunks) continue;
 #pragma unroll
         for (int r = 0; r < R; r++) {
-          const Vec<T> b = fetch(x, ldx, r * 16 + l, n, c0 + 4 * u);
+          const Vec<T> b = r == 0 ? b0[u] : fetch(x, ldx, r * 16 + l, n, c0 + 4 * u);
           if constexpr (sizeof(T) == 4) {
 #pragma unroll
             for (int e = 0; e < 4; e++)
@@ -220,16 +233,16 @@ __global__ __launch_bounds__(256) void k_few(const T* __restrict__ x, size_t ldx
 #pragma unroll
     for (int e = 0; e < 4; e++) {
       const uint32_t j = g * 16 + q * 4 + e;
-      z[e] = j < k ? z[e] * s2 : -INFINITY;
+      z[e] = j < k ? z[e] * scale : -INFINITY;
       if (j == lab && j < k) zlabel[mine] = z[e];
       top = fmaxf(top, z[e]);  // (passes over NaN: the sum keeps it)
     }
     top = fmaxf(top, __shfl_xor(top, 16, 64));
     top = fmaxf(top, __shfl_xor(top, 32, 64));
     const float b = fmaxf(m, top), bb = b == -INFINITY ? 0.f : b;
-    s *= __builtin_amdgcn_exp2f(m - bb);
+    s *= exp_of(m, bb);
 #pragma unroll
-    for (int e = 0; e < 4; e++) s += __builtin_amdgcn_exp2f(z[e] - bb);
+    for (int e = 0; e < 4; e++) s += exp_of(z[e], bb);
     m = b;
   }
   if (wave >= R) return;
@@ -248,11 +261,7 @@ __global__ __launch_bounds__(256) void k_join_few(const float2* __restrict__ par
   const uint32_t lab = labels[i];
   const float zl = zlabel[i];
   float m = -INFINITY, s = 0.f;
-  auto join = [&](float2 p) __attribute__((always_inline)) {
-    const float b = fmaxf(m, p.x), bb = b == -INFINITY ? 0.f : b;
-    s = s * __builtin_amdgcn_exp2f(m - bb) + p.y * __builtin_amdgcn_exp2f(p.x - bb);
-    m = b;
-  };
+  auto join = [&](float2 p) __attribute__((always_inline)) { join_sums(m, s, p); };
 #pragma unroll 4
   for (uint32_t t = threadIdx.x; t < nparts; t += 256) join(part[(size_t)i * nparts + t]);
   for (int o = 32; o > 0; o >>= 1) join(make_float2(__shfl_xor(m, o, 64), __shfl_xor(s, o, 64)));
@@ -261,10 +270,7 @@ __global__ __launch_bounds__(256) void k_join_few(const float2* __restrict__ par
   if (threadIdx.x != 0) return;
   m = sh[0].x, s = sh[0].y;
   for (int t = 1; t < 4; t++) join(sh[t]);
-  const float l2 = (m == -INFINITY ? 0.f : m) + log2f(s);
-  if (lse) lse[i] = l2 * LN2;
-  loss[i] = lab < k ? (l2 - zl) * LN2 : 0.f;
-  if (lab >= k && lab != NO_LABEL) small[SW_BAD_CLASS] = 1u;
+  finish_row(i, m, s, lab, k, zl, loss, lse, small);
 }
 
 // The parts' maxima and sums joined: 64 rows a workgroup, 16 shares of the parts.
@@ -276,11 +282,7 @@ __global__ __launch_bounds__(1024) void k_join(const float2* __restrict__ part, 
   const uint32_t c = threadIdx.x & 63, g = threadIdx.x >> 6;
   const uint32_t i = blockIdx.x * 64 + c;
   float m = -INFINITY, s = 0.f;
-  auto join = [&](float2 p) __attribute__((always_inline)) {
-    const float b = fmaxf(m, p.x), bb = b == -INFINITY ? 0.f : b;
-    s = s * __builtin_amdgcn_exp2f(m - bb) + p.y * __builtin_amdgcn_exp2f(p.x - bb);
-    m = b;
-  };
+  auto join = [&](float2 p) __attribute__((always_inline)) { join_sums(m, s, p); };
   if (i < n) {
     uint32_t t = g;
     for (; t + 48 < nparts; t += 64) {  // four loads in flight
@@ -296,11 +298,7 @@ __global__ __launch_bounds__(1024) void k_join(const float2* __restrict__ part, 
   m = -INFINITY, s = 0.f;
 #pragma unroll
   for (int t = 0; t < 16; t++) join(sh[t][c]);
-  const float l2 = (m == -INFINITY ? 0.f : m) + log2f(s);
-  const uint32_t lab = labels[i];
-  if (lse) lse[i] = l2 * LN2;
-  loss[i] = lab < k ? (l2 - zlabel[i]) * LN2 : 0.f;
-  if (lab >= k && lab != NO_LABEL) small[SW_BAD_CLASS] = 1u;
+  finish_row(i, m, s, labels[i], k, zlabel[i], loss, lse, small);
 }
 
 // out = the splits' sums added, in their order.
@@ -360,7 +358,7 @@ struct Laid {
     p[0] = w.take<char>(rows * dp * 2);
     if (m.kind == EMH_F32) {
       p[1] = w.take<char>(rows * dp * 2);
-      ex = w.take<int>(up(rows, 256));
+      ex = w.take<int>(up(rows, ALL_COLS));  // (the tiles read whole column tiles of them)
     }
   }
   Operand deep(const MatIn& m, size_t first, size_t rows) const {
@@ -398,7 +396,7 @@ void few(emh_ctx* c, const XentIn& in, float* loss, float* lse) {
   auto run = [&](auto kernel) {
     kernel<<<dim3(blocks), 256, 0, c->stream>>>((const T*)in.x.p, in.x.ld, n, (uint32_t)in.d,
                                                 (const T*)in.w.p, in.w.ld, k, in.labels,
-                                                in.scale * 1.44269504f, part, zlabel);
+                                                in.scale, part, zlabel);
   };
   if (n <= 16)
     run(k_few<T, 1>);
@@ -495,7 +493,7 @@ void launch_cross_entropy(emh_ctx* c, const XentIn& in, float* loss, float* lse)
     a.t.rtiles = p.rtiles, a.t.ctiles = p.ctiles, a.t.splits = 1;
     a.n = (uint32_t)m, a.m = a.k = (uint32_t)k;
     a.labels = in.labels + r0;
-    a.s2 = in.scale * 1.44269504f;
+    a.scale = in.scale;
     a.ex = f32 ? lx.ex + r0 : nullptr;
     a.ew = lw.ex;
     a.part = part, a.zlabel = zlabel;
@@ -517,10 +515,10 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
     return;
   }
   const size_t slabs = up(d, SLAB) / SLAB, passes = f32 ? 3 : 1, planes = f32 ? 4 : 1;
-  // Classes a piece: 1 GB of G.
-  const size_t np = up(n, 256);
-  const size_t piece =
-      std::min<size_t>(up(k, 256), std::max<size_t>(256, ((size_t(512) << 20) / (np * planes)) & ~(size_t)255));
+  // Classes a piece: 1 GB of G, in whole tiles both ways, whatever their shape is.
+  const size_t np = up(n, ALL_ROWS);
+  const size_t most = (size_t(512) << 20) / (np * planes) / ALL_COLS * ALL_COLS;
+  const size_t piece = std::min<size_t>(up(k, ALL_COLS), std::max<size_t>(ALL_COLS, most));
   const size_t ldg = piece * 2, pieces = (k + piece - 1) / piece, ldp = up(d, 4);
   const Plan px = plan_of(n, d, passes * ((std::min(piece, k) + SLAB - 1) / SLAB), c->cus, true);
   const Plan pw = plan_of(std::min(piece, k), d, passes * ((n + SLAB - 1) / SLAB), c->cus, true);
@@ -563,6 +561,8 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
   for (size_t v0 = 0; v0 < k; v0 += piece) {
     const size_t m = std::min(piece, k - v0);
     const Plan pg = plan_of(n, m, slabs * passes, c->cus, false);
+    if ((size_t)pg.rtiles * TILE_ROWS[pg.tile] > np || (size_t)pg.ctiles * TILE_COLS[pg.tile] > piece)
+      throw Failure("cross_entropy_grad: tiles beyond the piece");
     LogitArgs a{};
     a.t.r = xl.deep(in.x, 0, n);
     a.t.c = lw.deep(in.w, v0, m);
@@ -570,9 +570,9 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
     a.t.rtiles = pg.rtiles, a.t.ctiles = pg.ctiles, a.t.splits = 1;
     a.n = (uint32_t)n, a.m = (uint32_t)m, a.col0 = (uint32_t)v0, a.k = (uint32_t)k;
     a.labels = in.labels;
-    a.s2 = in.scale * 1.44269504f;
+    a.scale = in.scale;
     a.ex = lx.ex, a.ew = f32 ? lw.ex + v0 : nullptr;
-    a.lse = lse, a.gloss = gloss, a.st = st, a.scale = in.scale;
+    a.lse = lse, a.gloss = gloss, a.st = st;
     if (x_as_is && v0 == 0)
       a.odd = {c->small + SW_ODD_ROW, call, lx.p[0], lx.dp, (const char*)in.x.p, in.x.ld, d};
     for (int i = 0; i < 4; i++) a.g[i] = G[i];

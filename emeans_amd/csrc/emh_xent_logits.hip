@@ -5,8 +5,6 @@
 namespace emh {
 namespace {
 
-constexpr float LOG2E = 1.44269504f;
-
 // x with zeros in rows without a label (OddRows): every workgroup its share.
 template <class T>
 __device__ __forceinline__ void copy_rows(const LogitArgs& a) {
@@ -39,7 +37,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_logits(const LogitArgs a) {
   const uint32_t i0 = at.rt * S::TR + wr * S::WB * 32 + li;
   const uint32_t j0 = at.ct * S::TC + wc * S::WA * 32;
 
-  // To logits times log2(e).
+  // To logits.
   int ex[S::WB];
 #pragma unroll
   for (int y = 0; y < S::WB; y++) ex[y] = F32 ? a.ex[min(i0 + y * 32, a.n - 1)] : 0;
@@ -57,7 +55,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_logits(const LogitArgs a) {
 #pragma unroll
         for (int y = 0; y < S::WB; y++) {
           const float z = acc[b][y][4 * q + e];
-          acc[b][y][4 * q + e] = (F32 ? ldexpf(z, ex[y] + ew[e]) : z) * a.s2;
+          acc[b][y][4 * q + e] = (F32 ? ldexpf(z, ex[y] + ew[e]) : z) * a.scale;
         }
     }
 
@@ -102,7 +100,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_logits(const LogitArgs a) {
 #pragma unroll
       for (int b = 0; b < S::WA; b++)
 #pragma unroll
-        for (int r = 0; r < 16; r++) s += __builtin_amdgcn_exp2f(acc[b][y][r] - mm);
+        for (int r = 0; r < 16; r++) s += exp_of(acc[b][y][r], mm);
       s += __shfl_xor(s, 32, 64);
       if (h == 0 && i < a.n) a.part[(size_t)pi * a.n + i] = make_float2(m, s);
     }
@@ -114,7 +112,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_logits(const LogitArgs a) {
       const uint32_t ic = min(i, a.n - 1);
       const uint32_t lab = i < a.n ? a.labels[ic] : NO_LABEL;
       const bool has = lab < a.k;
-      const float l2 = a.lse[ic] * LOG2E;
+      const float lse = a.lse[ic];
       const float u = a.gloss ? a.gloss[ic] : 1.f;
       // The label's column (another piece's: none of this one), and the columns
       // there are, none in a row without a label, from the lane's first.
@@ -126,7 +124,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_logits(const LogitArgs a) {
 #pragma unroll
         for (int r = 0; r < 16; r++) {
           const int c = b * 32 + 8 * (r >> 2) + (r & 3);
-          const float soft = __builtin_amdgcn_exp2f(acc[b][y][r] - l2);
+          const float soft = exp_of(acc[b][y][r], lse);
           const float g = (soft - (own == (uint32_t)c ? 1.f : 0.f)) * u;
           acc[b][y][r] = c < have ? g : 0.f;
         }

@@ -105,6 +105,18 @@ def test_against_64_bits(dev, n, d, k, name):
     Run(dev, x, w, lab, name, gloss=gloss).check()
 
 
+# Enough rows, columns or classes for each of the products' tile shapes, and for
+# sums split over the depth, at sizes that end inside a tile.
+TILES = [(10_007, 300, 1000), (2100, 770, 1250), (4097, 190, 385), (700, 64, 4500), (5000, 384, 130)]
+
+
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n,d,k", TILES)
+def test_every_tile_shape(dev, n, d, k, name):
+    x, w, lab = _inputs(n, d, k, n + d + k)
+    Run(dev, x, w, lab, name).check()
+
+
 @pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("n,d,k", [(9, 40, 70), (270, 64, 300), (100, 33, 513)])
 @pytest.mark.parametrize("pad,off", [(0, 1), (3, 0), (8, 5)])
