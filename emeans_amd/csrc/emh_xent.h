@@ -63,6 +63,7 @@ struct OddRows {
   const char* x;
   size_t ld, d;
 };
+constexpr int XENT_LEAST = -120;  // least exponent of a row (its power of two is finite)
 constexpr int XENT_BIAS = 4096;  // (so that zero is less than any)
 
 struct LogitArgs {

@@ -71,7 +71,8 @@ __global__ __launch_bounds__(256) void k_pack32(const float* x, size_t ld, size_
   for (uint32_t q = 0; q < HELD; q++) top = largest(held[q], top);
   for (uint32_t c = lane * 4 + HELD * 256; c < d; c += 256) top = largest(get(c), top);
   top = lanes_max<64>(top);
-  const int e0 = top > 0.f ? max(ilogbf(top) - 13, -120) : 0;
+  // (A row of zeros takes the least exponent, which is no one's largest.)
+  const int e0 = top > 0.f ? max(ilogbf(top) - 13, XENT_LEAST) : XENT_LEAST;
   const float by = ldexpf(1.f, -e0);
   auto put = [&](uint32_t c, const Vec<float>& v) __attribute__((always_inline)) {
     uint16_t a[4], b[4];

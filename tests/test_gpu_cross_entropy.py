@@ -188,6 +188,33 @@ def test_wide_ranges_in_one_matrix(dev):
     Run(dev, x, w, lab, "f32").check()
 
 
+@pytest.mark.parametrize("n", [150, 3000])
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+def test_zero_rows_and_classes(dev, name, n):
+    """A row or a class of zeros (a cluster that was never used) has no size of its own
+    to be held to, and takes none of the others' precision."""
+    x, w, lab = _inputs(n, 64, 300, 12)
+    x[5], w[7], w[200:] = 0.0, 0.0, 0.0
+    Run(dev, x, w, lab, name).check()
+    Run(dev, 0 * x, w, lab, name).check()
+    Run(dev, x, 0 * w, lab, name).check()
+
+
+@pytest.mark.parametrize("n", [150, 3000])
+def test_a_few_rows_and_classes_of_another_size(dev, n):
+    """float32 rows and classes nearly of one size, and some of a thousandth of it or a thousand
+    times it."""
+    x, w, lab = _inputs(n, 64, 300, 13)
+    Run(dev, x, w, lab, "f32").check()
+    y, v = x.copy(), w.copy()
+    y[::7] *= 1e-3
+    Run(dev, y, w, lab, "f32").check()
+    v[::9] *= 1e-3
+    Run(dev, x, v, lab, "f32", gloss=np.random.default_rng(2).standard_normal(n)).check()
+    v[3] *= 1e3
+    Run(dev, y, v, lab, "f32").check()
+
+
 def test_labels_out_of_range_are_reported(dev):
     from emeans_amd import EmeansHipInvalid, F32
     x, w, lab = _inputs(50, 40, 30, 3, none=0.0)
