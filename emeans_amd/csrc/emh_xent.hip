@@ -20,35 +20,49 @@ __device__ __forceinline__ void finish_row(uint32_t i, float m, float s, uint32_
   if (lab >= k && lab != NO_LABEL) small[SW_BAD_CLASS] = 1u;
 }
 
-// Rows to 16-byte aligned rows of dp elements, the rest zero (dp a multiple of
-// SLAB). labels: rows without one become zeros. A wave a row.
+// One matrix to lay out: rows to 16-byte aligned rows of dp elements, the rest zero
+// (dp a multiple of SLAB); labels: rows without one become zeros.
+struct PackOne {
+  const void* x;
+  size_t ld, n;
+  const uint32_t* labels;
+  char *hi, *lo;
+  int* ex;
+};
+struct PackArgs {  // both operands in one launch, the first's workgroups first
+  PackOne m[2];
+  uint32_t d, dp, k, first;
+};
+
+// 16-bit rows. A wave a row.
 template <class T>
-__global__ __launch_bounds__(256) void k_pack16(const T* x, size_t ld, size_t n, uint32_t d,
-                                                uint32_t dp, const uint32_t* labels, uint32_t k,
-                                                T* out) {
-  const size_t i = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (i >= n) return;
+__global__ __launch_bounds__(256) void k_pack16(const PackArgs a) {
+  const bool second = blockIdx.x >= a.first;
+  const PackOne& m = a.m[second ? 1 : 0];
+  const size_t i = (size_t)(blockIdx.x - (second ? a.first : 0)) * 4 + (threadIdx.x >> 6);
+  if (i >= m.n) return;
   const uint32_t lane = threadIdx.x & 63;
-  const T* row = x + i * ld;
-  const bool zero = labels && labels[i] >= k;
-  for (uint32_t c = lane * 8; c < dp; c += 512) {
+  const T* row = reinterpret_cast<const T*>(m.x) + i * m.ld;
+  T* out = reinterpret_cast<T*>(m.hi) + i * a.dp;
+  const bool zero = m.labels && m.labels[i] >= a.k;
+  for (uint32_t c = lane * 8; c < a.dp; c += 512) {
     Vec<T> v{make_uint4(0u, 0u, 0u, 0u)};
-    if (!zero && c < d) v = c + 8 <= d ? load_vec(row + c) : load_some(row + c, (int)(d - c));
-    *reinterpret_cast<uint4*>(out + i * dp + c) = v.raw;
+    if (!zero && c < a.d) v = c + 8 <= a.d ? load_vec(row + c) : load_some(row + c, (int)(a.d - c));
+    *reinterpret_cast<uint4*>(out + c) = v.raw;
   }
 }
 
-// f32 rows to planes of f16 (emh_xent.h) and their exponents e (x = plane 2^e);
-// labels: rows without one become zeros. A wave a row, which it holds where it
-// has at most 1,024 elements, and reads twice beyond.
-__global__ __launch_bounds__(256) void k_pack32(const float* x, size_t ld, size_t n, uint32_t d,
-                                                uint32_t dp, const uint32_t* labels, uint32_t k,
-                                                f16* hi, f16* lo, int* ex) {
-  const size_t i = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (i >= n) return;
-  const uint32_t lane = threadIdx.x & 63;
-  const float* row = x + i * ld;
-  const bool zero = labels && labels[i] >= k;
+// f32 rows to planes of f16 (emh_xent.h) and their exponents e (x = plane 2^e). A
+// wave a row, which it holds where it has at most 1,024 elements, and reads twice
+// beyond.
+__global__ __launch_bounds__(256) void k_pack32(const PackArgs a) {
+  const bool second = blockIdx.x >= a.first;
+  const PackOne& m = a.m[second ? 1 : 0];
+  const size_t i = (size_t)(blockIdx.x - (second ? a.first : 0)) * 4 + (threadIdx.x >> 6);
+  if (i >= m.n) return;
+  const uint32_t lane = threadIdx.x & 63, d = a.d, dp = a.dp;
+  const float* row = reinterpret_cast<const float*>(m.x) + i * m.ld;
+  const bool zero = m.labels && m.labels[i] >= a.k;
   constexpr uint32_t HELD = 4;  // vectors of four a lane
   auto get = [&](uint32_t c) __attribute__((always_inline)) {
     Vec<float> v{make_uint4(0u, 0u, 0u, 0u)};
@@ -58,8 +72,8 @@ __global__ __launch_bounds__(256) void k_pack32(const float* x, size_t ld, size_
   auto largest = [](const Vec<float>& v, float top) __attribute__((always_inline)) {
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      const float m = fabsf(v.get(e));
-      top = fmaxf(top, m < INFINITY ? m : 0.f);
+      const float t = fabsf(v.get(e));
+      top = fmaxf(top, t < INFINITY ? t : 0.f);
     }
     return top;
   };
@@ -75,25 +89,25 @@ __global__ __launch_bounds__(256) void k_pack32(const float* x, size_t ld, size_
   const int e0 = top > 0.f ? max(ilogbf(top) - 13, XENT_LEAST) : XENT_LEAST;
   const float by = ldexpf(1.f, -e0);
   auto put = [&](uint32_t c, const Vec<float>& v) __attribute__((always_inline)) {
-    uint16_t a[4], b[4];
+    uint16_t h4[4], l4[4];
 #pragma unroll
     for (int e = 0; e < 4; e++) {
       const float t = v.get(e) * by;
       const f16 h = (f16)t;
-      a[e] = __builtin_bit_cast(uint16_t, h);
-      b[e] = __builtin_bit_cast(uint16_t, (f16)(t - (float)h));
+      h4[e] = __builtin_bit_cast(uint16_t, h);
+      l4[e] = __builtin_bit_cast(uint16_t, (f16)(t - (float)h));
     }
-    const size_t o = i * dp + c;
-    *reinterpret_cast<uint2*>(hi + o) =
-        make_uint2(a[0] | (uint32_t)a[1] << 16, a[2] | (uint32_t)a[3] << 16);
-    *reinterpret_cast<uint2*>(lo + o) =
-        make_uint2(b[0] | (uint32_t)b[1] << 16, b[2] | (uint32_t)b[3] << 16);
+    const size_t o = (i * dp + c) * 2;
+    *reinterpret_cast<uint2*>(m.hi + o) =
+        make_uint2(h4[0] | (uint32_t)h4[1] << 16, h4[2] | (uint32_t)h4[3] << 16);
+    *reinterpret_cast<uint2*>(m.lo + o) =
+        make_uint2(l4[0] | (uint32_t)l4[1] << 16, l4[2] | (uint32_t)l4[3] << 16);
   };
 #pragma unroll
   for (uint32_t q = 0; q < HELD; q++)
     if (lane * 4 + q * 256 < dp) put(lane * 4 + q * 256, held[q]);
   for (uint32_t c = lane * 4 + HELD * 256; c < dp; c += 256) put(c, get(c));
-  if (lane == 0) ex[i] = e0;
+  if (lane == 0) m.ex[i] = e0;
 }
 
 // The call's state, by workgroup 0 alone (a pass over the labels, and of f32
@@ -126,8 +140,9 @@ __global__ __launch_bounds__(1024) void k_survey(const T* x, size_t ld, uint32_t
     if (__ballot(odd) != 0ull && lane == 0) small[SW_ODD_ROW] = call;
     return;
   }
-  __shared__ int sh[3][16];
-  int count = 0, uexp = 0, ewmax = 0;
+  __shared__ int sh[5][16];
+  constexpr int MANY = 1 << 20;
+  int count = 0, uexp = 0, ewmax = 0, ulow = MANY, ewlow = MANY;
   bool bad = false;
 #pragma unroll 4
   for (uint32_t i = threadIdx.x; i < n; i += 1024) {
@@ -137,27 +152,38 @@ __global__ __launch_bounds__(1024) void k_survey(const T* x, size_t ld, uint32_t
     count += has ? 1 : 0;
     const float g = gloss ? fabsf(gloss[i]) : 1.f;
     const int e = (ex ? ex[i] : 0) + XENT_BIAS + (gloss ? ilogbf(g) : 0);
-    if (has && g > 0.f && g < INFINITY) uexp = max(uexp, e);
+    if (has && g > 0.f && g < INFINITY) {
+      uexp = max(uexp, e);
+      ulow = min(ulow, e);
+    }
   }
   if (ew) {
 #pragma unroll 8
-    for (uint32_t j = threadIdx.x; j < k; j += 1024) ewmax = max(ewmax, ew[j] + XENT_BIAS);
+    for (uint32_t j = threadIdx.x; j < k; j += 1024) {
+      ewmax = max(ewmax, ew[j] + XENT_BIAS);
+      ewlow = min(ewlow, ew[j] + XENT_BIAS);
+    }
   }
   if (bad) small[SW_BAD_CLASS] = 1u;
   for (int o = 32; o > 0; o >>= 1) {
     count += __shfl_xor(count, o, 64);
     uexp = max(uexp, __shfl_xor(uexp, o, 64));
     ewmax = max(ewmax, __shfl_xor(ewmax, o, 64));
+    ulow = min(ulow, __shfl_xor(ulow, o, 64));
+    ewlow = min(ewlow, __shfl_xor(ewlow, o, 64));
   }
-  if (lane == 0) sh[0][w] = count, sh[1][w] = uexp, sh[2][w] = ewmax;
+  if (lane == 0) sh[0][w] = count, sh[1][w] = uexp, sh[2][w] = ewmax, sh[3][w] = ulow, sh[4][w] = ewlow;
   __syncthreads();
   if (threadIdx.x != 0) return;
   for (int i = 1; i < 16; i++) {
     count += sh[0][i];
     uexp = max(uexp, sh[1][i]);
     ewmax = max(ewmax, sh[2][i]);
+    ulow = min(ulow, sh[3][i]);
+    ewlow = min(ewlow, sh[4][i]);
   }
-  *st = XentState{(uint32_t)count, uexp, ewmax};
+  const int span = max(uexp - ulow, 0) + max(ewmax - ewlow, 0);
+  *st = XentState{(uint32_t)count, uexp, ewmax, span <= XENT_SPAN ? 1 : 0};
 }
 
 typedef float v4f __attribute__((ext_vector_type(4)));
@@ -373,15 +399,24 @@ struct Laid {
   }
 };
 
-void pack(emh_ctx* c, const MatIn& m, size_t rows, size_t d, const Laid& l, const uint32_t* labels,
-          size_t k) {
-  const dim3 grid = grid1(rows, 4);
-  if (m.kind == EMH_F32)
-    k_pack32<<<grid, 256, 0, c->stream>>>((const float*)m.p, m.ld, rows, (uint32_t)d, l.dp, labels,
-                                          (uint32_t)k, (f16*)l.p[0], (f16*)l.p[1], l.ex);
+// Lays out the operands that need it; labels: see PackOne, for x.
+void pack(emh_ctx* c, const XentIn& in, const Laid& x, const Laid& w, const uint32_t* labels) {
+  PackArgs a{};
+  unsigned blocks = 0;
+  auto add = [&](PackOne& m, const MatIn& from, size_t rows, const Laid& to, const uint32_t* lab) {
+    m = {from.p, from.ld, rows, lab, to.p[0], to.p[1], to.ex};
+    blocks += (unsigned)((rows + 3) / 4);
+    a.dp = to.dp;
+  };
+  if (x.packed) add(a.m[0], in.x, in.n, x, labels);
+  a.first = blocks;
+  if (w.packed) add(a.m[1], in.w, in.k, w, nullptr);
+  if (blocks == 0) return;
+  a.d = (uint32_t)in.d, a.k = (uint32_t)in.k;
+  if (in.x.kind == EMH_F32)
+    k_pack32<<<dim3(blocks), 256, 0, c->stream>>>(a);
   else  // (16-bit words, whatever they stand for)
-    k_pack16<f16><<<grid, 256, 0, c->stream>>>((const f16*)m.p, m.ld, rows, (uint32_t)d, l.dp, labels,
-                                               (uint32_t)k, (f16*)l.p[0]);
+    k_pack16<f16><<<dim3(blocks), 256, 0, c->stream>>>(a);
 }
 
 // At most this many rows take the kernel that reads the classes once, as they lie.
@@ -482,8 +517,7 @@ void launch_cross_entropy(emh_ctx* c, const XentIn& in, float* loss, float* lse)
     zlabel = w.take<float>(rows);
     if (pass == 0) w.base = (char*)c->xent.get(w.used);
   }
-  if (lx.packed) pack(c, in.x, n, d, lx, nullptr, 0);
-  if (lw.packed) pack(c, in.w, k, d, lw, nullptr, 0);
+  pack(c, in, lx, lw, nullptr);
   for (size_t r0 = 0; r0 < n; r0 += rows) {
     const size_t m = std::min(rows, n - r0);
     const Plan p = plan_of(m, k, slabs * passes, c->cus, false);
@@ -542,8 +576,7 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
     if (pass == 0) w.base = (char*)c->xent.get(w.used);
   }
   const uint32_t call = ++c->xent_calls;
-  if (!x_as_is) pack(c, in.x, n, d, lx, in.labels, k);
-  if (lw.packed) pack(c, in.w, k, d, lw, nullptr, 0);
+  pack(c, in, x_as_is ? Laid{} : lx, lw, in.labels);
   {
     const dim3 grid(x_as_is ? 1 + (unsigned)((n + 255) / 256) : 1);
     auto run = [&](auto t) {
@@ -591,13 +624,16 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
       p.t.slabs = (uint32_t)((m + SLAB - 1) / SLAB);
       p.t.rtiles = px.rtiles, p.t.ctiles = px.ctiles, p.t.splits = px.splits;
       p.rows = (uint32_t)n, p.dw = false;
+      p.ex = lx.ex;
       p.out = dx.p, p.ldo = dx.ld;
       p.part = px_part ? partx : nullptr;
       p.add = v0 > 0;
       launch_prod(c->stream, p, in.x.kind, px.tile);
     }
     if (dw.p) {
-      p.t.r = {{f32 ? G[2] : G[0], G[3]}, (uint32_t)ldg, up(n, SLAB), (uint32_t)piece};
+      p.t.r = {{G[0], G[1]}, (uint32_t)ldg, up(n, SLAB), (uint32_t)piece};
+      p.gb[0] = G[2], p.gb[1] = G[3];
+      p.ex = a.ew;
       p.t.c = xl.deep(in.x, 0, n);
       p.t.c.wide = xl.packed ? xl.dp : (uint32_t)d;
       p.t.slabs = (uint32_t)((n + SLAB - 1) / SLAB);

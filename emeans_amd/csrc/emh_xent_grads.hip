@@ -11,6 +11,11 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_grads(const ProdArgs a) {
   v16f acc[S::WA][S::WB];
   TileIn t = a.t;
   if (DW && a.flag && *a.flag == a.call) t.c = a.alt;
+  bool one = false;
+  if constexpr (F32) {
+    one = a.st->one != 0;
+    if (DW && !one) t.r.p[0] = a.gb[0], t.r.p[1] = a.gb[1];
+  }
   tile_sums<T, S, !DW, false>(t, at, ring, acc);
 
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, li = lane & 31, h = lane >> 5;
@@ -25,10 +30,15 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_grads(const ProdArgs a) {
     if (i >= a.rows) continue;
     const bool zero = !DW && a.labels[i] >= a.k;
     int by = 0;
-    if constexpr (F32)
-      by = DW ? -rs.gexp : a.st->ewmax - XENT_BIAS - row_exp(a.gloss, i);
-    else if constexpr (__is_same(T, f16))
+    if constexpr (F32) {
+      const int ewmax = a.st->ewmax - XENT_BIAS;
+      if (one)
+        by = ewmax - a.ex[i] - rs.gexp;
+      else
+        by = DW ? -rs.gexp : ewmax - row_exp(a.gloss, i);
+    } else if constexpr (__is_same(T, f16)) {
       by = -rs.gexp;
+    }
 #pragma unroll
     for (int b = 0; b < S::WA; b++)
 #pragma unroll

@@ -135,15 +135,22 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_logits(const LogitArgs a) {
     RowScale rs;
     rs.init(a.st, a.gloss, a.scale);
     int ewmax = 0;
-    if constexpr (F32) ewmax = a.st->ewmax - XENT_BIAS;
+    bool one = false;
+    if constexpr (F32) {
+      ewmax = a.st->ewmax - XENT_BIAS;
+      one = a.st->one != 0;
+    }
     constexpr int CH = S::TC / 8;
     const uint32_t r0 = wr * S::WB * 32 + li;
 #pragma unroll
     for (int plane = 0; plane < (F32 ? 4 : 1); plane++) {
+      if (plane == 2 && one) break;
       __syncthreads();
 #pragma unroll
       for (int y = 0; y < S::WB; y++) {
-        const int ga = F32 ? row_exp(a.gloss, min(i0 + y * 32, a.n - 1)) : 0;
+        int ga = 0;
+        if constexpr (F32)
+          ga = one ? ex[y] + rs.gexp : row_exp(a.gloss, min(i0 + y * 32, a.n - 1));
         const uint32_t row = r0 + y * 32;
 #pragma unroll
         for (int b = 0; b < S::WA; b++)
