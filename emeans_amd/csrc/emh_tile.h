@@ -314,6 +314,20 @@ __device__ __forceinline__ void eight(const float* lo, const float* hi, float* o
     out[4 + e] = __uint_as_float(v[1]);
   }
 }
+// The same in a 16-bit type.
+template <class T>
+__device__ __forceinline__ Vec<T> eight_of(const float* lo, const float* hi) {
+  uint32_t out[4];
+#pragma unroll
+  for (int e = 0; e < 2; e++) {
+    const auto v = __builtin_amdgcn_permlane32_swap(pair_from_f32<T>(lo[2 * e], lo[2 * e + 1]),
+                                                    pair_from_f32<T>(hi[2 * e], hi[2 * e + 1]),
+                                                    false, false);
+    out[e] = v[0];
+    out[2 + e] = v[1];
+  }
+  return Vec<T>{make_uint4(out[0], out[1], out[2], out[3])};
+}
 
 }  // namespace
 }  // namespace emh

@@ -31,6 +31,13 @@ template <class T>
 __device__ __forceinline__ T from_f32(float v) {
   return (T)v;  // nearest, ties to even
 }
+// Two of a 16-bit type in one word, by one instruction.
+template <class T>
+__device__ __forceinline__ uint32_t pair_from_f32(float lo, float hi) {
+  typedef float F2 __attribute__((ext_vector_type(2)));
+  typedef T T2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((F2{lo, hi}), T2));
+}
 
 // A 16-byte vector's raw bits and its elements.
 template <class T>
@@ -75,11 +82,19 @@ __device__ __forceinline__ void store_vec(T* p, const float* v) {
     for (int e = 0; e < 4; e++) a.w[e] = __float_as_uint(v[e]);
   } else {
 #pragma unroll
-    for (int e = 0; e < 4; e++)
-      a.w[e] = (uint32_t)__builtin_bit_cast(uint16_t, from_f32<T>(v[2 * e])) |
-               (uint32_t)__builtin_bit_cast(uint16_t, from_f32<T>(v[2 * e + 1])) << 16;
+    for (int e = 0; e < 4; e++) a.w[e] = pair_from_f32<T>(v[2 * e], v[2 * e + 1]);
   }
   *reinterpret_cast<Any16*>(p) = a;
+}
+template <class T>
+__device__ __forceinline__ void store_vec(T* p, const Vec<T>& v) {
+  *reinterpret_cast<Any16*>(p) = Any16{{v.raw.x, v.raw.y, v.raw.z, v.raw.w}};
+}
+template <class T>
+__device__ __forceinline__ void store_some(T* p, const Vec<T>& v, int left) {
+#pragma unroll
+  for (int e = 0; e < VecOf<T>::N; e++)
+    if (e < left) p[e] = from_f32<T>(v.get(e));
 }
 template <class T>
 __device__ __forceinline__ void store_some(T* p, const float* v, int left) {

@@ -42,6 +42,10 @@ namespace emh {
 __device__ __forceinline__ float exp_of(float z, float of) {
   return __builtin_amdgcn_exp2f((z - of) * 1.44269504f);
 }
+// The same of z = sum scale, which is not rounded by itself.
+__device__ __forceinline__ float exp_of(float sum, float scale, float of) {
+  return __builtin_amdgcn_exp2f(fmaf(sum, scale, -of) * 1.44269504f);
+}
 // A row's maximum and sum of exponentials, joined with another's.
 __device__ __forceinline__ void join_sums(float& m, float& s, float2 p) {
   const float b = fmaxf(m, p.x), bb = b == -INFINITY ? 0.f : b;

@@ -43,7 +43,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_grads(const ProdArgs a) {
     for (int b = 0; b < S::WA; b++)
 #pragma unroll
       for (int p = 0; p < 2; p++) {
-        float v[2][4], g[8];
+        float v[2][4];
 #pragma unroll
         for (int f = 0; f < 2; f++)
 #pragma unroll
@@ -68,16 +68,25 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_grads(const ProdArgs a) {
           }
           continue;
         }
-        eight(v[0], v[1], g);
         const uint32_t j = j0 + b * 32 + 16 * p + 8 * h;
         O* o = reinterpret_cast<O*>(a.out) + (size_t)i * a.ldo + j;
-        if (j + 8 <= a.cols) {
-          store_vec(o, g);
-          if constexpr (sizeof(O) == 4) store_vec(o + 4, g + 4);
-        } else {
+        if constexpr (sizeof(O) == 4) {
+          float g[8];
+          eight(v[0], v[1], g);
+          if (j + 8 <= a.cols) {
+            store_vec(o, g);
+            store_vec(o + 4, g + 4);
+          } else {
 #pragma unroll
-          for (int e = 0; e < 8; e++)
-            if (j + e < a.cols) o[e] = from_f32<O>(g[e]);
+            for (int e = 0; e < 8; e++)
+              if (j + e < a.cols) o[e] = g[e];
+          }
+        } else {
+          const Vec<O> g = eight_of<O>(v[0], v[1]);
+          if (j + 8 <= a.cols)
+            store_vec(o, g);
+          else
+            store_some(o, g, (int)a.cols - (int)j);
         }
       }
   }

@@ -21,6 +21,37 @@ __device__ __forceinline__ void copy_rows(const LogitArgs& a) {
   }
 }
 
+// f(c, v) in place of every v of the lane's row y, c its column less the lane's
+// first, which is 4 (lane / 32).
+template <class S, class F>
+__device__ __forceinline__ void each(v16f (&acc)[S::WA][S::WB], int y, F&& f) {
+#pragma unroll
+  for (int b = 0; b < S::WA; b++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) acc[b][y][r] = f(b * 32 + 8 * (r >> 2) + (r & 3), acc[b][y][r]);
+}
+// The v whose c it is (below 32 WA, a multiple of 8 and at most 3): its block first,
+// half of the selections that a search of all takes.
+template <class S>
+__device__ __forceinline__ float at_column(const v16f (&acc)[S::WA][S::WB], int y, uint32_t c) {
+  v16f v = acc[0][y];
+#pragma unroll
+  for (int b = 1; b < S::WA; b++) {
+    const bool from = c >= (uint32_t)b * 32;
+#pragma unroll
+    for (int r = 0; r < 16; r++) v[r] = from ? acc[b][y][r] : v[r];
+  }
+  const uint32_t at = (c & 31) >> 3 << 2 | (c & 3);
+  float out = v[0];
+#pragma unroll
+  for (int r = 1; r < 16; r++) out = at == (uint32_t)r ? v[r] : out;
+  return out;
+}
+// Four classes' exponents (their buffer is a whole number of tiles long).
+__device__ __forceinline__ int4 four_exps(const int* ew, uint32_t j) {
+  return *reinterpret_cast<const int4*>(ew + j);
+}
+
 // F32: operands are planes of f16 with exponents.
 template <class T, class S, bool F32, bool GRAD>
 __global__ __launch_bounds__(S::THREADS, 2) void k_logits(const LogitArgs a) {
@@ -37,75 +68,75 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_logits(const LogitArgs a) {
   const uint32_t i0 = at.rt * S::TR + wr * S::WB * 32 + li;
   const uint32_t j0 = at.ct * S::TC + wc * S::WA * 32;
 
-  // To logits.
+  // The sums in their own units. The logits are these times the scale, which the
+  // exponentials take in their difference (exp_of). (The paths that few calls take
+  // are kept out of the others' way: a call's workgroups are few enough for the
+  // instructions' first reads to count.)
   int ex[S::WB];
 #pragma unroll
   for (int y = 0; y < S::WB; y++) ex[y] = F32 ? a.ex[min(i0 + y * 32, a.n - 1)] : 0;
+  if constexpr (F32) {
 #pragma unroll
-  for (int b = 0; b < S::WA; b++)
+    for (int b = 0; b < S::WA; b++)
 #pragma unroll
-    for (int q = 0; q < 4; q++) {
-      int ew[4] = {0, 0, 0, 0};
-      if constexpr (F32) {  // (the exponents' buffer is a whole number of tiles long)
-        const int4 v = *reinterpret_cast<const int4*>(a.ew + j0 + b * 32 + 8 * q + 4 * h);
-        ew[0] = v.x, ew[1] = v.y, ew[2] = v.z, ew[3] = v.w;
+      for (int q = 0; q < 4; q++) {
+        const int4 v = four_exps(a.ew, j0 + b * 32 + 8 * q + 4 * h);
+        const int ew[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+          for (int y = 0; y < S::WB; y++)
+            acc[b][y][4 * q + e] = ldexpf(acc[b][y][4 * q + e], ex[y] + ew[e]);
       }
-#pragma unroll
-      for (int e = 0; e < 4; e++)
-#pragma unroll
-        for (int y = 0; y < S::WB; y++) {
-          const float z = acc[b][y][4 * q + e];
-          acc[b][y][4 * q + e] = (F32 ? ldexpf(z, ex[y] + ew[e]) : z) * a.scale;
-        }
-    }
+  }
+  float scale = a.scale;
 
   // Columns of the wave that there are; all of them but in the last tile.
   const int left = (int)min(a.m - min(a.m, j0), (uint32_t)(S::WA * 32));
   const bool full = left == S::WA * 32;
   if constexpr (!GRAD) {
     const uint32_t pi = at.ct * S::NWC + wc;
-    if (!full) {
+    if (__builtin_expect(!(scale > 0.f), 0)) {  // the largest sum is not the largest logit's
+#pragma unroll
+      for (int y = 0; y < S::WB; y++)
+        each<S>(acc, y, [&](int, float v) { return v * scale; });
+      scale = 1.f;
+    }
+    if (__builtin_expect(!full, 0)) {
       int have = left - 4 * h;
       asm volatile("" : "+v"(have));  // (the comparisons are made here, not kept)
 #pragma unroll
-      for (int b = 0; b < S::WA; b++)
-#pragma unroll
-        for (int r = 0; r < 16; r++) {
-          const bool in = b * 32 + 8 * (r >> 2) + (r & 3) < have;
-#pragma unroll
-          for (int y = 0; y < S::WB; y++) acc[b][y][r] = in ? acc[b][y][r] : -INFINITY;
-        }
+      for (int y = 0; y < S::WB; y++)
+        each<S>(acc, y, [&](int c, float v) { return c < have ? v : -INFINITY; });
     }
 #pragma unroll
     for (int y = 0; y < S::WB; y++) {
       const uint32_t i = i0 + y * 32;
       const uint32_t lab = i < a.n ? a.labels[i] : NO_LABEL;
-      uint32_t own = lab - j0 - 4 * h;  // the label's column of the lane's, if it has it
-      asm volatile("" : "+v"(own));
-      float m = -INFINITY, z = 0.f;
-      bool mine = false;
+      const uint32_t own = lab - j0 - 4 * h;  // the label's column of the lane's, if it has it
+      const bool mine = lab < a.k && own < S::WA * 32 && !(own & 4);
+      if (__any(mine)) {
+        const float z = at_column<S>(acc, y, own) * scale;
+        if (mine) a.zlabel[i] = z;
+      }
+      float m = -INFINITY;
 #pragma unroll
       for (int b = 0; b < S::WA; b++)
 #pragma unroll
-        for (int r = 0; r < 16; r++) {
-          const bool is = own == (uint32_t)(b * 32 + 8 * (r >> 2) + (r & 3));
-          z = is ? acc[b][y][r] : z;
-          mine = mine || is;
+        for (int r = 0; r < 16; r++)
           m = fmaxf(m, acc[b][y][r]);  // (passes over NaN: the sum keeps it)
-        }
-      if (mine && lab < a.k) a.zlabel[i] = z;
-      m = fmaxf(m, __shfl_xor(m, 32, 64));
+      m = fmaxf(m, __shfl_xor(m, 32, 64)) * scale;
       const float mm = m == -INFINITY ? 0.f : m;
       float s = 0.f;
 #pragma unroll
       for (int b = 0; b < S::WA; b++)
 #pragma unroll
-        for (int r = 0; r < 16; r++) s += exp_of(acc[b][y][r], mm);
+        for (int r = 0; r < 16; r++) s += exp_of(acc[b][y][r], scale, mm);
       s += __shfl_xor(s, 32, 64);
       if (h == 0 && i < a.n) a.part[(size_t)pi * a.n + i] = make_float2(m, s);
     }
   } else {
-    // G in place of the logits.
+    // G in place of the sums.
 #pragma unroll
     for (int y = 0; y < S::WB; y++) {
       const uint32_t i = i0 + y * 32;
@@ -113,21 +144,21 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_logits(const LogitArgs a) {
       const uint32_t lab = i < a.n ? a.labels[ic] : NO_LABEL;
       const bool has = lab < a.k;
       const float lse = a.lse[ic];
-      const float u = a.gloss ? a.gloss[ic] : 1.f;
       // The label's column (another piece's: none of this one), and the columns
       // there are, none in a row without a label, from the lane's first.
       uint32_t own = lab - a.col0 - j0 - 4 * h;
       int have = (has ? left : 0) - 4 * h;
       asm volatile("" : "+v"(own), "+v"(have));
-#pragma unroll
-      for (int b = 0; b < S::WA; b++)
-#pragma unroll
-        for (int r = 0; r < 16; r++) {
-          const int c = b * 32 + 8 * (r >> 2) + (r & 3);
-          const float soft = exp_of(acc[b][y][r], lse);
-          const float g = (soft - (own == (uint32_t)c ? 1.f : 0.f)) * u;
-          acc[b][y][r] = c < have ? g : 0.f;
-        }
+      each<S>(acc, y, [&](int, float v) { return exp_of(v, scale, lse); });
+      // (Where there are many classes, few waves have a row's label.)
+      if (__any(own < S::WA * 32))
+        each<S>(acc, y, [&](int c, float v) { return own == (uint32_t)c ? v - 1.f : v; });
+      if (__builtin_expect(a.gloss != nullptr, 0)) {
+        const float u = a.gloss[ic];
+        each<S>(acc, y, [&](int, float v) { return v * u; });
+      }
+      if (__builtin_expect(__any(!has) || !full, 0))
+        each<S>(acc, y, [&](int c, float v) { return c < have ? v : 0.f; });
     }
     // Through LDS (the ring is free once every wave is here), so that a row's
     // 2 TC bytes go to memory together: eight columns a lane are one 16-byte chunk,
@@ -150,43 +181,32 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_logits(const LogitArgs a) {
       for (int y = 0; y < S::WB; y++) {
         int ga = 0;
         if constexpr (F32)
-          ga = one ? ex[y] + rs.gexp : row_exp(a.gloss, min(i0 + y * 32, a.n - 1));
+          ga = (one ? ex[y] + rs.gexp : row_exp(a.gloss, min(i0 + y * 32, a.n - 1))) - ewmax;
         const uint32_t row = r0 + y * 32;
 #pragma unroll
         for (int b = 0; b < S::WA; b++)
 #pragma unroll
           for (int p = 0; p < 2; p++) {
-            float lo[4], hi[4], g[8];
+            float g[2][4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-              lo[e] = acc[b][y][8 * p + e];
-              hi[e] = acc[b][y][8 * p + 4 + e];
-            }
-            eight(lo, hi, g);
-            if constexpr (F32) {
-              int by[8];
-              if (plane < 2) {
-                const uint32_t j = j0 + b * 32 + 16 * p + 8 * h;
-                const int4 w0 = *reinterpret_cast<const int4*>(a.ew + j);
-                const int4 w1 = *reinterpret_cast<const int4*>(a.ew + j + 4);
-                const int ew[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-#pragma unroll
-                for (int e = 0; e < 8; e++) by[e] = ew[e] - ewmax + ga;
-              } else {
-#pragma unroll
-                for (int e = 0; e < 8; e++) by[e] = ex[y] + rs.gexp;
+            for (int f = 0; f < 2; f++) {
+              int by[4] = {rs.gexp, rs.gexp, rs.gexp, rs.gexp};
+              if (F32 && plane < 2) {
+                const int4 v = four_exps(a.ew, j0 + b * 32 + 8 * (2 * p + f) + 4 * h);
+                by[0] = v.x + ga, by[1] = v.y + ga, by[2] = v.z + ga, by[3] = v.w + ga;
+              } else if (F32) {
+                by[0] = by[1] = by[2] = by[3] = ex[y] + rs.gexp;
               }
 #pragma unroll
-              for (int e = 0; e < 8; e++) {
-                const float t = ldexpf(g[e], by[e]);
-                g[e] = plane & 1 ? t - (float)(f16)t : t;
+              for (int e = 0; e < 4; e++) {
+                float t = acc[b][y][4 * (2 * p + f) + e];
+                if constexpr (__is_same(T, f16)) t = ldexpf(t, by[e]);
+                g[f][e] = F32 && (plane & 1) ? t - (float)(f16)t : t;
               }
-            } else if constexpr (__is_same(T, f16)) {
-#pragma unroll
-              for (int e = 0; e < 8; e++) g[e] = ldexpf(g[e], rs.gexp);
             }
             const uint32_t chunk = (wc * S::WA + b) * 4 + 2 * p + h;
-            store_vec(reinterpret_cast<T*>(ring + row * S::TC * 2 + ((chunk ^ (row & 7)) << 4)), g);
+            store_vec(reinterpret_cast<T*>(ring + row * S::TC * 2 + ((chunk ^ (row & 7)) << 4)),
+                      eight_of<T>(g[0], g[1]));
           }
       }
       __syncthreads();
