@@ -20,6 +20,8 @@
 // row of each 32 x 32 block and four consecutive columns at a time.
 #pragma once
 
+#include <algorithm>
+
 #include "emh_dma.h"
 #include "emh_learn.h"
 #include "emh_types.h"
@@ -94,9 +96,33 @@ struct TileIn {
   uint32_t slabs;   // of the depth; one operand is zero past it
   uint32_t passes;  // 1, or 3: planes (0, 0), (0, 1), (1, 0)
   uint32_t rtiles, ctiles, splits;  // workgroups: rtiles ctiles splits
+  // What a workgroup finds its tile by (prepare): divisions there, by whole words,
+  // were 300 instructions that every workgroup of a launch met cold.
+  uint32_t blocks, steps;  // all workgroups; steps of a split (the first `more`: one more)
+  uint32_t more;
+  uint32_t by_split, by_group, by_tail;
 };
+constexpr uint32_t GROUP = 8;  // row tiles taken together (tile_at)
+// floor(v / by) as umulhi(v, m), which is that or one more (v below 2^31, by > 1).
+inline uint32_t recip(uint32_t by) { return (uint32_t)((uint64_t(1) << 32) / by + 1); }
+inline unsigned prepare(TileIn& t) {
+  const uint32_t steps = t.slabs * t.passes;
+  t.blocks = t.rtiles * t.ctiles * t.splits;
+  t.steps = steps / t.splits;
+  t.more = steps % t.splits;
+  t.by_split = recip(t.rtiles * t.ctiles);
+  t.by_group = recip(GROUP * t.ctiles);
+  t.by_tail = recip(std::max(1u, t.rtiles % GROUP));
+  return t.blocks;
+}
 
 namespace {
+
+__device__ __forceinline__ uint32_t quotient(uint32_t v, uint32_t by, uint32_t m) {
+  if (by == 1) return v;
+  const uint32_t q = __umulhi(v, m);
+  return q * by > v ? q - 1 : q;
+}
 
 // Which tile, and which steps (pass, slab) of it, a workgroup takes.
 struct TileAt {
@@ -107,22 +133,20 @@ struct TileAt {
 // other, so that what its 32 CUs read at a time is a few row and column
 // slabs, shared in its L2.
 __device__ __forceinline__ TileAt tile_at(const TileIn& t) {
-  const uint32_t nb = gridDim.x, bid = blockIdx.x;
+  const uint32_t nb = t.blocks, bid = blockIdx.x;
   const uint32_t xcd = bid & 7, q = bid >> 3, m = nb >> 3, rem = nb & 7;
   uint32_t wi = xcd * m + min(xcd, rem) + q;
   TileAt a;
   const uint32_t tiles = t.rtiles * t.ctiles;
-  a.split = wi / tiles;
+  a.split = quotient(wi, tiles, t.by_split);
   wi -= a.split * tiles;
-  constexpr uint32_t GROUP = 8;
-  const uint32_t per = GROUP * t.ctiles, g = wi / per;
+  const uint32_t per = GROUP * t.ctiles, g = quotient(wi, per, t.by_group);
   const uint32_t have = min(GROUP, t.rtiles - g * GROUP);
   wi -= g * per;
-  a.ct = wi / have;
-  a.rt = g * GROUP + wi % have;
-  const uint32_t steps = t.slabs * t.passes;
-  a.s0 = (uint32_t)((uint64_t)steps * a.split / t.splits);
-  a.s1 = (uint32_t)((uint64_t)steps * (a.split + 1) / t.splits);
+  a.ct = have == GROUP ? wi / GROUP : quotient(wi, have, t.by_tail);
+  a.rt = g * GROUP + wi - a.ct * have;
+  a.s0 = a.split * t.steps + min(a.split, t.more);
+  a.s1 = a.s0 + t.steps + (a.split < t.more ? 1 : 0);
   return a;
 }
 
@@ -221,7 +245,8 @@ __device__ __forceinline__ void tile_sums(const TileIn& t, const TileAt& at, cha
 
   // Load cursor: pass, slab and stage of the next DMAs; past the last step it
   // stays there, and what it fetches again nothing reads.
-  uint32_t lpass = at.s0 / t.slabs, lslab = at.s0 % t.slabs, lleft = at.s1 - at.s0, lst = 0;
+  uint32_t lpass = 0, lslab = at.s0, lleft = at.s1 - at.s0, lst = 0;
+  while (lslab >= t.slabs) lslab -= t.slabs, lpass++;
   auto dma = [&](int q) __attribute__((always_inline)) {
     if (q < S::RD)
       R.dma(q, t.r.p[lpass == 2 ? 1 : 0] + r0, t.r, lslab,

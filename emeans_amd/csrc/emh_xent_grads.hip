@@ -7,10 +7,11 @@ namespace {
 template <class T, class S, bool F32, bool DW, class O>
 __global__ __launch_bounds__(S::THREADS, 2) void k_grads(const ProdArgs a) {
   __shared__ __attribute__((aligned(1024))) char ring[S::RING];
+  const bool alt = DW && a.flag && *a.flag == a.call;
   const TileAt at = tile_at(a.t);
   v16f acc[S::WA][S::WB];
   TileIn t = a.t;
-  if (DW && a.flag && *a.flag == a.call) t.c = a.alt;
+  if (alt) t.c = a.alt;
   bool one = false;
   if constexpr (F32) {
     one = a.st->one != 0;
@@ -93,10 +94,10 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_grads(const ProdArgs a) {
 }
 
 template <class T, bool F32, class O>
-void launch(hipStream_t s, const ProdArgs& a, Tile tile) {
+void launch(hipStream_t s, ProdArgs a, Tile tile) {
+  const unsigned blocks = prepare(a.t);
   by_tile(tile, [&](auto shape) {
     using S = decltype(shape);
-    const unsigned blocks = a.t.rtiles * a.t.ctiles * a.t.splits;
     if (a.dw)
       k_grads<T, S, F32, true, O><<<blocks, S::THREADS, 0, s>>>(a);
     else

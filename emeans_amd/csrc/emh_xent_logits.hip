@@ -9,7 +9,7 @@ namespace {
 template <class T>
 __device__ __forceinline__ void copy_rows(const LogitArgs& a) {
   const OddRows& o = a.odd;
-  for (uint32_t i = blockIdx.x; i < a.n; i += gridDim.x) {
+  for (uint32_t i = blockIdx.x; i < a.n; i += a.t.blocks) {
     const T* row = reinterpret_cast<const T*>(o.x) + i * o.ld;
     const bool has = a.labels[i] < a.k;
     for (uint32_t c = threadIdx.x * 8; c < o.dp; c += blockDim.x * 8) {
@@ -223,10 +223,11 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_logits(const LogitArgs a) {
 }
 
 template <class T, bool F32, bool GRAD>
-void launch(hipStream_t s, const LogitArgs& a, Tile tile) {
+void launch(hipStream_t s, LogitArgs a, Tile tile) {
+  const unsigned blocks = prepare(a.t);
   by_tile(tile, [&](auto shape) {
     using S = decltype(shape);
-    k_logits<T, S, F32, GRAD><<<a.t.rtiles * a.t.ctiles, S::THREADS, 0, s>>>(a);
+    k_logits<T, S, F32, GRAD><<<blocks, S::THREADS, 0, s>>>(a);
   });
 }
 
