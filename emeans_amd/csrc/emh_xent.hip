@@ -188,24 +188,45 @@ __global__ __launch_bounds__(1024) void k_survey(const T* x, size_t ld, uint32_t
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 
+// One chunk of 16 classes (a) and 16 rows (b).
+__device__ __forceinline__ v4f mfma_few(const Vec<float>& a, const Vec<float>& b, v4f c) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.get(e), b.get(e), c, 0, 0, 0);
+  return c;
+}
+__device__ __forceinline__ v4f mfma_few(const Vec<f16>& a, const Vec<f16>& b, v4f c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a.raw),
+                                                __builtin_bit_cast(v8h, b.raw), c, 0, 0, 0);
+}
+__device__ __forceinline__ v4f mfma_few(const Vec<bf16>& a, const Vec<bf16>& b, v4f c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a.raw),
+                                                 __builtin_bit_cast(v8bf, b.raw), c, 0, 0, 0);
+}
+
 // Few rows (at most 16 R) against all classes, the operands read as they lie, once:
-// a workgroup takes 16 classes at a time, its four waves a quarter of the depth
+// a workgroup takes 16 C classes at a time, its four waves a quarter of the depth
 // each (every fourth 64 bytes of a row), with 16 x 16 MFMAs, the classes as their A: a
 // lane then holds four classes of one row. f32 in f32 MFMAs. The workgroup's maximum
 // and sum of its classes go to part[row][workgroup].
-// Bound by the classes' bytes from HBM, or by latency: 16 rows of 384 against
-// 256 classes are 25 KB a CU.
-template <class T, int R>
+// Bound by the classes' bytes from HBM (16 rows of 1,024 against 131,071 classes in
+// bf16 48 us with the join, 5.6 TB/s), or by latency: 16 rows of 384 against 256 classes
+// are 25 KB a CU and take 5.4 us, the join 3.2.
+// Many waves do more than many loads of one: with eight chunks in flight, 16 rows of
+// 384 against 20,000 took 15.0 us, now 10.0. C = 4 where there are classes enough for
+// every CU: the rows' loads, which are as many as the classes' with C = 1, are shared
+// (16 rows by 131,071: 64.8 us before, 64 rows 150, now 74; but 64 classes at a time,
+// 16 by 4,096, take 9.8 us and 16 at a time 7.5).
+template <class T, int R, int C>
 __global__ __launch_bounds__(256) void k_few(const T* __restrict__ x, size_t ldx, uint32_t n,
                                              uint32_t d, const T* __restrict__ w, size_t ldw,
                                              uint32_t k, const uint32_t* __restrict__ labels,
                                              float scale, float2* part, float* zlabel) {
   constexpr int N = VecOf<T>::N, DEEP = 4 * N;  // a chunk: DEEP of the depth, N a lane
-  constexpr int U = R == 4 ? 4 : 8;             // chunks in flight
-  __shared__ v4f sum[4][R][64];
+  constexpr int U = C == 1 && R < 4 ? 2 : 1;    // chunks a wave has in flight
+  __shared__ v4f sum[4][R][C][64];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint32_t l = lane & 15, q = lane >> 4;
-  const uint32_t groups = (k + 15) / 16, chunks = (d + DEEP - 1) / DEEP;
+  const uint32_t groups = (k + 16 * C - 1) / (16 * C), chunks = (d + DEEP - 1) / DEEP;
   float m = -INFINITY, s = 0.f;  // of the row that this lane keeps (wave r: rows 16 r ..)
   const uint32_t mine = wave * 16 + l;
   const uint32_t lab = wave < R && mine < n ? labels[mine] : NO_LABEL;
@@ -216,60 +237,61 @@ __global__ __launch_bounds__(256) void k_few(const T* __restrict__ x, size_t ldx
     return load_some(at + min(col, d), (int)d - (int)col);
   };
   for (uint32_t g = blockIdx.x; g < groups; g += gridDim.x) {
-    v4f acc[R];
+    v4f acc[R][C];
 #pragma unroll
-    for (int r = 0; r < R; r++) acc[r] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int r = 0; r < R; r++)
+#pragma unroll
+      for (int i = 0; i < C; i++) acc[r][i] = v4f{0.f, 0.f, 0.f, 0.f};
     for (uint32_t c0 = wave; c0 < chunks; c0 += 4 * U) {
       // (Past the last chunk it is read again, and not used: no load waits for a branch.)
-      Vec<T> a[U], b0[U];
+      Vec<T> a[U][C], b[U][R];
 #pragma unroll
       for (int u = 0; u < U; u++) {
         const uint32_t c = min(c0 + 4 * u, chunks - 1);
-        a[u] = fetch(w, ldw, g * 16 + l, k, c);
-        b0[u] = fetch(x, ldx, l, n, c);
+#pragma unroll
+        for (int i = 0; i < C; i++) a[u][i] = fetch(w, ldw, (g * C + i) * 16 + l, k, c);
+#pragma unroll
+        for (int r = 0; r < R; r++) b[u][r] = fetch(x, ldx, r * 16 + l, n, c);
       }
 #pragma unroll
       for (int u = 0; u < U; u++) {
         if (c0 + 4 * u >= chunks) continue;
 #pragma unroll
-        for (int r = 0; r < R; r++) {
-          const Vec<T> b = r == 0 ? b0[u] : fetch(x, ldx, r * 16 + l, n, c0 + 4 * u);
-          if constexpr (sizeof(T) == 4) {
+        for (int r = 0; r < R; r++)
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-              acc[r] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[u].get(e), b.get(e), acc[r], 0, 0, 0);
-          } else if constexpr (__is_same(T, f16)) {
-            acc[r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a[u].raw),
-                                                            __builtin_bit_cast(v8h, b.raw), acc[r], 0, 0, 0);
-          } else {
-            acc[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a[u].raw),
-                                                             __builtin_bit_cast(v8bf, b.raw), acc[r], 0, 0, 0);
-          }
-        }
+          for (int i = 0; i < C; i++) acc[r][i] = mfma_few(a[u][i], b[u][r], acc[r][i]);
       }
     }
     __syncthreads();  // the last group's sums have been read
 #pragma unroll
-    for (int r = 0; r < R; r++) sum[wave][r][lane] = acc[r];
+    for (int r = 0; r < R; r++)
+#pragma unroll
+      for (int i = 0; i < C; i++) sum[wave][r][i][lane] = acc[r][i];
     __syncthreads();
     if (wave >= R) continue;
-    v4f z = sum[0][wave][lane];
-#pragma unroll
-    for (int i = 1; i < 4; i++) z += sum[i][wave][lane];
+    v4f z[C];
     float top = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const uint32_t j = g * 16 + q * 4 + e;
-      z[e] = j < k ? z[e] * scale : -INFINITY;
-      if (j == lab && j < k) zlabel[mine] = z[e];
-      top = fmaxf(top, z[e]);  // (passes over NaN: the sum keeps it)
+    for (int i = 0; i < C; i++) {
+      z[i] = sum[0][wave][i][lane];
+#pragma unroll
+      for (int o = 1; o < 4; o++) z[i] += sum[o][wave][i][lane];
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const uint32_t j = (g * C + i) * 16 + q * 4 + e;
+        z[i][e] = j < k ? z[i][e] * scale : -INFINITY;
+        if (j == lab && j < k) zlabel[mine] = z[i][e];
+        top = fmaxf(top, z[i][e]);  // (passes over NaN: the sum keeps it)
+      }
     }
     top = fmaxf(top, __shfl_xor(top, 16, 64));
     top = fmaxf(top, __shfl_xor(top, 32, 64));
     const float b = fmaxf(m, top), bb = b == -INFINITY ? 0.f : b;
     s *= exp_of(m, bb);
 #pragma unroll
-    for (int e = 0; e < 4; e++) s += exp_of(z[e], bb);
+    for (int i = 0; i < C; i++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) s += exp_of(z[i][e], bb);
     m = b;
   }
   if (wave >= R) return;
@@ -419,13 +441,19 @@ void pack(emh_ctx* c, const XentIn& in, const Laid& x, const Laid& w, const uint
     k_pack16<f16><<<dim3(blocks), 256, 0, c->stream>>>(a);
 }
 
-// At most this many rows take the kernel that reads the classes once, as they lie.
+// At most this many rows take the kernel that reads the classes once, as they lie. (64
+// rows of 768 in bf16 by 16,384 classes 12.8 us, in tiles 14.0; by 131,071 56.7 and 53.0;
+// f32, which the tiles have laid out first, by 65,536 87 and 129.)
 constexpr size_t FEW_ROWS = 64;
 constexpr uint32_t FEW_BLOCKS = 2048;
 template <class T>
 void few(emh_ctx* c, const XentIn& in, float* loss, float* lse) {
   const uint32_t n = (uint32_t)in.n, k = (uint32_t)in.k;
-  const uint32_t blocks = std::min((k + 15) / 16, FEW_BLOCKS);
+  // 16 of 768 in bf16 by 8,192: 9.8 us wide, 8.8 not; by 16,384: 9.7 and 11.2. One row,
+  // which stays in the L1: by 16,384 10.1 and 9.1, f32 by 65,536 37.3 and 40.4.
+  const bool wide = k >= (n > 4 ? 16384u : 65536u);
+  const uint32_t per = wide ? 64 : 16;
+  const uint32_t blocks = std::min((k + per - 1) / per, FEW_BLOCKS);
   char* ws = (char*)c->xent.get((size_t)blocks * n * sizeof(float2) + n * 4);
   float2* part = (float2*)ws;
   float* zlabel = (float*)(part + (size_t)blocks * n);
@@ -435,11 +463,11 @@ void few(emh_ctx* c, const XentIn& in, float* loss, float* lse) {
                                                 in.scale, part, zlabel);
   };
   if (n <= 16)
-    run(k_few<T, 1>);
+    wide ? run(k_few<T, 1, 4>) : run(k_few<T, 1, 1>);
   else if (n <= 32)
-    run(k_few<T, 2>);
+    wide ? run(k_few<T, 2, 4>) : run(k_few<T, 2, 1>);
   else
-    run(k_few<T, 4>);
+    wide ? run(k_few<T, 4, 4>) : run(k_few<T, 4, 1>);
   // (A launch of its own: the fence and the ticket that let the last workgroup join
   // the parts cost 70 us with 1,024 workgroups, 6 with 16.)
   k_join_few<<<dim3(n), 256, 0, c->stream>>>(part, blocks, in.labels, k, zlabel, loss, lse, c->small);

@@ -117,6 +117,20 @@ def test_every_tile_shape(dev, n, d, k, name):
     Run(dev, x, w, lab, name).check()
 
 
+# Few rows, so many classes that several are taken together, at either side of the
+# sizes where they are.
+FEW = [(1, 40, 65_537), (4, 37, 65_536), (4, 33, 65_535), (5, 64, 16_384), (5, 64, 16_383),
+       (16, 33, 20_001), (30, 48, 17_001), (50, 20, 16_999), (64, 64, 16_401)]
+
+
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n,d,k", FEW)
+def test_few_rows_many_classes(dev, n, d, k, name):
+    x, w, lab = _inputs(n, d, k, n + d + k)
+    lab[0] = k - 1
+    Run(dev, x, w, lab, name, scale=1.5, pad=n % 2, off=d % 2, grad=False).check()
+
+
 @pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("n,d,k", [(9, 40, 70), (270, 64, 300), (100, 33, 513)])
 @pytest.mark.parametrize("pad,off", [(0, 1), (3, 0), (8, 5)])
