@@ -60,6 +60,24 @@ __device__ __forceinline__ Vec<T> load_vec(const T* p) {
   const Any16 a = *reinterpret_cast<const Any16*>(p);
   return Vec<T>{make_uint4(a.w[0], a.w[1], a.w[2], a.w[3])};
 }
+// The same of a 16-bit type where addresses may be odd multiples of two bytes, by whole
+// words: lanes apart from each other are served a word at a time there otherwise.
+// (What the words hold besides is not used; each holds an element of p's.)
+template <class T>
+__device__ __forceinline__ Vec<T> load_vec_words(const T* p) {
+  static_assert(sizeof(T) == 2, "16 bits");
+  const uint32_t odd = (uint32_t)(uintptr_t)p & 2;
+  const T* from = reinterpret_cast<const T*>((uintptr_t)p - odd);
+  struct __attribute__((packed, aligned(4))) Words {
+    uint32_t w[4];
+  };
+  const Words a = *reinterpret_cast<const Words*>(from);
+  const uint32_t last = *reinterpret_cast<const uint32_t*>(from + (odd ? 8 : 6));
+  const uint32_t by = odd * 8;
+  return Vec<T>{make_uint4(
+      __builtin_amdgcn_alignbit(a.w[1], a.w[0], by), __builtin_amdgcn_alignbit(a.w[2], a.w[1], by),
+      __builtin_amdgcn_alignbit(a.w[3], a.w[2], by), __builtin_amdgcn_alignbit(last, a.w[3], by))};
+}
 // The elements p[0 .. left), left < N; the others zero.
 template <class T>
 __device__ __forceinline__ Vec<T> load_some(const T* p, int left) {

@@ -3,6 +3,7 @@
 // (emh_xent.h), the operands laid out for them, and the joins of their parts.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "emh_xent.h"
 
@@ -216,7 +217,8 @@ __device__ __forceinline__ v4f mfma_few(const Vec<bf16>& a, const Vec<bf16>& b, 
 // every CU: the rows' loads, which are as many as the classes' with C = 1, are shared
 // (16 rows by 131,071: 64.8 us before, 64 rows 150, now 74; but 64 classes at a time,
 // 16 by 4,096, take 9.8 us and 16 at a time 7.5).
-template <class T, int R, int C>
+// ODD: rows may begin at odd multiples of two bytes.
+template <class T, int R, int C, bool ODD>
 __global__ __launch_bounds__(256) void k_few(const T* __restrict__ x, size_t ldx, uint32_t n,
                                              uint32_t d, const T* __restrict__ w, size_t ldw,
                                              uint32_t k, const uint32_t* __restrict__ labels,
@@ -233,7 +235,11 @@ __global__ __launch_bounds__(256) void k_few(const T* __restrict__ x, size_t ldx
   auto fetch = [&](const T* p, size_t ld, uint32_t row, uint32_t rows, uint32_t c) __attribute__((always_inline)) {
     const T* at = p + (size_t)min(row, rows - 1) * ld;
     const uint32_t col = c * DEEP + q * N;
-    if (col + N <= d) return load_vec(at + col);
+    if constexpr (ODD) {
+      if (col + N <= d) return load_vec_words(at + col);
+    } else {
+      if (col + N <= d) return load_vec(at + col);
+    }
     return load_some(at + min(col, d), (int)d - (int)col);
   };
   for (uint32_t g = blockIdx.x; g < groups; g += gridDim.x) {
@@ -462,12 +468,22 @@ void few(emh_ctx* c, const XentIn& in, float* loss, float* lse) {
                                                 (const T*)in.w.p, in.w.ld, k, in.labels,
                                                 in.scale, part, zlabel);
   };
-  if (n <= 16)
-    wide ? run(k_few<T, 1, 4>) : run(k_few<T, 1, 1>);
-  else if (n <= 32)
-    wide ? run(k_few<T, 2, 4>) : run(k_few<T, 2, 1>);
-  else
-    wide ? run(k_few<T, 4, 4>) : run(k_few<T, 4, 1>);
+  auto shaped = [&](auto odd) {
+    constexpr bool ODD = decltype(odd)::value;
+    if (n <= 16)
+      wide ? run(k_few<T, 1, 4, ODD>) : run(k_few<T, 1, 1, ODD>);
+    else if (n <= 32)
+      wide ? run(k_few<T, 2, 4, ODD>) : run(k_few<T, 2, 1, ODD>);
+    else
+      wide ? run(k_few<T, 4, 4, ODD>) : run(k_few<T, 4, 1, ODD>);
+  };
+  auto odd = [](const MatIn& m) { return m.ld % 2 != 0 || (uintptr_t)m.p % 4 != 0; };
+  if constexpr (sizeof(T) == 2) {
+    // (57 rows of 641 in bf16 by 59,673: 71 us without, 44 with.)
+    odd(in.x) || odd(in.w) ? shaped(std::true_type{}) : shaped(std::false_type{});
+  } else {
+    shaped(std::false_type{});
+  }
   // (A launch of its own: the fence and the ticket that let the last workgroup join
   // the parts cost 70 us with 1,024 workgroups, 6 with 16.)
   k_join_few<<<dim3(n), 256, 0, c->stream>>>(part, blocks, in.labels, k, zlabel, loss, lse, c->small);

@@ -117,6 +117,16 @@ def test_every_tile_shape(dev, n, d, k, name):
     Run(dev, x, w, lab, name).check()
 
 
+# 16-bit rows and classes at every alignment that an element may have, at either side of
+# the last vector's end.
+@pytest.mark.parametrize("name", ["f16", "bf16"])
+@pytest.mark.parametrize("d", [8, 31, 32, 33, 39, 41, 65, 127])
+@pytest.mark.parametrize("pad,off", [(0, 0), (0, 1), (1, 2), (1, 3)])
+def test_few_rows_at_any_alignment(dev, name, d, pad, off):
+    x, w, lab = _inputs(11 + 3 * d % 50, d, 83, d)
+    Run(dev, x, w, lab, name, pad=pad, off=off, grad=False).check()
+
+
 # Few rows, so many classes that several are taken together, at either side of the
 # sizes where they are.
 FEW = [(1, 40, 65_537), (4, 37, 65_536), (4, 33, 65_535), (5, 64, 16_384), (5, 64, 16_383),
