@@ -76,6 +76,7 @@ typedef TileShape<2, 2, 2, 2> TileS;  // 128 x 128, 4 waves (two workgroups a CU
 enum Tile : int { TILE_L, TILE_M, TILE_S, TILES };
 constexpr uint32_t TILE_ROWS[TILES] = {TileL::TR, TileM::TR, TileS::TR};
 constexpr uint32_t TILE_COLS[TILES] = {TileL::TC, TileM::TC, TileS::TC};
+constexpr uint32_t TILE_WAVES[TILES] = {TileL::NWR, TileM::NWR, TileS::NWR};  // down the rows
 // Rows and columns of whole tiles of any shape.
 constexpr uint32_t ALL_ROWS = 256, ALL_COLS = 768;
 static_assert(ALL_ROWS % TileL::TR == 0 && ALL_ROWS % TileM::TR == 0 && ALL_ROWS % TileS::TR == 0 &&

@@ -62,13 +62,13 @@ struct XentState {
 };
 constexpr int XENT_SPAN = 8;
 // Rows without a label have zeros in G, which silence any finite value of x in dw.
-// f32 rows are laid out for the call anyway, and are made zeros there. 16-bit rows
-// that the tiles can read as they lie are looked at (k_survey): only when one
-// without a label holds a value that is not finite, which the call's number in
-// `flag` then says, the kernel of the logits makes the copy `rows` of x with
-// zeros in their place, and dw reads that.
+// f32 rows are laid out for the call anyway, and are made zeros there. Of 16-bit rows
+// that the tiles can read as they lie the kernel of the logits looks at a logit: where
+// a row holds a value that is not finite, none of its logits is. Only when one without
+// a label is so, which the call's number in `flag` then says, dx's kernel (or one of its
+// own) makes the copy `rows` of x with zeros in their place, and dw reads that.
 struct OddRows {
-  const uint32_t* flag;  // null: nothing to do
+  uint32_t* flag;  // null: nothing to do
   uint32_t call;
   char* rows;
   uint32_t dp;           // elements of a row there
@@ -91,7 +91,9 @@ struct LogitArgs {
   const float* lse; // gradients
   const float* gloss;
   const XentState* st;
-  OddRows odd;
+  uint32_t* counts; // or null: [row tile][wave of it] rows with a label (RowScale)
+  uint32_t* small;
+  OddRows odd;      // flag and call
   char* g[4];       // G; f32: the planes of G' or Ga, and of Gb
   size_t ldg;       // bytes (rows and columns to full tiles)
 };
@@ -105,6 +107,9 @@ struct ProdArgs {
   uint32_t k;
   const float* gloss;
   const XentState* st;
+  const uint32_t* counts;  // or null: as in LogitArgs
+  uint32_t ncounts;
+  OddRows odd;          // dx: the copy to make
   const int* ex;        // f32: as in LogitArgs (dx: of the rows, dw: of the classes)
   const char* gb[2];    // f32, dw: Gb's planes (t.r: those of G')
   float scale;
@@ -118,16 +123,41 @@ struct ProdArgs {
   Operand alt;
 };
 void launch_prod(hipStream_t s, const ProdArgs& a, int kind, Tile tile);
+void launch_copy_rows(emh_ctx* c, const OddRows& o, uint32_t n, const uint32_t* labels, uint32_t k);
 
-// A row's weight in G, the powers of two of G (see above) and the factor left for the
-// results: all from the call's state.
+// The powers of two of G (see above), and the factor left for the results, from the
+// call's state. A mean over rows of 16 bits has all weights 1 in G and needs nothing of
+// its rows but how many have a label: the kernel of the logits counts them on the way,
+// in MANY_COUNTS words at most, which the products' workgroups add. (k_survey would be
+// a launch, 5 us of 139 at 16,384 x 768 by 1,024.)
+constexpr uint32_t MANY_COUNTS = 512;
 struct RowScale {
-  float by;   // scale, and without gloss 1 / rows with a label
-  int gexp;   // f16: G's exponent; f32: gb
-  __device__ __forceinline__ void init(const XentState* st, const float* gloss, float scale) {
-    const uint32_t c = st->count;
-    by = gloss ? scale : c ? scale / (float)c : 0.f;
-    gexp = st->uexp ? 14 - (st->uexp - XENT_BIAS + 1) : 0;  // |weight_i| 2^ex_i < 2^(uexp + 1)
+  // f16: G's exponent; f32: gb.
+  static __device__ __forceinline__ int exponent(const XentState* st, const uint32_t* counts) {
+    if (counts) return 13;
+    return st->uexp ? 14 - (st->uexp - XENT_BIAS + 1) : 0;  // |weight_i| 2^ex_i < 2^(uexp + 1)
+  }
+  // scale, and without gloss 1 / rows with a label. By whole waves.
+  static __device__ __forceinline__ float factor(const XentState* st, const uint32_t* counts,
+                                                 uint32_t ncounts, const float* gloss,
+                                                 float scale) {
+    if (gloss) return scale;
+    uint32_t c = 0;
+    if (counts) {
+      const uint32_t i = (threadIdx.x & 63) * 4;  // (the buffer holds MANY_COUNTS)
+      static_assert(MANY_COUNTS == 512, "two loads a lane");
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const uint4 v = *reinterpret_cast<const uint4*>(counts + h * 256 + i);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 4; e++) c += h * 256 + i + e < ncounts ? w[e] : 0u;
+      }
+      for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o, 64);
+    } else {
+      c = st->count;
+    }
+    return c ? scale / (float)c : 0.f;
   }
 };
 // The exponent that brings a row's weight below 2^14.

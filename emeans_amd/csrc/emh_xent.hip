@@ -112,38 +112,16 @@ __global__ __launch_bounds__(256) void k_pack32(const PackArgs a) {
   if (lane == 0) m.ex[i] = e0;
 }
 
-// The call's state, by workgroup 0 alone (a pass over the labels, and of f32
-// operands over the exponents); the others, for 16-bit rows that are read as they
-// lie (OddRows), look at the rows without a label, a wave at sixteen labels. Bound by
-// latency: 16,384 rows 5.4 us, of f32 7.1. (A workgroup: joining several would take a
-// launch more, or a fence and a ticket, which cost more.)
-template <class T>
-__global__ __launch_bounds__(1024) void k_survey(const T* x, size_t ld, uint32_t n, uint32_t d,
-                                                 const uint32_t* __restrict__ labels, uint32_t k,
-                                                 const float* __restrict__ gloss,
+// The call's state, by one workgroup: a pass over the labels and weights, and of f32
+// operands over the exponents. Bound by latency: 16,384 rows 5.4 us, of f32 7.1. (A
+// workgroup: joining several would take a launch more, or a fence and a ticket, which
+// cost more. Calls that need only how many rows have a label do without: RowScale.)
+__global__ __launch_bounds__(1024) void k_survey(uint32_t n, const uint32_t* __restrict__ labels,
+                                                 uint32_t k, const float* __restrict__ gloss,
                                                  const int* __restrict__ ex,
                                                  const int* __restrict__ ew, XentState* st,
-                                                 uint32_t* small, uint32_t call) {
+                                                 uint32_t* small) {
   const uint32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  if (blockIdx.x > 0) {
-    const uint32_t first = (blockIdx.x - 1) * 256 + w * 16;
-    const bool none = lane < 16 && first + lane < n && labels[first + lane] >= k;
-    unsigned long long left = __ballot(none);
-    bool odd = false;
-    while (left) {
-      const int r = __ffsll((long long)left) - 1;
-      left &= left - 1;
-      const T* row = x + (size_t)(first + r) * ld;
-#pragma unroll 4
-      for (uint32_t c = lane * 8; c < d; c += 512) {
-        const Vec<T> v = c + 8 <= d ? load_vec(row + c) : load_some(row + c, (int)(d - c));
-#pragma unroll
-        for (int q = 0; q < 8; q++) odd = odd || !(fabsf(v.get(q)) < INFINITY);
-      }
-    }
-    if (__ballot(odd) != 0ull && lane == 0) small[SW_ODD_ROW] = call;
-    return;
-  }
   __shared__ int sh[5][16];
   constexpr int MANY = 1 << 20;
   int count = 0, uexp = 0, ewmax = 0, ulow = MANY, ewlow = MANY;
@@ -616,11 +594,13 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
   Carve w;
   Laid lx, lw;
   XentState* st = nullptr;
+  uint32_t* counts = nullptr;
   char* G[4] = {};
   float *partx = nullptr, *partw = nullptr;
   for (int pass = 0; pass < 2; pass++) {
     w.used = 0;
     st = w.take<XentState>(1);
+    counts = w.take<uint32_t>(MANY_COUNTS);
     lx.size(w, in.x, n, d, true);
     lw.size(w, in.w, k, d, !direct(in.w, d, true));
     for (size_t i = 0; i < planes; i++) G[i] = w.take<char>(np * ldg);
@@ -630,18 +610,13 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
   }
   const uint32_t call = ++c->xent_calls;
   pack(c, in, x_as_is ? Laid{} : lx, lw, in.labels);
-  {
-    const dim3 grid(x_as_is ? 1 + (unsigned)((n + 255) / 256) : 1);
-    auto run = [&](auto t) {
-      using T = decltype(t);
-      k_survey<T><<<grid, 1024, 0, c->stream>>>((const T*)in.x.p, in.x.ld, (uint32_t)n, (uint32_t)d,
-                                                in.labels, (uint32_t)k, gloss, lx.ex, lw.ex, st,
-                                                c->small, call);
-    };
-    if (in.x.kind == EMH_BF16)
-      run(bf16{});
-    else
-      run(f16{});  // (f32 rows are laid out: none is looked at)
+  const Plan first = plan_of(n, std::min(piece, k), slabs * passes, c->cus, false);
+  const size_t waves = (size_t)first.rtiles * TILE_WAVES[first.tile];
+  const bool counted = !f32 && !gloss && waves <= MANY_COUNTS;
+  if (!counted) {
+    k_survey<<<dim3(1), 1024, 0, c->stream>>>((uint32_t)n, in.labels, (uint32_t)k, gloss, lx.ex, lw.ex,
+                                              st, c->small);
+    EMH_HIP(hipGetLastError());
   }
   Laid as_is;
   const Laid& xl = x_as_is ? as_is : lx;
@@ -660,14 +635,19 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
     a.scale = in.scale;
     a.ex = lx.ex, a.ew = f32 ? lw.ex + v0 : nullptr;
     a.lse = lse, a.gloss = gloss, a.st = st;
-    if (x_as_is && v0 == 0)
-      a.odd = {c->small + SW_ODD_ROW, call, lx.p[0], lx.dp, (const char*)in.x.p, in.x.ld, d};
+    a.small = c->small;
+    if (counted) a.counts = counts;
+    OddRows odd{};
+    if (x_as_is && dw.p && v0 == 0)
+      odd = {c->small + SW_ODD_ROW, call, lx.p[0], lx.dp, (const char*)in.x.p, in.x.ld, d};
+    a.odd = odd;
     for (int i = 0; i < 4; i++) a.g[i] = G[i];
     a.ldg = ldg;
     launch_logits(c->stream, a, in.x.kind, pg.tile, true);
     ProdArgs p{};
     p.labels = in.labels, p.k = (uint32_t)k;
     p.gloss = gloss, p.st = st, p.scale = in.scale;
+    if (counted) p.counts = counts, p.ncounts = (uint32_t)waves;
     p.t.passes = (uint32_t)passes;
     p.cols = (uint32_t)d, p.ldp = ldp;
     if (dx.p) {
@@ -681,7 +661,10 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
       p.out = dx.p, p.ldo = dx.ld;
       p.part = px_part ? partx : nullptr;
       p.add = v0 > 0;
+      p.odd = odd;
       launch_prod(c->stream, p, in.x.kind, px.tile);
+    } else if (odd.flag) {
+      launch_copy_rows(c, odd, (uint32_t)n, in.labels, (uint32_t)k);
     }
     if (dw.p) {
       p.t.r = {{G[0], G[1]}, (uint32_t)ldg, up(n, SLAB), (uint32_t)gcols};

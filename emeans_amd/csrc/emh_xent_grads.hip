@@ -4,6 +4,27 @@
 namespace emh {
 namespace {
 
+// x with zeros in rows without a label (OddRows): every workgroup of `blocks` its share.
+template <class T>
+__device__ __forceinline__ void copy_rows(const OddRows& o, uint32_t n, const uint32_t* labels,
+                                          uint32_t k, uint32_t blocks) {
+  for (uint32_t i = blockIdx.x; i < n; i += blocks) {
+    const T* row = reinterpret_cast<const T*>(o.x) + i * o.ld;
+    const bool has = labels[i] < k;
+    for (uint32_t c = threadIdx.x * 8; c < o.dp; c += blockDim.x * 8) {
+      Vec<T> v{make_uint4(0u, 0u, 0u, 0u)};
+      if (has && c < o.d)
+        v = c + 8 <= o.d ? load_vec(row + c) : load_some(row + c, (int)(o.d - c));
+      *reinterpret_cast<uint4*>(o.rows + ((size_t)i * o.dp + c) * 2) = v.raw;
+    }
+  }
+}
+// Where no dx is asked for. (16-bit words, whatever they stand for.)
+__global__ __launch_bounds__(256) void k_copy_rows(const OddRows o, uint32_t n,
+                                                   const uint32_t* labels, uint32_t k) {
+  if (*o.flag == o.call) copy_rows<f16>(o, n, labels, k, gridDim.x);
+}
+
 // A tile of dx (rows: G's, as they lie; columns: w's, across) or of dw (both across), or
 // its sums over one split of the depth or one piece of the classes. Bound by the MFMAs
 // (emh_tile.h). In bf16: 16,384 x 768 by 1,024 30 us (dx) and 34 (dw, 16 splits); 8,192
@@ -12,6 +33,10 @@ template <class T, class S, bool F32, bool DW, class O>
 __global__ __launch_bounds__(S::THREADS, 2) void k_grads(const ProdArgs a) {
   __shared__ __attribute__((aligned(1024))) char ring[S::RING];
   const bool alt = DW && a.flag && *a.flag == a.call;
+  if constexpr (!DW && !F32) {
+    if (a.odd.flag && *a.odd.flag == a.odd.call)
+      copy_rows<T>(a.odd, a.rows, a.labels, a.k, a.t.blocks);
+  }
   const TileAt at = tile_at(a.t);
   v16f acc[S::WA][S::WB];
   TileIn t = a.t;
@@ -27,8 +52,8 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_grads(const ProdArgs a) {
   const int wr = w % S::NWR, wc = w / S::NWR;
   const uint32_t i0 = at.rt * S::TR + wr * S::WB * 32 + li;
   const uint32_t j0 = at.ct * S::TC + wc * S::WA * 32;
-  RowScale rs;
-  rs.init(a.st, a.gloss, a.scale);
+  const int gexp = __is_same(T, f16) ? RowScale::exponent(a.st, a.counts) : 0;
+  const float factor = RowScale::factor(a.st, a.counts, a.ncounts, a.gloss, a.scale);
 #pragma unroll
   for (int y = 0; y < S::WB; y++) {
     const uint32_t i = i0 + y * 32;
@@ -38,11 +63,11 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_grads(const ProdArgs a) {
     if constexpr (F32) {
       const int ewmax = a.st->ewmax - XENT_BIAS;
       if (one)
-        by = ewmax - a.ex[i] - rs.gexp;
+        by = ewmax - a.ex[i] - gexp;
       else
-        by = DW ? -rs.gexp : ewmax - row_exp(a.gloss, i);
+        by = DW ? -gexp : ewmax - row_exp(a.gloss, i);
     } else if constexpr (__is_same(T, f16)) {
-      by = -rs.gexp;
+      by = -gexp;
     }
 #pragma unroll
     for (int b = 0; b < S::WA; b++)
@@ -54,7 +79,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_grads(const ProdArgs a) {
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             const float t = acc[b][y][4 * (2 * p + f) + e];
-            v[f][e] = zero ? 0.f : (__is_same(T, f16) ? ldexpf(t, by) : t) * rs.by;
+            v[f][e] = zero ? 0.f : (__is_same(T, f16) ? ldexpf(t, by) : t) * factor;
           }
         if (a.part) {
           // Whole fours: ldp is a multiple of 4.
@@ -110,6 +135,11 @@ void launch(hipStream_t s, ProdArgs a, Tile tile) {
 }
 
 }  // namespace
+
+void launch_copy_rows(emh_ctx* c, const OddRows& o, uint32_t n, const uint32_t* labels, uint32_t k) {
+  k_copy_rows<<<dim3(std::min<uint32_t>(n, (uint32_t)c->cus * 4)), 256, 0, c->stream>>>(o, n, labels, k);
+  EMH_HIP(hipGetLastError());
+}
 
 void launch_prod(hipStream_t s, const ProdArgs& a, int kind, Tile tile) {
   if (kind == EMH_F32)

@@ -5,22 +5,6 @@
 namespace emh {
 namespace {
 
-// x with zeros in rows without a label (OddRows): every workgroup its share.
-template <class T>
-__device__ __forceinline__ void copy_rows(const LogitArgs& a) {
-  const OddRows& o = a.odd;
-  for (uint32_t i = blockIdx.x; i < a.n; i += a.t.blocks) {
-    const T* row = reinterpret_cast<const T*>(o.x) + i * o.ld;
-    const bool has = a.labels[i] < a.k;
-    for (uint32_t c = threadIdx.x * 8; c < o.dp; c += blockDim.x * 8) {
-      Vec<T> v{make_uint4(0u, 0u, 0u, 0u)};
-      if (has && c < o.d)
-        v = c + 8 <= o.d ? load_vec(row + c) : load_some(row + c, (int)(o.d - c));
-      *reinterpret_cast<uint4*>(o.rows + ((size_t)i * o.dp + c) * 2) = v.raw;
-    }
-  }
-}
-
 // f(c, v) in place of every v of the lane's row y, c its column less the lane's
 // first, which is 4 (lane / 32).
 template <class S, class F>
@@ -60,9 +44,6 @@ __device__ __forceinline__ int4 four_exps(const int* ew, uint32_t j) {
 template <class T, class S, bool F32, bool GRAD>
 __global__ __launch_bounds__(S::THREADS, 2) void k_logits(const LogitArgs a) {
   __shared__ __attribute__((aligned(1024))) char ring[S::RING];
-  if constexpr (GRAD && !F32) {
-    if (a.odd.flag && *a.odd.flag == a.odd.call) copy_rows<T>(a);
-  }
   const TileAt at = tile_at(a.t);
   v16f acc[S::WA][S::WB];
   tile_sums<T, S, true, true>(a.t, at, ring, acc);
@@ -141,6 +122,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_logits(const LogitArgs a) {
     }
   } else {
     // G in place of the sums.
+    uint32_t count = 0;
 #pragma unroll
     for (int y = 0; y < S::WB; y++) {
       const uint32_t i = i0 + y * 32;
@@ -148,6 +130,12 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_logits(const LogitArgs a) {
       const uint32_t lab = i < a.n ? a.labels[ic] : NO_LABEL;
       const bool has = lab < a.k;
       const float lse = a.lse[ic];
+      if constexpr (!F32) {
+        count += __popcll(__ballot(has && h == 0));
+        if (a.counts && lab != NO_LABEL && !has) a.small[SW_BAD_CLASS] = 1u;
+        if (a.odd.flag && i < a.n && !has && !(fabsf(acc[0][y][0]) < INFINITY))
+          *a.odd.flag = a.odd.call;
+      }
       // The label's column (another piece's: none of this one), and the columns
       // there are, none in a row without a label, from the lane's first.
       uint32_t own = lab - a.col0 - j0 - 4 * h;
@@ -164,11 +152,14 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_logits(const LogitArgs a) {
       if (__builtin_expect(__any(!has) || !full, 0))
         each<S>(acc, y, [&](int c, float v) { return c < have ? v : 0.f; });
     }
+    if constexpr (!F32) {
+      if (a.counts && a.col0 == 0 && at.ct == 0 && wc == 0 && lane == 0)
+        a.counts[at.rt * S::NWR + wr] = count;
+    }
     // Through LDS (the ring is free once every wave is here), so that a row's
     // 2 TC bytes go to memory together: eight columns a lane are one 16-byte chunk,
     // XOR-swizzled by the row.
-    RowScale rs;
-    rs.init(a.st, a.gloss, a.scale);
+    const int gexp = __is_same(T, f16) ? RowScale::exponent(a.st, a.counts) : 0;
     int ewmax = 0;
     bool one = false;
     if constexpr (F32) {
@@ -185,7 +176,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_logits(const LogitArgs a) {
       for (int y = 0; y < S::WB; y++) {
         int ga = 0;
         if constexpr (F32)
-          ga = (one ? ex[y] + rs.gexp : row_exp(a.gloss, min(i0 + y * 32, a.n - 1))) - ewmax;
+          ga = (one ? ex[y] + gexp : row_exp(a.gloss, min(i0 + y * 32, a.n - 1))) - ewmax;
         const uint32_t row = r0 + y * 32;
 #pragma unroll
         for (int b = 0; b < S::WA; b++)
@@ -194,12 +185,12 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_logits(const LogitArgs a) {
             float g[2][4];
 #pragma unroll
             for (int f = 0; f < 2; f++) {
-              int by[4] = {rs.gexp, rs.gexp, rs.gexp, rs.gexp};
+              int by[4] = {gexp, gexp, gexp, gexp};
               if (F32 && plane < 2) {
                 const int4 v = four_exps(a.ew, j0 + b * 32 + 8 * (2 * p + f) + 4 * h);
                 by[0] = v.x + ga, by[1] = v.y + ga, by[2] = v.z + ga, by[3] = v.w + ga;
               } else if (F32) {
-                by[0] = by[1] = by[2] = by[3] = ex[y] + rs.gexp;
+                by[0] = by[1] = by[2] = by[3] = ex[y] + gexp;
               }
 #pragma unroll
               for (int e = 0; e < 4; e++) {

@@ -117,6 +117,61 @@ def test_every_tile_shape(dev, n, d, k, name):
     Run(dev, x, w, lab, name).check()
 
 
+@pytest.mark.parametrize("name", ["f16", "bf16"])
+@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("n,k,want_dx", [(300, 140, False), (300, 140, True), (4000, 700, False),
+                                         (33_000, 65, True), (33_000, 65, False)])
+def test_rows_without_a_label_keep_out_of_dw(dev, name, value, n, k, want_dx):
+    """One value of such a row that is not finite, where some classes have a zero, at
+    few rows and at more than are counted on the way; with dx and without."""
+    from emeans_amd import F32
+    d = 64
+    x, w, lab = _inputs(n, d, k, n + k)
+    lab[[3, n // 2, n - 1]] = NONE
+    w[::3, 17] = 0.0
+    clean = R.Padded(dev, x, name).value
+    y = x.copy()
+    y[3, 17], y[n // 2, 17], y[n - 1, 17] = value, value, value
+    px, pw, lb = R.Padded(dev, y, name), R.Padded(dev, w, name), dev.upload_u32(lab)
+    loss, lse = dev.zeros(n, F32), dev.zeros(n, F32)
+    dx, dw = dev.zeros(n * d, R.kind(name)), dev.zeros(k * d, R.kind(name))
+    dev.cross_entropy(px.buf, n, d, pw.buf, k, lb, loss, lse)
+    dev.cross_entropy_grad(px.buf, n, d, pw.buf, k, lb, lse, dx if want_dx else None, dw)
+    got = R.decode(dev.read(dw), name).reshape(k, d)
+    has = lab != NONE
+    _, lse64, p, z = R.cross_entropy(clean, pw.value, lab, 1.0)
+    up = np.where(has, 1.0 / has.sum(), 0.0)
+    _, want, g = R.cross_entropy_grad(clean, pw.value, lab, 1.0, p, up)
+    # (The bounds of Run.check, coarser: a logit within 2^-15 of its terms' sizes.)
+    ez = 2.0 ** -15 * (np.abs(clean) @ np.abs(pw.value).T + np.abs(lse64)[:, None] + 1)
+    unit = {"f16": 2.0 ** -11, "bf16": 2.0 ** -8}[name]
+    eg = up[:, None] * p * ez + 1.01 * unit * np.abs(g) + 2.0 ** -36 * up.max()
+    eg[~has] = 0.0
+    tol = eg.T @ np.abs(clean) + (n + 64) * U * (np.abs(g).T @ np.abs(clean))
+    assert np.all(np.abs(got - want) <= tol + 1.01 * R.UNIT[name] * np.abs(want) + R.TINY[name])
+    if want_dx:
+        assert not R.decode(dev.read(dx), name).reshape(n, d)[~has].any()
+
+
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n", [5, 300, 40_000])
+def test_a_wrong_label_is_an_error_of_the_gradient_too(dev, name, n):
+    from emeans_amd import EmeansHipInvalid, F32
+    x, w, lab = _inputs(n, 16, 9, n)
+    px, pw = R.Padded(dev, x, name), R.Padded(dev, w, name)
+    loss, lse = dev.zeros(n, F32), dev.zeros(n, F32)
+    dx, dw = dev.zeros(n * 16, R.kind(name)), dev.zeros(9 * 16, R.kind(name))
+    dev.cross_entropy(px.buf, n, 16, pw.buf, 9, dev.upload_u32(lab), loss, lse)
+    dev.sync()
+    bad = lab.copy()
+    bad[n - 2] = 9
+    dev.cross_entropy_grad(px.buf, n, 16, pw.buf, 9, dev.upload_u32(bad), lse, dx, dw)
+    with pytest.raises(EmeansHipInvalid, match="label out of range"):
+        dev.sync()
+    dev.cross_entropy_grad(px.buf, n, 16, pw.buf, 9, dev.upload_u32(lab), lse, dx, dw)
+    dev.sync()
+
+
 # 16-bit rows and classes at every alignment that an element may have, at either side of
 # the last vector's end.
 @pytest.mark.parametrize("name", ["f16", "bf16"])
