@@ -3,7 +3,9 @@
 //
 // A workgroup owns a tile of TR rows x TC columns of the result. The depth goes by in
 // slabs of 64, each operand's slab (TR or TC by 64, 128 bytes a row) moved to LDS by
-// DMA into one of two stages. An operand lies in memory in one of two ways:
+// DMA into one of two stages, or of four for a small tile that has its CU to itself,
+// whose slab is done in less than the memory takes to answer (0.6 us a slab with four
+// stages, 0.75 with two). An operand lies in memory in one of two ways:
 //   DEEP  its rows run along the depth (x and w for the logits): a slab is 128
 //         bytes of each row, and a wave's operand is one 16-byte read a lane;
 //   WIDE  its rows run across it (w and x for the gradients: the depth is the
@@ -61,27 +63,32 @@ __device__ __forceinline__ v16f mfma16(bf16, v8s a, v8s b, v16f c) {
 constexpr int SLAB = 64;  // depth of a slab
 
 // A workgroup's shape: waves of NWR x NWC, each WB x WA blocks of 32 x 32.
-template <int NWR_, int NWC_, int WB_, int WA_>
+// STAGES slabs are in the ring.
+template <int NWR_, int NWC_, int WB_, int WA_, int STAGES_>
 struct TileShape {
   static constexpr int NWR = NWR_, NWC = NWC_, WB = WB_, WA = WA_;
   static constexpr int NW = NWR * NWC, THREADS = 64 * NW;
   static constexpr int TR = NWR * WB * 32, TC = NWC * WA * 32;
   static constexpr int RBYTES = TR * SLAB * 2, CBYTES = TC * SLAB * 2;
-  static constexpr int STAGE = RBYTES + CBYTES, RING = 2 * STAGE;
+  static constexpr int STAGES = STAGES_, STAGE = RBYTES + CBYTES, RING = STAGES * STAGE;
   static constexpr int RD = RBYTES / (1024 * NW), CD = CBYTES / (1024 * NW);  // DMAs a wave
 };
-typedef TileShape<4, 2, 2, 4> TileL;  // 256 x 256, 8 waves
-typedef TileShape<4, 2, 2, 3> TileM;  // 256 x 192, 8 waves
-typedef TileShape<2, 2, 2, 2> TileS;  // 128 x 128, 4 waves (two workgroups a CU)
-enum Tile : int { TILE_L, TILE_M, TILE_S, TILES };
-constexpr uint32_t TILE_ROWS[TILES] = {TileL::TR, TileM::TR, TileS::TR};
-constexpr uint32_t TILE_COLS[TILES] = {TileL::TC, TileM::TC, TileS::TC};
-constexpr uint32_t TILE_WAVES[TILES] = {TileL::NWR, TileM::NWR, TileS::NWR};  // down the rows
+typedef TileShape<4, 2, 2, 4, 2> TileL;  // 256 x 256, 8 waves
+typedef TileShape<4, 2, 2, 3, 2> TileM;  // 256 x 192, 8 waves
+typedef TileShape<2, 2, 2, 2, 2> TileS;  // 128 x 128, 4 waves (two workgroups a CU)
+typedef TileShape<4, 2, 1, 2, 4> TileD;  // 128 x 128, 8 waves, three slabs on their way
+enum Tile : int { TILE_L, TILE_M, TILE_S, TILE_D, TILES };
+constexpr uint32_t TILE_ROWS[TILES] = {TileL::TR, TileM::TR, TileS::TR, TileD::TR};
+constexpr uint32_t TILE_COLS[TILES] = {TileL::TC, TileM::TC, TileS::TC, TileD::TC};
+// Waves down the rows.
+constexpr uint32_t TILE_WAVES[TILES] = {TileL::NWR, TileM::NWR, TileS::NWR, TileD::NWR};
 // Rows and columns of whole tiles of any shape.
 constexpr uint32_t ALL_ROWS = 256, ALL_COLS = 768;
-static_assert(ALL_ROWS % TileL::TR == 0 && ALL_ROWS % TileM::TR == 0 && ALL_ROWS % TileS::TR == 0 &&
-                  ALL_COLS % TileL::TC == 0 && ALL_COLS % TileM::TC == 0 && ALL_COLS % TileS::TC == 0,
-              "whole tiles");
+constexpr uint32_t PARTS = 2;  // waves across a tile's columns
+template <class S>
+constexpr bool whole_tiles = ALL_ROWS % S::TR == 0 && ALL_COLS % S::TC == 0 && S::NWC == PARTS;
+static_assert(whole_tiles<TileL> && whole_tiles<TileM> && whole_tiles<TileS> && whole_tiles<TileD>,
+              "whole tiles, and parts of their rows");
 // Runs f with the shape as a type.
 template <class F>
 void by_tile(Tile t, F&& f) {
@@ -89,8 +96,10 @@ void by_tile(Tile t, F&& f) {
     f(TileL{});
   else if (t == TILE_M)
     f(TileM{});
-  else
+  else if (t == TILE_S)
     f(TileS{});
+  else
+    f(TileD{});
 }
 
 // One operand. f32 matrices come as two planes of fp16 (emh_xent.h).
@@ -237,7 +246,8 @@ struct Side16 {
 // next step's as soon as its MFMAs are issued. The last MFMA step's operands
 // are in registers before it begins, so its stage is free then: every wave has
 // waited for its own reads and DMAs (the next slab's) and met the others at the
-// barrier, and the DMAs of the slab after the next go out between its MFMAs.
+// barrier, and the DMAs of the slab that takes the stage next (the one after the next,
+// with two) go out between its MFMAs.
 template <class T, class S, bool RDEEP, bool CDEEP>
 __device__ __forceinline__ void tile_sums(const TileIn& t, const TileAt& at, char* ring,
                                           v16f (&acc)[S::WA][S::WB]) {
@@ -257,6 +267,10 @@ __device__ __forceinline__ void tile_sums(const TileIn& t, const TileAt& at, cha
   // Load cursor: pass, slab and stage of the next DMAs; past the last step it
   // stays there, and what it fetches again nothing reads.
   uint32_t lpass = 0, lslab = at.s0, lleft = at.s1 - at.s0, lst = 0;
+  auto after = [](uint32_t stage) __attribute__((always_inline)) {
+    if constexpr (S::STAGES == 2) return S::STAGE - stage;
+    return stage + S::STAGE == S::RING ? 0u : stage + S::STAGE;
+  };
   while (lslab >= t.slabs) lslab -= t.slabs, lpass++;
   auto dma = [&](int q) __attribute__((always_inline)) {
     if (q < S::RD)
@@ -267,7 +281,7 @@ __device__ __forceinline__ void tile_sums(const TileIn& t, const TileAt& at, cha
             ldst + lst + S::RBYTES + (uint32_t)(q - S::RD) * S::NW * 1024);
   };
   auto advance = [&]() __attribute__((always_inline)) {
-    lst = S::STAGE - lst;
+    lst = after(lst);
     if (lleft > 1) {
       lleft--;
       if (++lslab == t.slabs) {
@@ -285,12 +299,12 @@ __device__ __forceinline__ void tile_sums(const TileIn& t, const TileAt& at, cha
 
   constexpr int PER = S::RD + S::CD;
 #pragma unroll
-  for (int s = 0; s < 2; s++) {
+  for (int s = 0; s < S::STAGES; s++) {
 #pragma unroll
     for (int q = 0; q < PER; q++) dma(q);
     advance();
   }
-  wait_vm<PER>();  // the first slab is in, the second in flight
+  wait_vm<(S::STAGES - 1) * PER>();  // the first slab is in, the others in flight
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
@@ -304,13 +318,13 @@ __device__ __forceinline__ void tile_sums(const TileIn& t, const TileAt& at, cha
 #pragma unroll
     for (int ks = 0; ks < 4; ks++) {
       if (ks == 3) {
-        wait_vm<0>();
+        wait_vm<(S::STAGES - 2) * PER>();
         __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
       }
-      const uint32_t from = ks == 3 ? S::STAGE - st : st;
+      const uint32_t from = ks == 3 ? after(st) : st;
 #pragma unroll
       for (int a = 0; a < S::WA; a++) {
 #pragma unroll
@@ -330,7 +344,7 @@ __device__ __forceinline__ void tile_sums(const TileIn& t, const TileAt& at, cha
       }
     }
     advance();
-    st = S::STAGE - st;
+    st = after(st);
   }
   wait_vm<0>();  // the DMAs past the last step have landed
   asm volatile("" ::: "memory");

@@ -481,11 +481,11 @@ struct Plan {
   uint32_t rtiles = 1, ctiles = 1, splits = 1;
 };
 Plan plan_of(size_t rows, size_t cols, size_t steps, int cus, bool may_split) {
-  // us a slab on a full card (256 x 256: 1.18 PFLOP/s), workgroups a CU. Small tiles
-  // alone on their CUs are faster (10,007 x 300 by 1,000 f32: dx without splits, dw in 10
-  // instead of 30, 171 us a training pass instead of 177).
-  constexpr double STEP[TILES] = {1.8, 1.4, 1.2}, STEP_ALONE = 0.75;
-  constexpr int PER_CU[TILES] = {1, 1, 2};
+  // us a slab on a full card (256 x 256: 1.18 PFLOP/s), workgroups a CU. 128 x 128 two
+  // a CU for many tiles, else one with a deeper ring (10,007 x 300 by 1,000 f32: dx
+  // without splits, dw in 10 instead of 30, 165 us a training pass, 177 without).
+  constexpr double STEP[TILES] = {1.8, 1.4, 1.2, 0.6};
+  constexpr int PER_CU[TILES] = {1, 1, 2, 1};
   Plan best;
   double least = 1e300;
   for (int tile = 0; tile < TILES; tile++) {
@@ -494,8 +494,7 @@ Plan plan_of(size_t rows, size_t cols, size_t steps, int cus, bool may_split) {
     for (size_t s = 1; s <= (may_split ? 32 : 1); s++) {
       if (s > 1 && steps < 4 * s) break;
       const double rounds = std::ceil((double)(rt * ct * s) / ((double)cus * PER_CU[tile]));
-      const bool alone = PER_CU[tile] > 1 && rt * ct * s <= (size_t)cus;
-      double us = rounds * ((double)((steps + s - 1) / s) * (alone ? STEP_ALONE : STEP[tile]) + 4.0);
+      double us = rounds * ((double)((steps + s - 1) / s) * STEP[tile] + 4.0);
       if (s > 1) us += 3.0 + 1.2e-6 * (double)s * (double)rows * (double)cols;
       if (us < least) {
         least = us;
@@ -563,7 +562,7 @@ void launch_cross_entropy(emh_ctx* c, const XentIn& in, float* loss, float* lse)
     a.ew = lw.ex;
     a.part = part, a.zlabel = zlabel;
     launch_logits(c->stream, a, in.x.kind, p.tile, false);
-    k_join<<<grid1(m, 64), 1024, 0, c->stream>>>(part, p.ctiles * 2, (uint32_t)m, in.labels + r0,
+    k_join<<<grid1(m, 64), 1024, 0, c->stream>>>(part, p.ctiles * PARTS, (uint32_t)m, in.labels + r0,
                                                  (uint32_t)k, zlabel, loss + r0,
                                                  lse ? lse + r0 : nullptr, c->small);
     EMH_HIP(hipGetLastError());
