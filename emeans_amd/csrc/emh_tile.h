@@ -89,6 +89,11 @@ template <class S>
 constexpr bool whole_tiles = ALL_ROWS % S::TR == 0 && ALL_COLS % S::TC == 0 && S::NWC == PARTS;
 static_assert(whole_tiles<TileL> && whole_tiles<TileM> && whole_tiles<TileS> && whole_tiles<TileD>,
               "whole tiles, and parts of their rows");
+// Whether f32's planes are taken together: where two stages of both are in the ring.
+template <class S>
+constexpr bool takes_both = S::STAGES >= 4;
+constexpr bool TILE_BOTH[TILES] = {takes_both<TileL>, takes_both<TileM>, takes_both<TileS>,
+                                   takes_both<TileD>};
 // Runs f with the shape as a type.
 template <class F>
 void by_tile(Tile t, F&& f) {
@@ -114,7 +119,7 @@ struct Operand {
 struct TileIn {
   Operand r, c;
   uint32_t slabs;   // of the depth; one operand is zero past it
-  uint32_t passes;  // 1, or 3: planes (0, 0), (0, 1), (1, 0)
+  uint32_t passes;  // 1, or 3: planes (0, 0), (0, 1), (1, 0) one after another
   uint32_t rtiles, ctiles, splits;  // workgroups: rtiles ctiles splits
   // What a workgroup finds its tile by (prepare): divisions there, by whole words,
   // were 300 instructions that every workgroup of a launch met cold.
@@ -248,7 +253,12 @@ struct Side16 {
 // waited for its own reads and DMAs (the next slab's) and met the others at the
 // barrier, and the DMAs of the slab that takes the stage next (the one after the next,
 // with two) go out between its MFMAs.
-template <class T, class S, bool RDEEP, bool CDEEP>
+//
+// BOTH (f32's planes, where one pass over the depth can have them all in LDS): a stage
+// holds both planes of both operands, and a step takes the three products from it: two
+// thirds of the DMAs and of the LDS reads. (10,007 x 300 by 1,000: dx 37 us with three
+// passes, 31 with both; dw 36 and 30.)
+template <class T, class S, bool RDEEP, bool CDEEP, bool BOTH>
 __device__ __forceinline__ void tile_sums(const TileIn& t, const TileAt& at, char* ring,
                                           v16f (&acc)[S::WA][S::WB]) {
   const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -263,22 +273,26 @@ __device__ __forceinline__ void tile_sums(const TileIn& t, const TileAt& at, cha
   const size_t r0 = RDEEP ? (size_t)at.rt * S::TR * t.r.ld : 0;
   const size_t c0 = CDEEP ? (size_t)at.ct * S::TC * t.c.ld : 0;
   const uint32_t ldst = lds0 + (uint32_t)w * 1024;
+  constexpr int P = BOTH ? 2 : 1, STAGES = S::STAGES / P, STAGE = S::STAGE * P;
+  static_assert(STAGES >= 2, "a stage to fill and one to read");
 
   // Load cursor: pass, slab and stage of the next DMAs; past the last step it
   // stays there, and what it fetches again nothing reads.
   uint32_t lpass = 0, lslab = at.s0, lleft = at.s1 - at.s0, lst = 0;
   auto after = [](uint32_t stage) __attribute__((always_inline)) {
-    if constexpr (S::STAGES == 2) return S::STAGE - stage;
-    return stage + S::STAGE == S::RING ? 0u : stage + S::STAGE;
+    if constexpr (STAGES == 2) return STAGE - stage;
+    return stage + STAGE == STAGES * STAGE ? 0u : stage + STAGE;
   };
   while (lslab >= t.slabs) lslab -= t.slabs, lpass++;
-  auto dma = [&](int q) __attribute__((always_inline)) {
+  auto dma = [&](int i) __attribute__((always_inline)) {
+    const int q = i % (S::RD + S::CD), plane = i / (S::RD + S::CD);
+    const uint32_t to = ldst + lst + (uint32_t)plane * S::STAGE;
     if (q < S::RD)
-      R.dma(q, t.r.p[lpass == 2 ? 1 : 0] + r0, t.r, lslab,
-            ldst + lst + (uint32_t)q * S::NW * 1024);
+      R.dma(q, t.r.p[BOTH ? plane : lpass == 2 ? 1 : 0] + r0, t.r, lslab,
+            to + (uint32_t)q * S::NW * 1024);
     else
-      C.dma(q - S::RD, t.c.p[lpass == 1 ? 1 : 0] + c0, t.c, lslab,
-            ldst + lst + S::RBYTES + (uint32_t)(q - S::RD) * S::NW * 1024);
+      C.dma(q - S::RD, t.c.p[BOTH ? plane : lpass == 1 ? 1 : 0] + c0, t.c, lslab,
+            to + S::RBYTES + (uint32_t)(q - S::RD) * S::NW * 1024);
   };
   auto advance = [&]() __attribute__((always_inline)) {
     lst = after(lst);
@@ -297,54 +311,97 @@ __device__ __forceinline__ void tile_sums(const TileIn& t, const TileAt& at, cha
 #pragma unroll
       for (int r = 0; r < 16; r++) acc[a][y][r] = 0.f;
 
-  constexpr int PER = S::RD + S::CD;
+  constexpr int PER = (S::RD + S::CD) * P;
 #pragma unroll
-  for (int s = 0; s < S::STAGES; s++) {
+  for (int s = 0; s < STAGES; s++) {
 #pragma unroll
     for (int q = 0; q < PER; q++) dma(q);
     advance();
   }
-  wait_vm<(S::STAGES - 1) * PER>();  // the first slab is in, the others in flight
+  wait_vm<(STAGES - 1) * PER>();  // the first slab is in, the others in flight
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
-  v8s rb[2][S::WB], ca[S::WA];
-#pragma unroll
-  for (int y = 0; y < S::WB; y++) rb[0][y] = R.read(0, 0, y);
-#pragma unroll
-  for (int a = 0; a < S::WA; a++) ca[a] = C.read(0, 0, a);
+  // The next slab is in, and what this one's stage held is in registers.
+  auto meet = [&]() __attribute__((always_inline)) {
+    wait_vm<(STAGES - 2) * PER>();
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
   uint32_t st = 0;
-  for (uint32_t s = at.s0; s < at.s1; s++) {
+  if constexpr (BOTH) {
+    constexpr int ROWS = 2 * S::WB, READS = ROWS + 2 * S::WA, MS = 3 * S::WA;
+    v8s op[2][READS];  // [row block][plane], then [column block][plane]
+    auto read = [&](int i, uint32_t stage, int ks) __attribute__((always_inline)) {
+      const uint32_t at_plane = stage + (uint32_t)(i & 1) * S::STAGE;
+      return i < ROWS ? R.read(at_plane, ks, i / 2) : C.read(at_plane, ks, (i - ROWS) / 2);
+    };
 #pragma unroll
-    for (int ks = 0; ks < 4; ks++) {
-      if (ks == 3) {
-        wait_vm<(S::STAGES - 2) * PER>();
-        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-      }
-      const uint32_t from = ks == 3 ? after(st) : st;
+    for (int i = 0; i < READS; i++) op[0][i] = read(i, 0, 0);
+    for (uint32_t s = at.s0; s < at.s1; s++) {
 #pragma unroll
-      for (int a = 0; a < S::WA; a++) {
+      for (int ks = 0; ks < 4; ks++) {
+        if (ks == 3) meet();
+        const uint32_t from = ks == 3 ? after(st) : st;
 #pragma unroll
-        for (int y = 0; y < S::WB; y++)
-          acc[a][y] = mfma16(T{}, ca[a], rb[ks & 1][y], acc[a][y]);
-        __builtin_amdgcn_sched_barrier(0);
-        if (a == 0) {
+        for (int m = 0; m < MS; m++) {  // (h, h) of every block, (h, l), (l, h)
+          const int a = m % S::WA, pass = m / S::WA;
 #pragma unroll
-          for (int y = 0; y < S::WB; y++) rb[(ks + 1) & 1][y] = R.read(from, (ks + 1) & 3, y);
+          for (int y = 0; y < S::WB; y++)
+            acc[a][y] = mfma16(T{}, op[ks & 1][ROWS + 2 * a + (pass == 1)],
+                               op[ks & 1][2 * y + (pass == 2)], acc[a][y]);
+          __builtin_amdgcn_sched_barrier(0);
+          // The next step's operands by the middle of this one.
+          constexpr int BY = (MS + 1) / 2;
+          if (m < BY) {
+#pragma unroll
+            for (int i = m * READS / BY; i < (m + 1) * READS / BY; i++)
+              op[(ks + 1) & 1][i] = read(i, from, (ks + 1) & 3);
+          }
+          if (ks == 3) {
+#pragma unroll
+            for (int q = m * PER / MS; q < (m + 1) * PER / MS; q++) dma(q);
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
-        ca[a] = C.read(from, (ks + 1) & 3, a);
-        if (ks == 3) {
-#pragma unroll
-          for (int q = a * PER / S::WA; q < (a + 1) * PER / S::WA; q++) dma(q);
-        }
-        __builtin_amdgcn_sched_barrier(0);
       }
+      advance();
+      st = after(st);
     }
-    advance();
-    st = after(st);
+  } else {
+    v8s rb[2][S::WB], ca[S::WA];
+#pragma unroll
+    for (int y = 0; y < S::WB; y++) rb[0][y] = R.read(0, 0, y);
+#pragma unroll
+    for (int a = 0; a < S::WA; a++) ca[a] = C.read(0, 0, a);
+    for (uint32_t s = at.s0; s < at.s1; s++) {
+#pragma unroll
+      for (int ks = 0; ks < 4; ks++) {
+        if (ks == 3) meet();
+        const uint32_t from = ks == 3 ? after(st) : st;
+#pragma unroll
+        for (int a = 0; a < S::WA; a++) {
+#pragma unroll
+          for (int y = 0; y < S::WB; y++)
+            acc[a][y] = mfma16(T{}, ca[a], rb[ks & 1][y], acc[a][y]);
+          __builtin_amdgcn_sched_barrier(0);
+          if (a == 0) {
+#pragma unroll
+            for (int y = 0; y < S::WB; y++) rb[(ks + 1) & 1][y] = R.read(from, (ks + 1) & 3, y);
+          }
+          ca[a] = C.read(from, (ks + 1) & 3, a);
+          if (ks == 3) {
+#pragma unroll
+            for (int q = a * PER / S::WA; q < (a + 1) * PER / S::WA; q++) dma(q);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      advance();
+      st = after(st);
+    }
   }
   wait_vm<0>();  // the DMAs past the last step have landed
   asm volatile("" ::: "memory");

@@ -474,32 +474,35 @@ void few(emh_ctx* c, const XentIn& in, float* loss, float* lse) {
   EMH_HIP(hipGetLastError());
 }
 
-// The shape and splits of a product of rows x cols over `steps` slabs: the
+// The shape and splits of a product of rows x cols over `slabs` (of f32's planes): the
 // fewest rounds of workgroups times a workgroup's time, with the cost of
 // writing and adding the splits' sums.
 struct Plan {
   Tile tile = TILE_L;
-  uint32_t rtiles = 1, ctiles = 1, splits = 1;
+  uint32_t rtiles = 1, ctiles = 1, splits = 1, passes = 1;
 };
-Plan plan_of(size_t rows, size_t cols, size_t steps, int cus, bool may_split) {
+Plan plan_of(size_t rows, size_t cols, size_t slabs, bool planes, int cus, bool may_split) {
   // us a slab on a full card (256 x 256: 1.18 PFLOP/s), workgroups a CU. 128 x 128 two
   // a CU for many tiles, else one with a deeper ring (10,007 x 300 by 1,000 f32: dx
-  // without splits, dw in 10 instead of 30, 165 us a training pass, 177 without).
-  constexpr double STEP[TILES] = {1.8, 1.4, 1.2, 0.6};
+  // without splits, dw in 10 instead of 30, 165 us a training pass, 177 without). Of a
+  // slab of both of f32's planes (TILE_BOTH) STEP_BOTH.
+  constexpr double STEP[TILES] = {1.8, 1.4, 1.2, 0.6}, STEP_BOTH = 1.2;
   constexpr int PER_CU[TILES] = {1, 1, 2, 1};
   Plan best;
   double least = 1e300;
   for (int tile = 0; tile < TILES; tile++) {
     const size_t rt = (rows + TILE_ROWS[tile] - 1) / TILE_ROWS[tile];
     const size_t ct = (cols + TILE_COLS[tile] - 1) / TILE_COLS[tile];
+    const bool both = planes && TILE_BOTH[tile];
+    const size_t passes = planes && !both ? 3 : 1, steps = passes * slabs;
     for (size_t s = 1; s <= (may_split ? 32 : 1); s++) {
       if (s > 1 && steps < 4 * s) break;
       const double rounds = std::ceil((double)(rt * ct * s) / ((double)cus * PER_CU[tile]));
-      double us = rounds * ((double)((steps + s - 1) / s) * STEP[tile] + 4.0);
+      double us = rounds * ((double)((steps + s - 1) / s) * (both ? STEP_BOTH : STEP[tile]) + 4.0);
       if (s > 1) us += 3.0 + 1.2e-6 * (double)s * (double)rows * (double)cols;
       if (us < least) {
         least = us;
-        best = {(Tile)tile, (uint32_t)rt, (uint32_t)ct, (uint32_t)s};
+        best = {(Tile)tile, (uint32_t)rt, (uint32_t)ct, (uint32_t)s, (uint32_t)passes};
       }
     }
   }
@@ -531,7 +534,7 @@ void launch_cross_entropy(emh_ctx* c, const XentIn& in, float* loss, float* lse)
       few<bf16>(c, in, loss, lse);
     return;
   }
-  const size_t slabs = up(d, SLAB) / SLAB, passes = f32 ? 3 : 1;
+  const size_t slabs = up(d, SLAB) / SLAB;
   // Rows at a time: what bounds them is the parts' maxima and sums (512 MB).
   const size_t all = (k + 127) / 128 * 2;
   const size_t rows = std::min(n, std::max<size_t>(256, ((size_t(64) << 20) / all) & ~(size_t)255));
@@ -550,11 +553,11 @@ void launch_cross_entropy(emh_ctx* c, const XentIn& in, float* loss, float* lse)
   pack(c, in, lx, lw, nullptr);
   for (size_t r0 = 0; r0 < n; r0 += rows) {
     const size_t m = std::min(rows, n - r0);
-    const Plan p = plan_of(m, k, slabs * passes, c->cus, false);
+    const Plan p = plan_of(m, k, slabs, f32, c->cus, false);
     LogitArgs a{};
     a.t.r = lx.deep(in.x, r0, m);
     a.t.c = lw.deep(in.w, 0, k);
-    a.t.slabs = (uint32_t)slabs, a.t.passes = (uint32_t)passes;
+    a.t.slabs = (uint32_t)slabs, a.t.passes = p.passes;
     a.t.rtiles = p.rtiles, a.t.ctiles = p.ctiles, a.t.splits = 1;
     a.n = (uint32_t)m, a.m = a.k = (uint32_t)k;
     a.labels = in.labels + r0;
@@ -579,7 +582,7 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
     EMH_HIP(hipGetLastError());
     return;
   }
-  const size_t slabs = up(d, SLAB) / SLAB, passes = f32 ? 3 : 1, planes = f32 ? 4 : 1;
+  const size_t slabs = up(d, SLAB) / SLAB, planes = f32 ? 4 : 1;
   // The classes in pieces of one size (a small last one, in a few workgroups, took as
   // long as 0.17 of a whole one: 8,192 rows of 1,024 against 131,071, 8.43 ms a training
   // pass, now 8.29), whole rows of dw's tiles each, with 1 GB of G at most, but for its
@@ -589,8 +592,8 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
   const size_t pieces = (k + most - 1) / most;
   const size_t piece = pieces == 1 ? k : up((k + pieces - 1) / pieces, ALL_ROWS);
   const size_t gcols = up(piece, ALL_COLS), ldg = gcols * 2, ldp = up(d, 4);
-  const Plan px = plan_of(n, d, passes * ((piece + SLAB - 1) / SLAB), c->cus, true);
-  const Plan pw = plan_of(piece, d, passes * ((n + SLAB - 1) / SLAB), c->cus, true);
+  const Plan px = plan_of(n, d, (piece + SLAB - 1) / SLAB, f32, c->cus, true);
+  const Plan pw = plan_of(piece, d, (n + SLAB - 1) / SLAB, f32, c->cus, true);
   const bool px_part = px.splits > 1 || pieces > 1, pw_part = pw.splits > 1;
   // Rows without a label: see OddRows.
   const bool x_as_is = direct(in.x, d, true);
@@ -613,7 +616,7 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
   }
   const uint32_t call = ++c->xent_calls;
   pack(c, in, x_as_is ? Laid{} : lx, lw, in.labels);
-  const Plan first = plan_of(n, std::min(piece, k), slabs * passes, c->cus, false);
+  const Plan first = plan_of(n, std::min(piece, k), slabs, f32, c->cus, false);
   const size_t waves = (size_t)first.rtiles * TILE_WAVES[first.tile];
   const bool counted = !f32 && !gloss && waves <= MANY_COUNTS;
   if (!counted) {
@@ -625,13 +628,13 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
   const Laid& xl = x_as_is ? as_is : lx;
   for (size_t v0 = 0; v0 < k; v0 += piece) {
     const size_t m = std::min(piece, k - v0);
-    const Plan pg = plan_of(n, m, slabs * passes, c->cus, false);
+    const Plan pg = plan_of(n, m, slabs, f32, c->cus, false);
     if ((size_t)pg.rtiles * TILE_ROWS[pg.tile] > np || (size_t)pg.ctiles * TILE_COLS[pg.tile] > gcols)
       throw Failure("cross_entropy_grad: tiles beyond the piece");
     LogitArgs a{};
     a.t.r = xl.deep(in.x, 0, n);
     a.t.c = lw.deep(in.w, v0, m);
-    a.t.slabs = (uint32_t)slabs, a.t.passes = (uint32_t)passes;
+    a.t.slabs = (uint32_t)slabs, a.t.passes = pg.passes;
     a.t.rtiles = pg.rtiles, a.t.ctiles = pg.ctiles, a.t.splits = 1;
     a.n = (uint32_t)n, a.m = (uint32_t)m, a.col0 = (uint32_t)v0, a.k = (uint32_t)k;
     a.labels = in.labels;
@@ -651,7 +654,6 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
     p.labels = in.labels, p.k = (uint32_t)k;
     p.gloss = gloss, p.st = st, p.scale = in.scale;
     if (counted) p.counts = counts, p.ncounts = (uint32_t)waves;
-    p.t.passes = (uint32_t)passes;
     p.cols = (uint32_t)d, p.ldp = ldp;
     if (dx.p) {
       p.t.r = {{G[0], G[1]}, (uint32_t)ldg, (uint32_t)n, 0};
@@ -659,6 +661,7 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
       p.t.c.wide = lw.packed ? lw.dp : (uint32_t)d;
       p.t.slabs = (uint32_t)((m + SLAB - 1) / SLAB);
       p.t.rtiles = px.rtiles, p.t.ctiles = px.ctiles, p.t.splits = px.splits;
+      p.t.passes = px.passes;
       p.rows = (uint32_t)n, p.dw = false;
       p.ex = lx.ex;
       p.out = dx.p, p.ldo = dx.ld;
@@ -677,7 +680,7 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
       p.t.c.wide = xl.packed ? xl.dp : (uint32_t)d;
       p.t.slabs = (uint32_t)((n + SLAB - 1) / SLAB);
       p.t.rtiles = ((uint32_t)m + TILE_ROWS[pw.tile] - 1) / TILE_ROWS[pw.tile];
-      p.t.ctiles = pw.ctiles, p.t.splits = pw.splits;
+      p.t.ctiles = pw.ctiles, p.t.splits = pw.splits, p.t.passes = pw.passes;
       p.rows = (uint32_t)m, p.dw = true;
       p.out = (char*)dw.p + v0 * dw.ld * kind_bytes(dw.kind), p.ldo = dw.ld;
       p.part = pw_part ? partw : nullptr;

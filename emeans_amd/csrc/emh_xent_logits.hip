@@ -46,7 +46,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_logits(const LogitArgs a) {
   __shared__ __attribute__((aligned(1024))) char ring[S::RING];
   const TileAt at = tile_at(a.t);
   v16f acc[S::WA][S::WB];
-  tile_sums<T, S, true, true>(a.t, at, ring, acc);
+  tile_sums<T, S, true, true, F32 && takes_both<S>>(a.t, at, ring, acc);
 
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, li = lane & 31, h = lane >> 5;
   const int wr = w % S::NWR, wc = w / S::NWR;
