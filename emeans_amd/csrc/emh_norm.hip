@@ -14,6 +14,7 @@
 //
 // Bound by HBM: 2 (forward) and 3 (backward) elements moved per element.
 #include <algorithm>
+#include <type_traits>
 
 #include "emh_learn.h"
 #include "emh_types.h"
@@ -449,12 +450,25 @@ void launch_layer_norm_grad(emh_ctx* c, const MatIn& dy, const MatIn& x, size_t 
     const bool held = by_shape<T>(d, [&](auto s) {
       using S = decltype(s);
       // A workgroup a CU, of as many waves as the registers allow: few rows of
-      // sums to write and add.
-      constexpr int TB = S::NV * VecOf<T>::N < 16 ? 1024 : S::NV * VecOf<T>::N == 16 ? 768 : 512;
-      constexpr size_t G = TB / S::LPR;
-      parts = std::min((rows + G - 1) / G, (size_t)c->cus);
-      if (sums) a.part = (float*)c->norm_part.get(parts * 2 * d * 4);
-      k_norm_grad<T, S::LPR, S::NV, TB><<<dim3((unsigned)parts), TB, 0, c->stream>>>(a);
+      // sums to write and add. (Twelve elements a thread fill 1,024 threads' registers
+      // and a few more: whole rows take that, 200,000 x 768 f32 592 us a training pass and
+      // 598 with 768 threads; 30,000 x 641 takes 75 and 67.)
+      auto go = [&](auto threads) {
+        constexpr int TB = decltype(threads)::value;
+        constexpr size_t G = TB / S::LPR;
+        parts = std::min((rows + G - 1) / G, (size_t)c->cus);
+        if (sums) a.part = (float*)c->norm_part.get(parts * 2 * d * 4);
+        k_norm_grad<T, S::LPR, S::NV, TB><<<dim3((unsigned)parts), TB, 0, c->stream>>>(a);
+      };
+      constexpr int HELD = S::NV * VecOf<T>::N;
+      if constexpr (HELD > 16)
+        go(std::integral_constant<int, 512>{});
+      else if constexpr (HELD == 16)
+        go(std::integral_constant<int, 768>{});
+      else if (HELD < 12 || d == (size_t)S::LPR * HELD)
+        go(std::integral_constant<int, 1024>{});
+      else if constexpr (HELD == 12)
+        go(std::integral_constant<int, 768>{});
     });
     if (held) return;
     if (sums) {  // before dx, which may overwrite dy
