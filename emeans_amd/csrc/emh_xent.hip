@@ -484,7 +484,7 @@ struct Plan {
 Plan plan_of(size_t rows, size_t cols, size_t slabs, bool planes, int cus, bool may_split) {
   // us a slab on a full card (256 x 256: 1.18 PFLOP/s), workgroups a CU. 128 x 128 two
   // a CU for many tiles, else one with a deeper ring (10,007 x 300 by 1,000 f32: dx
-  // without splits, dw in 10 instead of 30, 165 us a training pass, 177 without). Of a
+  // without splits, dw in 10 instead of 30, 12 us less a training pass). Of a
   // slab of both of f32's planes (TILE_BOTH) STEP_BOTH.
   constexpr double STEP[TILES] = {1.8, 1.4, 1.2, 0.6}, STEP_BOTH = 1.2;
   constexpr int PER_CU[TILES] = {1, 1, 2, 1};
