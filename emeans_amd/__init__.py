@@ -449,6 +449,10 @@ class HipDevice:
         EXACT_BELOW); 0 screens every call the mode screens. Same bits."""
         check(lib().emh_set_exact_below(self._ctx, int(items)))
 
+    def set_xent_workspace(self, size: int):
+        """The most bytes of softmax that cross_entropy_grad holds at a time (0: 1 GiB)."""
+        check(lib().emh_set_xent_workspace(self._ctx, int(size)))
+
 
 def _h(b: Optional[DevBuf]):
     return None if b is None else b.h

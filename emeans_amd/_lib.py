@@ -81,6 +81,13 @@ class DedupResult(C.Structure):
                 ("split_components", C.c_uint64)]
 
 
+class XentProduct(C.Structure):
+    _fields_ = [("what", C.c_int), ("tile_rows", C.c_uint32), ("tile_cols", C.c_uint32),
+                ("row_tiles", C.c_uint32), ("col_tiles", C.c_uint32), ("splits", C.c_uint32),
+                ("slabs", C.c_uint32), ("passes", C.c_uint32), ("row0", C.c_uint64),
+                ("rows", C.c_uint64), ("class0", C.c_uint64), ("classes", C.c_uint64)]
+
+
 class AdamTensor(C.Structure):
     _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("m", C.c_void_p),
                 ("v", C.c_void_p), ("m_scale", C.c_void_p), ("v_scale", C.c_void_p),
@@ -124,6 +131,7 @@ SIGNATURES = {
     "emh_cross_entropy": (_i, [_vp, _vp, _sz, _sz, _sz, _vp, _sz, _sz, _vp, _f, _vp, _vp]),
     "emh_cross_entropy_grad": (_i, [_vp, _vp, _sz, _sz, _sz, _vp, _sz, _sz, _vp, _f, _vp, _vp, _vp,
                                     _sz, _vp, _sz]),
+    "emh_set_xent_workspace": (_i, [_vp, _u64]),
     "emh_adamw_create": (_i, [_vp, _vp, _sz, _pp]),
     "emh_adamw_step": (_i, [_vp, _vp]),
     "emh_adamw_destroy": (_i, [_vp]),
@@ -164,6 +172,7 @@ SIGNATURES = {
     "emh_host_scheduled_alpha": (_d, [_d, _u64, _u64]),
     "emh_host_plan_revival": (_u64, [_vp, _u64, _d, _u32, _vp]),
     "emh_host_numpy_sum_f32": (_f, [_vp, _u64]),
+    "emh_host_xent_products": (_i, [_u64, _u64, _u64, _i, _i, _u64, _vp, _u64, C.POINTER(_u64)]),
 }
 
 _lib = None

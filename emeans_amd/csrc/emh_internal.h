@@ -136,6 +136,8 @@ enum ScreenMode : int { SCREEN_OFF = 0, SCREEN_ON = 1, SCREEN_F32 = 2, SCREEN_F1
 // than the screen's three (d = 768: the screen ~60 us at any size up to 8,192
 // rows for k <= 16, ~85 us for k = 64 .. 256 up to 4,096 rows).
 constexpr size_t EXACT_BELOW = 4096;
+// Bytes of G that a cross entropy gradient holds at a time by default.
+constexpr size_t XENT_WORKSPACE = size_t(1) << 30;
 // Direct selections of at most this many items of the latency-bound scan
 // (k_queued1: 4 rows x 16 centroids each, plus one per 4 rows for L2) take
 // that scan instead of k_exact1 (~13 us against ~32 us at 64 items).
@@ -225,6 +227,7 @@ struct emh_ctx {
   int cus = 256;
   int screen = emh::SCREEN_ON;
   size_t exact_below = emh::EXACT_BELOW;  // emh_set_exact_below
+  size_t xent_workspace = emh::XENT_WORKSPACE;  // emh_set_xent_workspace
   uint32_t* small = nullptr;  // SW_WORDS u32 on the device
   float* scales = nullptr;    // (s, 1 / s) of each SCALE_* matrix (emh_lines.h), after small
   char* scratch = nullptr;    // the device's fixed scratch block (emh_top1_noalloc)

@@ -183,6 +183,7 @@ int emh_layer_norm_grad(emh_ctx* c, const emh_buf* dy, size_t lddy, const emh_bu
 }  // extern "C"
 
 namespace {
+constexpr size_t XENT_D = size_t(1) << 21, XENT_K = size_t(1) << 30, XENT_N = size_t(1) << 30;
 struct XentCall {
   emh::XentIn in;
   Range x, w, labels;
@@ -190,9 +191,9 @@ struct XentCall {
 XentCall check_xent(emh_ctx* c, const emh_buf* x, size_t ldx, size_t n, size_t d, const emh_buf* w,
                     size_t ldw, size_t k, const emh_buf* labels, float scale) {
   EMH_ENSURE(c, "null context");
-  EMH_ENSURE(d > 0 && d <= (size_t(1) << 21), "d must be 1 to 2^21");
-  EMH_ENSURE(k > 0 && k <= (size_t(1) << 30), "k must be 1 to 2^30");
-  EMH_ENSURE(n <= (size_t(1) << 30), "too many rows");
+  EMH_ENSURE(d > 0 && d <= XENT_D, "d must be 1 to 2^21");
+  EMH_ENSURE(k > 0 && k <= XENT_K, "k must be 1 to 2^30");
+  EMH_ENSURE(n <= XENT_N, "too many rows");
   EMH_ENSURE(x && real_kind(x->kind), "x must be an f32, f16 or bf16 buffer");
   EMH_ENSURE(w && w->kind == x->kind, "w must be of x's kind");
   EMH_ENSURE(labels && labels->kind == EMH_U32, "labels must be a u32 buffer");
@@ -266,6 +267,27 @@ int emh_cross_entropy_grad(emh_ctx* c, const emh_buf* x, size_t ldx, size_t n, s
     }
     emh::launch_cross_entropy_grad(c, t.in, (const float*)lse->ptr,
                                    gloss ? (const float*)gloss->ptr : nullptr, mo[0], mo[1]);
+  });
+}
+
+int emh_set_xent_workspace(emh_ctx* c, uint64_t bytes) {
+  return guard([&] {
+    EMH_ENSURE(c, "null context");
+    c->xent_workspace = bytes ? (size_t)bytes : emh::XENT_WORKSPACE;
+  });
+}
+
+int emh_host_xent_products(uint64_t n, uint64_t d, uint64_t k, int kind, int cus, uint64_t workspace,
+                           emh_xent_product* out, uint64_t cap, uint64_t* count) {
+  return guard([&] {
+    EMH_ENSURE(count && (out || cap == 0), "null argument");
+    EMH_ENSURE(d > 0 && d <= XENT_D && k > 0 && k <= XENT_K && n <= XENT_N, "size out of range");
+    EMH_ENSURE(real_kind(kind), "kind must be f32, f16 or bf16");
+    EMH_ENSURE(cus > 0, "cus must be positive");
+    const auto all = emh::cross_entropy_products(n, d, k, kind == EMH_F32, cus,
+                                                 workspace ? (size_t)workspace : emh::XENT_WORKSPACE);
+    *count = all.size();
+    std::copy_n(all.begin(), std::min<size_t>(all.size(), cap), out);
   });
 }
 

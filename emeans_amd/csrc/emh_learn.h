@@ -2,6 +2,8 @@
 // the arguments that their entry points (emh_learn.cpp) have checked.
 #pragma once
 
+#include <vector>
+
 #include "emh_internal.h"
 
 namespace emh {
@@ -39,6 +41,10 @@ void launch_cross_entropy(emh_ctx* c, const XentIn& in, float* loss, float* lse)
 // gloss (n entries): the gradients of the rows' losses, or null: of their mean.
 void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, const float* gloss,
                                const MatOut& dx, const MatOut& dw);
+// The tiled products that launch_cross_entropy_grad queues, in their order, for both
+// gradients (host arithmetic alone).
+std::vector<emh_xent_product> cross_entropy_products(size_t n, size_t d, size_t k, bool f32, int cus,
+                                                     size_t workspace);
 
 // ---- emh_adamw.hip
 struct AdamTensor {  // as the kernel reads it

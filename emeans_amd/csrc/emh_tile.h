@@ -120,7 +120,8 @@ struct TileIn {
   Operand r, c;
   uint32_t slabs;   // of the depth; one operand is zero past it
   uint32_t passes;  // 1, or 3: planes (0, 0), (0, 1), (1, 0) one after another
-  uint32_t rtiles, ctiles, splits;  // workgroups: rtiles ctiles splits
+  uint32_t rtiles, ctiles, splits;  // workgroups: rtiles ctiles splits (at most slabs passes:
+                                    // each has a step, whose loads go out unasked)
   // What a workgroup finds its tile by (prepare): divisions there, by whole words,
   // were 300 instructions that every workgroup of a launch met cold.
   uint32_t blocks, steps;  // all workgroups; steps of a split (the first `more`: one more)
@@ -132,6 +133,7 @@ constexpr uint32_t GROUP = 8;  // row tiles taken together (tile_at)
 inline uint32_t recip(uint32_t by) { return (uint32_t)((uint64_t(1) << 32) / by + 1); }
 inline unsigned prepare(TileIn& t) {
   const uint32_t steps = t.slabs * t.passes;
+  if (t.splits == 0 || t.splits > steps) throw Failure("a product's split without a step");
   t.blocks = t.rtiles * t.ctiles * t.splits;
   t.steps = steps / t.splits;
   t.more = steps % t.splits;

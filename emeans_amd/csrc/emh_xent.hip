@@ -4,6 +4,7 @@
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
+#include <vector>
 
 #include "emh_xent.h"
 
@@ -403,8 +404,8 @@ struct Laid {
   Operand deep(const MatIn& m, size_t first, size_t rows) const {
     Operand o{};
     o.ld = packed ? dp * 2 : (uint32_t)(m.ld * 2);
-    for (int i = 0; i < 2; i++)
-      o.p[i] = (packed ? p[i] : (char*)m.p) + (p[1] || i == 0 ? first * o.ld : 0);
+    for (int i = 0; i < 2; i++)  // (of 16 bits there is one plane)
+      o.p[i] = (packed ? p[p[1] ? i : 0] : (char*)m.p) + first * o.ld;
     o.rows = (uint32_t)rows;
     o.wide = packed ? dp : 0;
     return o;
@@ -479,7 +480,7 @@ void few(emh_ctx* c, const XentIn& in, float* loss, float* lse) {
 // writing and adding the splits' sums.
 struct Plan {
   Tile tile = TILE_L;
-  uint32_t rtiles = 1, ctiles = 1, splits = 1, passes = 1;
+  uint32_t rtiles = 1, ctiles = 1, splits = 1, passes = 1, slabs = 1;
 };
 Plan plan_of(size_t rows, size_t cols, size_t slabs, bool planes, int cus, bool may_split) {
   // us a slab on a full card (256 x 256: 1.18 PFLOP/s), workgroups a CU. 128 x 128 two
@@ -502,11 +503,59 @@ Plan plan_of(size_t rows, size_t cols, size_t slabs, bool planes, int cus, bool 
       if (s > 1) us += 3.0 + 1.2e-6 * (double)s * (double)rows * (double)cols;
       if (us < least) {
         least = us;
-        best = {(Tile)tile, (uint32_t)rt, (uint32_t)ct, (uint32_t)s, (uint32_t)passes};
+        best = {(Tile)tile, (uint32_t)rt, (uint32_t)ct, (uint32_t)s, (uint32_t)passes,
+                (uint32_t)slabs};
       }
     }
   }
   return best;
+}
+
+void set_plan(TileIn& t, const Plan& p) {
+  t.slabs = p.slabs, t.passes = p.passes;
+  t.rtiles = p.rtiles, t.ctiles = p.ctiles, t.splits = p.splits;
+}
+
+// A gradient's classes in pieces, and the shapes and splits of its products of a whole one.
+// The pieces are all of one size (a small last one, in a few workgroups, took as
+// long as 0.17 of a whole one: 8,192 rows of 1,024 against 131,071, 8.43 ms a training
+// pass, now 8.29), whole rows of dw's tiles each, with `workspace` bytes of G at most, but for its
+// rows and columns to whole tiles, whatever their shape is.
+struct GradPlan {
+  size_t n, d, planes, np, piece, pieces, gcols;  // np x gcols: G, in whole tiles
+  bool f32;
+  int cus;
+  Plan px, pw;
+};
+GradPlan grad_plan(size_t n, size_t d, size_t k, bool f32, int cus, size_t workspace) {
+  GradPlan g{};
+  g.n = n, g.d = d, g.f32 = f32, g.cus = cus;
+  g.planes = f32 ? 4 : 1;
+  g.np = up(n, ALL_ROWS);
+  const size_t most = std::max<size_t>(ALL_COLS, workspace / (2 * g.np * g.planes));
+  g.pieces = (k + most - 1) / most;
+  g.piece = g.pieces == 1 ? k : up((k + g.pieces - 1) / g.pieces, ALL_ROWS);
+  g.gcols = up(g.piece, ALL_COLS);
+  g.px = plan_of(n, d, (g.piece + SLAB - 1) / SLAB, f32, cus, true);
+  g.pw = plan_of(g.piece, d, (n + SLAB - 1) / SLAB, f32, cus, true);
+  return g;
+}
+// The products of a piece of m classes.
+Plan logits_plan(const GradPlan& g, size_t m) {
+  return plan_of(g.n, m, up(g.d, SLAB) / SLAB, g.f32, g.cus, false);
+}
+Plan dx_plan(const GradPlan& g, size_t m) {
+  Plan p = g.px;
+  p.slabs = (uint32_t)((m + SLAB - 1) / SLAB);
+  // The last piece may have fewer steps than the others have splits. (Their sums, of
+  // all splits, are there by then: it adds to the first of them.)
+  p.splits = std::min(p.splits, p.slabs * p.passes);
+  return p;
+}
+Plan dw_plan(const GradPlan& g, size_t m) {
+  Plan p = g.pw;
+  p.rtiles = (uint32_t)((m + TILE_ROWS[p.tile] - 1) / TILE_ROWS[p.tile]);
+  return p;
 }
 
 void join_splits(emh_ctx* c, const float* part, uint32_t splits, size_t rows, size_t cols, size_t ldp,
@@ -557,8 +606,7 @@ void launch_cross_entropy(emh_ctx* c, const XentIn& in, float* loss, float* lse)
     LogitArgs a{};
     a.t.r = lx.deep(in.x, r0, m);
     a.t.c = lw.deep(in.w, 0, k);
-    a.t.slabs = (uint32_t)slabs, a.t.passes = p.passes;
-    a.t.rtiles = p.rtiles, a.t.ctiles = p.ctiles, a.t.splits = 1;
+    set_plan(a.t, p);
     a.n = (uint32_t)m, a.m = a.k = (uint32_t)k;
     a.labels = in.labels + r0;
     a.scale = in.scale;
@@ -582,19 +630,9 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
     EMH_HIP(hipGetLastError());
     return;
   }
-  const size_t slabs = up(d, SLAB) / SLAB, planes = f32 ? 4 : 1;
-  // The classes in pieces of one size (a small last one, in a few workgroups, took as
-  // long as 0.17 of a whole one: 8,192 rows of 1,024 against 131,071, 8.43 ms a training
-  // pass, now 8.29), whole rows of dw's tiles each, with 1 GB of G at most, but for its
-  // rows and columns to whole tiles, whatever their shape is.
-  const size_t np = up(n, ALL_ROWS);
-  const size_t most = std::max<size_t>(ALL_COLS, (size_t(512) << 20) / (np * planes));
-  const size_t pieces = (k + most - 1) / most;
-  const size_t piece = pieces == 1 ? k : up((k + pieces - 1) / pieces, ALL_ROWS);
-  const size_t gcols = up(piece, ALL_COLS), ldg = gcols * 2, ldp = up(d, 4);
-  const Plan px = plan_of(n, d, (piece + SLAB - 1) / SLAB, f32, c->cus, true);
-  const Plan pw = plan_of(piece, d, (n + SLAB - 1) / SLAB, f32, c->cus, true);
-  const bool px_part = px.splits > 1 || pieces > 1, pw_part = pw.splits > 1;
+  const GradPlan gp = grad_plan(n, d, k, f32, c->cus, c->xent_workspace);
+  const size_t planes = gp.planes, piece = gp.piece, ldg = gp.gcols * 2, ldp = up(d, 4);
+  const bool px_part = gp.px.splits > 1 || gp.pieces > 1, pw_part = gp.pw.splits > 1;
   // Rows without a label: see OddRows.
   const bool x_as_is = direct(in.x, d, true);
   Carve w;
@@ -609,14 +647,14 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
     counts = w.take<uint32_t>(MANY_COUNTS);
     lx.size(w, in.x, n, d, true);
     lw.size(w, in.w, k, d, !direct(in.w, d, true));
-    for (size_t i = 0; i < planes; i++) G[i] = w.take<char>(np * ldg);
-    if (dx.p && px_part) partx = w.take<float>(px.splits * n * ldp);
-    if (dw.p && pw_part) partw = w.take<float>((size_t)pw.splits * piece * ldp);
+    for (size_t i = 0; i < planes; i++) G[i] = w.take<char>(gp.np * ldg);
+    if (dx.p && px_part) partx = w.take<float>(gp.px.splits * n * ldp);
+    if (dw.p && pw_part) partw = w.take<float>((size_t)gp.pw.splits * piece * ldp);
     if (pass == 0) w.base = (char*)c->xent.get(w.used);
   }
   const uint32_t call = ++c->xent_calls;
   pack(c, in, x_as_is ? Laid{} : lx, lw, in.labels);
-  const Plan first = plan_of(n, std::min(piece, k), slabs, f32, c->cus, false);
+  const Plan first = logits_plan(gp, std::min(piece, k));
   const size_t waves = (size_t)first.rtiles * TILE_WAVES[first.tile];
   const bool counted = !f32 && !gloss && waves <= MANY_COUNTS;
   if (!counted) {
@@ -628,14 +666,14 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
   const Laid& xl = x_as_is ? as_is : lx;
   for (size_t v0 = 0; v0 < k; v0 += piece) {
     const size_t m = std::min(piece, k - v0);
-    const Plan pg = plan_of(n, m, slabs, f32, c->cus, false);
-    if ((size_t)pg.rtiles * TILE_ROWS[pg.tile] > np || (size_t)pg.ctiles * TILE_COLS[pg.tile] > gcols)
+    const Plan pg = logits_plan(gp, m), px = dx_plan(gp, m), pw = dw_plan(gp, m);
+    if ((size_t)pg.rtiles * TILE_ROWS[pg.tile] > gp.np ||
+        (size_t)pg.ctiles * TILE_COLS[pg.tile] > gp.gcols)
       throw Failure("cross_entropy_grad: tiles beyond the piece");
     LogitArgs a{};
     a.t.r = xl.deep(in.x, 0, n);
     a.t.c = lw.deep(in.w, v0, m);
-    a.t.slabs = (uint32_t)slabs, a.t.passes = pg.passes;
-    a.t.rtiles = pg.rtiles, a.t.ctiles = pg.ctiles, a.t.splits = 1;
+    set_plan(a.t, pg);
     a.n = (uint32_t)n, a.m = (uint32_t)m, a.col0 = (uint32_t)v0, a.k = (uint32_t)k;
     a.labels = in.labels;
     a.scale = in.scale;
@@ -656,12 +694,10 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
     if (counted) p.counts = counts, p.ncounts = (uint32_t)waves;
     p.cols = (uint32_t)d, p.ldp = ldp;
     if (dx.p) {
-      p.t.r = {{G[0], G[1]}, (uint32_t)ldg, (uint32_t)n, 0};
+      p.t.r = {{G[0], G[f32 ? 1 : 0]}, (uint32_t)ldg, (uint32_t)n, 0};
       p.t.c = lw.deep(in.w, v0, m);
       p.t.c.wide = lw.packed ? lw.dp : (uint32_t)d;
-      p.t.slabs = (uint32_t)((m + SLAB - 1) / SLAB);
-      p.t.rtiles = px.rtiles, p.t.ctiles = px.ctiles, p.t.splits = px.splits;
-      p.t.passes = px.passes;
+      set_plan(p.t, px);
       p.rows = (uint32_t)n, p.dw = false;
       p.ex = lx.ex;
       p.out = dx.p, p.ldo = dx.ld;
@@ -673,14 +709,12 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
       launch_copy_rows(c, odd, (uint32_t)n, in.labels, (uint32_t)k);
     }
     if (dw.p) {
-      p.t.r = {{G[0], G[1]}, (uint32_t)ldg, up(n, SLAB), (uint32_t)gcols};
+      p.t.r = {{G[0], G[f32 ? 1 : 0]}, (uint32_t)ldg, up(n, SLAB), (uint32_t)gp.gcols};
       p.gb[0] = G[2], p.gb[1] = G[3];
       p.ex = a.ew;
       p.t.c = xl.deep(in.x, 0, n);
       p.t.c.wide = xl.packed ? xl.dp : (uint32_t)d;
-      p.t.slabs = (uint32_t)((n + SLAB - 1) / SLAB);
-      p.t.rtiles = ((uint32_t)m + TILE_ROWS[pw.tile] - 1) / TILE_ROWS[pw.tile];
-      p.t.ctiles = pw.ctiles, p.t.splits = pw.splits, p.t.passes = pw.passes;
+      set_plan(p.t, pw);
       p.rows = (uint32_t)m, p.dw = true;
       p.out = (char*)dw.p + v0 * dw.ld * kind_bytes(dw.kind), p.ldo = dw.ld;
       p.part = pw_part ? partw : nullptr;
@@ -694,8 +728,26 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
       if (pw_part) join_splits(c, partw, pw.splits, m, d, ldp, p.out, dw.ld, dw.kind);
     }
   }
-  if (dx.p && px_part) join_splits(c, partx, px.splits, n, d, ldp, dx.p, dx.ld, dx.kind);
+  if (dx.p && px_part) join_splits(c, partx, gp.px.splits, n, d, ldp, dx.p, dx.ld, dx.kind);
   EMH_HIP(hipGetLastError());
+}
+
+std::vector<emh_xent_product> cross_entropy_products(size_t n, size_t d, size_t k, bool f32, int cus,
+                                                     size_t workspace) {
+  std::vector<emh_xent_product> out;
+  if (n == 0) return out;
+  const GradPlan gp = grad_plan(n, d, k, f32, cus, workspace);
+  auto add = [&](int what, const Plan& p, size_t v0, size_t m) {
+    out.push_back({what, TILE_ROWS[p.tile], TILE_COLS[p.tile], p.rtiles, p.ctiles, p.splits, p.slabs,
+                   p.passes, 0, n, v0, m});
+  };
+  for (size_t v0 = 0; v0 < k; v0 += gp.piece) {
+    const size_t m = std::min(gp.piece, k - v0);
+    add(EMH_XENT_LOGITS, logits_plan(gp, m), v0, m);
+    add(EMH_XENT_DX, dx_plan(gp, m), v0, m);
+    add(EMH_XENT_DW, dw_plan(gp, m), v0, m);
+  }
+  return out;
 }
 
 }  // namespace emh

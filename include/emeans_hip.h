@@ -384,12 +384,16 @@ int emh_cross_entropy(emh_ctx* ctx, const emh_buf* x, size_t ldx, size_t n, size
  * lse[i]) - [v = labels[i]]), zero in rows without a label: dx_i = sum_v g_iv
  * w_v (n x d), dw_v = sum_i g_iv x_i (k x d), both of x's kind, overwritten; either
  * may be NULL. A row without a label has no part in dw, whatever it holds.
- * The logits are computed again, for pieces of the classes. The sums' order
- * depends on the sizes alone. */
+ * The logits are computed again, for pieces of the classes (emh_set_xent_workspace).
+ * The sums' order depends on the sizes and the workspace alone. */
 int emh_cross_entropy_grad(emh_ctx* ctx, const emh_buf* x, size_t ldx, size_t n, size_t d,
                            const emh_buf* w, size_t ldw, size_t k, const emh_buf* labels,
                            float scale, const emh_buf* lse, const emh_buf* gloss, emh_buf* dx,
                            size_t lddx, emh_buf* dw, size_t lddw);
+
+/* The most bytes that a gradient's softmax of a piece of the classes may take (default
+ * 1 GiB; 0: the default): the fewer, the more pieces, of 768 classes at least. */
+int emh_set_xent_workspace(emh_ctx* ctx, uint64_t bytes);
 
 /* One tensor of an AdamW step. param: f32, f16 or bf16; grad: f32, f16 or bf16,
  * as long. copy (f16 or bf16, as long, may be NULL) gets the new parameters
@@ -449,6 +453,20 @@ uint64_t emh_host_plan_revival(const float* usage, uint64_t k, double tau, uint3
                                uint32_t* pairs);
 /* numpy_sum_f32 (model.rs:970-1002): numpy's pairwise f32 sum. */
 float emh_host_numpy_sum_f32(const float* a, uint64_t n);
+/* The tiled products that emh_cross_entropy_grad queues for both gradients of these
+ * sizes on a device of `cus` CUs, in their order (the first `cap` written to out):
+ * rows (row0 ..) by classes (class0 ..), over a depth of `slabs` slabs of 64, taken
+ * `passes` times one after another, the slabs * passes steps dealt to `splits`. */
+#define EMH_XENT_LOGITS 0 /* over d */
+#define EMH_XENT_DX 1     /* rows by d, over the classes */
+#define EMH_XENT_DW 2     /* classes by d, over the rows */
+typedef struct emh_xent_product {
+  int what; /* EMH_XENT_* */
+  uint32_t tile_rows, tile_cols, row_tiles, col_tiles, splits, slabs, passes;
+  uint64_t row0, rows, class0, classes;
+} emh_xent_product;
+int emh_host_xent_products(uint64_t n, uint64_t d, uint64_t k, int kind, int cus, uint64_t workspace,
+                           emh_xent_product* out, uint64_t cap, uint64_t* count);
 
 /* ------------------------------------------------------------ diagnostics */
 /* Which screen a top-1 or top-k call ran (emh_screen_report.variant). */
