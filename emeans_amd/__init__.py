@@ -499,9 +499,9 @@ class AdamW:
 
     def close(self):
         """Free the plan (not the tensors)."""
-        if self._h and self._dev._ctx:
-            check(lib().emh_adamw_destroy(self._h))
-        self._h = None
+        h, self._h = self._h, None
+        if h:
+            check(lib().emh_adamw_destroy(h))
 
     def __del__(self):
         try:

@@ -14,6 +14,7 @@
 #include <vector>
 
 #include "emh_internal.h"
+#include "emh_learn.h"
 
 namespace {
 thread_local std::string g_last_error;
@@ -354,6 +355,7 @@ int emh_destroy(emh_ctx* c) {
     (void)hipStreamSynchronize(c->stream);
     if (c->copy_stream)
       (void)hipStreamSynchronize(c->copy_stream);  // copies may still read pinned staging
+    emh::drop_plans(c);
     for (emh::Scratch* s : {&c->cand, &c->fblist, &c->order, &c->start, &c->misc, &c->knn_tmp,
                             &c->xnorm, &c->bigj, &c->chunkcnt, &c->tickets,
                             &c->preview_ticket, &c->xsplit, &c->xsplit_norm, &c->csplit, &c->csplit_norm, &c->csplit_part,

@@ -211,6 +211,7 @@ struct emh_buf {
   mutable bool exposed = false;
 };
 
+struct emh_adamw;
 struct emh_ctx {
   int device = 0;
   hipStream_t stream = nullptr;
@@ -255,6 +256,7 @@ struct emh_ctx {
   // carved from a block kept between calls, since hipFree waits for the
   // whole device, the other contexts' streams included.
   emh::Scratch trun, kpp, iscore, cnorm;
+  std::vector<emh_adamw*> plans;  // made with it and not destroyed (emh_learn.cpp)
   uint32_t xent_calls = 0;  // gradients of the cross entropy so far (see SW_ODD_ROW)
   emh::Scratch norm_part;  // layer_norm_grad: the blocks' sums of dweight and dbias
   emh::Scratch xent;       // cross_entropy's parts, gradients of a piece and laid-out operands

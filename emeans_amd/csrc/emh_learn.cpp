@@ -5,12 +5,13 @@
 #include <cmath>
 #include <exception>
 #include <memory>
+#include <mutex>
 #include <vector>
 
 #include "emh_learn.h"
 
 struct emh_adamw {
-  emh_ctx* ctx = nullptr;
+  emh_ctx* ctx = nullptr;  // null once it is destroyed
   emh::AdamTensor* tensors = nullptr;  // on the device
   uint2* chunks = nullptr;
   size_t nchunks = 0, chunk = emh::ADAM_CHUNK;
@@ -34,6 +35,16 @@ int guard(F&& f) {
     emh::set_last_error("unknown error");
     return EMH_ERROR;
   }
+}
+
+// A context's list of plans: a plan may be destroyed on another thread than its context.
+std::mutex g_plans_mu;
+
+void free_tables(emh_adamw* p) {
+  if (p->tensors) (void)hipFree(p->tensors);
+  if (p->chunks) (void)hipFree(p->chunks);
+  p->tensors = nullptr;
+  p->chunks = nullptr;
 }
 
 void use_device(emh_ctx* c) { EMH_HIP(hipSetDevice(c->device)); }
@@ -387,10 +398,16 @@ int emh_adamw_create(emh_ctx* c, const emh_adamw_tensor* tensors, size_t count, 
                                hipMemcpyHostToDevice, c->stream));
         EMH_HIP(hipStreamSynchronize(c->stream));  // the host's tables go away
       } catch (...) {
-        if (plan->tensors) (void)hipFree(plan->tensors);
-        if (plan->chunks) (void)hipFree(plan->chunks);
+        free_tables(plan.get());
         throw;
       }
+    }
+    std::lock_guard<std::mutex> g(g_plans_mu);
+    try {
+      c->plans.push_back(plan.get());
+    } catch (...) {
+      free_tables(plan.get());
+      throw;
     }
     *out = plan.release();
   });
@@ -399,6 +416,7 @@ int emh_adamw_create(emh_ctx* c, const emh_adamw_tensor* tensors, size_t count, 
 int emh_adamw_step(emh_adamw* plan, const emh_adamw_config* cfg) {
   return guard([&] {
     EMH_ENSURE(plan && cfg, "null argument");
+    EMH_ENSURE(plan->ctx, "the plan's context is destroyed");
     EMH_ENSURE(cfg->step >= 1, "step counts from 1");
     EMH_ENSURE(cfg->beta1 >= 0 && cfg->beta1 < 1 && cfg->beta2 >= 0 && cfg->beta2 < 1,
                "beta1 and beta2 must be in [0, 1)");
@@ -424,11 +442,26 @@ int emh_adamw_destroy(emh_adamw* plan) {
   return guard([&] {
     if (!plan) return;
     std::unique_ptr<emh_adamw> hold(plan);
+    std::lock_guard<std::mutex> g(g_plans_mu);
+    if (!plan->ctx) return;  // its context went first, and the tables with it
+    auto& plans = plan->ctx->plans;
+    plans.erase(std::remove(plans.begin(), plans.end(), plan), plans.end());
     use_device(plan->ctx);
-    EMH_HIP(hipStreamSynchronize(plan->ctx->stream));  // a queued step may read the tables
-    if (plan->tensors) EMH_HIP(hipFree(plan->tensors));
-    if (plan->chunks) EMH_HIP(hipFree(plan->chunks));
+    const hipError_t e = hipStreamSynchronize(plan->ctx->stream);  // a queued step may read the tables
+    free_tables(plan);
+    EMH_HIP(e);
   });
 }
 
 }  // extern "C"
+
+namespace emh {
+void drop_plans(emh_ctx* c) {
+  std::lock_guard<std::mutex> g(g_plans_mu);
+  for (emh_adamw* p : c->plans) {
+    free_tables(p);
+    p->ctx = nullptr;
+  }
+  c->plans.clear();
+}
+}  // namespace emh

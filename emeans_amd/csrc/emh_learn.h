@@ -68,6 +68,9 @@ struct AdamScalars {
 // flight a thread, or, in a plan of few elements, one, and four times the workgroups.
 constexpr size_t ADAM_CHUNK = 4096, ADAM_CHUNK_FEW = 1024;
 constexpr size_t ADAM_FEW = size_t(2) << 20;
+// The plans made with c step no more, and what they hold on the device is freed (c's
+// stream is idle).
+void drop_plans(emh_ctx* c);
 // chunks[i]: the tensor and the chunk in it that workgroup i takes.
 void launch_adamw(emh_ctx* c, const AdamTensor* tensors, const uint2* chunks, size_t nchunks,
                   size_t chunk, const AdamScalars& s);

@@ -418,9 +418,9 @@ typedef struct emh_adamw_config {
   uint64_t step;     /* 1 for the first */
 } emh_adamw_config;
 typedef struct emh_adamw emh_adamw;
-/* A plan over count tensors, which keeps their addresses: the buffers outlive it,
- * and it its context's last step. No tensor that the step writes may overlap
- * another. */
+/* A plan over count tensors, which keeps their addresses: the buffers outlive its last
+ * step. Once its context is destroyed it is refused there (and still to be destroyed).
+ * No tensor that the step writes may overlap another. */
 int emh_adamw_create(emh_ctx* ctx, const emh_adamw_tensor* tensors, size_t count, emh_adamw** out);
 /* One step over all of them, in one launch: g = grad_scale grad, m = beta1 m + (1 - beta1) g,
  * v = beta2 v + (1 - beta2) g^2, param = param (1 - lr weight_decay) - lr
