@@ -367,8 +367,7 @@ int emh_adamw_create(emh_ctx* c, const emh_adamw_tensor* tensors, size_t count, 
         chunks.push_back(make_uint2((unsigned)table.size(), (unsigned)k));
       table.push_back(a);
     }
-    EMH_ENSURE(chunks.size() < (size_t(1) << 31) && table.size() < (size_t(1) << 31),
-               "too many elements for one plan");
+    EMH_ENSURE(chunks.size() < (size_t(1) << 24), "too many tensors or elements for one plan");
     // What is written is written once.
     std::sort(written.begin(), written.end(),
               [](const Written& a, const Written& b) { return a.r.lo < b.r.lo; });

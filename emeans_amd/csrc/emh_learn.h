@@ -20,6 +20,11 @@ struct MatOut {
   int kind = EMH_F32;
 };
 
+// A launch has fewer than 2^32 threads (more are cut off without an error): the most
+// workgroups of 256 or 1,024 that a kernel whose work may exceed that is given, which
+// strides over the rest.
+constexpr size_t MAX_GROUPS = size_t(1) << 21;
+
 // ---- emh_norm.hip
 void launch_layer_norm(emh_ctx* c, const MatIn& x, size_t rows, size_t d, const MatIn& weight,
                        const MatIn& bias, float eps, const MatOut& y, float* mean, float* rstd);

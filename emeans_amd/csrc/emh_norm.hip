@@ -275,43 +275,48 @@ __global__ __launch_bounds__(TB, TB / 256) void k_norm_grad(const NormArgs a) {
 template <class T>
 __global__ __launch_bounds__(256) void k_norm_wide(const NormArgs a) {
   __shared__ float red[4][4];
-  const T* x = reinterpret_cast<const T*>(a.x) + (size_t)blockIdx.x * a.ldx;
-  T* y = reinterpret_cast<T*>(a.y) + (size_t)blockIdx.x * a.ldy;
-  float s = 0.f;
-  for (int i = threadIdx.x; i < a.d; i += 256) s += to_f32(x[i]);
-  const float mean = row_sum<256, 256>(s, red, 0) / (float)a.d;
-  float q = 0.f;
-  for (int i = threadIdx.x; i < a.d; i += 256) {
-    const float o = to_f32(x[i]) - mean;
-    q = fmaf(o, o, q);
+  // (A row's second sum has a barrier between the reads of the first and the next row's.)
+  for (size_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T* x = reinterpret_cast<const T*>(a.x) + row * a.ldx;
+    T* y = reinterpret_cast<T*>(a.y) + row * a.ldy;
+    float s = 0.f;
+    for (int i = threadIdx.x; i < a.d; i += 256) s += to_f32(x[i]);
+    const float mean = row_sum<256, 256>(s, red, 0) / (float)a.d;
+    float q = 0.f;
+    for (int i = threadIdx.x; i < a.d; i += 256) {
+      const float o = to_f32(x[i]) - mean;
+      q = fmaf(o, o, q);
+    }
+    const float rstd = 1.0f / sqrtf(row_sum<256, 256>(q, red, 1) / (float)a.d + a.eps);
+    for (int i = threadIdx.x; i < a.d; i += 256) {
+      const float h = (to_f32(x[i]) - mean) * rstd;
+      y[i] = from_f32<T>(fmaf(h, a.w ? load_kind(a.w, a.wkind, i) : 1.f,
+                              a.b ? load_kind(a.b, a.bkind, i) : 0.f));
+    }
+    if (threadIdx.x == 0 && a.mean) a.mean[row] = mean;
+    if (threadIdx.x == 0 && a.rstd) a.rstd[row] = rstd;
   }
-  const float rstd = 1.0f / sqrtf(row_sum<256, 256>(q, red, 1) / (float)a.d + a.eps);
-  for (int i = threadIdx.x; i < a.d; i += 256) {
-    const float h = (to_f32(x[i]) - mean) * rstd;
-    y[i] = from_f32<T>(fmaf(h, a.w ? load_kind(a.w, a.wkind, i) : 1.f,
-                            a.b ? load_kind(a.b, a.bkind, i) : 0.f));
-  }
-  if (threadIdx.x == 0 && a.mean) a.mean[blockIdx.x] = mean;
-  if (threadIdx.x == 0 && a.rstd) a.rstd[blockIdx.x] = rstd;
 }
 template <class T>
 __global__ __launch_bounds__(256) void k_norm_grad_wide(const NormArgs a) {
   __shared__ float red[4][4];
-  const T* x = reinterpret_cast<const T*>(a.x) + (size_t)blockIdx.x * a.ldx;
-  const T* dy = reinterpret_cast<const T*>(a.dy) + (size_t)blockIdx.x * a.lddy;
-  T* o = reinterpret_cast<T*>(a.y) + (size_t)blockIdx.x * a.ldy;
-  const float mean = a.mean[blockIdx.x], rstd = a.rstd[blockIdx.x];
-  float c1 = 0.f, c2 = 0.f;
-  for (int i = threadIdx.x; i < a.d; i += 256) {
-    const float u = to_f32(dy[i]) * (a.w ? load_kind(a.w, a.wkind, i) : 1.f);
-    c1 += u;
-    c2 = fmaf(u, (to_f32(x[i]) - mean) * rstd, c2);
-  }
-  c1 = row_sum<256, 256>(c1, red, 0) / (float)a.d;
-  c2 = row_sum<256, 256>(c2, red, 1) / (float)a.d;
-  for (int i = threadIdx.x; i < a.d; i += 256) {
-    const float u = to_f32(dy[i]) * (a.w ? load_kind(a.w, a.wkind, i) : 1.f);
-    o[i] = from_f32<T>(rstd * (u - c1 - (to_f32(x[i]) - mean) * rstd * c2));
+  for (size_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T* x = reinterpret_cast<const T*>(a.x) + row * a.ldx;
+    const T* dy = reinterpret_cast<const T*>(a.dy) + row * a.lddy;
+    T* o = reinterpret_cast<T*>(a.y) + row * a.ldy;
+    const float mean = a.mean[row], rstd = a.rstd[row];
+    float c1 = 0.f, c2 = 0.f;
+    for (int i = threadIdx.x; i < a.d; i += 256) {
+      const float u = to_f32(dy[i]) * (a.w ? load_kind(a.w, a.wkind, i) : 1.f);
+      c1 += u;
+      c2 = fmaf(u, (to_f32(x[i]) - mean) * rstd, c2);
+    }
+    c1 = row_sum<256, 256>(c1, red, 0) / (float)a.d;
+    c2 = row_sum<256, 256>(c2, red, 1) / (float)a.d;
+    for (int i = threadIdx.x; i < a.d; i += 256) {
+      const float u = to_f32(dy[i]) * (a.w ? load_kind(a.w, a.wkind, i) : 1.f);
+      o[i] = from_f32<T>(rstd * (u - c1 - (to_f32(x[i]) - mean) * rstd * c2));
+    }
   }
 }
 // Their sums over rows: a thread a column, blockIdx.y a share of the rows.
@@ -340,22 +345,27 @@ __global__ __launch_bounds__(1024) void k_norm_sums(const float* __restrict__ pa
                                                     int dbkind) {
   __shared__ float s[64][17];
   const int c = threadIdx.x & 15, g = threadIdx.x >> 4;
-  const int col = blockIdx.x * 16 + c;
-  float v = 0.f;
-  if (col < 2 * d) {
+  const size_t cols = (size_t)d * 2;
+  for (size_t c0 = (size_t)blockIdx.x * 16; c0 < cols; c0 += (size_t)gridDim.x * 16) {
+    const size_t col = c0 + c;
+    float v = 0.f;
+    if (col < cols) {
 #pragma unroll 8
-    for (int i = g; i < nparts; i += 64) v += part[(size_t)i * 2 * d + col];
-  }
-  s[g][c] = v;
-  __syncthreads();
-  if (g != 0 || col >= 2 * d) return;
-  v = 0.f;
+      for (int i = g; i < nparts; i += 64) v += part[(size_t)i * cols + col];
+    }
+    s[g][c] = v;
+    __syncthreads();
+    if (g == 0 && col < cols) {
+      v = 0.f;
 #pragma unroll
-  for (int i = 0; i < 64; i++) v += s[i][c];
-  if (col < d) {
-    if (dw) store_kind(dw, dwkind, col, v);
-  } else if (db) {
-    store_kind(db, dbkind, col - d, v);
+      for (int i = 0; i < 64; i++) v += s[i][c];
+      if (col < (size_t)d) {
+        if (dw) store_kind(dw, dwkind, col, v);
+      } else if (db) {
+        store_kind(db, dbkind, col - d, v);
+      }
+    }
+    __syncthreads();  // the next columns' sums take their place
   }
 }
 // No rows: the sums are zero.
@@ -424,7 +434,8 @@ void launch_layer_norm(emh_ctx* c, const MatIn& x, size_t rows, size_t d, const 
       const size_t blocks = std::min((rows + G - 1) / G, (size_t)c->cus * 8);
       k_norm<T, S::LPR, S::NV><<<dim3((unsigned)blocks), 256, 0, c->stream>>>(a);
     });
-    if (!held) k_norm_wide<T><<<dim3((unsigned)rows), 256, 0, c->stream>>>(a);
+    if (!held)
+      k_norm_wide<T><<<dim3((unsigned)std::min(rows, MAX_GROUPS)), 256, 0, c->stream>>>(a);
   });
   EMH_HIP(hipGetLastError());
 }
@@ -476,11 +487,12 @@ void launch_layer_norm_grad(emh_ctx* c, const MatIn& dy, const MatIn& x, size_t 
       a.part = (float*)c->norm_part.get(parts * 2 * d * 4);
       k_norm_cols<T><<<dim3((unsigned)((d + 255) / 256), (unsigned)parts), 256, 0, c->stream>>>(a);
     }
-    if (dx.p) k_norm_grad_wide<T><<<dim3((unsigned)rows), 256, 0, c->stream>>>(a);
+    if (dx.p)
+      k_norm_grad_wide<T><<<dim3((unsigned)std::min(rows, MAX_GROUPS)), 256, 0, c->stream>>>(a);
   });
   if (sums)
-    k_norm_sums<<<grid1(2 * d, 16), 1024, 0, c->stream>>>(a.part, (int)parts, (int)d, dweight.p,
-                                                          dweight.kind, dbias.p, dbias.kind);
+    k_norm_sums<<<dim3((unsigned)std::min((2 * d + 15) / 16, MAX_GROUPS)), 1024, 0, c->stream>>>(
+        a.part, (int)parts, (int)d, dweight.p, dweight.kind, dbias.p, dbias.kind);
   EMH_HIP(hipGetLastError());
 }
 

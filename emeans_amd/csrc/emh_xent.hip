@@ -30,6 +30,12 @@ struct PackOne {
   const uint32_t* labels;
   char *hi, *lo;
   int* ex;
+  uint32_t blocks;
+  // A wave's first row, and from one to the next.
+  __device__ __forceinline__ size_t first(uint32_t block) const {
+    return (size_t)block * 4 + (threadIdx.x >> 6);
+  }
+  __device__ __forceinline__ size_t step() const { return (size_t)blocks * 4; }
 };
 struct PackArgs {  // both operands in one launch, the first's workgroups first
   PackOne m[2];
@@ -41,16 +47,16 @@ template <class T>
 __global__ __launch_bounds__(256) void k_pack16(const PackArgs a) {
   const bool second = blockIdx.x >= a.first;
   const PackOne& m = a.m[second ? 1 : 0];
-  const size_t i = (size_t)(blockIdx.x - (second ? a.first : 0)) * 4 + (threadIdx.x >> 6);
-  if (i >= m.n) return;
   const uint32_t lane = threadIdx.x & 63;
-  const T* row = reinterpret_cast<const T*>(m.x) + i * m.ld;
-  T* out = reinterpret_cast<T*>(m.hi) + i * a.dp;
-  const bool zero = m.labels && m.labels[i] >= a.k;
-  for (uint32_t c = lane * 8; c < a.dp; c += 512) {
-    Vec<T> v{make_uint4(0u, 0u, 0u, 0u)};
-    if (!zero && c < a.d) v = c + 8 <= a.d ? load_vec(row + c) : load_some(row + c, (int)(a.d - c));
-    *reinterpret_cast<uint4*>(out + c) = v.raw;
+  for (size_t i = m.first(blockIdx.x - (second ? a.first : 0)); i < m.n; i += m.step()) {
+    const T* row = reinterpret_cast<const T*>(m.x) + i * m.ld;
+    T* out = reinterpret_cast<T*>(m.hi) + i * a.dp;
+    const bool zero = m.labels && m.labels[i] >= a.k;
+    for (uint32_t c = lane * 8; c < a.dp; c += 512) {
+      Vec<T> v{make_uint4(0u, 0u, 0u, 0u)};
+      if (!zero && c < a.d) v = c + 8 <= a.d ? load_vec(row + c) : load_some(row + c, (int)(a.d - c));
+      *reinterpret_cast<uint4*>(out + c) = v.raw;
+    }
   }
 }
 
@@ -61,56 +67,56 @@ __global__ __launch_bounds__(256) void k_pack16(const PackArgs a) {
 __global__ __launch_bounds__(256) void k_pack32(const PackArgs a) {
   const bool second = blockIdx.x >= a.first;
   const PackOne& m = a.m[second ? 1 : 0];
-  const size_t i = (size_t)(blockIdx.x - (second ? a.first : 0)) * 4 + (threadIdx.x >> 6);
-  if (i >= m.n) return;
   const uint32_t lane = threadIdx.x & 63, d = a.d, dp = a.dp;
-  const float* row = reinterpret_cast<const float*>(m.x) + i * m.ld;
-  const bool zero = m.labels && m.labels[i] >= a.k;
-  constexpr uint32_t HELD = 4;  // vectors of four a lane
-  auto get = [&](uint32_t c) __attribute__((always_inline)) {
-    Vec<float> v{make_uint4(0u, 0u, 0u, 0u)};
-    if (!zero && c < d) v = c + 4 <= d ? load_vec(row + c) : load_some(row + c, (int)(d - c));
-    return v;
-  };
-  auto largest = [](const Vec<float>& v, float top) __attribute__((always_inline)) {
+  for (size_t i = m.first(blockIdx.x - (second ? a.first : 0)); i < m.n; i += m.step()) {
+    const float* row = reinterpret_cast<const float*>(m.x) + i * m.ld;
+    const bool zero = m.labels && m.labels[i] >= a.k;
+    constexpr uint32_t HELD = 4;  // vectors of four a lane
+    auto get = [&](uint32_t c) __attribute__((always_inline)) {
+      Vec<float> v{make_uint4(0u, 0u, 0u, 0u)};
+      if (!zero && c < d) v = c + 4 <= d ? load_vec(row + c) : load_some(row + c, (int)(d - c));
+      return v;
+    };
+    auto largest = [](const Vec<float>& v, float top) __attribute__((always_inline)) {
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const float t = fabsf(v.get(e));
-      top = fmaxf(top, t < INFINITY ? t : 0.f);
-    }
-    return top;
-  };
-  Vec<float> held[HELD];
-  float top = 0.f;
+      for (int e = 0; e < 4; e++) {
+        const float t = fabsf(v.get(e));
+        top = fmaxf(top, t < INFINITY ? t : 0.f);
+      }
+      return top;
+    };
+    Vec<float> held[HELD];
+    float top = 0.f;
 #pragma unroll
-  for (uint32_t q = 0; q < HELD; q++) held[q] = get(lane * 4 + q * 256);
+    for (uint32_t q = 0; q < HELD; q++) held[q] = get(lane * 4 + q * 256);
 #pragma unroll
-  for (uint32_t q = 0; q < HELD; q++) top = largest(held[q], top);
-  for (uint32_t c = lane * 4 + HELD * 256; c < d; c += 256) top = largest(get(c), top);
-  top = lanes_max<64>(top);
-  // (A row of zeros takes the least exponent, which is no one's largest.)
-  const int e0 = top > 0.f ? max(ilogbf(top) - 13, XENT_LEAST) : XENT_LEAST;
-  const float by = ldexpf(1.f, -e0);
-  auto put = [&](uint32_t c, const Vec<float>& v) __attribute__((always_inline)) {
-    uint16_t h4[4], l4[4];
+    for (uint32_t q = 0; q < HELD; q++) top = largest(held[q], top);
+    for (uint32_t c = lane * 4 + HELD * 256; c < d; c += 256) top = largest(get(c), top);
+    top = lanes_max<64>(top);
+    // (A row of zeros takes the least exponent, which is no one's largest.)
+    const int e0 = top > 0.f ? max(ilogbf(top) - 13, XENT_LEAST) : XENT_LEAST;
+    const float by = ldexpf(1.f, -e0);
+    auto put = [&](uint32_t c, const Vec<float>& v) __attribute__((always_inline)) {
+      uint16_t h4[4], l4[4];
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const float t = v.get(e) * by;
-      const f16 h = (f16)t;
-      h4[e] = __builtin_bit_cast(uint16_t, h);
-      l4[e] = __builtin_bit_cast(uint16_t, (f16)(t - (float)h));
-    }
-    const size_t o = (i * dp + c) * 2;
-    *reinterpret_cast<uint2*>(m.hi + o) =
-        make_uint2(h4[0] | (uint32_t)h4[1] << 16, h4[2] | (uint32_t)h4[3] << 16);
-    *reinterpret_cast<uint2*>(m.lo + o) =
-        make_uint2(l4[0] | (uint32_t)l4[1] << 16, l4[2] | (uint32_t)l4[3] << 16);
-  };
+      for (int e = 0; e < 4; e++) {
+        const float t = v.get(e) * by;
+        const f16 h = (f16)t;
+        h4[e] = __builtin_bit_cast(uint16_t, h);
+        l4[e] = __builtin_bit_cast(uint16_t, (f16)(t - (float)h));
+      }
+      const size_t o = (i * dp + c) * 2;
+      *reinterpret_cast<uint2*>(m.hi + o) =
+          make_uint2(h4[0] | (uint32_t)h4[1] << 16, h4[2] | (uint32_t)h4[3] << 16);
+      *reinterpret_cast<uint2*>(m.lo + o) =
+          make_uint2(l4[0] | (uint32_t)l4[1] << 16, l4[2] | (uint32_t)l4[3] << 16);
+    };
 #pragma unroll
-  for (uint32_t q = 0; q < HELD; q++)
-    if (lane * 4 + q * 256 < dp) put(lane * 4 + q * 256, held[q]);
-  for (uint32_t c = lane * 4 + HELD * 256; c < dp; c += 256) put(c, get(c));
-  if (lane == 0) m.ex[i] = e0;
+    for (uint32_t q = 0; q < HELD; q++)
+      if (lane * 4 + q * 256 < dp) put(lane * 4 + q * 256, held[q]);
+    for (uint32_t c = lane * 4 + HELD * 256; c < dp; c += 256) put(c, get(c));
+    if (lane == 0) m.ex[i] = e0;
+  }
 }
 
 // The call's state, by one workgroup: a pass over the labels and weights, and of f32
@@ -346,21 +352,23 @@ template <class T>
 __global__ __launch_bounds__(256) void k_splits(const float* __restrict__ part, uint32_t splits,
                                                 size_t rows, uint32_t cols, size_t ldp, T* out,
                                                 size_t ldo) {
-  const size_t t = (size_t)blockIdx.x * 256 + threadIdx.x;
-  const size_t per = ldp / 4, i = t / per;
-  if (i >= rows) return;
-  const uint32_t j = (uint32_t)(t % per) * 4;
-  if (j >= cols) return;
-  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  const size_t per = ldp / 4;
+  for (size_t t = (size_t)blockIdx.x * 256 + threadIdx.x; t < rows * per;
+       t += (size_t)gridDim.x * 256) {
+    const size_t i = t / per;
+    const uint32_t j = (uint32_t)(t % per) * 4;
+    if (j >= cols) continue;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (uint32_t s = 0; s < splits; s++) {
-    const float4 p = *reinterpret_cast<const float4*>(part + (s * rows + i) * ldp + j);
-    v[0] += p.x, v[1] += p.y, v[2] += p.z, v[3] += p.w;
-  }
-  T* o = out + i * ldo + j;
+    for (uint32_t s = 0; s < splits; s++) {
+      const float4 p = *reinterpret_cast<const float4*>(part + (s * rows + i) * ldp + j);
+      v[0] += p.x, v[1] += p.y, v[2] += p.z, v[3] += p.w;
+    }
+    T* o = out + i * ldo + j;
 #pragma unroll
-  for (int e = 0; e < 4; e++)
-    if (j + e < cols) o[e] = from_f32<T>(v[e]);
+    for (int e = 0; e < 4; e++)
+      if (j + e < cols) o[e] = from_f32<T>(v[e]);
+  }
 }
 
 // Scratch of one call, 256-byte aligned pieces (first sized, then taken).
@@ -417,8 +425,9 @@ void pack(emh_ctx* c, const XentIn& in, const Laid& x, const Laid& w, const uint
   PackArgs a{};
   unsigned blocks = 0;
   auto add = [&](PackOne& m, const MatIn& from, size_t rows, const Laid& to, const uint32_t* lab) {
-    m = {from.p, from.ld, rows, lab, to.p[0], to.p[1], to.ex};
-    blocks += (unsigned)((rows + 3) / 4);
+    m = {from.p, from.ld, rows, lab, to.p[0], to.p[1], to.ex,
+         (uint32_t)std::min((rows + 3) / 4, MAX_GROUPS)};
+    blocks += m.blocks;
     a.dp = to.dp;
   };
   if (x.packed) add(a.m[0], in.x, in.n, x, labels);
@@ -498,6 +507,7 @@ Plan plan_of(size_t rows, size_t cols, size_t slabs, bool planes, int cus, bool 
     const size_t passes = planes && !both ? 3 : 1, steps = passes * slabs;
     for (size_t s = 1; s <= (may_split ? 32 : 1); s++) {
       if (s > 1 && steps < 4 * s) break;
+      if (rt * ct * s >= size_t(1) << 23) break;  // (512 threads each: a launch's limit)
       const double rounds = std::ceil((double)(rt * ct * s) / ((double)cus * PER_CU[tile]));
       double us = rounds * ((double)((steps + s - 1) / s) * (both ? STEP_BOTH : STEP[tile]) + 4.0);
       if (s > 1) us += 3.0 + 1.2e-6 * (double)s * (double)rows * (double)cols;
@@ -508,6 +518,7 @@ Plan plan_of(size_t rows, size_t cols, size_t slabs, bool planes, int cus, bool 
       }
     }
   }
+  if (least == 1e300) throw Failure("cross_entropy: more tiles than a launch holds");
   return best;
 }
 
@@ -560,7 +571,7 @@ Plan dw_plan(const GradPlan& g, size_t m) {
 
 void join_splits(emh_ctx* c, const float* part, uint32_t splits, size_t rows, size_t cols, size_t ldp,
                  void* out, size_t ldo, int kind) {
-  const dim3 grid = grid1(rows * (ldp / 4), 256);
+  const dim3 grid((unsigned)std::min((rows * (ldp / 4) + 255) / 256, MAX_GROUPS));
   if (kind == EMH_F32)
     k_splits<float><<<grid, 256, 0, c->stream>>>(part, splits, rows, (uint32_t)cols, ldp, (float*)out, ldo);
   else if (kind == EMH_F16)

@@ -72,6 +72,14 @@ def test_any_sizes():
         check(n, d, k, r.choice([_lib.EMH_F32, _lib.EMH_BF16]), workspace)
 
 
+def test_a_launch_holds_the_tiles():
+    """Fewer than 2^32 threads of at most 512 a tile, at sizes whose matrices fit a device."""
+    for n, d, k in ((1 << 30, 1, 2), (1 << 30, 64, 1), (100, 1, 1 << 30), (1 << 24, 1024, 5)):
+        for kind in (_lib.EMH_F32, _lib.EMH_BF16):
+            for p in products(n, d, k, kind):
+                assert p.row_tiles * p.col_tiles * p.splits < 1 << 23, (n, d, k, kind, p.what)
+
+
 def test_refusals():
     lib, count = _lib.lib(), C.c_uint64()
     for bad in ((1, 0, 1, 0, CUS), (1, 1, 0, 0, CUS), (1, 1, 1, _lib.EMH_U32, CUS), (1, 1, 1, 0, 0),
