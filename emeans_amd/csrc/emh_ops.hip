@@ -10,6 +10,8 @@
 // so one wave owns a row: its lanes square the elements in parallel into LDS
 // and one lane adds them in order.
 
+#include <algorithm>
+
 #include "emh_halves.h"
 #include "emh_internal.h"
 
@@ -21,8 +23,9 @@ constexpr int WAVES = 4;   // waves per workgroup
 constexpr int CH = 1024;   // elements per LDS chunk of one row
 
 __global__ __launch_bounds__(256) void k_fill_u32(uint32_t* p, size_t n, uint32_t v) {
-  size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i < n) p[i] = v;
+  for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n;
+       i += (size_t)gridDim.x * blockDim.x)
+    p[i] = v;
 }
 
 constexpr int NU = CH / WAVE;  // values per lane in one chunk
@@ -652,7 +655,9 @@ void launch_gather_rows(emh_ctx* c, const float* x, size_t nx, size_t d, const u
 
 void launch_fill_u32(emh_ctx* c, uint32_t* p, size_t n, uint32_t v) {
   if (n == 0) return;
-  hipLaunchKernelGGL(k_fill_u32, grid1(n, 256), dim3(256), 0, c->stream, p, n, v);
+  // (A launch of 2^32 threads would be cut off without an error.)
+  const dim3 grid = grid1(std::min(n, size_t(1) << 31), 256);
+  hipLaunchKernelGGL(k_fill_u32, grid, dim3(256), 0, c->stream, p, n, v);
   EMH_HIP(hipGetLastError());
 }
 

@@ -85,3 +85,15 @@ def test_cross_entropy_of_very_many_rows(dev):
     tol = 16 * U * (1 + np.abs(z).max(1))
     assert np.all(np.abs(got[at] - want) <= tol) and np.all(np.abs(got_lse[at] - lse64) <= tol)
     assert np.all(got_lse != 0.0) and not got[::1001].any()
+
+
+def test_zeros_of_more_than_a_launch_of_words(dev):
+    """On memory that was not zero before, where the allocator gives the same again."""
+    from emeans_amd import F8
+    n = (1 << 34) + 1027
+    for _ in range(2):
+        b = dev.zeros(n, F8)
+        for lo in (0, (1 << 34) - 1500, n - 1027):
+            assert not dev.read(b, (lo, lo + 1000)).any()
+            dev.write(b, lo, np.full(1000, 7, np.uint8))
+        del b
