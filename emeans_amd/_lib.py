@@ -85,7 +85,8 @@ class XentProduct(C.Structure):
     _fields_ = [("what", C.c_int), ("tile_rows", C.c_uint32), ("tile_cols", C.c_uint32),
                 ("row_tiles", C.c_uint32), ("col_tiles", C.c_uint32), ("splits", C.c_uint32),
                 ("slabs", C.c_uint32), ("passes", C.c_uint32), ("row0", C.c_uint64),
-                ("rows", C.c_uint64), ("class0", C.c_uint64), ("classes", C.c_uint64)]
+                ("rows", C.c_uint64), ("class0", C.c_uint64), ("classes", C.c_uint64),
+                ("softmax_bytes", C.c_uint64)]
 
 
 class AdamTensor(C.Structure):

@@ -80,7 +80,7 @@ constexpr int XENT_BIAS = 4096;  // (so that zero is less than any)
 
 struct LogitArgs {
   TileIn t;
-  uint32_t n, m;    // rows, classes of the piece
+  uint32_t n, m;    // rows of the block, classes of the piece
   uint32_t col0, k; // its first class, all classes
   const uint32_t* labels;
   float scale;
@@ -115,9 +115,9 @@ struct ProdArgs {
   float scale;
   void* out;            // the result in its kind, or
   size_t ldo;           // (elements)
-  float* part;          // one split's sums: [split][row][ldp] in f32
-  size_t ldp;
-  bool add;             // into what an earlier piece left
+  float* part;          // one split's sums: [split][part_rows][ldp] in f32
+  size_t ldp, part_rows;
+  bool add;             // into what an earlier piece or block left
   const uint32_t* flag; // dw: where it is `call`, x is read from alt
   uint32_t call;
   Operand alt;

@@ -527,46 +527,65 @@ void set_plan(TileIn& t, const Plan& p) {
   t.rtiles = p.rtiles, t.ctiles = p.ctiles, t.splits = p.splits;
 }
 
-// A gradient's classes in pieces, and the shapes and splits of its products of a whole one.
-// The pieces are all of one size (a small last one, in a few workgroups, took as
+// A gradient's classes in pieces and its rows in blocks, and the shapes and splits of the
+// products of a whole block and piece. What bounds them is G's bytes, `workspace` (and a
+// sixteenth more, for whole tiles of every shape; 256 x 768 of it at least). The
+// pieces are all of one size (a small last one, in a few workgroups, took as
 // long as 0.17 of a whole one: 8,192 rows of 1,024 against 131,071, 8.43 ms a training
-// pass, now 8.29), whole rows of dw's tiles each, with `workspace` bytes of G at most, but for its
-// rows and columns to whole tiles, whatever their shape is.
+// pass, now 8.29), whole rows of dw's tiles each. The rows are one block where 768 classes
+// of them fit, else blocks of one size that hold up to CUT_COLS classes: deep enough
+// for both products, whose sums over blocks and pieces are added in memory.
 struct GradPlan {
-  size_t n, d, planes, np, piece, pieces, gcols;  // np x gcols: G, in whole tiles
+  size_t n, d, planes, pieces, piece, blocks, block, grows, gcols;  // G: grows x gcols
   bool f32;
   int cus;
   Plan px, pw;
 };
+constexpr size_t CUT_COLS = 5 * ALL_COLS;
 GradPlan grad_plan(size_t n, size_t d, size_t k, bool f32, int cus, size_t workspace) {
   GradPlan g{};
   g.n = n, g.d = d, g.f32 = f32, g.cus = cus;
   g.planes = f32 ? 4 : 1;
-  g.np = up(n, ALL_ROWS);
-  const size_t most = std::max<size_t>(ALL_COLS, workspace / (2 * g.np * g.planes));
+  const size_t room = workspace / (2 * g.planes);  // elements of G
+  g.blocks = 1, g.block = n;
+  if (up(n, ALL_ROWS) > room / ALL_COLS) {
+    const size_t cols = std::min<size_t>(up(k, ALL_COLS), CUT_COLS);
+    const size_t rows = std::max<size_t>(ALL_ROWS, room / cols / ALL_ROWS * ALL_ROWS);
+    g.blocks = (n + rows - 1) / rows;
+    if (g.blocks > 1) g.block = up((n + g.blocks - 1) / g.blocks, ALL_ROWS);
+    g.blocks = (n + g.block - 1) / g.block;
+  }
+  g.grows = up(g.block, ALL_ROWS);
+  size_t most = std::max<size_t>(ALL_COLS, room / g.grows);
+  if (most < 16 * ALL_COLS) most -= most % ALL_COLS;
   g.pieces = (k + most - 1) / most;
   g.piece = g.pieces == 1 ? k : up((k + g.pieces - 1) / g.pieces, ALL_ROWS);
+  g.pieces = (k + g.piece - 1) / g.piece;
   g.gcols = up(g.piece, ALL_COLS);
-  g.px = plan_of(n, d, (g.piece + SLAB - 1) / SLAB, f32, cus, true);
-  g.pw = plan_of(g.piece, d, (n + SLAB - 1) / SLAB, f32, cus, true);
+  g.px = plan_of(g.block, d, (g.piece + SLAB - 1) / SLAB, f32, cus, true);
+  g.pw = plan_of(g.piece, d, (g.block + SLAB - 1) / SLAB, f32, cus, true);
   return g;
 }
-// The products of a piece of m classes.
-Plan logits_plan(const GradPlan& g, size_t m) {
-  return plan_of(g.n, m, up(g.d, SLAB) / SLAB, g.f32, g.cus, false);
+// The products of a block of nr rows and a piece of m classes. A last one may have fewer
+// steps than the others have splits. (Their sums, of all splits, are there by then: it
+// adds to the first of them.)
+Plan logits_plan(const GradPlan& g, size_t nr, size_t m) {
+  return plan_of(nr, m, up(g.d, SLAB) / SLAB, g.f32, g.cus, false);
 }
-Plan dx_plan(const GradPlan& g, size_t m) {
-  Plan p = g.px;
-  p.slabs = (uint32_t)((m + SLAB - 1) / SLAB);
-  // The last piece may have fewer steps than the others have splits. (Their sums, of
-  // all splits, are there by then: it adds to the first of them.)
+Plan cut(Plan p, size_t rows, size_t depth) {
+  p.rtiles = (uint32_t)((rows + TILE_ROWS[p.tile] - 1) / TILE_ROWS[p.tile]);
+  p.slabs = (uint32_t)((depth + SLAB - 1) / SLAB);
   p.splits = std::min(p.splits, p.slabs * p.passes);
   return p;
 }
-Plan dw_plan(const GradPlan& g, size_t m) {
-  Plan p = g.pw;
-  p.rtiles = (uint32_t)((m + TILE_ROWS[p.tile] - 1) / TILE_ROWS[p.tile]);
-  return p;
+Plan dx_plan(const GradPlan& g, size_t nr, size_t m) { return cut(g.px, nr, m); }
+Plan dw_plan(const GradPlan& g, size_t nr, size_t m) { return cut(g.pw, m, nr); }
+// f(first row, rows, first class, classes) for every block of every piece.
+template <class F>
+void by_part(const GradPlan& g, size_t k, F&& f) {
+  for (size_t v0 = 0; v0 < k; v0 += g.piece)
+    for (size_t r0 = 0; r0 < g.n; r0 += g.block)
+      f(r0, std::min(g.block, g.n - r0), v0, std::min(g.piece, k - v0));
 }
 
 void join_splits(emh_ctx* c, const float* part, uint32_t splits, size_t rows, size_t cols, size_t ldp,
@@ -595,7 +614,8 @@ void launch_cross_entropy(emh_ctx* c, const XentIn& in, float* loss, float* lse)
     return;
   }
   const size_t slabs = up(d, SLAB) / SLAB;
-  // Rows at a time: what bounds them is the parts' maxima and sums (512 MB).
+  // Rows at a time: what bounds them is the parts' maxima and sums (512 MB, or those of
+  // 256 rows: 32 bytes a class).
   const size_t all = (k + 127) / 128 * 2;
   const size_t rows = std::min(n, std::max<size_t>(256, ((size_t(64) << 20) / all) & ~(size_t)255));
   Carve w;
@@ -642,10 +662,11 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
     return;
   }
   const GradPlan gp = grad_plan(n, d, k, f32, c->cus, c->xent_workspace);
-  const size_t planes = gp.planes, piece = gp.piece, ldg = gp.gcols * 2, ldp = up(d, 4);
-  const bool px_part = gp.px.splits > 1 || gp.pieces > 1, pw_part = gp.pw.splits > 1;
-  // Rows without a label: see OddRows.
-  const bool x_as_is = direct(in.x, d, true);
+  const size_t planes = gp.planes, ldg = gp.gcols * 2, ldp = up(d, 4);
+  const bool px_part = gp.px.splits > 1 || gp.pieces > 1, pw_part = gp.pw.splits > 1 || gp.blocks > 1;
+  // Rows without a label: see OddRows. (Several blocks would need a flag each: their rows are
+  // laid out for the call.)
+  const bool x_as_is = direct(in.x, d, true) && gp.blocks == 1;
   Carve w;
   Laid lx, lw;
   XentState* st = nullptr;
@@ -658,16 +679,16 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
     counts = w.take<uint32_t>(MANY_COUNTS);
     lx.size(w, in.x, n, d, true);
     lw.size(w, in.w, k, d, !direct(in.w, d, true));
-    for (size_t i = 0; i < planes; i++) G[i] = w.take<char>(gp.np * ldg);
+    for (size_t i = 0; i < planes; i++) G[i] = w.take<char>(gp.grows * ldg);
     if (dx.p && px_part) partx = w.take<float>(gp.px.splits * n * ldp);
-    if (dw.p && pw_part) partw = w.take<float>((size_t)gp.pw.splits * piece * ldp);
+    if (dw.p && pw_part) partw = w.take<float>((size_t)gp.pw.splits * gp.piece * ldp);
     if (pass == 0) w.base = (char*)c->xent.get(w.used);
   }
   const uint32_t call = ++c->xent_calls;
   pack(c, in, x_as_is ? Laid{} : lx, lw, in.labels);
-  const Plan first = logits_plan(gp, std::min(piece, k));
+  const Plan first = logits_plan(gp, gp.block, gp.piece);
   const size_t waves = (size_t)first.rtiles * TILE_WAVES[first.tile];
-  const bool counted = !f32 && !gloss && waves <= MANY_COUNTS;
+  const bool counted = !f32 && !gloss && waves <= MANY_COUNTS && gp.blocks == 1;
   if (!counted) {
     k_survey<<<dim3(1), 1024, 0, c->stream>>>((uint32_t)n, in.labels, (uint32_t)k, gloss, lx.ex, lw.ex,
                                               st, c->small);
@@ -675,21 +696,20 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
   }
   Laid as_is;
   const Laid& xl = x_as_is ? as_is : lx;
-  for (size_t v0 = 0; v0 < k; v0 += piece) {
-    const size_t m = std::min(piece, k - v0);
-    const Plan pg = logits_plan(gp, m), px = dx_plan(gp, m), pw = dw_plan(gp, m);
-    if ((size_t)pg.rtiles * TILE_ROWS[pg.tile] > gp.np ||
+  by_part(gp, k, [&](size_t r0, size_t nr, size_t v0, size_t m) {
+    const Plan pg = logits_plan(gp, nr, m), px = dx_plan(gp, nr, m), pw = dw_plan(gp, nr, m);
+    if ((size_t)pg.rtiles * TILE_ROWS[pg.tile] > gp.grows ||
         (size_t)pg.ctiles * TILE_COLS[pg.tile] > gp.gcols)
       throw Failure("cross_entropy_grad: tiles beyond the piece");
     LogitArgs a{};
-    a.t.r = xl.deep(in.x, 0, n);
+    a.t.r = xl.deep(in.x, r0, nr);
     a.t.c = lw.deep(in.w, v0, m);
     set_plan(a.t, pg);
-    a.n = (uint32_t)n, a.m = (uint32_t)m, a.col0 = (uint32_t)v0, a.k = (uint32_t)k;
-    a.labels = in.labels;
+    a.n = (uint32_t)nr, a.m = (uint32_t)m, a.col0 = (uint32_t)v0, a.k = (uint32_t)k;
+    a.labels = in.labels + r0;
     a.scale = in.scale;
-    a.ex = lx.ex, a.ew = f32 ? lw.ex + v0 : nullptr;
-    a.lse = lse, a.gloss = gloss, a.st = st;
+    a.ex = f32 ? lx.ex + r0 : nullptr, a.ew = f32 ? lw.ex + v0 : nullptr;
+    a.lse = lse + r0, a.gloss = gloss ? gloss + r0 : nullptr, a.st = st;
     a.small = c->small;
     if (counted) a.counts = counts;
     OddRows odd{};
@@ -700,19 +720,20 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
     a.ldg = ldg;
     launch_logits(c->stream, a, in.x.kind, pg.tile, true);
     ProdArgs p{};
-    p.labels = in.labels, p.k = (uint32_t)k;
-    p.gloss = gloss, p.st = st, p.scale = in.scale;
+    p.labels = a.labels, p.k = (uint32_t)k;
+    p.gloss = a.gloss, p.st = st, p.scale = in.scale;
     if (counted) p.counts = counts, p.ncounts = (uint32_t)waves;
     p.cols = (uint32_t)d, p.ldp = ldp;
     if (dx.p) {
-      p.t.r = {{G[0], G[f32 ? 1 : 0]}, (uint32_t)ldg, (uint32_t)n, 0};
+      p.t.r = {{G[0], G[f32 ? 1 : 0]}, (uint32_t)ldg, (uint32_t)nr, 0};
       p.t.c = lw.deep(in.w, v0, m);
       p.t.c.wide = lw.packed ? lw.dp : (uint32_t)d;
       set_plan(p.t, px);
-      p.rows = (uint32_t)n, p.dw = false;
-      p.ex = lx.ex;
-      p.out = dx.p, p.ldo = dx.ld;
-      p.part = px_part ? partx : nullptr;
+      p.rows = (uint32_t)nr, p.dw = false;
+      p.ex = a.ex;
+      p.out = (char*)dx.p + r0 * dx.ld * kind_bytes(dx.kind), p.ldo = dx.ld;
+      p.part = px_part ? partx + r0 * ldp : nullptr;
+      p.part_rows = n;
       p.add = v0 > 0;
       p.odd = odd;
       launch_prod(c->stream, p, in.x.kind, px.tile);
@@ -720,25 +741,27 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
       launch_copy_rows(c, odd, (uint32_t)n, in.labels, (uint32_t)k);
     }
     if (dw.p) {
-      p.t.r = {{G[0], G[f32 ? 1 : 0]}, (uint32_t)ldg, up(n, SLAB), (uint32_t)gp.gcols};
+      p.t.r = {{G[0], G[f32 ? 1 : 0]}, (uint32_t)ldg, up(nr, SLAB), (uint32_t)gp.gcols};
       p.gb[0] = G[2], p.gb[1] = G[3];
       p.ex = a.ew;
-      p.t.c = xl.deep(in.x, 0, n);
+      p.t.c = xl.deep(in.x, r0, nr);
       p.t.c.wide = xl.packed ? xl.dp : (uint32_t)d;
       set_plan(p.t, pw);
       p.rows = (uint32_t)m, p.dw = true;
       p.out = (char*)dw.p + v0 * dw.ld * kind_bytes(dw.kind), p.ldo = dw.ld;
       p.part = pw_part ? partw : nullptr;
-      p.add = false;
+      p.part_rows = m;
+      p.add = r0 > 0;
       if (x_as_is) {
         p.flag = c->small + SW_ODD_ROW;
         p.call = call;
         p.alt = lx.deep(in.x, 0, n);
       }
       launch_prod(c->stream, p, in.x.kind, pw.tile);
-      if (pw_part) join_splits(c, partw, pw.splits, m, d, ldp, p.out, dw.ld, dw.kind);
+      if (pw_part && r0 + nr == n)
+        join_splits(c, partw, gp.pw.splits, m, d, ldp, p.out, dw.ld, dw.kind);
     }
-  }
+  });
   if (dx.p && px_part) join_splits(c, partx, gp.px.splits, n, d, ldp, dx.p, dx.ld, dx.kind);
   EMH_HIP(hipGetLastError());
 }
@@ -748,16 +771,15 @@ std::vector<emh_xent_product> cross_entropy_products(size_t n, size_t d, size_t 
   std::vector<emh_xent_product> out;
   if (n == 0) return out;
   const GradPlan gp = grad_plan(n, d, k, f32, cus, workspace);
-  auto add = [&](int what, const Plan& p, size_t v0, size_t m) {
-    out.push_back({what, TILE_ROWS[p.tile], TILE_COLS[p.tile], p.rtiles, p.ctiles, p.splits, p.slabs,
-                   p.passes, 0, n, v0, m});
-  };
-  for (size_t v0 = 0; v0 < k; v0 += gp.piece) {
-    const size_t m = std::min(gp.piece, k - v0);
-    add(EMH_XENT_LOGITS, logits_plan(gp, m), v0, m);
-    add(EMH_XENT_DX, dx_plan(gp, m), v0, m);
-    add(EMH_XENT_DW, dw_plan(gp, m), v0, m);
-  }
+  by_part(gp, k, [&](size_t r0, size_t nr, size_t v0, size_t m) {
+    auto add = [&](int what, const Plan& p) {
+      out.push_back({what, TILE_ROWS[p.tile], TILE_COLS[p.tile], p.rtiles, p.ctiles, p.splits,
+                     p.slabs, p.passes, r0, nr, v0, m, gp.grows * gp.gcols * 2 * gp.planes});
+    };
+    add(EMH_XENT_LOGITS, logits_plan(gp, nr, m));
+    add(EMH_XENT_DX, dx_plan(gp, nr, m));
+    add(EMH_XENT_DW, dw_plan(gp, nr, m));
+  });
   return out;
 }
 

@@ -135,7 +135,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_grads(const ProdArgs a) {
             const uint32_t j = j0 + b * 32 + 8 * (2 * p + f) + 4 * h;
             if (j >= a.cols) continue;
             float4* o = reinterpret_cast<float4*>(
-                a.part + ((size_t)at.split * a.rows + i) * a.ldp + j);
+                a.part + (at.split * a.part_rows + i) * a.ldp + j);
             float4 s = make_float4(v[f][0], v[f][1], v[f][2], v[f][3]);
             if (a.add) {
               const float4 had = *o;

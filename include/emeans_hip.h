@@ -384,15 +384,18 @@ int emh_cross_entropy(emh_ctx* ctx, const emh_buf* x, size_t ldx, size_t n, size
  * lse[i]) - [v = labels[i]]), zero in rows without a label: dx_i = sum_v g_iv
  * w_v (n x d), dw_v = sum_i g_iv x_i (k x d), both of x's kind, overwritten; either
  * may be NULL. A row without a label has no part in dw, whatever it holds.
- * The logits are computed again, for pieces of the classes (emh_set_xent_workspace).
- * The sums' order depends on the sizes and the workspace alone. */
+ * The logits are computed again, for pieces of the classes and blocks of the rows
+ * (emh_set_xent_workspace). The sums' order depends on the sizes and the workspace alone. */
 int emh_cross_entropy_grad(emh_ctx* ctx, const emh_buf* x, size_t ldx, size_t n, size_t d,
                            const emh_buf* w, size_t ldw, size_t k, const emh_buf* labels,
                            float scale, const emh_buf* lse, const emh_buf* gloss, emh_buf* dx,
                            size_t lddx, emh_buf* dw, size_t lddw);
 
-/* The most bytes that a gradient's softmax of a piece of the classes may take (default
- * 1 GiB; 0: the default): the fewer, the more pieces, of 768 classes at least. */
+/* The bytes that a gradient's softmax of a piece of the classes and a block of the rows may
+ * take, and a sixteenth more (default 1 GiB; 0: the default). It is held in 2 bytes an
+ * element, 8 of f32 rows; 256 rows by 768 classes are taken at least. Beside it a
+ * gradient holds f32 sums of its results that more than one piece, block or part of
+ * a product adds to, and rows and classes laid out (2 bytes an element, 4 of f32). */
 int emh_set_xent_workspace(emh_ctx* ctx, uint64_t bytes);
 
 /* One tensor of an AdamW step. param: f32, f16 or bf16; grad: f32, f16 or bf16,
@@ -464,6 +467,7 @@ typedef struct emh_xent_product {
   int what; /* EMH_XENT_* */
   uint32_t tile_rows, tile_cols, row_tiles, col_tiles, splits, slabs, passes;
   uint64_t row0, rows, class0, classes;
+  uint64_t softmax_bytes; /* of a whole block and piece, in memory */
 } emh_xent_product;
 int emh_host_xent_products(uint64_t n, uint64_t d, uint64_t k, int kind, int cus, uint64_t workspace,
                            emh_xent_product* out, uint64_t cap, uint64_t* count);

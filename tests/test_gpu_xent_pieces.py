@@ -1,5 +1,5 @@
-"""The cross entropy's gradients in many pieces of the classes (a workspace that holds the
-least of them), the last of one class and more, against 64 bits."""
+"""The cross entropy's gradients in many pieces of the classes and blocks of the rows (a small
+workspace), the last of one class and more, against 64 bits."""
 
 import numpy as np
 import pytest
@@ -14,16 +14,23 @@ pytestmark = pytest.mark.gpu
 def dev():
     from emeans_amd import HipDevice
     d = HipDevice()
-    d.set_xent_workspace(1)
     yield d
     d.close()
 
 
+def _small(dev, n, name, blocks):
+    """Pieces of 768 classes of all rows, or blocks of 256 rows, too."""
+    planes = 4 if name == "f32" else 1
+    dev.set_xent_workspace(1 if blocks else -(-n // 256) * 256 * 768 * 2 * planes)
+
+
 # d = 64: rows as they lie; others are laid out. Few rows and columns: dx in splits.
 @pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("n,d", [(300, 40), (300, 64), (65, 500), (1000, 200)])
+@pytest.mark.parametrize("n,d", [(300, 40), (300, 64), (65, 500), (1000, 200), (513, 64)])
 @pytest.mark.parametrize("last", [1, 63, 65, 257])
-def test_a_short_last_piece(dev, name, n, d, last):
+@pytest.mark.parametrize("blocks", [False, True])
+def test_a_short_last_piece(dev, name, n, d, last, blocks):
+    _small(dev, n, name, blocks)
     k = 2 * 768 + last
     x, w, lab = _inputs(n, d, k, n + d + last)
     lab[:3] = k - 1, 767, 768
@@ -32,9 +39,20 @@ def test_a_short_last_piece(dev, name, n, d, last):
 
 
 @pytest.mark.parametrize("name", ["f32", "bf16"])
-def test_one_gradient_alone(dev, name):
+@pytest.mark.parametrize("n,k", [(300, 40), (1025, 1000)])
+def test_blocks_of_rows_alone(dev, name, n, k):
+    """All classes in one piece or two: dx as it comes, dw a sum over the blocks."""
+    _small(dev, n, name, True)
+    x, w, lab = _inputs(n, 50, k, n)
+    Run(dev, x, w, lab, name, pad=3).check()
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("blocks", [False, True])
+def test_one_gradient_alone(dev, name, blocks):
     from emeans_amd import F32
-    n, d, k = 200, 72, 2 * 768 + 5
+    n, d, k = 300, 72, 2 * 768 + 5
+    _small(dev, n, name, blocks)
     x, w, lab = _inputs(n, d, k, 5)
     both = Run(dev, x, w, lab, name).check()
     xb, wb = R.Padded(dev, x, name), R.Padded(dev, w, name)
@@ -48,10 +66,12 @@ def test_one_gradient_alone(dev, name):
 @pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("d", [40, 64])
 @pytest.mark.parametrize("want_dx", [False, True])
-def test_a_row_without_a_label_that_is_not_finite(dev, name, d, want_dx):
+@pytest.mark.parametrize("blocks", [False, True])
+def test_a_row_without_a_label_that_is_not_finite(dev, name, d, want_dx, blocks):
     """Found with the first piece, and kept out of dw in the others."""
     from emeans_amd import F32
     n, k = 300, 2 * 768 + 1
+    _small(dev, n, name, blocks)
     x, w, lab = _inputs(n, d, k, d)
     lab[[2, 299]] = NONE
     w[::3, 17] = 0.0

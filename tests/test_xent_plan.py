@@ -25,6 +25,8 @@ def products(n, d, k, kind, workspace=0):
 def check(n, d, k, kind, workspace=0):
     got = products(n, d, k, kind, workspace)
     area = {LOGITS: 0, DX: 0, DW: 0}
+    planes = 4 if kind == _lib.EMH_F32 else 1
+    most = max((workspace or 1 << 30) * 17 // 16, 256 * 768 * 2 * planes)
     for p in got:
         where = (n, d, k, kind, workspace, p.what, p.row0, p.rows, p.class0, p.classes)
         assert p.rows > 0 and p.classes > 0, where
@@ -38,6 +40,8 @@ def check(n, d, k, kind, workspace=0):
         # Every workgroup has a step: an empty split's loads would come from nowhere.
         assert 1 <= p.splits <= p.slabs * p.passes, where
         assert p.passes == 1 or (p.passes == 3 and kind == _lib.EMH_F32), where
+        # The softmax in memory holds the product, in the workspace.
+        assert p.rows * p.classes * 2 * planes <= p.softmax_bytes <= most, where
         area[p.what] += p.rows * p.classes
     assert all(a == n * k for a in area.values()), (n, d, k, kind, workspace)
 
@@ -67,9 +71,16 @@ def test_any_sizes():
     for _ in range(3000):
         n, d, k = size(1, 1_000_000), size(1, 4096), size(1, 3_000_000)
         workspace = r.choice([0, 0, 1, 1 << 20, 1 << 26, 1 << 32])
-        if n * k > (1 << 24) * max(1, workspace >> 6 or 1 << 24):  # (a few hundred pieces at most)
+        if n * k > 200 * max(1 << 17, (workspace or 1 << 30) >> 4):  # (a few hundred parts)
             continue
         check(n, d, k, r.choice([_lib.EMH_F32, _lib.EMH_BF16]), workspace)
+
+
+@pytest.mark.parametrize("kind", [_lib.EMH_F32, _lib.EMH_BF16])
+def test_many_rows_in_the_default_workspace(kind):
+    for n in (170_000, 200_000, 700_000, 1_000_000, 10_000_001):
+        for d, k in ((768, 1024), (40, 10), (64, 5000)):
+            check(n, d, k, kind)
 
 
 def test_a_launch_holds_the_tiles():
