@@ -476,10 +476,12 @@ class AdamTensor:
 
 class AdamW:
     """AdamW over many tensors in one launch: a plan that keeps their addresses
-    (and the buffers alive)."""
+    (and the buffers alive). seed: 8-bit states are rounded at random, by numbers
+    that follow from it and the step, as a training of more than a few steps needs
+    (emh_adamw_set_seed); without one to the nearest code."""
     BLOCK = EMH_ADAMW_BLOCK
 
-    def __init__(self, dev: HipDevice, tensors: List[AdamTensor]):
+    def __init__(self, dev: HipDevice, tensors: List[AdamTensor], seed: Optional[int] = None):
         self._h = None
         self._dev, self._tensors = dev, list(tensors)
         table = (_CAdamTensor * max(len(self._tensors), 1))()
@@ -490,6 +492,8 @@ class AdamW:
         h = C.c_void_p()
         check(lib().emh_adamw_create(dev._ctx, table, len(self._tensors), C.byref(h)))
         self._h = h
+        if seed is not None:
+            check(lib().emh_adamw_set_seed(h, seed))
 
     def step(self, lr: float, step: int, beta1: float = 0.9, beta2: float = 0.999,
              eps: float = 1e-8, grad_scale: float = 1.0):

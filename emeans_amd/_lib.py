@@ -135,6 +135,7 @@ SIGNATURES = {
     "emh_set_xent_workspace": (_i, [_vp, _u64]),
     "emh_adamw_create": (_i, [_vp, _vp, _sz, _pp]),
     "emh_adamw_step": (_i, [_vp, _vp]),
+    "emh_adamw_set_seed": (_i, [_vp, _u64]),
     "emh_adamw_destroy": (_i, [_vp]),
     "emh_buf_ptr": (_vp, [_vp]),
     "emh_buf_len": (_sz, [_vp]),

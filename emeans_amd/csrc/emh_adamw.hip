@@ -9,7 +9,9 @@
 // m and the root of v are what is held in 8 bits, as e4m3 codes times the block's
 // scale. The root, because its codes reach 2^17 below the block's largest (v
 // itself would need twice the exponents); a positive v never gets the code zero,
-// which would divide m by eps alone.
+// which would divide m by eps alone. Rounded to the nearest code, a state follows its
+// average only where a step moves it by half a code, which beta2 near 1 never does; a plan
+// with a seed rounds at random (RANDOM), in the proportion that keeps the mean.
 //
 // Bound by HBM: 28 bytes an element with f32 parameters, gradients and states,
 // 16 with 8-bit states, 10 with those and 16-bit parameters and gradients.
@@ -98,8 +100,9 @@ __device__ __forceinline__ void decode4(uint32_t w, float scale, float* v) {
 // and its remainder): a code one step off changes a small root by up to half, and
 // the parameter's step with it. A quotient is at most 448 (1 + 2^-23), which rounds to
 // 448; infinities and NaN become the NaN code.
-template <bool LEAST>
-__device__ __forceinline__ uint32_t encode4(const float* v, float& scale) {
+// RANDOM: the code above or below, as bits' top 20 decide.
+template <bool LEAST, bool RANDOM>
+__device__ __forceinline__ uint32_t encode4(const float* v, float& scale, const uint32_t* bits) {
   float top = lanes_max<64>(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))));
   top = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(top)));  // (the wave's)
   if (!(top < INFINITY)) {  // without the infinite ones (the maximum passes over NaN)
@@ -126,8 +129,41 @@ __device__ __forceinline__ uint32_t encode4(const float* v, float& scale) {
 #pragma unroll
     for (int e = 0; e < 4; e++) q[e] = v[e] > 0.f && q[e] < F8_LEAST ? F8_LEAST : q[e];
   }
+  if constexpr (RANDOM) {
+    // (Bits below the code's last are added to and cut off; past 448 lies the NaN.)
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+      q[e] = fabsf(q[e]) < INFINITY ? fminf(fmaxf(q[e], -F8_TOP), F8_TOP) : q[e];
+    int w = __builtin_amdgcn_cvt_sr_fp8_f32(q[0], (int)bits[0], 0, 0);
+    w = __builtin_amdgcn_cvt_sr_fp8_f32(q[1], (int)bits[1], w, 1);
+    w = __builtin_amdgcn_cvt_sr_fp8_f32(q[2], (int)bits[2], w, 2);
+    return (uint32_t)__builtin_amdgcn_cvt_sr_fp8_f32(q[3], (int)bits[3], w, 3);
+  }
   const uint32_t w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], (int)w, true);
+}
+
+// Random bits for a lane's four elements of block `block` of a tensor: for m, and, the
+// same backwards, for v (20 of 32 bits each count, the first twelve of them alone in one
+// of the two). Multiplications by odd numbers between shifts; of lanes, elements,
+// blocks, tensors and steps no two are correlated beyond chance over 2^20 samples.
+__device__ __forceinline__ uint32_t mixed(uint32_t h) {
+  h = (h ^ h >> 16) * 0x9E3779B1u;
+  h = (h ^ h >> 14) * 0xA2F9836Bu;
+  return h ^ h >> 15;
+}
+__device__ __forceinline__ void random4(const AdamScalars& s, uint32_t tensor, size_t block,
+                                        uint32_t* m, uint32_t* v) {
+  const uint32_t b = mixed(mixed(s.key0 + tensor) ^ (uint32_t)block) + s.key1 +
+                     (uint32_t)(block >> 32) * 0x9E3779B1u;
+  const uint32_t l = mixed(b ^ (threadIdx.x & 63));
+#pragma unroll
+  for (uint32_t e = 0; e < 4; e++) {
+    uint32_t h = l + e * 0x9E3779B1u;
+    h = (h ^ h >> 15) * 0xA2F9836Bu;
+    m[e] = h ^ h >> 16;
+    v[e] = __brev(m[e]);
+  }
 }
 
 // One element's step; r: the root of the new v.
@@ -187,8 +223,9 @@ __device__ __forceinline__ u32x4_any pack32(const float* v) {
 }
 
 // A whole chunk: every load goes out before the first is used.
-template <int U, bool P16, bool G16, bool EIGHT>
-__device__ __forceinline__ void whole_chunk(const AdamTensor& t, const AdamScalars& s, size_t base) {
+template <int U, bool P16, bool G16, bool EIGHT, bool RANDOM>
+__device__ __forceinline__ void whole_chunk(const AdamTensor& t, uint32_t tensor,
+                                            const AdamScalars& s, size_t base) {
   const float keep = (float)(1.0 - s.lr * t.weight_decay);
   const size_t i0 = base + threadIdx.x * 4;
   u32x4_any p4[P16 ? 1 : U], g4[G16 ? 1 : U], m4[EIGHT ? 1 : U], v4[EIGHT ? 1 : U];
@@ -247,7 +284,11 @@ __device__ __forceinline__ void whole_chunk(const AdamTensor& t, const AdamScala
     if (t.copy) gstore(t.copy, i * 2, pack16(p, t.copy_kind));
     if constexpr (EIGHT) {
       float ms, vs;
-      const uint32_t a = encode4<false>(m, ms), b = encode4<true>(r, vs);
+      uint32_t rm[4], rv[4];
+      if constexpr (RANDOM)
+        random4(s, tensor, (base >> 8) + u * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6),
+                rm, rv);
+      const uint32_t a = encode4<false, RANDOM>(m, ms, rm), b = encode4<true, RANDOM>(r, vs, rv);
       gstore<u32_any>(t.m, i, a);
       gstore<u32_any>(t.v, i, b);
       if ((threadIdx.x & 63) == 0) {
@@ -262,8 +303,9 @@ __device__ __forceinline__ void whole_chunk(const AdamTensor& t, const AdamScala
 }
 
 // A tensor's last chunk: fours that may be cut short.
-__device__ __forceinline__ void last_chunk(const AdamTensor& t, const AdamScalars& s, size_t base,
-                                           int count) {
+template <bool RANDOM>
+__device__ __forceinline__ void last_chunk(const AdamTensor& t, uint32_t tensor,
+                                           const AdamScalars& s, size_t base, int count) {
   const float keep = (float)(1.0 - s.lr * t.weight_decay);
   for (int o = (int)threadIdx.x * 4; o < ((count + 255) & ~255); o += 1024) {
     const int left = count - o;  // (whole waves come here together: a block's scale is theirs)
@@ -293,7 +335,9 @@ __device__ __forceinline__ void last_chunk(const AdamTensor& t, const AdamScalar
         m[e] = e < left ? m[e] : 0.f;
       }
       float ms, vs;
-      const uint32_t a = encode4<false>(m, ms), b = encode4<true>(r, vs);
+      uint32_t rm[4], rv[4];
+      if constexpr (RANDOM) random4(s, tensor, i / EMH_ADAMW_BLOCK, rm, rv);
+      const uint32_t a = encode4<false, RANDOM>(m, ms, rm), b = encode4<true, RANDOM>(r, vs, rv);
       store4_codes(t.m, i, left, a);
       store4_codes(t.v, i, left, b);
       if ((threadIdx.x & 63) == 0) {
@@ -308,8 +352,8 @@ __device__ __forceinline__ void last_chunk(const AdamTensor& t, const AdamScalar
 }
 
 // A chunk: 1024 U elements. 131,071 x 1,024 and two layers in bf16 with 8-bit states,
-// 10 bytes an element: 270 us, 5.0 TB/s; 256 x 384 f32 3.3 us, a launch.
-template <int U>
+// 10 bytes an element: 275 us, 4.9 TB/s, rounded at random 316; 256 x 384 f32 3.3 us, a launch.
+template <int U, bool RANDOM>
 __global__ __launch_bounds__(256) void k_adamw(const AdamTensor* __restrict__ tensors,
                                                const uint2* __restrict__ chunks,
                                                const AdamScalars s) {
@@ -318,33 +362,39 @@ __global__ __launch_bounds__(256) void k_adamw(const AdamTensor* __restrict__ te
   const size_t base = (size_t)at.y * (1024 * U);
   const size_t here = t.len - base;  // > 0
   if (here < (size_t)(1024 * U)) {
-    last_chunk(t, s, base, (int)here);
+    last_chunk<RANDOM>(t, at.x, s, base, (int)here);
     return;
   }
   const bool p16 = t.param_kind != EMH_F32, g16 = t.grad_kind != EMH_F32;
   if (t.m_scale) {
     if (p16)
-      g16 ? whole_chunk<U, true, true, true>(t, s, base) : whole_chunk<U, true, false, true>(t, s, base);
+      g16 ? whole_chunk<U, true, true, true, RANDOM>(t, at.x, s, base)
+          : whole_chunk<U, true, false, true, RANDOM>(t, at.x, s, base);
     else
-      g16 ? whole_chunk<U, false, true, true>(t, s, base) : whole_chunk<U, false, false, true>(t, s, base);
+      g16 ? whole_chunk<U, false, true, true, RANDOM>(t, at.x, s, base)
+          : whole_chunk<U, false, false, true, RANDOM>(t, at.x, s, base);
   } else {
     if (p16)
-      g16 ? whole_chunk<U, true, true, false>(t, s, base) : whole_chunk<U, true, false, false>(t, s, base);
+      g16 ? whole_chunk<U, true, true, false, RANDOM>(t, at.x, s, base)
+          : whole_chunk<U, true, false, false, RANDOM>(t, at.x, s, base);
     else
-      g16 ? whole_chunk<U, false, true, false>(t, s, base) : whole_chunk<U, false, false, false>(t, s, base);
+      g16 ? whole_chunk<U, false, true, false, RANDOM>(t, at.x, s, base)
+          : whole_chunk<U, false, false, false, RANDOM>(t, at.x, s, base);
   }
 }
 
 }  // namespace
 
 void launch_adamw(emh_ctx* c, const AdamTensor* tensors, const uint2* chunks, size_t nchunks,
-                  size_t chunk, const AdamScalars& s) {
+                  size_t chunk, bool random, const AdamScalars& s) {
   if (nchunks == 0) return;
   const dim3 grid((unsigned)nchunks);
+  auto go = [&](auto kernel) { kernel<<<grid, 256, 0, c->stream>>>(tensors, chunks, s); };
+  constexpr int MANY = (int)(ADAM_CHUNK / 1024), FEW = (int)(ADAM_CHUNK_FEW / 1024);
   if (chunk == ADAM_CHUNK)
-    k_adamw<(int)(ADAM_CHUNK / 1024)><<<grid, 256, 0, c->stream>>>(tensors, chunks, s);
+    random ? go(k_adamw<MANY, true>) : go(k_adamw<MANY, false>);
   else
-    k_adamw<(int)(ADAM_CHUNK_FEW / 1024)><<<grid, 256, 0, c->stream>>>(tensors, chunks, s);
+    random ? go(k_adamw<FEW, true>) : go(k_adamw<FEW, false>);
   EMH_HIP(hipGetLastError());
 }
 

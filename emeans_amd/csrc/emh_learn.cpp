@@ -15,6 +15,8 @@ struct emh_adamw {
   emh::AdamTensor* tensors = nullptr;  // on the device
   uint2* chunks = nullptr;
   size_t nchunks = 0, chunk = emh::ADAM_CHUNK;
+  bool random = false;  // emh_adamw_set_seed
+  uint64_t seed = 0;
   std::vector<emh_buf*> written;
 };
 
@@ -412,6 +414,14 @@ int emh_adamw_create(emh_ctx* c, const emh_adamw_tensor* tensors, size_t count, 
   });
 }
 
+int emh_adamw_set_seed(emh_adamw* plan, uint64_t seed) {
+  return guard([&] {
+    EMH_ENSURE(plan, "null argument");
+    plan->random = true;
+    plan->seed = seed;
+  });
+}
+
 int emh_adamw_step(emh_adamw* plan, const emh_adamw_config* cfg) {
   return guard([&] {
     EMH_ENSURE(plan && cfg, "null argument");
@@ -431,9 +441,16 @@ int emh_adamw_step(emh_adamw* plan, const emh_adamw_config* cfg) {
     s.eps = (float)cfg->eps;
     s.gscale = (float)cfg->grad_scale;
     s.lr = cfg->lr;
+    uint64_t key = plan->seed * 0xD1342543DE82EF95u + cfg->step * 0x9E3779B97F4A7C15u +
+                   0x632BE59BD9B4E019u;
+    for (int i = 0; i < 2; i++) key = (key ^ key >> 32) * 0xD6E8FEB86659FD93u;
+    key ^= key >> 32;
+    s.key0 = (uint32_t)key;
+    s.key1 = (uint32_t)(key >> 32);
     use_device(plan->ctx);
     for (emh_buf* b : plan->written) ++b->gen;
-    emh::launch_adamw(plan->ctx, plan->tensors, plan->chunks, plan->nchunks, plan->chunk, s);
+    emh::launch_adamw(plan->ctx, plan->tensors, plan->chunks, plan->nchunks, plan->chunk,
+                      plan->random, s);
   });
 }
 

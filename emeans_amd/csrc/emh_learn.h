@@ -68,6 +68,7 @@ struct AdamScalars {
   float beta1, beta2, new1, new2;  // new = 1 - beta
   float rate, root2, eps, gscale;  // lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t)
   double lr;
+  uint32_t key0, key1;             // of a step whose 8-bit states are rounded at random
 };
 // Elements of a workgroup's share of one tensor: four loads of each array in
 // flight a thread, or, in a plan of few elements, one, and four times the workgroups.
@@ -78,6 +79,6 @@ constexpr size_t ADAM_FEW = size_t(2) << 20;
 void drop_plans(emh_ctx* c);
 // chunks[i]: the tensor and the chunk in it that workgroup i takes.
 void launch_adamw(emh_ctx* c, const AdamTensor* tensors, const uint2* chunks, size_t nchunks,
-                  size_t chunk, const AdamScalars& s);
+                  size_t chunk, bool random, const AdamScalars& s);
 
 }  // namespace emh

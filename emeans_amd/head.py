@@ -38,8 +38,8 @@ def _encode(a, kind):
 class ClusterHead:
     """d: columns of the rows; k: clusters; kind: what rows and the classes' working
     copy are held as (F32, F16 or BF16; the parameters themselves are F32);
-    state_bits: 32, or 8 for AdamW states of one byte; centroids: k x d initial
-    weights (else small random ones); scale: factor of the logits."""
+    state_bits: 32, or 8 for AdamW states of one byte (rounded at random); centroids: k x d
+    initial weights (else small random ones); seed: of both random choices; scale: factor of the logits."""
 
     EPS = 1e-5
 
@@ -74,7 +74,7 @@ class ClusterHead:
         self._plan = AdamW(self.dev, [
             self._tensor(self.w, self._dw, state_bits, weight_decay, copy),
             self._tensor(self.norm_weight, self._dweight, state_bits, 0.0),
-            self._tensor(self.norm_bias, self._dbias, state_bits, 0.0)])
+            self._tensor(self.norm_bias, self._dbias, state_bits, 0.0)], seed=seed)
         self._rows = 0
 
     def _tensor(self, param, grad, bits, decay, copy=None):
