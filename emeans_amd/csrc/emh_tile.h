@@ -61,6 +61,8 @@ __device__ __forceinline__ v16f mfma16(bf16, v8s a, v8s b, v16f c) {
 }  // namespace
 
 constexpr int SLAB = 64;  // depth of a slab
+// What plane 1 of an f32 operand counts of plane 0's unit (emh_xent.h).
+constexpr float LOW_UNIT = 1.f / 2048;
 
 // A workgroup's shape: waves of NWR x NWC, each WB x WA blocks of 32 x 32.
 // STAGES slabs are in the ring.
@@ -119,7 +121,7 @@ struct Operand {
 struct TileIn {
   Operand r, c;
   uint32_t slabs;   // of the depth; one operand is zero past it
-  uint32_t passes;  // 1, or 3: planes (0, 0), (0, 1), (1, 0) one after another
+  uint32_t passes;  // 1, or 3: planes (0, 1), (1, 0), (0, 0) one after another
   uint32_t rtiles, ctiles, splits;  // workgroups: rtiles ctiles splits (at most slabs passes:
                                     // each has a step, whose loads go out unasked)
   // What a workgroup finds its tile by (prepare): divisions there, by whole words,
@@ -256,11 +258,14 @@ struct Side16 {
 // barrier, and the DMAs of the slab that takes the stage next (the one after the next,
 // with two) go out between its MFMAs.
 //
+// PLANES (f32): plane 1 counts LOW_UNIT, so the products with one are made first and
+// scaled once, when the (0, 0) follow or the split ends.
 // BOTH (f32's planes, where one pass over the depth can have them all in LDS): a stage
 // holds both planes of both operands, and a step takes the three products from it: two
-// thirds of the DMAs and of the LDS reads. (10,007 x 300 by 1,000: dx 37 us with three
+// thirds of the DMAs and of the LDS reads; the products with a plane 1 have sums of their
+// own. (10,007 x 300 by 1,000: dx 37 us with three
 // passes, 31 with both; dw 36 and 30.)
-template <class T, class S, bool RDEEP, bool CDEEP, bool BOTH>
+template <class T, class S, bool RDEEP, bool CDEEP, bool PLANES>
 __device__ __forceinline__ void tile_sums(const TileIn& t, const TileAt& at, char* ring,
                                           v16f (&acc)[S::WA][S::WB]) {
   const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -275,6 +280,7 @@ __device__ __forceinline__ void tile_sums(const TileIn& t, const TileAt& at, cha
   const size_t r0 = RDEEP ? (size_t)at.rt * S::TR * t.r.ld : 0;
   const size_t c0 = CDEEP ? (size_t)at.ct * S::TC * t.c.ld : 0;
   const uint32_t ldst = lds0 + (uint32_t)w * 1024;
+  constexpr bool BOTH = PLANES && takes_both<S>;
   constexpr int P = BOTH ? 2 : 1, STAGES = S::STAGES / P, STAGE = S::STAGE * P;
   static_assert(STAGES >= 2, "a stage to fill and one to read");
 
@@ -290,10 +296,10 @@ __device__ __forceinline__ void tile_sums(const TileIn& t, const TileAt& at, cha
     const int q = i % (S::RD + S::CD), plane = i / (S::RD + S::CD);
     const uint32_t to = ldst + lst + (uint32_t)plane * S::STAGE;
     if (q < S::RD)
-      R.dma(q, t.r.p[BOTH ? plane : lpass == 2 ? 1 : 0] + r0, t.r, lslab,
+      R.dma(q, t.r.p[BOTH ? plane : PLANES && lpass == 1 ? 1 : 0] + r0, t.r, lslab,
             to + (uint32_t)q * S::NW * 1024);
     else
-      C.dma(q - S::RD, t.c.p[BOTH ? plane : lpass == 1 ? 1 : 0] + c0, t.c, lslab,
+      C.dma(q - S::RD, t.c.p[BOTH ? plane : PLANES && lpass == 0 ? 1 : 0] + c0, t.c, lslab,
             to + S::RBYTES + (uint32_t)(q - S::RD) * S::NW * 1024);
   };
   auto advance = [&]() __attribute__((always_inline)) {
@@ -336,6 +342,13 @@ __device__ __forceinline__ void tile_sums(const TileIn& t, const TileAt& at, cha
   if constexpr (BOTH) {
     constexpr int ROWS = 2 * S::WB, READS = ROWS + 2 * S::WA, MS = 3 * S::WA;
     v8s op[2][READS];  // [row block][plane], then [column block][plane]
+    v16f low[S::WA][S::WB];
+#pragma unroll
+    for (int a = 0; a < S::WA; a++)
+#pragma unroll
+      for (int y = 0; y < S::WB; y++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) low[a][y][r] = 0.f;
     auto read = [&](int i, uint32_t stage, int ks) __attribute__((always_inline)) {
       const uint32_t at_plane = stage + (uint32_t)(i & 1) * S::STAGE;
       return i < ROWS ? R.read(at_plane, ks, i / 2) : C.read(at_plane, ks, (i - ROWS) / 2);
@@ -351,9 +364,11 @@ __device__ __forceinline__ void tile_sums(const TileIn& t, const TileAt& at, cha
         for (int m = 0; m < MS; m++) {  // (h, h) of every block, (h, l), (l, h)
           const int a = m % S::WA, pass = m / S::WA;
 #pragma unroll
-          for (int y = 0; y < S::WB; y++)
-            acc[a][y] = mfma16(T{}, op[ks & 1][ROWS + 2 * a + (pass == 1)],
-                               op[ks & 1][2 * y + (pass == 2)], acc[a][y]);
+          for (int y = 0; y < S::WB; y++) {
+            v16f& to = pass == 0 ? acc[a][y] : low[a][y];
+            to = mfma16(T{}, op[ks & 1][ROWS + 2 * a + (pass == 1)],
+                        op[ks & 1][2 * y + (pass == 2)], to);
+          }
           __builtin_amdgcn_sched_barrier(0);
           // The next step's operands by the middle of this one.
           constexpr int BY = (MS + 1) / 2;
@@ -372,13 +387,28 @@ __device__ __forceinline__ void tile_sums(const TileIn& t, const TileAt& at, cha
       advance();
       st = after(st);
     }
+#pragma unroll
+    for (int a = 0; a < S::WA; a++)
+#pragma unroll
+      for (int y = 0; y < S::WB; y++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) acc[a][y][r] = fmaf(low[a][y][r], LOW_UNIT, acc[a][y][r]);
   } else {
     v8s rb[2][S::WB], ca[S::WA];
 #pragma unroll
     for (int y = 0; y < S::WB; y++) rb[0][y] = R.read(0, 0, y);
 #pragma unroll
     for (int a = 0; a < S::WA; a++) ca[a] = C.read(0, 0, a);
+    auto units = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int a = 0; a < S::WA; a++)
+#pragma unroll
+        for (int y = 0; y < S::WB; y++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) acc[a][y][r] *= LOW_UNIT;
+    };
     for (uint32_t s = at.s0; s < at.s1; s++) {
+      if (PLANES && s == 2 * t.slabs) units();  // (at a split's first step the sums are zero)
 #pragma unroll
       for (int ks = 0; ks < 4; ks++) {
         if (ks == 3) meet();
@@ -404,6 +434,7 @@ __device__ __forceinline__ void tile_sums(const TileIn& t, const TileAt& at, cha
       advance();
       st = after(st);
     }
+    if (PLANES && at.s1 <= 2 * t.slabs) units();
   }
   wait_vm<0>();  // the DMAs past the last step have landed
   asm volatile("" ::: "memory");

@@ -12,11 +12,13 @@
 // rounded once to their type (f16: times a power of two that brings the largest
 // possible element to 2^13 .. 2^14, or the gradients of a mean over many rows would be
 // subnormal). float32 operands are two planes of f16: a row times a power of two
-// 2^-e that brings its largest element to 2^13 .. 2^14, h = f16(x), l = f16(x - h),
-// which hold 22 bits and more of every element down to 2^-26 of the row's
-// largest; h h + h l + l h leaves out 2^-22 of a product at most, as f32's own
-// rounding would over a few terms, and takes three MFMAs of the f16 rate where
-// the f32 MFMA takes sixteen.
+// 2^-e that brings its largest element to 2^13 .. 2^14, h = f16(x), l = f16(2^11 (x - h)),
+// which hold every element to 2^-22 of itself, or to 2^-49 of the row's largest where that is
+// more (an element below 2^-27 of it); h h + 2^-11 (h l + l h) leaves out 2^-22 of a product,
+// as f32's own rounding would over a few terms, and takes three MFMAs of the f16 rate
+// where the f32 MFMA takes sixteen. (Without the 2^11, l ends in f16's subnormals from
+// 2^-16 of the largest on: columns of 1e4 and 1e-4, which the classes make up for, left
+// logits 2e-3 off, now 1.3e-6, as f32 does; of 1e5 and 1e-5 0.2, now 1e-4.)
 // The exponents: z = sum 2^(ex_i + ew_v). The gradient products sum over the
 // class or the row, whose exponent then has to be in G, and the other one's may be. Where
 // all exponents together span little (XENT_SPAN; a row of zeros does not), one G
@@ -27,7 +29,7 @@
 //   Ga = G 2^(ew_v - ewmax + ga_i)  for dx_i = 2^(ewmax - ga_i) sum_v Ga w_v,
 //   Gb = G 2^(ex_i + gb)            for dw_v = 2^-gb sum_i Gb x_i,
 // with ga_i and gb such that the largest element is below 2^14: what is lost of
-// the others is 2^-39 of that (of G', 2^-39 of 2^SPAN times an element's own bound).
+// the others is 2^-50 of that (of G', 2^-50 of 2^SPAN times an element's own bound).
 // 10,007 x 300 by 1,000: with two G, 82 MB, their kernel takes 44 us, with one 38.
 #pragma once
 

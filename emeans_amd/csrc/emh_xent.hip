@@ -103,7 +103,7 @@ __global__ __launch_bounds__(256) void k_pack32(const PackArgs a) {
         const float t = v.get(e) * by;
         const f16 h = (f16)t;
         h4[e] = __builtin_bit_cast(uint16_t, h);
-        l4[e] = __builtin_bit_cast(uint16_t, (f16)(t - (float)h));
+        l4[e] = __builtin_bit_cast(uint16_t, (f16)((t - (float)h) * (1.f / LOW_UNIT)));
       }
       const size_t o = (i * dp + c) * 2;
       *reinterpret_cast<uint2*>(m.hi + o) =

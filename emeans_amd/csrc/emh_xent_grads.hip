@@ -47,7 +47,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_grads(const ProdArgs a) {
     one = a.st->one != 0;
     if (DW && !one) t.r.p[0] = a.gb[0], t.r.p[1] = a.gb[1];
   }
-  tile_sums<T, S, !DW, false, F32 && takes_both<S>>(t, at, ring, acc);
+  tile_sums<T, S, !DW, false, F32>(t, at, ring, acc);
 
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, li = lane & 31, h = lane >> 5;
   const int wr = w % S::NWR, wc = w / S::NWR;

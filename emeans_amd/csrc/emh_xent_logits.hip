@@ -46,7 +46,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_logits(const LogitArgs a) {
   __shared__ __attribute__((aligned(1024))) char ring[S::RING];
   const TileAt at = tile_at(a.t);
   v16f acc[S::WA][S::WB];
-  tile_sums<T, S, true, true, F32 && takes_both<S>>(a.t, at, ring, acc);
+  tile_sums<T, S, true, true, F32>(a.t, at, ring, acc);
 
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, li = lane & 31, h = lane >> 5;
   const int wr = w % S::NWR, wc = w / S::NWR;
@@ -196,7 +196,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_logits(const LogitArgs a) {
               for (int e = 0; e < 4; e++) {
                 float t = acc[b][y][4 * (2 * p + f) + e];
                 if constexpr (__is_same(T, f16)) t = ldexpf(t, by[e]);
-                g[f][e] = F32 && (plane & 1) ? t - (float)(f16)t : t;
+                g[f][e] = F32 && (plane & 1) ? (t - (float)(f16)t) * (1.f / LOW_UNIT) : t;
               }
             }
             const uint32_t chunk = (wc * S::WA + b) * 4 + 2 * p + h;

@@ -374,7 +374,10 @@ int emh_layer_norm_grad(emh_ctx* ctx, const emh_buf* dy, size_t lddy, const emh_
  * = scale x_i . w_v, lse[i] = log sum_v exp z_iv and loss[i] = lse[i] -
  * z_i,labels[i] (f32, n entries each). labels: a u32 each, 0xFFFFFFFF for a
  * row without one (loss 0); any other label >= k is an error at the next
- * synchronizing call (the row counts as one without a label). lse may be NULL. */
+ * synchronizing call (the row counts as one without a label). lse may be NULL.
+ * Bits: products and sums are f32. Of more than 64 rows f32 operands are held as two
+ * parts of f16: an element to 2^-22 of itself, or, where that is less, to 2^-49 of the
+ * largest of its row. */
 int emh_cross_entropy(emh_ctx* ctx, const emh_buf* x, size_t ldx, size_t n, size_t d,
                       const emh_buf* w, size_t ldw, size_t k, const emh_buf* labels, float scale,
                       emh_buf* loss, emh_buf* lse);
