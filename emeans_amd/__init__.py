@@ -298,12 +298,14 @@ class HipDevice:
     def cross_entropy_grad(self, x: DevBuf, n: int, d: int, w: DevBuf, k: int, labels: DevBuf,
                            lse: DevBuf, dx: Optional[DevBuf], dw: Optional[DevBuf],
                            gloss: Optional[DevBuf] = None, scale: float = 1.0, ldx: int = 0,
-                           ldw: int = 0, lddx: int = 0, lddw: int = 0):
+                           ldw: int = 0, lddx: int = 0, lddw: int = 0, loss_scale: float = 1.0):
         """The gradients of cross_entropy's losses weighted by gloss (F32), or of
         the mean over the rows with a label, into dx (n x d) and dw (k x d), of
-        x's kind; either may be None."""
-        check(lib().emh_cross_entropy_grad(self._ctx, x.h, ldx, n, d, w.h, ldw, k, labels.h, scale,
-                                           lse.h, _h(gloss), _h(dx), lddx, _h(dw), lddw))
+        x's kind; either may be None. loss_scale: factor of both, before they are
+        rounded (F16: a mean over many rows has gradients below its range)."""
+        check(lib().emh_cross_entropy_grad_scaled(
+            self._ctx, x.h, ldx, n, d, w.h, ldw, k, labels.h, scale, lse.h, _h(gloss), loss_scale,
+            _h(dx), lddx, _h(dw), lddw))
 
     # -- Assigner::assign (assign_all over assign_on)
     def assign(self, x, d: int, centroids, metric, chunk: int = 65536):

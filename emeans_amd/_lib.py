@@ -132,6 +132,8 @@ SIGNATURES = {
     "emh_cross_entropy": (_i, [_vp, _vp, _sz, _sz, _sz, _vp, _sz, _sz, _vp, _f, _vp, _vp]),
     "emh_cross_entropy_grad": (_i, [_vp, _vp, _sz, _sz, _sz, _vp, _sz, _sz, _vp, _f, _vp, _vp, _vp,
                                     _sz, _vp, _sz]),
+    "emh_cross_entropy_grad_scaled": (_i, [_vp, _vp, _sz, _sz, _sz, _vp, _sz, _sz, _vp, _f, _vp,
+                                           _vp, _f, _vp, _sz, _vp, _sz]),
     "emh_set_xent_workspace": (_i, [_vp, _u64]),
     "emh_adamw_create": (_i, [_vp, _vp, _sz, _pp]),
     "emh_adamw_step": (_i, [_vp, _vp]),

@@ -252,7 +252,17 @@ int emh_cross_entropy_grad(emh_ctx* c, const emh_buf* x, size_t ldx, size_t n, s
                            const emh_buf* w, size_t ldw, size_t k, const emh_buf* labels,
                            float scale, const emh_buf* lse, const emh_buf* gloss, emh_buf* dx,
                            size_t lddx, emh_buf* dw, size_t lddw) {
+  return emh_cross_entropy_grad_scaled(c, x, ldx, n, d, w, ldw, k, labels, scale, lse, gloss, 1.f, dx,
+                                       lddx, dw, lddw);
+}
+
+int emh_cross_entropy_grad_scaled(emh_ctx* c, const emh_buf* x, size_t ldx, size_t n, size_t d,
+                                  const emh_buf* w, size_t ldw, size_t k, const emh_buf* labels,
+                                  float scale, const emh_buf* lse, const emh_buf* gloss,
+                                  float loss_scale, emh_buf* dx, size_t lddx, emh_buf* dw,
+                                  size_t lddw) {
   return guard([&] {
+    EMH_ENSURE(std::isfinite(loss_scale), "loss_scale must be finite");
     const XentCall t = check_xent(c, x, ldx, n, d, w, ldw, k, labels, scale);
     const Range rs = check_f32(lse, n, "lse");
     Range rg;
@@ -279,7 +289,8 @@ int emh_cross_entropy_grad(emh_ctx* c, const emh_buf* x, size_t ldx, size_t n, s
       mo[i] = {o[i]->ptr, *ld[i], o[i]->kind};
     }
     emh::launch_cross_entropy_grad(c, t.in, (const float*)lse->ptr,
-                                   gloss ? (const float*)gloss->ptr : nullptr, mo[0], mo[1]);
+                                   gloss ? (const float*)gloss->ptr : nullptr, loss_scale, mo[0],
+                                   mo[1]);
   });
 }
 

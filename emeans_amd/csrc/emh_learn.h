@@ -43,9 +43,10 @@ struct XentIn {
 };
 constexpr uint32_t NO_LABEL = 0xFFFFFFFFu;
 void launch_cross_entropy(emh_ctx* c, const XentIn& in, float* loss, float* lse);
-// gloss (n entries): the gradients of the rows' losses, or null: of their mean.
+// gloss (n entries): the gradients of the rows' losses, or null: of their mean; all of
+// loss_scale times it.
 void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, const float* gloss,
-                               const MatOut& dx, const MatOut& dw);
+                               float loss_scale, const MatOut& dx, const MatOut& dw);
 // The tiled products that launch_cross_entropy_grad queues, in their order, for both
 // gradients (host arithmetic alone).
 std::vector<emh_xent_product> cross_entropy_products(size_t n, size_t d, size_t k, bool f32, int cus,

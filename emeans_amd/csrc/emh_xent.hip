@@ -653,7 +653,7 @@ void launch_cross_entropy(emh_ctx* c, const XentIn& in, float* loss, float* lse)
 }
 
 void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, const float* gloss,
-                               const MatOut& dx, const MatOut& dw) {
+                               float loss_scale, const MatOut& dx, const MatOut& dw) {
   const size_t n = in.n, d = in.d, k = in.k;
   const bool f32 = in.x.kind == EMH_F32;
   if (n == 0) {  // no row, no gradient
@@ -721,7 +721,7 @@ void launch_cross_entropy_grad(emh_ctx* c, const XentIn& in, const float* lse, c
     launch_logits(c->stream, a, in.x.kind, pg.tile, true);
     ProdArgs p{};
     p.labels = a.labels, p.k = (uint32_t)k;
-    p.gloss = a.gloss, p.st = st, p.scale = in.scale;
+    p.gloss = a.gloss, p.st = st, p.scale = in.scale * loss_scale;
     if (counted) p.counts = counts, p.ncounts = (uint32_t)waves;
     p.cols = (uint32_t)d, p.ldp = ldp;
     if (dx.p) {

@@ -42,6 +42,11 @@ class ClusterHead:
     initial weights (else small random ones); seed: of both random choices; scale: factor of the logits."""
 
     EPS = 1e-5
+    # F16 gradients are those of so many times the loss, and AdamW divides by it. (A mean over
+    # 16,384 rows has rows' gradients of 6e-5 of their classes' weights, about F16's least
+    # normal number. A class's is at most the scale times its largest element of a
+    # normalized row: in range for elements below 64.)
+    F16_LOSS_SCALE = 1024.0
 
     def __init__(self, d: int, k: int, kind: int = F32, state_bits: int = 32, centroids=None,
                  scale: float = 1.0, weight_decay: float = 0.01, seed: int = 1234,
@@ -53,6 +58,7 @@ class ClusterHead:
         if state_bits not in (32, 8):
             raise ValueError("state_bits must be 32 or 8")
         self.d, self.k, self.kind, self.scale, self.steps = d, k, kind, float(scale), 0
+        self.loss_scale = self.F16_LOSS_SCALE if kind == F16 else 1.0
         self.dev = dev if dev is not None else make_assigner()
         if centroids is None:
             r = np.random.default_rng(seed)
@@ -127,10 +133,11 @@ class ClusterHead:
         self.steps += 1
         self._forward(x, labels, n)
         self.dev.cross_entropy_grad(self._y, n, self.d, self._w, self.k, labels, self._lse,
-                                    self._dy, self._dw, scale=self.scale)
+                                    self._dy, self._dw, scale=self.scale,
+                                    loss_scale=self.loss_scale)
         self.dev.layer_norm_grad(self._dy, x, n, self.d, self.norm_weight, self._mean, self._rstd,
                                  None, self._dweight, self._dbias)
-        self._plan.step(lr, self.steps)
+        self._plan.step(lr, self.steps, grad_scale=1.0 / self.loss_scale)
         return self._loss
 
     def fit(self, x, labels, epochs: int = 1, batch: int = 16384, lr: float = 1e-3,

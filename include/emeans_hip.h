@@ -393,6 +393,13 @@ int emh_cross_entropy_grad(emh_ctx* ctx, const emh_buf* x, size_t ldx, size_t n,
                            const emh_buf* w, size_t ldw, size_t k, const emh_buf* labels,
                            float scale, const emh_buf* lse, const emh_buf* gloss, emh_buf* dx,
                            size_t lddx, emh_buf* dw, size_t lddw);
+/* The same times loss_scale, which is applied in f32 before the results are rounded: a mean's
+ * gradients over many rows lie among the smallest f16 numbers, or below them. */
+int emh_cross_entropy_grad_scaled(emh_ctx* ctx, const emh_buf* x, size_t ldx, size_t n, size_t d,
+                                  const emh_buf* w, size_t ldw, size_t k, const emh_buf* labels,
+                                  float scale, const emh_buf* lse, const emh_buf* gloss,
+                                  float loss_scale, emh_buf* dx, size_t lddx, emh_buf* dw,
+                                  size_t lddw);
 
 /* The bytes that a gradient's softmax of a piece of the classes and a block of the rows may
  * take, and a sixteenth more (default 1 GiB; 0: the default). It is held in 2 bytes an
