@@ -130,14 +130,14 @@ class ClusterHead:
 
     def step(self, x: DevBuf, labels: DevBuf, n: int, lr: float) -> DevBuf:
         """One training step on n resident rows; the buffer that gets their losses."""
-        self.steps += 1
         self._forward(x, labels, n)
         self.dev.cross_entropy_grad(self._y, n, self.d, self._w, self.k, labels, self._lse,
                                     self._dy, self._dw, scale=self.scale,
                                     loss_scale=self.loss_scale)
         self.dev.layer_norm_grad(self._dy, x, n, self.d, self.norm_weight, self._mean, self._rstd,
                                  None, self._dweight, self._dbias)
-        self._plan.step(lr, self.steps, grad_scale=1.0 / self.loss_scale)
+        self._plan.step(lr, self.steps + 1, grad_scale=1.0 / self.loss_scale)
+        self.steps += 1  # (a step that was refused is none)
         return self._loss
 
     def fit(self, x, labels, epochs: int = 1, batch: int = 16384, lr: float = 1e-3,
