@@ -120,6 +120,8 @@ class ClusterHead:
     def labels(self, labels) -> DevBuf:
         """Host labels as a device buffer; negative ones (rows without a cluster) are NONE."""
         a = np.asarray(labels)
+        if a.size and a.max() > NONE:
+            raise ValueError("a label has more than 32 bits")
         a = np.where(a < 0, NONE, a) if np.issubdtype(a.dtype, np.signedinteger) else a
         return self.dev.upload_u32(a)
 

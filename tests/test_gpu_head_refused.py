@@ -34,3 +34,14 @@ def test_a_refused_step_does_not_count(dev):
         return dev.read_f32(head.w)
 
     assert np.array_equal(run(True), run(False))
+
+
+def test_labels_of_more_than_32_bits(dev):
+    from emeans_amd import NONE
+    from emeans_amd.head import ClusterHead
+    head = ClusterHead(8, 4, dev=dev)
+    with pytest.raises(ValueError):
+        head.labels(np.array([1, (1 << 32) + 1]))
+    for kind in (np.int8, np.int32, np.int64):
+        assert list(dev.read_u32(head.labels(np.array([3, -1, -7], kind)))) == [3, NONE, NONE]
+    assert list(dev.read_u32(head.labels(np.array([3, NONE], np.uint32)))) == [3, NONE]
