@@ -462,8 +462,7 @@ void launch_layer_norm_grad(emh_ctx* c, const MatIn& dy, const MatIn& x, size_t 
       using S = decltype(s);
       // A workgroup a CU, of as many waves as the registers allow: few rows of
       // sums to write and add. (Twelve elements a thread fill 1,024 threads' registers
-      // and a few more: whole rows take that, 200,000 x 768 f32 592 us a training pass and
-      // 598 with 768 threads; 30,000 x 641 takes 75 and 67.)
+      // and a few more: 30,000 x 641 f32 75 us a training pass, with 768 threads 67.)
       auto go = [&](auto threads) {
         constexpr int TB = decltype(threads)::value;
         constexpr size_t G = TB / S::LPR;
@@ -474,12 +473,10 @@ void launch_layer_norm_grad(emh_ctx* c, const MatIn& dy, const MatIn& x, size_t 
       constexpr int HELD = S::NV * VecOf<T>::N;
       if constexpr (HELD > 16)
         go(std::integral_constant<int, 512>{});
-      else if constexpr (HELD == 16)
+      else if constexpr (HELD >= 12)
         go(std::integral_constant<int, 768>{});
-      else if (HELD < 12 || d == (size_t)S::LPR * HELD)
+      else
         go(std::integral_constant<int, 1024>{});
-      else if constexpr (HELD == 12)
-        go(std::integral_constant<int, 768>{});
     });
     if (held) return;
     if (sums) {  // before dx, which may overwrite dy
