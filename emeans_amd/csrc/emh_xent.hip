@@ -562,7 +562,8 @@ GradPlan grad_plan(size_t n, size_t d, size_t k, bool f32, int cus, size_t works
   g.piece = g.pieces == 1 ? k : up((k + g.pieces - 1) / g.pieces, ALL_ROWS);
   g.pieces = (k + g.piece - 1) / g.piece;
   g.gcols = up(g.piece, ALL_COLS);
-  g.px = plan_of(g.block, d, (g.piece + SLAB - 1) / SLAB, f32, cus, true);
+  // (dx's sums are those of all rows: in splits only where the rows are one block.)
+  g.px = plan_of(g.block, d, (g.piece + SLAB - 1) / SLAB, f32, cus, g.blocks == 1);
   g.pw = plan_of(g.piece, d, (g.block + SLAB - 1) / SLAB, f32, cus, true);
   return g;
 }

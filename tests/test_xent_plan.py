@@ -42,6 +42,8 @@ def check(n, d, k, kind, workspace=0):
         assert p.passes == 1 or (p.passes == 3 and kind == _lib.EMH_F32), where
         # The softmax in memory holds the product, in the workspace.
         assert p.rows * p.classes * 2 * planes <= p.softmax_bytes <= most, where
+        if p.what == DX and p.rows < n:  # (the sums of dx are of all rows)
+            assert p.splits == 1, where
         area[p.what] += p.rows * p.classes
     assert all(a == n * k for a in area.values()), (n, d, k, kind, workspace)
 
