@@ -60,8 +60,8 @@ class ClusterHead:
         self.d, self.k, self.kind, self.scale, self.steps = d, k, kind, float(scale), 0
         self.loss_scale = self.F16_LOSS_SCALE if kind == F16 else 1.0
         self.dev = dev if dev is not None else make_assigner()
+        r = np.random.default_rng(seed)
         if centroids is None:
-            r = np.random.default_rng(seed)
             w = (r.standard_normal((k, d)) / np.sqrt(d)).astype(np.float32)
         else:
             w = np.ascontiguousarray(centroids, np.float32).reshape(-1)
@@ -80,7 +80,8 @@ class ClusterHead:
         self._plan = AdamW(self.dev, [
             self._tensor(self.w, self._dw, state_bits, weight_decay, copy),
             self._tensor(self.norm_weight, self._dweight, state_bits, 0.0),
-            self._tensor(self.norm_bias, self._dbias, state_bits, 0.0)], seed=seed)
+            self._tensor(self.norm_bias, self._dbias, state_bits, 0.0)],
+            seed=int(r.integers(1 << 63)))
         self._rows = 0
 
     def _tensor(self, param, grad, bits, decay, copy=None):
