@@ -301,7 +301,8 @@ class HipDevice:
                            ldw: int = 0, lddx: int = 0, lddw: int = 0, loss_scale: float = 1.0):
         """The gradients of cross_entropy's losses weighted by gloss (F32), or of
         the mean over the rows with a label, into dx (n x d) and dw (k x d), of
-        x's kind; either may be None. loss_scale: factor of both, before they are
+        x's kind; either may be None. The softmax less the labels is rounded to
+        x's kind before the products (F32: two parts of F16). loss_scale: factor of both, before they are
         rounded (F16: a mean over many rows has gradients below its range)."""
         check(lib().emh_cross_entropy_grad_scaled(
             self._ctx, x.h, ldx, n, d, w.h, ldw, k, labels.h, scale, lse.h, _h(gloss), loss_scale,

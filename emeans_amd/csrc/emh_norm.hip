@@ -161,7 +161,7 @@ __global__ __launch_bounds__(256) void k_norm(const NormArgs a) {
 // Backward, TB threads. The row's elements stay packed and are unpacked again for
 // the result: what that takes is fewer registers, so more waves, whose rows are in
 // flight together. AHEAD: the next row is on its way, too, where there are registers.
-// 200,000 x 768 f32 363 us, 5.1 TB/s; 16,384 x 768 bf16 17.7 us, 4.3 TB/s.
+// 200,000 x 768 f32 371 us, 5.0 TB/s; 16,384 x 768 bf16 17.9 us, 4.2 TB/s.
 template <class T, int LPR, int NV, int TB>
 __global__ __launch_bounds__(TB, TB / 256) void k_norm_grad(const NormArgs a) {
   constexpr int N = VecOf<T>::N, G = TB / LPR;

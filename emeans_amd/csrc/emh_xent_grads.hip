@@ -27,9 +27,9 @@ __global__ __launch_bounds__(256) void k_copy_rows(const OddRows o, uint32_t n,
 
 // A tile of dx (rows: G's, as they lie; columns: w's, across) or of dw (both across), or
 // its sums over one split of the depth or one piece of the classes. Bound by the MFMAs
-// (emh_tile.h). In bf16: 16,384 x 768 by 1,024 31 us (dx) and 39 (dw in 5 splits; in 16
+// (emh_tile.h). In bf16: 16,384 x 768 by 1,024 31 us (dx) and 38 (dw in 5 splits; in 16
 // of 256 x 192 tiles 35, but their sums take 9 us instead of 5); 8,192 x 1,024 by
-// 131,071 1.90 ms each, 1.16 PFLOP/s.
+// 131,071 1.86 and 1.82 ms, 1.18 and 1.21 PFLOP/s.
 template <class T, class S, bool F32, bool DW, class O>
 __global__ __launch_bounds__(S::THREADS, 2) void k_grads(const ProdArgs a) {
   __shared__ __attribute__((aligned(1024))) char ring[S::RING];

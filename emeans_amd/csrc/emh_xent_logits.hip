@@ -39,8 +39,8 @@ __device__ __forceinline__ int4 four_exps(const int* ew, uint32_t j) {
 // A tile of logits, never in memory. !GRAD: its rows' maxima and sums of exponentials;
 // GRAD: G instead of it. F32: operands are planes of f16 with exponents.
 // Bound by the MFMAs (emh_tile.h), then by the exponentials (5 instructions an element)
-// and G's bytes. In bf16: 16,384 x 768 by 1,024 27 us, and 34 with G, of which the
-// loop takes 19; 8,192 x 1,024 by 131,071 1.95 ms (1.13 PFLOP/s), 2.43 with G (2.1 GB).
+// and G's bytes. In bf16: 16,384 x 768 by 1,024 28 us, and 35 with G, of which the
+// loop takes 19; 8,192 x 1,024 by 131,071 1.91 ms (1.15 PFLOP/s), 2.47 with G (2.1 GB).
 template <class T, class S, bool F32, bool GRAD>
 __global__ __launch_bounds__(S::THREADS, 2) void k_logits(const LogitArgs a) {
   __shared__ __attribute__((aligned(1024))) char ring[S::RING];

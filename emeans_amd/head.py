@@ -7,9 +7,9 @@ labels that `assign` or a training gave, AdamW.
     head = ClusterHead(768, 1024, centroids=model.centroids())
     losses = head.fit(other_view_of_x, labels, epochs=3, batch=16384)
 
-Everything between the batches' upload and the losses runs on the GPU: one step is
-layer_norm, cross_entropy, cross_entropy_grad, layer_norm_grad and one AdamW
-step over all parameters, queued on the device's stream without a wait.
+`step` takes resident rows: layer_norm, cross_entropy, cross_entropy_grad,
+layer_norm_grad and one AdamW step over all parameters, queued on the device's stream
+without a wait. `fit` uploads each batch of host rows, and waits for its losses.
 
 `python -m emeans_amd.head` runs this on synthetic rows.
 """

@@ -388,7 +388,12 @@ int emh_cross_entropy(emh_ctx* ctx, const emh_buf* x, size_t ldx, size_t n, size
  * w_v (n x d), dw_v = sum_i g_iv x_i (k x d), both of x's kind, overwritten; either
  * may be NULL. A row without a label has no part in dw, whatever it holds.
  * The logits are computed again, for pieces of the classes and blocks of the rows
- * (emh_set_xent_workspace). The sums' order depends on the sizes and the workspace alone. */
+ * (emh_set_xent_workspace). The sums' order depends on the sizes and the workspace alone.
+ * Bits: between the logits and the products, exp(z - lse) - [v = label] times gloss is
+ * rounded once to x's kind (bf16: 2^-8 of itself; f16: 2^-11, or 2^-38 of the largest gloss
+ * where that is more) or held as two parts of f16 (f32; the operands too, whatever the
+ * number of rows). Scale and the mean's 1 / rows are applied to the products' sums in
+ * f32, which are rounded once more. */
 int emh_cross_entropy_grad(emh_ctx* ctx, const emh_buf* x, size_t ldx, size_t n, size_t d,
                            const emh_buf* w, size_t ldw, size_t k, const emh_buf* labels,
                            float scale, const emh_buf* lse, const emh_buf* gloss, emh_buf* dx,
@@ -441,7 +446,8 @@ int emh_adamw_create(emh_ctx* ctx, const emh_adamw_tensor* tensors, size_t count
  * m and v. 8-bit states are rounded anew: a block's scale is its largest
  * magnitude / 448, its values the nearest codes of value / scale (a positive v at least
  * the least positive code; an element that is not finite gets a NaN and has no
- * part in the scale), or one of the two around it, at random (emh_adamw_set_seed). */
+ * part in the scale), or one of the two around it, at random (emh_adamw_set_seed). The
+ * arithmetic is f32, the quotient of the step within two units of its last place. */
 int emh_adamw_step(emh_adamw* plan, const emh_adamw_config* cfg);
 /* From the next step on 8-bit states are rounded at random, up or down in the proportion
  * that keeps their mean, by numbers that follow from the seed, the step's number, the
