@@ -263,6 +263,7 @@ int emh_cross_entropy_grad_scaled(emh_ctx* c, const emh_buf* x, size_t ldx, size
                                   size_t lddw) {
   return guard([&] {
     EMH_ENSURE(std::isfinite(loss_scale), "loss_scale must be finite");
+    EMH_ENSURE(std::isfinite(scale * loss_scale), "scale times loss_scale must be finite");
     const XentCall t = check_xent(c, x, ldx, n, d, w, ldw, k, labels, scale);
     const Range rs = check_f32(lse, n, "lse");
     Range rg;

@@ -81,3 +81,6 @@ def test_a_loss_scale_that_is_not_finite_is_refused(dev):
     with pytest.raises(EmeansHipInvalid):
         dev.cross_entropy_grad(z(6), 2, 3, z(12), 4, dev.zeros(2, U32), z(2), z(6), z(12),
                                loss_scale=float("inf"))
+    with pytest.raises(EmeansHipInvalid):
+        dev.cross_entropy_grad(z(6), 2, 3, z(12), 4, dev.zeros(2, U32), z(2), z(6), z(12),
+                               scale=1e30, loss_scale=1e30)
