@@ -21,8 +21,8 @@ from typing import List, Optional, Tuple
 import numpy as np
 
 from . import model_file
-from ._lib import (EMH_ADAMW_BLOCK, EMH_BF16, EMH_F16, EMH_F32, EMH_F8, EMH_IP, EMH_L2,
-                   EMH_PROF_EMA, EMH_PROF_SCATTER, EMH_PROF_SCREEN, EMH_U32,
+from ._lib import (EMH_ADAMW_BLOCK, EMH_BF16, EMH_CODE_BLOCK, EMH_F16, EMH_F32, EMH_F8, EMH_IP,
+                   EMH_L2, EMH_MAX_TOP, EMH_PROF_EMA, EMH_PROF_SCATTER, EMH_PROF_SCREEN, EMH_U32,
                    AdamConfig as _CAdamConfig, AdamTensor as _CAdamTensor, Config as _CConfig, DedupConfig as _CDedupConfig,
                    DedupInput as _CDedupInput, DedupResult as _CDedupResult, EmeansHipError,
                    EmeansHipInvalid, EpochStats as _CEpoch, TrainInit as _CTrainInit,
@@ -34,7 +34,7 @@ __all__ = [
     "knn_self", "knn", "dedup", "dedup_with_neighbors", "make_assigner", "available_backends",
     "Backend", "BACKEND_NAME", "EmeansHipError", "EmeansHipInvalid",
     "GPU_KMAX", "KLONG", "NONE",
-    "AdamTensor", "AdamW", "F32", "U32", "F16", "BF16", "F8",
+    "AdamTensor", "AdamW", "GradNorm", "MAX_TOP", "F32", "U32", "F16", "BF16", "F8",
 ]
 
 BACKEND_NAME = "hip"
@@ -43,6 +43,7 @@ KLONG = 4096           # the exact top-k's largest k beyond GPU_KMAX (no CPU fal
 NONE = 0xFFFFFFFF      # emeans-core/src/knn.rs:19
 # What a buffer's elements are (HipDevice.wrap, zeros).
 F32, U32, F16, BF16, F8 = EMH_F32, EMH_U32, EMH_F16, EMH_BF16, EMH_F8
+MAX_TOP = EMH_MAX_TOP  # the most alternatives of HipDevice.log_probs
 
 
 def _metric(m) -> int:
@@ -308,6 +309,74 @@ class HipDevice:
             self._ctx, x.h, ldx, n, d, w.h, ldw, k, labels.h, scale, lse.h, _h(gloss), loss_scale,
             _h(dx), lddx, _h(dw), lddw))
 
+    # -- answering and tuning operators
+    CODE_BLOCK = EMH_CODE_BLOCK  # columns (and rows of classes) that share a scale of codes
+
+    @staticmethod
+    def code_blocks(n: int) -> int:
+        """Scales for n columns of codes (or for n classes)."""
+        return -(-n // EMH_CODE_BLOCK)
+
+    @staticmethod
+    def code_stride(d: int) -> int:
+        """Bytes of a row of d codes: rows begin at multiples of 16."""
+        return -(-d // 16) * 16
+
+    def rms_norm(self, x: DevBuf, rows: int, d: int, weight: Optional[DevBuf], y: DevBuf,
+                 residual: Optional[DevBuf] = None, h: Optional[DevBuf] = None,
+                 scales: Optional[DevBuf] = None, rstd: Optional[DevBuf] = None,
+                 eps: float = 1e-6, ldx: int = 0, ldr: int = 0, ldh: int = 0, ldy: int = 0,
+                 lds: int = 0):
+        """h = x + residual in x's kind (F32, F16 or BF16), y = h rstd weight with rstd = 1 /
+        sqrt(mean(h^2) + eps) (rows x d; ld...: row strides in elements, 0 = the row). y is of
+        x's kind, or F8 with scales (F32: rows x code_blocks(d)): codes of code_stride(d) bytes
+        a row. h, rstd (F32, rows entries) and residual may be None; h may be x or residual."""
+        check(lib().emh_rms_norm(self._ctx, x.h, ldx, _h(residual), ldr, rows, d, _h(weight), eps,
+                                 _h(h), ldh, y.h, ldy, _h(scales), lds, _h(rstd)))
+
+    def rms_norm_grad(self, dy: DevBuf, h: DevBuf, rows: int, d: int, weight: Optional[DevBuf],
+                      rstd: DevBuf, dx: Optional[DevBuf], dweight: Optional[DevBuf] = None,
+                      dh: Optional[DevBuf] = None, lddy: int = 0, ldh: int = 0, lddx: int = 0,
+                      lddh: int = 0):
+        """The gradients of rms_norm's rows (x's and residual's alike; may be dy or dh) and
+        weight (F32 or h's kind) from those of its result, dy, and of h, dh; either may be None."""
+        check(lib().emh_rms_norm_grad(self._ctx, dy.h, lddy, _h(dh), lddh, h.h, ldh, rows, d,
+                                      _h(weight), rstd.h, _h(dx), lddx, _h(dweight)))
+
+    def quantize(self, x: DevBuf, rows: int, d: int, q: DevBuf, scales: DevBuf,
+                 tile_rows: int = 1, ldx: int = 0, ldq: int = 0, lds: int = 0):
+        """8-bit codes q (F8, rows x code_stride(d)) of x, with a scale (F32) for every
+        tile_rows rows (1, or CODE_BLOCK: what product8 takes as classes) and CODE_BLOCK columns."""
+        check(lib().emh_quantize(self._ctx, x.h, ldx, rows, d, tile_rows, q.h, ldq, scales.h, lds))
+
+    def product8(self, x: DevBuf, xscales: DevBuf, n: int, d: int, w: DevBuf, wscales: DevBuf,
+                 k: int, y: DevBuf, ldx: int = 0, ldxs: int = 0, ldw: int = 0, ldws: int = 0,
+                 ldy: int = 0):
+        """y = x w^T (n x k, F32, F16 or BF16) of codes as quantize makes them: x with a scale
+        for every row, w for every CODE_BLOCK rows; sums in f32."""
+        check(lib().emh_product8(self._ctx, x.h, ldx, xscales.h, ldxs, n, d, w.h, ldw, wscales.h,
+                                 ldws, k, y.h, ldy))
+
+    def log_probs(self, z: DevBuf, n: int, k: int, tokens: Optional[DevBuf],
+                  logp: Optional[DevBuf], lse: DevBuf, entropy: Optional[DevBuf] = None,
+                  top: int = 0, top_ids: Optional[DevBuf] = None,
+                  top_logp: Optional[DevBuf] = None, scale: float = 1.0, ldz: int = 0):
+        """Of rows of logits z (n x k), times scale (> 0): lse, the log probability of each
+        row's class in tokens (U32, NONE: 0), the entropy, and the `top` likeliest classes (at
+        most MAX_TOP; n x top, U32; equal ones by class) with their log probabilities. Classes
+        of -inf have no probability; places that none takes have NONE and -inf."""
+        check(lib().emh_log_probs(self._ctx, z.h, ldz, n, k, _h(tokens), scale, _h(logp), lse.h,
+                                  _h(entropy), top, _h(top_ids), _h(top_logp)))
+
+    def log_probs_grad(self, z: DevBuf, n: int, k: int, tokens: Optional[DevBuf], lse: DevBuf,
+                       dz: DevBuf, entropy: Optional[DevBuf] = None,
+                       glogp: Optional[DevBuf] = None, gentropy: Optional[DevBuf] = None,
+                       scale: float = 1.0, ldz: int = 0, lddz: int = 0):
+        """The logits' gradient (z's kind, may be z) of the log probabilities weighted by glogp
+        and the entropies weighted by gentropy (F32, n entries)."""
+        check(lib().emh_log_probs_grad(self._ctx, z.h, ldz, n, k, _h(tokens), scale, lse.h,
+                                       _h(entropy), _h(glogp), _h(gentropy), dz.h, lddz))
+
     # -- Assigner::assign (assign_all over assign_on)
     def assign(self, x, d: int, centroids, metric, chunk: int = 65536):
         x, c = _f32(x), _f32(centroids)
@@ -499,16 +568,61 @@ class AdamW:
             check(lib().emh_adamw_set_seed(h, seed))
 
     def step(self, lr: float, step: int, beta1: float = 0.9, beta2: float = 0.999,
-             eps: float = 1e-8, grad_scale: float = 1.0):
-        """One step over all tensors; step counts from 1."""
+             eps: float = 1e-8, grad_scale: float = 1.0, clip: Optional[DevBuf] = None):
+        """One step over all tensors; step counts from 1. clip: what GradNorm.norm left of these
+        gradients; they count times its factor, and where their norm is not finite the step
+        changes nothing."""
         cfg = _CAdamConfig(lr, beta1, beta2, eps, grad_scale, step)
-        check(lib().emh_adamw_step(self._h, C.byref(cfg)))
+        if clip is None:
+            check(lib().emh_adamw_step(self._h, C.byref(cfg)))
+        else:
+            check(lib().emh_adamw_step_clipped(self._h, C.byref(cfg), clip.h))
 
     def close(self):
         """Free the plan (not the tensors)."""
         h, self._h = self._h, None
         if h:
             check(lib().emh_adamw_destroy(h))
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class GradNorm:
+    """The global norm of many gradients (F32, F16 or BF16), and clipping: a plan that keeps
+    their addresses (and the buffers alive). outs: where clipped gradients go, else in
+    place."""
+
+    def __init__(self, dev: HipDevice, grads: List[DevBuf], outs: Optional[List[DevBuf]] = None):
+        self._h = None
+        self._dev, self._grads = dev, list(grads)
+        self._outs = None if outs is None else list(outs)
+        if self._outs is not None and len(self._outs) != len(self._grads):
+            raise ValueError("outs must have an entry for every gradient")
+        table = lambda l: (C.c_void_p * max(len(l), 1))(*[b.h for b in l])  # noqa: E731
+        h = C.c_void_p()
+        check(lib().emh_grad_norm_create(dev._ctx, table(self._grads),
+                                         None if self._outs is None else table(self._outs),
+                                         len(self._grads), C.byref(h)))
+        self._h = h
+
+    def norm(self, out: DevBuf, max_norm: float = float("inf"), scale: float = 1.0):
+        """out (F32, 2 entries) = the norm of scale times the gradients, and the factor that
+        brings it to max_norm (1 where it is below; NaN where it is not finite)."""
+        check(lib().emh_grad_norm_measure(self._h, scale, max_norm, out.h))
+
+    def clip(self, out: DevBuf, max_norm: float, scale: float = 1.0):
+        """The same, and the gradients times the factor (as they are where it is NaN)."""
+        check(lib().emh_grad_norm_clip(self._h, scale, max_norm, out.h))
+
+    def close(self):
+        """Free the plan (not the tensors)."""
+        h, self._h = self._h, None
+        if h:
+            check(lib().emh_grad_norm_destroy(h))
 
     def __del__(self):
         try:

@@ -14,6 +14,7 @@ EMH_OK, EMH_INVALID, EMH_ERROR = 0, 1, 2
 EMH_L2, EMH_IP = 0, 1
 EMH_F32, EMH_U32, EMH_F16, EMH_BF16, EMH_F8 = 0, 1, 2, 3, 4
 EMH_ADAMW_BLOCK = 256
+EMH_CODE_BLOCK, EMH_MAX_TOP = 128, 32
 EMH_PROF_SCREEN, EMH_PROF_SCATTER, EMH_PROF_EMA = 0, 1, 2
 
 
@@ -139,6 +140,19 @@ SIGNATURES = {
     "emh_adamw_step": (_i, [_vp, _vp]),
     "emh_adamw_set_seed": (_i, [_vp, _u64]),
     "emh_adamw_destroy": (_i, [_vp]),
+    "emh_adamw_step_clipped": (_i, [_vp, _vp, _vp]),
+    "emh_rms_norm": (_i, [_vp, _vp, _sz, _vp, _sz, _sz, _sz, _vp, _f, _vp, _sz, _vp, _sz, _vp, _sz,
+                          _vp]),
+    "emh_rms_norm_grad": (_i, [_vp, _vp, _sz, _vp, _sz, _vp, _sz, _sz, _sz, _vp, _vp, _vp, _sz,
+                               _vp]),
+    "emh_quantize": (_i, [_vp, _vp, _sz, _sz, _sz, _sz, _vp, _sz, _vp, _sz]),
+    "emh_product8": (_i, [_vp, _vp, _sz, _vp, _sz, _sz, _sz, _vp, _sz, _vp, _sz, _sz, _vp, _sz]),
+    "emh_log_probs": (_i, [_vp, _vp, _sz, _sz, _sz, _vp, _f, _vp, _vp, _vp, _sz, _vp, _vp]),
+    "emh_log_probs_grad": (_i, [_vp, _vp, _sz, _sz, _sz, _vp, _f, _vp, _vp, _vp, _vp, _vp, _sz]),
+    "emh_grad_norm_create": (_i, [_vp, _vp, _vp, _sz, _pp]),
+    "emh_grad_norm_measure": (_i, [_vp, _f, _f, _vp]),
+    "emh_grad_norm_clip": (_i, [_vp, _f, _f, _vp]),
+    "emh_grad_norm_destroy": (_i, [_vp]),
     "emh_buf_ptr": (_vp, [_vp]),
     "emh_buf_len": (_sz, [_vp]),
     "emh_top1": (_i, [_vp, _vp, _sz, _vp, _sz, _sz, _vp, _vp, _sz, _i, _vp, _vp]),

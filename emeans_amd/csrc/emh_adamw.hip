@@ -15,6 +15,8 @@
 //
 // Bound by HBM: 28 bytes an element with f32 parameters, gradients and states,
 // 16 with 8-bit states, 10 with those and 16-bit parameters and gradients.
+#include <type_traits>
+
 #include "emh_learn.h"
 #include "emh_types.h"
 
@@ -353,10 +355,18 @@ __device__ __forceinline__ void last_chunk(const AdamTensor& t, uint32_t tensor,
 
 // A chunk: 1024 U elements. 131,071 x 1,024 and two layers in bf16 with 8-bit states,
 // 10 bytes an element: 275 us, 4.9 TB/s, rounded at random 316; 256 x 384 f32 3.3 us, a launch.
-template <int U, bool RANDOM>
+// CLIP: the gradients times clip[1] too; a NaN there leaves everything as it is.
+template <int U, bool RANDOM, bool CLIP>
 __global__ __launch_bounds__(256) void k_adamw(const AdamTensor* __restrict__ tensors,
                                                const uint2* __restrict__ chunks,
-                                               const AdamScalars s) {
+                                               const AdamScalars given,
+                                               const float* __restrict__ clip) {
+  AdamScalars s = given;
+  if constexpr (CLIP) {
+    const float f = clip[1];
+    if (!(f == f)) return;
+    s.gscale *= f;
+  }
   const uint2 at = chunks[blockIdx.x];
   const AdamTensor t = tensors[at.x];
   const size_t base = (size_t)at.y * (1024 * U);
@@ -386,15 +396,19 @@ __global__ __launch_bounds__(256) void k_adamw(const AdamTensor* __restrict__ te
 }  // namespace
 
 void launch_adamw(emh_ctx* c, const AdamTensor* tensors, const uint2* chunks, size_t nchunks,
-                  size_t chunk, bool random, const AdamScalars& s) {
+                  size_t chunk, bool random, const AdamScalars& s, const float* clip) {
   if (nchunks == 0) return;
   const dim3 grid((unsigned)nchunks);
-  auto go = [&](auto kernel) { kernel<<<grid, 256, 0, c->stream>>>(tensors, chunks, s); };
+  auto go = [&](auto kernel) { kernel<<<grid, 256, 0, c->stream>>>(tensors, chunks, s, clip); };
   constexpr int MANY = (int)(ADAM_CHUNK / 1024), FEW = (int)(ADAM_CHUNK_FEW / 1024);
-  if (chunk == ADAM_CHUNK)
-    random ? go(k_adamw<MANY, true>) : go(k_adamw<MANY, false>);
-  else
-    random ? go(k_adamw<FEW, true>) : go(k_adamw<FEW, false>);
+  auto with = [&](auto clipped) {
+    constexpr bool CLIP = decltype(clipped)::value;
+    if (chunk == ADAM_CHUNK)
+      random ? go(k_adamw<MANY, true, CLIP>) : go(k_adamw<MANY, false, CLIP>);
+    else
+      random ? go(k_adamw<FEW, true, CLIP>) : go(k_adamw<FEW, false, CLIP>);
+  };
+  clip ? with(std::true_type{}) : with(std::false_type{});
   EMH_HIP(hipGetLastError());
 }
 

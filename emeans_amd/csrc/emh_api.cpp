@@ -14,7 +14,7 @@
 #include <vector>
 
 #include "emh_internal.h"
-#include "emh_learn.h"
+#include "emh_answer.h"
 
 namespace {
 thread_local std::string g_last_error;
@@ -275,7 +275,7 @@ void check_device_flags(emh_ctx* c) {
     emh::launch_fill_u32(c, c->small + emh::SW_BAD_ID, 1, 0);
     emh::launch_fill_u32(c, c->small + emh::SW_BAD_CLASS, 1, 0);
     EMH_HIP(hipStreamSynchronize(c->stream));
-    EMH_ENSURE(!bad_class, "cross_entropy: label out of range");
+    EMH_ENSURE(!bad_class, "cross_entropy or log_probs: label out of range");
     EMH_ENSURE(!bad_label, "scatter_add: label out of range");
     EMH_ENSURE(!bad_id, "row id out of range");
   }
@@ -356,6 +356,9 @@ int emh_destroy(emh_ctx* c) {
     if (c->copy_stream)
       (void)hipStreamSynchronize(c->copy_stream);  // copies may still read pinned staging
     emh::drop_plans(c);
+    emh::drop_norms(c);
+    c->rms_part.release();
+    c->logp_part.release();
     for (emh::Scratch* s : {&c->cand, &c->fblist, &c->order, &c->start, &c->misc, &c->knn_tmp,
                             &c->xnorm, &c->bigj, &c->chunkcnt, &c->tickets,
                             &c->preview_ticket, &c->xsplit, &c->xsplit_norm, &c->csplit, &c->csplit_norm, &c->csplit_part,

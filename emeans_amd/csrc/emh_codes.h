@@ -1,0 +1,66 @@
+// 8-bit codes (e4m3) of a block that shares a scale: scale = largest magnitude / 448, code =
+// the nearest to value / scale. Both quotients are correctly rounded, so that the codes
+// follow from the values alone: a code one step off is a sixteenth of its value.
+#pragma once
+
+#include "emh_types.h"
+
+namespace emh {
+
+constexpr int CODE_BLOCK = EMH_CODE_BLOCK;  // columns that share a scale
+
+// The largest magnitude counts finite values alone (an element that is not finite gets the
+// NaN code and has no part in the scale).
+__device__ __forceinline__ float finite_abs(float v) {
+  const float a = fabsf(v);
+  return a < INFINITY ? a : 0.f;
+}
+
+struct Coder {
+  float scale, by;
+  bool quick;  // (whole waves agree)
+  __device__ __forceinline__ explicit Coder(float top) {
+    scale = top / 448.f;
+    quick = __all((scale > 1e-30f && scale < 1e30f) || scale == 0.f);
+    const float r0 = __builtin_amdgcn_rcpf(scale > 0.f ? scale : 1.f);
+    by = fmaf(r0, fmaf(-scale, r0, 1.f), r0);
+    if (!(scale > 0.f)) by = 1.f;
+  }
+  // A quotient: one reciprocal a block, refined, then a product and its remainder. At most
+  // 448 (1 + 2^-23), which rounds to 448. (Without a scale the values are zeros, or below
+  // what a code can hold of them.)
+  __device__ __forceinline__ float quotient(float v) const {
+    if (quick) {
+      const float q = v * by, back = fmaf(fmaf(-scale, q, v), by, q);
+      // (The remainder of a negative zero is a positive one.)
+      return scale > 0.f && fabsf(v) < INFINITY ? copysignf(back, v) : v;
+    }
+    // (A scale among the last subnormal numbers may be small by half of itself.)
+    const float q = scale > 0.f ? v / scale : v;
+    return fabsf(q) < INFINITY ? fminf(fmaxf(q, -448.f), 448.f) : q;
+  }
+  __device__ __forceinline__ uint32_t four(const float* v) const {
+    const uint32_t w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(quotient(v[0]), quotient(v[1]), 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(quotient(v[2]), quotient(v[3]), (int)w, true);
+  }
+};
+
+// The codes of N (4 or 8) columns from `col` on, the first `skip` of v other columns', to a
+// row of codes (its start 16-byte aligned); zeros from the row's d columns to its next
+// multiple of 16.
+template <int N>
+__device__ __forceinline__ void store_codes(uint8_t* row, int col, int skip, int d, const Coder& c,
+                                            const float* v) {
+  static_assert(N == 4 || N == 8, "codes of a vector");
+  if constexpr (N == 8) {
+    uint64_t w = (uint64_t)c.four(v) | (uint64_t)c.four(v + 4) << 32;
+    w >>= 8 * skip;
+    *reinterpret_cast<uint2*>(row + col) = make_uint2((uint32_t)w, (uint32_t)(w >> 32));
+  } else {
+    *reinterpret_cast<uint32_t*>(row + col) = c.four(v) >> (8 * skip);
+  }
+  if (col + N >= d)
+    for (int t = col + N; t < ((d + 15) & ~15); t += 4) *reinterpret_cast<uint32_t*>(row + t) = 0u;
+}
+
+}  // namespace emh

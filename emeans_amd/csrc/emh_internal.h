@@ -4,6 +4,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <cstdio>
 #include <stdexcept>
@@ -81,6 +82,35 @@ struct Scratch {
   void release() {
     if (ptr) (void)hipFree(ptr);
     ptr = nullptr;
+    bytes = 0;
+  }
+};
+
+// Device scratch that grows without giving up what it has handed out: a graph captured
+// with a smaller block may still be replayed. Blocks at least double, so all of them hold at
+// most twice the last.
+struct Kept {
+  std::vector<void*> blocks;
+  size_t bytes = 0;  // of the last
+  void* get(size_t need, hipStream_t s) {
+    if (need > bytes) {
+      hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+      EMH_HIP(hipStreamIsCapturing(s, &st));
+      if (st != hipStreamCaptureStatusNone)
+        throw Invalid("the call needs a larger workspace than the context has: make it once "
+                      "before the capture");
+      const size_t b = std::max(need, 2 * bytes) + 4096;
+      blocks.reserve(blocks.size() + 1);
+      void* p = nullptr;
+      EMH_HIP(hipMalloc(&p, b));
+      blocks.push_back(p);
+      bytes = b;
+    }
+    return blocks.back();
+  }
+  void release() {
+    for (void* p : blocks) (void)hipFree(p);
+    blocks.clear();
     bytes = 0;
   }
 };
@@ -212,6 +242,7 @@ struct emh_buf {
 };
 
 struct emh_adamw;
+struct emh_grad_norm;
 struct emh_ctx {
   int device = 0;
   hipStream_t stream = nullptr;
@@ -259,6 +290,9 @@ struct emh_ctx {
   std::vector<emh_adamw*> plans;  // made with it and not destroyed (emh_learn.cpp)
   uint32_t xent_calls = 0;  // gradients of the cross entropy so far (see SW_ODD_ROW)
   emh::Scratch norm_part;  // layer_norm_grad: the blocks' sums of dweight and dbias
+  std::vector<emh_grad_norm*> norms;  // as plans (emh_answer.cpp)
+  emh::Kept rms_part;      // rms_norm_grad: the workgroups' sums of dweight
+  emh::Kept logp_part;     // log_probs: what the parts of a row found
   emh::Scratch xent;       // cross_entropy's parts, gradients of a piece and laid-out operands
   emh::Scratch preview_ticket;  // k_mass_preview's last-block ticket (left at zero)
   // Host staging of the device loop: masses, plan, flags, epoch orders and

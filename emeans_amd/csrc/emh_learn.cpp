@@ -3,12 +3,11 @@
 
 #include <algorithm>
 #include <cmath>
-#include <exception>
 #include <memory>
 #include <mutex>
 #include <vector>
 
-#include "emh_learn.h"
+#include "emh_check.h"
 
 struct emh_adamw {
   emh_ctx* ctx = nullptr;  // null once it is destroyed
@@ -18,26 +17,10 @@ struct emh_adamw {
   bool random = false;  // emh_adamw_set_seed
   uint64_t seed = 0;
   std::vector<emh_buf*> written;
+  std::vector<Range> ranges;  // of what a step writes
 };
 
 namespace {
-
-template <class F>
-int guard(F&& f) {
-  try {
-    f();
-    return EMH_OK;
-  } catch (const emh::Invalid& e) {
-    emh::set_last_error(e.what());
-    return EMH_INVALID;
-  } catch (const std::exception& e) {
-    emh::set_last_error(e.what());
-    return EMH_ERROR;
-  } catch (...) {
-    emh::set_last_error("unknown error");
-    return EMH_ERROR;
-  }
-}
 
 // A context's list of plans: a plan may be destroyed on another thread than its context.
 std::mutex g_plans_mu;
@@ -47,64 +30,6 @@ void free_tables(emh_adamw* p) {
   if (p->chunks) (void)hipFree(p->chunks);
   p->tensors = nullptr;
   p->chunks = nullptr;
-}
-
-void use_device(emh_ctx* c) { EMH_HIP(hipSetDevice(c->device)); }
-
-bool real_kind(int k) { return k == EMH_F32 || k == EMH_F16 || k == EMH_BF16; }
-
-// The bytes that an operand covers.
-struct Range {
-  const char* lo = nullptr;
-  const char* hi = nullptr;
-  bool meets(const Range& o) const { return lo < o.hi && o.lo < hi; }
-  bool same(const Range& o) const { return lo == o.lo && hi == o.hi; }
-};
-Range range_of(const void* p, size_t len, int kind) {
-  return {(const char*)p, (const char*)p + len * emh::kind_bytes(kind)};
-}
-
-void check_address(const emh_buf* b, const char* what) {
-  EMH_ENSURE((uintptr_t)b->ptr % emh::kind_bytes(b->kind) == 0,
-             "%s does not begin at an element's address", what);
-}
-
-// A rows x d matrix with row stride ld (0: d) in b; its stride and range.
-Range check_matrix(const emh_buf* b, size_t rows, size_t d, size_t& ld, const char* what) {
-  if (ld == 0) ld = d;
-  EMH_ENSURE(ld >= d, "%s: the row stride %zu is less than the row's %zu", what, ld, d);
-  check_address(b, what);
-  size_t span = 0;
-  if (rows > 0)
-    EMH_ENSURE(!__builtin_mul_overflow(rows - 1, ld, &span) &&
-                   !__builtin_add_overflow(span, d, &span) && span <= b->len,
-               "%s: the buffer's %zu elements do not hold %zu rows of %zu (stride %zu)", what,
-               b->len, rows, d, ld);
-  return range_of(b->ptr, span, b->kind);
-}
-Range check_vector(const emh_buf* b, size_t len, const char* what) {
-  EMH_ENSURE(b->len >= len, "%s: the buffer's %zu elements are fewer than %zu", what, b->len, len);
-  check_address(b, what);
-  return range_of(b->ptr, len, b->kind);
-}
-Range check_f32(const emh_buf* b, size_t len, const char* what) {
-  EMH_ENSURE(b && b->kind == EMH_F32, "%s must be an f32 buffer", what);
-  return check_vector(b, len, what);
-}
-void apart(const Range& out, const Range& in, const char* a, const char* b) {
-  EMH_ENSURE(!out.meets(in), "%s overlaps %s", a, b);
-}
-void apart_or_same(const Range& out, const Range& in, bool same_ld, const char* a, const char* b) {
-  EMH_ENSURE(!out.meets(in) || (out.same(in) && same_ld), "%s overlaps %s in part", a, b);
-}
-constexpr size_t MAX_D = size_t(1) << 30;
-
-// A norm's weight or bias: d entries of x's kind or f32.
-emh::MatIn check_affine(const emh_buf* b, size_t d, int kind, const char* what, Range& r) {
-  if (!b) return {};
-  EMH_ENSURE(b->kind == EMH_F32 || b->kind == kind, "%s must be f32 or of x's kind", what);
-  r = check_vector(b, d, what);
-  return {b->ptr, d, b->kind};
 }
 
 }  // namespace
@@ -388,6 +313,7 @@ int emh_adamw_create(emh_ctx* c, const emh_adamw_tensor* tensors, size_t count, 
     std::vector<Written> kept;  // not empty
     for (const Written& w : written)
       if (w.r.lo < w.r.hi) kept.push_back(w);
+    for (const Written& w : kept) plan->ranges.push_back(w.r);
     for (size_t i = 1; i < kept.size(); i++)
       EMH_ENSURE(kept[i - 1].r.hi <= kept[i].r.lo,
                  "tensors %zu and %zu: two of what the step writes overlap", kept[i - 1].tensor,
@@ -434,10 +360,15 @@ int emh_adamw_set_seed(emh_adamw* plan, uint64_t seed) {
   });
 }
 
-int emh_adamw_step(emh_adamw* plan, const emh_adamw_config* cfg) {
+static int adamw_step(emh_adamw* plan, const emh_adamw_config* cfg, const emh_buf* clip,
+                      bool clipped) {
   return guard([&] {
     EMH_ENSURE(plan && cfg, "null argument");
     EMH_ENSURE(plan->ctx, "the plan's context is destroyed");
+    if (clipped) {
+      const Range r = check_f32(clip, 2, "clip");
+      for (const Range& w : plan->ranges) apart(w, r, "what the step writes", "clip");
+    }
     EMH_ENSURE(cfg->step >= 1, "step counts from 1");
     EMH_ENSURE(cfg->beta1 >= 0 && cfg->beta1 < 1 && cfg->beta2 >= 0 && cfg->beta2 < 1,
                "beta1 and beta2 must be in [0, 1)");
@@ -462,8 +393,14 @@ int emh_adamw_step(emh_adamw* plan, const emh_adamw_config* cfg) {
     use_device(plan->ctx);
     for (emh_buf* b : plan->written) ++b->gen;
     emh::launch_adamw(plan->ctx, plan->tensors, plan->chunks, plan->nchunks, plan->chunk,
-                      plan->random, s);
+                      plan->random, s, clipped ? (const float*)clip->ptr : nullptr);
   });
+}
+int emh_adamw_step(emh_adamw* plan, const emh_adamw_config* cfg) {
+  return adamw_step(plan, cfg, nullptr, false);
+}
+int emh_adamw_step_clipped(emh_adamw* plan, const emh_adamw_config* cfg, const emh_buf* clip) {
+  return adamw_step(plan, cfg, clip, true);
 }
 
 int emh_adamw_destroy(emh_adamw* plan) {

@@ -78,8 +78,9 @@ constexpr size_t ADAM_FEW = size_t(2) << 20;
 // The plans made with c step no more, and what they hold on the device is freed (c's
 // stream is idle).
 void drop_plans(emh_ctx* c);
-// chunks[i]: the tensor and the chunk in it that workgroup i takes.
+// chunks[i]: the tensor and the chunk in it that workgroup i takes. clip: a gradient norm's
+// output, or null.
 void launch_adamw(emh_ctx* c, const AdamTensor* tensors, const uint2* chunks, size_t nchunks,
-                  size_t chunk, bool random, const AdamScalars& s);
+                  size_t chunk, bool random, const AdamScalars& s, const float* clip);
 
 }  // namespace emh

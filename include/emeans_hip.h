@@ -459,6 +459,92 @@ int emh_adamw_step(emh_adamw* plan, const emh_adamw_config* cfg);
 int emh_adamw_set_seed(emh_adamw* plan, uint64_t seed);
 int emh_adamw_destroy(emh_adamw* plan);
 
+/* ------------------------------------------- answering and tuning operators */
+/* What a classifier over the clusters answers with, in 8 bits, and is tuned with (no counterpart
+ * in the reference): a root-mean-square norm, 8-bit codes and their product, log probabilities
+ * of logits, their gradients, and the norm of all gradients. The conventions are those of the
+ * learning operators. A graph captured from the context's stream may be replayed as long
+ * as the buffers live; graphs of one context share its workspace, so one replay follows another.
+ * A call whose workspace does not exist yet is refused during a capture: make it once before.
+ *
+ * Codes: an f8 matrix has rows that begin at multiples of 16 bytes (its address and its
+ * stride; stride 0 = the row's length rounded up to 16, and the buffer holds the last row up to
+ * there), and f32 scales, one for every EMH_CODE_BLOCK columns (the last block may be shorter)
+ * of one row, or of EMH_CODE_BLOCK rows; ceil(d / EMH_CODE_BLOCK) scales a row are its length.
+ * A value is code times scale. scale = the block's largest finite magnitude / 448, code = the
+ * nearest to value / scale, both quotients correctly rounded; an element that is not
+ * finite gets the NaN code. Codes from a row's end to its next multiple of 16 are written as
+ * zeros, and never read as anything else. */
+#define EMH_CODE_BLOCK 128
+
+/* h = x + residual (rows x d, f32, f16 or bf16, one kind; residual NULL: h = x), rounded to
+ * their kind; rstd = 1 / sqrt(mean(h^2) + eps), y = h rstd weight. weight (d entries, x's kind or
+ * f32) may be NULL (ones). h may be NULL, x or residual. y: x's kind, may be x or residual (not
+ * what h is), scales NULL; or f8 codes of the unrounded result with a scale for every row and
+ * block. rstd (f32, rows entries; may be NULL) is for the gradient. Squares are f32: a row's
+ * largest element lies below 2^63. d <= 2^24. */
+int emh_rms_norm(emh_ctx* ctx, const emh_buf* x, size_t ldx, const emh_buf* residual, size_t ldr,
+                 size_t rows, size_t d, const emh_buf* weight, float eps, emh_buf* h, size_t ldh,
+                 emh_buf* y, size_t ldy, emh_buf* scales, size_t lds, emh_buf* rstd);
+/* Its gradient, with h and rstd as emh_rms_norm left them, dy that of y and dh (may be NULL) that
+ * of h from elsewhere: with u = h rstd and g = dy weight, dx = dh + rstd (g - u mean(g u)),
+ * which is both x's and residual's (h's kind, may be dy or dh), dweight = sum over rows of dy u (d
+ * entries, f32 or h's kind, overwritten). Either may be NULL. The sums' order depends on the
+ * sizes alone. */
+int emh_rms_norm_grad(emh_ctx* ctx, const emh_buf* dy, size_t lddy, const emh_buf* dh, size_t lddh,
+                      const emh_buf* h, size_t ldh, size_t rows, size_t d, const emh_buf* weight,
+                      const emh_buf* rstd, emh_buf* dx, size_t lddx, emh_buf* dweight);
+/* Codes of x (rows x d, f32, f16 or bf16), a scale for every tile_rows rows (1, or
+ * EMH_CODE_BLOCK: what emh_product8 takes as classes) and block of columns. d <= 2^24. */
+int emh_quantize(emh_ctx* ctx, const emh_buf* x, size_t ldx, size_t rows, size_t d,
+                 size_t tile_rows, emh_buf* q, size_t ldq, emh_buf* scales, size_t lds);
+/* y = x w^T (n x k, f32, f16 or bf16) of codes: x n x d with a scale for every row and block, w k x
+ * d with a scale for every EMH_CODE_BLOCK rows and block. y_iv = sum over blocks b of
+ * xscales_ib wscales_(v / EMH_CODE_BLOCK)b times the sum of the codes' products, all in f32 and
+ * rounded once to y's kind. d <= 2^21. */
+int emh_product8(emh_ctx* ctx, const emh_buf* x, size_t ldx, const emh_buf* xscales, size_t ldxs,
+                 size_t n, size_t d, const emh_buf* w, size_t ldw, const emh_buf* wscales,
+                 size_t ldws, size_t k, emh_buf* y, size_t ldy);
+/* Of rows of logits z (n x k, f32, f16 or bf16), times scale (positive: an inverse
+ * temperature): lse = log sum_v exp z_v; logp = z_t - lse of the row's class t = tokens[i] (u32,
+ * 0xFFFFFFFF for none: 0; any other t >= k is an error at the next synchronizing call, and
+ * counts as none); entropy = -sum_v p_v log p_v with p_v = exp(z_v - lse); the `top` (at most
+ * EMH_MAX_TOP) likeliest classes and their log probabilities, the likeliest first, of equal logits
+ * the lower class first, n x top. f32 all but the ids (u32). tokens and logp may both be NULL,
+ * entropy too, and of the top outputs one, or both with top = 0. A class of logit -infinity
+ * has probability 0 and is never among the likeliest: places that no class takes have the id
+ * 0xFFFFFFFF and -infinity. A row of such classes alone has lse and log probabilities of
+ * -infinity and entropy 0; a row with a NaN or +infinity NaN everywhere, and no ids. */
+#define EMH_MAX_TOP 32
+int emh_log_probs(emh_ctx* ctx, const emh_buf* z, size_t ldz, size_t n, size_t k,
+                  const emh_buf* tokens, float scale, emh_buf* logp, emh_buf* lse,
+                  emh_buf* entropy, size_t top, emh_buf* top_ids, emh_buf* top_logp);
+/* The gradient of sum_i glogp[i] logp[i] + gentropy[i] entropy[i] (f32; tokens and glogp may both
+ * be NULL, entropy and gentropy too), with lse and entropy as emh_log_probs left them: dz_v =
+ * scale (glogp ([v = t] - p_v) - gentropy p_v (log p_v + entropy)), z's kind, may be z. A row
+ * without a class that has a probability gets zeros. */
+int emh_log_probs_grad(emh_ctx* ctx, const emh_buf* z, size_t ldz, size_t n, size_t k,
+                       const emh_buf* tokens, float scale, const emh_buf* lse,
+                       const emh_buf* entropy, const emh_buf* glogp, const emh_buf* gentropy,
+                       emh_buf* dz, size_t lddz);
+
+/* A plan over count gradients (f32, f16 or bf16), which keeps their addresses: the buffers
+ * outlive its last call. outs (of the gradients' kinds and lengths): where clipped gradients
+ * go; NULL: in place. Nothing that is written may overlap another tensor. */
+typedef struct emh_grad_norm emh_grad_norm;
+int emh_grad_norm_create(emh_ctx* ctx, const emh_buf* const* grads, emh_buf* const* outs,
+                         size_t count, emh_grad_norm** out);
+/* out[0] = norm = |scale| sqrt(sum of all elements' squares) (summed in f64), out[1] = min(1,
+ * max_norm / norm) (f32, 2 entries; max_norm may be infinite; scale: 1 / the loss's, if it was
+ * scaled). A norm that is not finite has a NaN as out[1]. */
+int emh_grad_norm_measure(emh_grad_norm* plan, float scale, float max_norm, emh_buf* out);
+/* The same, and every gradient times out[1] (where that is a NaN, as it is) to its output. */
+int emh_grad_norm_clip(emh_grad_norm* plan, float scale, float max_norm, emh_buf* out);
+int emh_grad_norm_destroy(emh_grad_norm* plan);
+/* emh_adamw_step with the gradients times clip[1] as well (clip: what a measurement of them left,
+ * read on the device). Where that is a NaN the step changes nothing. */
+int emh_adamw_step_clipped(emh_adamw* plan, const emh_adamw_config* cfg, const emh_buf* clip);
+
 /* ------------------------------------------------- host replay (no device) */
 /* The seeded host-side pieces of the device loop, exported so that callers and
  * tests can check them without a GPU. They never touch the device. */
