@@ -51,6 +51,15 @@ __device__ __forceinline__ void dma16a(const void* base, uint32_t off, uint32_t 
       : "v"(off), "s"(base), "s"(lds)
       : "memory");
 }
+__device__ __forceinline__ void dma4a(const void* base, uint32_t off, uint32_t lds) {
+  uint32_t saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\t"
+      "global_load_lds_dword %1, %2\n\ts_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "v"(off), "s"(base), "s"(lds)
+      : "memory");
+}
 __device__ __forceinline__ void dma4(const void* g, void* lds) {
   uint32_t saved;
   asm volatile(

@@ -1,17 +1,31 @@
 // Rows in 8 bits times classes in 8 bits: y(i, v) = sum over blocks b of 128 columns of
 // xs(i, b) ws(v / 128, b) (sum over the block's columns of x(i, c) w(v, c)).
 //
-// A block's sum is one MFMA of depth 128 (products of codes are exact in f32); it is scaled and
-// added in f32, one fused multiply-add an element.
+// A block's sum comes from the MFMAs and is scaled and added in f32, one fused multiply-add an
+// element of the result and block.
+//
+// Two kinds of MFMA. The 8-bit ones (16 x 16 x 128, twice the 16-bit rate) align the products of
+// eight neighbouring columns to the largest and keep 13 bits below it: a sum is off by up to 7
+// 2^-13 of the largest product of each eight, 1.4e-5 of results from normal data, which 16-bit
+// results (2^-9, 2^-12) do not show. f32 results, and few rows, whose time is the classes'
+// bytes, take the f16 MFMA instead (an f16 holds every code exactly): 5e-8.
+//
+// Few rows read the classes once, as they lie. More of them go in tiles: a workgroup owns 256 x
+// 256 or 128 x 128 of the result, and a block of the depth, 128 bytes a row of both operands,
+// goes by in one step, moved to LDS by DMA into one of two stages, its 16-byte chunks
+// XOR-swizzled so that sixteen rows' equal chunks meet no bank twice.
 #include "emh_answer.h"
 #include "emh_codes.h"
+#include "emh_tile.h"
 
 namespace emh {
 namespace {
 
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef int v8i __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
-typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef v4u __attribute__((address_space(3)))* lds_v4u;
 
 // Eight codes as f16, which holds each exactly.
 __device__ __forceinline__ v8h halves8(uint32_t lo, uint32_t hi) {
@@ -25,7 +39,7 @@ __device__ __forceinline__ v8h halves8(uint32_t lo, uint32_t hi) {
 struct Halves {
   v8h v[4];
   __device__ __forceinline__ Halves() {}
-  __device__ __forceinline__ Halves(uint4 a, uint4 b)
+  __device__ __forceinline__ Halves(v4u a, v4u b)
       : v{halves8(a.x, a.y), halves8(a.z, a.w), halves8(b.x, b.y), halves8(b.z, b.w)} {}
 };
 // 16 x 16 x 128. Lane l gives row l % 16 of a and of b and 32 of the depth's codes, the same
@@ -38,20 +52,23 @@ __device__ __forceinline__ v4f block16(const Halves& a, const Halves& b) {
   return t;
 }
 
-// The 16 codes of a row from column c on, zeros from column d on.
-__device__ __forceinline__ uint4 codes16(const uint8_t* row, size_t c, size_t d) {
-  if (c >= d) return make_uint4(0u, 0u, 0u, 0u);
-  const uint4 v = *reinterpret_cast<const uint4*>(row + c);
-  if (c + 16 <= d) return v;
-  const int left = (int)(d - c);
-  uint32_t w[4] = {v.x, v.y, v.z, v.w};
+// The first `left` of 16 codes, then zeros.
+__device__ __forceinline__ v4u first_codes(v4u v, int left) {
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     const int have = left - 4 * i;
-    w[i] = have >= 4 ? w[i] : have <= 0 ? 0u : w[i] & ((1u << (8 * have)) - 1u);
+    v[i] = have >= 4 ? v[i] : have <= 0 ? 0u : v[i] & ((1u << (8 * have)) - 1u);
   }
-  return make_uint4(w[0], w[1], w[2], w[3]);
+  return v;
 }
+// The 16 codes of a row from column c on, zeros from column d on.
+__device__ __forceinline__ v4u codes16(const uint8_t* row, size_t c, size_t d) {
+  if (c >= d) return v4u{0u, 0u, 0u, 0u};
+  v4u v = *reinterpret_cast<const v4u*>(row + c);
+  if (c + 16 <= d) return v;
+  return first_codes(v, (int)(d - c));
+}
+
 // Few rows: a workgroup takes 16 classes and 16 YB rows, its four waves the blocks of the depth
 // by turns; operands come from memory as they lie.
 template <int YB>
@@ -106,6 +123,356 @@ __global__ __launch_bounds__(256) void k_few8(const CodedIn x, size_t n, size_t 
   }
 }
 
+// ------------------------------------------------------------------ tiles
+// Waves of NWR x NWC, each 16 YB rows by 16 AB classes. A stage holds a block of the depth of
+// both operands, the rows' scales of it (TR) and the classes' (64, by turns the tile's two).
+template <int NWR_, int NWC_, int YB_, int AB_, int PER_CU_>
+struct Shape8 {
+  static constexpr int NWR = NWR_, NWC = NWC_, YB = YB_, AB = AB_, PER_CU = PER_CU_;
+  static constexpr int NW = NWR * NWC, THREADS = 64 * NW;
+  static constexpr int TR = NWR * YB * 16, TC = NWC * AB * 16;
+  static constexpr int RBYTES = TR * CODE_BLOCK, CBYTES = TC * CODE_BLOCK;
+  static constexpr int CODES = RBYTES + CBYTES, STAGE = CODES + TR * 4 + 256;
+  static constexpr int RD = RBYTES / (1024 * NW), CD = CBYTES / (1024 * NW);  // DMAs a wave
+  static constexpr int XW = TR / 64;  // waves that move the rows' scales; the next the classes'
+  static_assert(NW % 2 == 0 && XW < NW && CODE_BLOCK % (AB * 16) == 0,
+                "a wave's classes share a scale");
+};
+typedef Shape8<4, 2, 4, 8, 1> Large8;  // 256 x 256, 8 waves
+typedef Shape8<2, 2, 4, 4, 2> Small8;  // 128 x 128, 4 waves, two workgroups a CU
+
+// Bytes of results from which they go past the caches.
+constexpr size_t STREAM_FROM = size_t(256) << 20;
+
+struct Prod8Args {
+  TileIn t;  // r: the rows, c: the classes; slabs: blocks of the depth
+  uint32_t n, k, d;
+  const float* xs;
+  uint32_t ldxs;  // bytes
+  const float* ws;
+  size_t ldws;
+  void* y;
+  size_t ldy;
+};
+
+struct Frag {  // a lane's 32 codes of a block's row
+  v4u a, b;
+  __device__ __forceinline__ void read(uint32_t at) {
+    a = *(lds_v4u)(uintptr_t)at;
+    b = *(lds_v4u)(uintptr_t)(at ^ 64u);
+  }
+  __device__ __forceinline__ v8i codes() const {
+    return __builtin_bit_cast(v8i, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+};
+typedef const float __attribute__((address_space(3)))* lds_f32;
+
+// Sixteen bytes of a lane's results in the blocks from acc[0] on: f32 as they are; of 16 bits two
+// blocks' fours swapped between lanes, so that each has eight columns of one.
+template <class T, int YB>
+__device__ __forceinline__ void sixteen(const v4f (*acc)[YB], int y, uint32_t* out) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) out[e] = __float_as_uint(acc[0][y][e]);
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const auto v = __builtin_amdgcn_permlane16_swap(
+          pair_from_f32<T>(acc[0][y][2 * h], acc[0][y][2 * h + 1]),
+          pair_from_f32<T>(acc[1][y][2 * h], acc[1][y][2 * h + 1]), false, false);
+      out[h] = v[0];
+      out[2 + h] = v[1];
+    }
+  }
+}
+// A store of what no cache need keep.
+template <class T>
+__device__ __forceinline__ void stream_vec(T* p, const Vec<T>& v) {
+  typedef uint32_t any16 __attribute__((ext_vector_type(4), aligned(2)));
+  __builtin_nontemporal_store(any16{v.raw.x, v.raw.y, v.raw.z, v.raw.w}, reinterpret_cast<any16*>(p));
+}
+
+// EXACT: f32 results by f16 MFMAs; else T results by 8-bit ones. STREAM: results that are
+// larger than the caches go past them.
+//
+// A workgroup takes tiles in turn, and the blocks of all its tiles are one stream: while a
+// tile's last blocks are multiplied, the next one's first are on their way, and while its
+// results go out of the registers, too.
+template <class T, class S, bool EXACT, bool STREAM>
+__global__ __launch_bounds__(S::THREADS, 2) void k_tile8(const Prod8Args a) {
+  __shared__ __attribute__((aligned(1024))) char ring[2 * S::STAGE];
+  const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int wr = w % S::NWR, wc = w / S::NWR;
+  const uint32_t lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
+  const uint32_t steps = a.t.slabs;
+  const uint32_t lds0 = lds_addr(ring);
+  // The last block may be short: chunks past the row's sixteens read the last one, and
+  // what lies past d is made zeros in LDS. (A lane moves the same chunk of a row in all its DMAs:
+  // a wave's rows are 8 apart times an even number.)
+  const uint32_t tail = a.d - (steps - 1) * CODE_BLOCK, lastc = (tail + 15) / 16 - 1;
+  const uint32_t chunk = (lane & 7) ^ (((uint32_t)w * 4 + (lane >> 4)) & 7);
+  const uint32_t back = chunk > lastc ? (chunk - lastc) << 4 : 0u;
+
+  // The next DMAs: their tile and block. Past the last tile they fetch its last block again.
+  uint32_t lbid = blockIdx.x, lslab = 0, lst = lds0;
+  const char *rp, *cp, *xp, *wp;
+  uint32_t roff, rlast, coff, clast, soff;
+  auto aim = [&]() __attribute__((always_inline)) {
+    const TileAt at = tile_at(a.t, lbid);
+    const uint32_t row = (uint32_t)w * 8 + (lane >> 3), ch = chunk << 4;
+    rp = a.t.r.p[0] + (size_t)at.rt * S::TR * a.t.r.ld;
+    cp = a.t.c.p[0] + (size_t)at.ct * S::TC * a.t.c.ld;
+    const uint32_t r1 = a.t.r.rows - 1 - at.rt * S::TR, c1 = a.t.c.rows - 1 - at.ct * S::TC;
+    roff = row * a.t.r.ld + ch;
+    rlast = min(r1, (uint32_t)S::TR - 1) * a.t.r.ld + ch;
+    coff = row * a.t.c.ld + ch;
+    clast = min(c1, (uint32_t)S::TC - 1) * a.t.c.ld + ch;
+    // Scales: waves below XW move the rows', the one after them the classes'.
+    xp = reinterpret_cast<const char*>(a.xs) + (size_t)at.rt * S::TR * a.ldxs;
+    const uint32_t v0 = at.ct * S::TC / CODE_BLOCK;
+    wp = reinterpret_cast<const char*>(a.ws + v0 * a.ldws);
+    soff = w < S::XW ? min((uint32_t)w * 64 + lane, r1) * a.ldxs
+                     : (uint32_t)(min(v0 + (lane & 1), (a.k - 1) / CODE_BLOCK) - v0) *
+                           (uint32_t)a.ldws * 4u;
+  };
+  constexpr int PER = S::RD + S::CD + 1;
+  auto dma = [&](int q) __attribute__((always_inline)) {
+    const uint32_t by = lslab + 1 == steps ? back : 0u;
+    const size_t from = (size_t)lslab * CODE_BLOCK;
+    if (q < S::RD) {
+      const uint32_t o = min(roff + (uint32_t)q * S::NW * 8 * a.t.r.ld, rlast);
+      dma16a(rp + from, o - by, lst + (uint32_t)(q * S::NW + w) * 1024);
+    } else if (q < S::RD + S::CD) {
+      const int j = q - S::RD;
+      const uint32_t o = min(coff + (uint32_t)j * S::NW * 8 * a.t.c.ld, clast);
+      dma16a(cp + from, o - by, lst + S::RBYTES + (uint32_t)(j * S::NW + w) * 1024);
+    } else if (w <= S::XW) {
+      dma4a((w < S::XW ? xp : wp) + (size_t)lslab * 4, soff, lst + S::CODES + (uint32_t)w * 256);
+    }
+  };
+  auto advance = [&]() __attribute__((always_inline)) {
+    lst = 2 * lds0 + S::STAGE - lst;
+    if (++lslab == steps) {
+      if (lbid + gridDim.x < a.t.blocks) {
+        lbid += gridDim.x;
+        lslab = 0;
+        aim();
+      } else {
+        lslab = steps - 1;
+      }
+    }
+  };
+  auto barrier = [&]() __attribute__((always_inline)) {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  // Zeros past d in the last block's stage, which has landed.
+  auto cut = [&](uint32_t stage) __attribute__((always_inline)) {
+    for (uint32_t r = threadIdx.x; r < (uint32_t)(S::TR + S::TC); r += S::THREADS) {
+      const uint32_t row = stage + r * CODE_BLOCK;
+      for (uint32_t c = tail / 16; c < 8; c++) {
+        lds_v4u p = (lds_v4u)(uintptr_t)(row + ((c ^ deep_swz(r)) << 4));
+        v4u v{0u, 0u, 0u, 0u};
+        if (c * 16 < tail) v = first_codes(*p, (int)(tail - c * 16));
+        *p = v;
+      }
+    }
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+    barrier();
+  };
+
+  aim();
+#pragma unroll
+  for (int s = 0; s < 2; s++) {
+#pragma unroll
+    for (int q = 0; q < PER; q++) dma(q);
+    advance();
+  }
+  wait_vm<PER - 1>();  // the first block is in (a wave without a DMA of scales has PER - 1 a block)
+  barrier();
+  if (steps == 1 && tail < CODE_BLOCK) cut(lds0);
+
+  const uint32_t swz = (g ^ deep_swz(li)) << 4;
+  const uint32_t rat = (uint32_t)(wr * S::YB * 16 + li) * CODE_BLOCK + swz;
+  const uint32_t cat = S::RBYTES + (uint32_t)(wc * S::AB * 16 + li) * CODE_BLOCK + swz;
+  const uint32_t xat = S::CODES + (uint32_t)(wr * S::YB * 16 + li) * 4;
+  const uint32_t wat = S::CODES + S::TR * 4 + (uint32_t)(wc * S::AB * 16 / CODE_BLOCK) * 4;
+  constexpr uint32_t BLOCK16 = 16 * CODE_BLOCK;
+  constexpr int ALL = S::AB * S::YB, SLOTS = 4, AHEAD = SLOTS - 1;
+  static_assert(S::YB == 4 && S::AB % SLOTS == 0, "t and ca by turns");
+
+  uint32_t st = lds0;
+  Frag rb[S::YB], ca[SLOTS];
+  float f[S::YB], fx[S::YB], fw;
+  auto read_scales = [&](uint32_t stage) __attribute__((always_inline)) {
+    fw = *(lds_f32)(uintptr_t)(stage + wat);
+#pragma unroll
+    for (int y = 0; y < S::YB; y++) fx[y] = *(lds_f32)(uintptr_t)(stage + xat + y * 64);
+  };
+  read_scales(st);
+#pragma unroll
+  for (int y = 0; y < S::YB; y++) rb[y].read(st + rat + y * BLOCK16);
+#pragma unroll
+  for (int i = 0; i < AHEAD; i++) ca[i].read(st + cat + i * BLOCK16);
+#pragma unroll
+  for (int y = 0; y < S::YB; y++) f[y] = fx[y] * fw;
+
+  // Sixteen bytes of results a lane.
+  constexpr int EL = 16 / sizeof(T), STRIDE = EL / 4, STORES = S::YB * S::AB / STRIDE;
+  bool stored = false;  // the last tile's results went out in STORES stores of every wave
+  for (uint32_t bid = blockIdx.x; bid < a.t.blocks; bid += gridDim.x) {
+    v4f acc[S::AB][S::YB];
+#pragma unroll
+    for (int i = 0; i < S::AB; i++)
+#pragma unroll
+      for (int y = 0; y < S::YB; y++) acc[i][y] = v4f{0.f, 0.f, 0.f, 0.f};
+    float fp[2] = {0.f, 0.f};  // the last block's scales of its last two sums
+    v4f t[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) t[i] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (uint32_t s = 0; s < steps; s++) {
+      Halves rh[EXACT ? S::YB : 1];
+      if constexpr (EXACT) {
+#pragma unroll
+        for (int y = 0; y < S::YB; y++) rh[y] = Halves(rb[y].a, rb[y].b);
+      }
+      const uint32_t other = 2 * lds0 + S::STAGE - st;
+#pragma unroll
+      for (int i = 0; i < S::AB; i++) {
+        // The class blocks are read AHEAD of their MFMAs: before these the last of the stage's
+        // are in registers.
+        constexpr int MEET = S::AB - AHEAD;
+        if (i == MEET) {
+          // The next block is in. (What a wave queues is done in order: stores of the last
+          // tile's results went out after it.)
+          if (s == 0 && stored)
+            wait_vm<STORES>();
+          else
+            wait_vm<0>();
+          __builtin_amdgcn_s_waitcnt(0xc07f);
+          barrier();
+          // (Of this tile, or of the next one, whose only block it then is.)
+          if (tail < CODE_BLOCK && (s + 2 == steps || steps == 1)) cut(other);
+          read_scales(other);
+        }
+        if (i + AHEAD < S::AB)
+          ca[(i + AHEAD) % SLOTS].read(st + cat + (i + AHEAD) * BLOCK16);
+        else
+          ca[(i + AHEAD) % SLOTS].read(other + cat + (i + AHEAD - S::AB) * BLOCK16);
+        Halves ch;
+        if constexpr (EXACT) ch = Halves(ca[i % SLOTS].a, ca[i % SLOTS].b);
+#pragma unroll
+        for (int y = 0; y < S::YB; y++) {
+          const int m = i * S::YB + y, o = (m + ALL - 2) % ALL;  // the MFMA, and whose sums are due
+          if constexpr (EXACT)
+            t[m & 3] = block16(ch, rh[y]);
+          else
+            t[m & 3] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                ca[i % SLOTS].codes(), rb[y].codes(), v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+          const float by = m < 2 ? fp[m] : f[o % S::YB];
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            acc[o / S::YB][o % S::YB][e] = fmaf(t[o & 3][e], by, acc[o / S::YB][o % S::YB][e]);
+          // (Here, not at the step's end, with all the blocks' sums kept until then.)
+          asm volatile("" : "+v"(acc[o / S::YB][o % S::YB]));
+          if (i == S::AB - 1) rb[y].read(other + rat + y * BLOCK16);
+          __builtin_amdgcn_sched_barrier(0);
+          if (i >= MEET) {
+            constexpr int LEFT = (S::AB - MEET) * S::YB;
+            const int from = m - MEET * S::YB;
+#pragma unroll
+            for (int q = from * PER / LEFT; q < (from + 1) * PER / LEFT; q++) dma(q);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+      }
+      fp[0] = f[S::YB - 2];
+      fp[1] = f[S::YB - 1];
+#pragma unroll
+      for (int y = 0; y < S::YB; y++) f[y] = fx[y] * fw;
+      advance();
+      st = other;
+    }
+#pragma unroll
+    for (int m = 0; m < 2; m++) {
+      const int o = ALL - 2 + m;
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        acc[o / S::YB][o % S::YB][e] = fmaf(t[o & 3][e], fp[m], acc[o / S::YB][o % S::YB][e]);
+    }
+
+    // A row's 128 bytes go out together, sixteen a lane.
+    const TileAt at = tile_at(a.t, bid);
+    stored = (at.rt + 1) * S::TR <= a.n && (at.ct + 1) * S::TC <= a.k;
+    const bool low = li < 8;
+#pragma unroll
+    for (int y = 0; y < S::YB; y++) {
+      const uint32_t row0 = at.rt * S::TR + (uint32_t)(wr * S::YB + y) * 16 + (li & 7);
+#pragma unroll
+      for (int i = 0; i < S::AB; i += 2 * STRIDE) {
+        uint32_t q[2][4];
+#pragma unroll
+        for (int h = 0; h < 2; h++) sixteen<T>(&acc[i + h * STRIDE], y, q[h]);
+        // Lanes li < 8 hand their second sixteen bytes to li + 8 and get its first: then eight
+        // lanes have a row's 128 bytes, first of the rows li, then of li + 8.
+        uint32_t o[2][4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const uint32_t give = low ? q[1][e] : q[0][e];
+          const uint32_t got = __float_as_uint(lane_perm<0x128>(__uint_as_float(give)));
+          o[0][e] = low ? q[0][e] : got;
+          o[1][e] = low ? got : q[1][e];
+        }
+        const uint32_t col = at.ct * S::TC + (uint32_t)(wc * S::AB + i + (low ? 0 : STRIDE)) * 16 +
+                             (sizeof(T) == 4 ? 4 * g : 16 * (g & 1) + 8 * (g >> 1));
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const uint32_t row = row0 + 8 * h;
+          T* const p = reinterpret_cast<T*>(a.y) + (size_t)row * a.ldy + col;
+          const Vec<T> v{make_uint4(o[h][0], o[h][1], o[h][2], o[h][3])};
+          if (stored || (row < a.n && col + EL <= a.k))
+            STREAM ? stream_vec(p, v) : store_vec(p, v);
+          else if (row < a.n && col < a.k)
+            store_some(p, v, (int)(a.k - col));
+        }
+      }
+    }
+  }
+  wait_vm<0>();  // the DMAs past the last step have landed
+}
+
+template <class T, class S, bool EXACT>
+void launch_tiles(emh_ctx* c, const CodedIn& x, size_t n, size_t d, const CodedIn& w, size_t k,
+                  const MatOut& y) {
+  Prod8Args a{};
+  a.k = (uint32_t)k, a.d = (uint32_t)d;
+  a.ws = w.scale, a.ldws = w.lds, a.ldxs = (uint32_t)(x.lds * 4), a.ldy = y.ld;
+  a.t.c = {{(const char*)w.q, nullptr}, (uint32_t)w.ld, (uint32_t)k, 0};
+  a.t.slabs = (uint32_t)((d + CODE_BLOCK - 1) / CODE_BLOCK);
+  a.t.passes = 1, a.t.splits = 1;
+  // Where rows begin at whole 64 bytes: pieces of them are put together in the caches.
+  const bool stream = n * k * sizeof(T) >= STREAM_FROM && y.ld * sizeof(T) % 64 == 0 &&
+                      (uintptr_t)y.p % 64 == 0;
+  a.t.ctiles = (uint32_t)((k + S::TC - 1) / S::TC);
+  // Bands of rows whose tiles 32 bits number.
+  const size_t most = std::max<size_t>(1, (size_t(1) << 30) / a.t.ctiles / GROUP) * S::TR;
+  for (size_t r0 = 0; r0 < n; r0 += most) {
+    const size_t rows = std::min(n - r0, most);
+    a.n = (uint32_t)rows;
+    a.xs = x.scale + r0 * x.lds;
+    a.y = (T*)y.p + r0 * y.ld;
+    a.t.r = {{(const char*)x.q + r0 * x.ld, nullptr}, (uint32_t)x.ld, (uint32_t)rows, 0};
+    a.t.rtiles = (uint32_t)((rows + S::TR - 1) / S::TR);
+    const unsigned blocks = prepare(a.t);
+    const unsigned grid = std::min(blocks, (unsigned)(c->cus * S::PER_CU));
+    if (stream)
+      k_tile8<T, S, EXACT, true><<<grid, S::THREADS, 0, c->stream>>>(a);
+    else
+      k_tile8<T, S, EXACT, false><<<grid, S::THREADS, 0, c->stream>>>(a);
+  }
+}
+
 }  // namespace
 
 void launch_product8(emh_ctx* c, const CodedIn& x, size_t n, size_t d, const CodedIn& w, size_t k,
@@ -117,12 +484,27 @@ void launch_product8(emh_ctx* c, const CodedIn& x, size_t n, size_t d, const Cod
     k_few8<YB><<<dim3((unsigned)std::min(groups, MAX_GROUPS)), 256, 0, c->stream>>>(
         x, n, d, w, k, y.p, y.ld, y.kind, (uint32_t)rg, groups);
   };
-  if (n <= 16)
+  // (A tile's offsets are 32 bits, rows of one launch too.)
+  const bool far = std::max({x.ld, w.ld, x.lds * 4, w.lds * 4}) >= (size_t(1) << 23);
+  if (n > 64 && !far) {
+    if (y.kind == EMH_F32) {
+      launch_tiles<float, Small8, true>(c, x, n, d, w, k, y);
+    } else {
+      const bool large = ((n + 255) / 256) * ((k + 255) / 256) >= (size_t)c->cus;
+      auto go = [&](auto t) {
+        using T = decltype(t);
+        large ? launch_tiles<T, Large8, false>(c, x, n, d, w, k, y)
+              : launch_tiles<T, Small8, false>(c, x, n, d, w, k, y);
+      };
+      y.kind == EMH_F16 ? go(f16{}) : go(bf16{});
+    }
+  } else if (n <= 16) {
     few(std::integral_constant<int, 1>{});
-  else if (n <= 32)
+  } else if (n <= 32) {
     few(std::integral_constant<int, 2>{});
-  else
+  } else {
     few(std::integral_constant<int, 4>{});
+  }
   EMH_HIP(hipGetLastError());
 }
 

@@ -161,8 +161,8 @@ struct TileAt {
 // consecutive items, in which the tiles of GROUP row tiles and a column tile follow each
 // other, so that what its 32 CUs read at a time is a few row and column
 // slabs, shared in its L2.
-__device__ __forceinline__ TileAt tile_at(const TileIn& t) {
-  const uint32_t nb = t.blocks, bid = blockIdx.x;
+__device__ __forceinline__ TileAt tile_at(const TileIn& t, uint32_t bid) {
+  const uint32_t nb = t.blocks;
   const uint32_t xcd = bid & 7, q = bid >> 3, m = nb >> 3, rem = nb & 7;
   uint32_t wi = xcd * m + min(xcd, rem) + q;
   TileAt a;
@@ -178,6 +178,8 @@ __device__ __forceinline__ TileAt tile_at(const TileIn& t) {
   a.s1 = a.s0 + t.steps + (a.split < t.more ? 1 : 0);
   return a;
 }
+
+__device__ __forceinline__ TileAt tile_at(const TileIn& t) { return tile_at(t, blockIdx.x); }
 
 __device__ __forceinline__ uint32_t deep_swz(uint32_t row) { return (row >> 1) & 7; }
 
