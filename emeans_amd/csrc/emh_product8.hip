@@ -153,6 +153,7 @@ struct Prod8Args {
   size_t ldws;
   void* y;
   size_t ldy;
+  bool odd;  // 16 bits: rows of y may begin at odd multiples of two bytes
 };
 
 struct Frag {  // a lane's 32 codes of a block's row
@@ -190,6 +191,39 @@ template <class T>
 __device__ __forceinline__ void stream_vec(T* p, const Vec<T>& v) {
   typedef uint32_t any16 __attribute__((ext_vector_type(4), aligned(2)));
   __builtin_nontemporal_store(any16{v.raw.x, v.raw.y, v.raw.z, v.raw.w}, reinterpret_cast<any16*>(p));
+}
+
+// A lane's pieces of a row (eight elements each, 64 apart; the lane has the row's `place` of
+// eight) to p, of which `left` elements from p on are the row's, where rows may begin at odd
+// multiples of two bytes: a row that does goes out an element later, by whole words.
+template <class T, int PIECES>
+__device__ __forceinline__ void store_odd(T* p, const uint32_t (*o)[4], uint32_t place,
+                                          uint32_t left) {
+  const uint32_t odd = (uint32_t)((uintptr_t)p >> 1) & 1, by = 16 * odd;
+  // Where the next eight of the row are: the lane of the next place.
+  const uint32_t lane = threadIdx.x & 63, q = (place + 1) & 7;
+  const uint32_t next = (lane & 7) + (q >> 2) * 8 + ((q >> 1 & 1) | (q & 1) << 1) * 16;
+#pragma unroll
+  for (int i = 0; i < PIECES; i++) {
+    const uint32_t give = place == 0 && i + 1 < PIECES ? o[i + 1 < PIECES ? i + 1 : i][0] : o[i][0];
+    const uint32_t after = (uint32_t)__builtin_amdgcn_ds_bpermute((int)(next * 4), (int)give);
+    uint32_t v[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+      v[e] = __builtin_amdgcn_alignbit(e < 3 ? o[i][e < 3 ? e + 1 : 3] : after, o[i][e], by);
+    const uint32_t at = (uint32_t)i * 64 + odd;
+    // The last of the pieces ends with its own eight.
+    const uint32_t have = i + 1 == PIECES && place == 7 ? 8 - odd : 8;
+    // (`left > at ? left - at : 0` lets the compiler take left for at least `odd` below.)
+    const uint32_t n = min(max(left, at) - at, have);
+    const Vec<T> out{make_uint4(v[0], v[1], v[2], v[3])};
+    if (n == 8)
+      store_vec(p + at, out);
+    else if (n > 0)
+      store_some(p + at, out, (int)n);
+    if (i == 0 && odd && place == 0 && left > 0)
+      *p = __builtin_bit_cast(T, (uint16_t)o[0][0]);
+  }
 }
 
 // EXACT: f32 results by f16 MFMAs; else T results by 8-bit ones. STREAM: results that are
@@ -402,39 +436,48 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_tile8(const Prod8Args a) {
         acc[o / S::YB][o % S::YB][e] = fmaf(t[o & 3][e], fp[m], acc[o / S::YB][o % S::YB][e]);
     }
 
-    // A row's 128 bytes go out together, sixteen a lane.
+    // A row's 128 bytes go out together, sixteen a lane, `place` of eight.
     const TileAt at = tile_at(a.t, bid);
     stored = (at.rt + 1) * S::TR <= a.n && (at.ct + 1) * S::TC <= a.k;
     const bool low = li < 8;
+    const uint32_t place = (low ? 0u : 4u) + (sizeof(T) == 4 ? g : 2 * (g & 1) + (g >> 1));
+    const uint32_t col0 = at.ct * S::TC + (uint32_t)(wc * S::AB) * 16 + place * EL;
+    constexpr int PIECES = S::AB / (2 * STRIDE);
 #pragma unroll
     for (int y = 0; y < S::YB; y++) {
-      const uint32_t row0 = at.rt * S::TR + (uint32_t)(wr * S::YB + y) * 16 + (li & 7);
+      uint32_t o[2][PIECES][4];
 #pragma unroll
-      for (int i = 0; i < S::AB; i += 2 * STRIDE) {
+      for (int i = 0; i < PIECES; i++) {
         uint32_t q[2][4];
 #pragma unroll
-        for (int h = 0; h < 2; h++) sixteen<T>(&acc[i + h * STRIDE], y, q[h]);
+        for (int h = 0; h < 2; h++) sixteen<T>(&acc[(2 * i + h) * STRIDE], y, q[h]);
         // Lanes li < 8 hand their second sixteen bytes to li + 8 and get its first: then eight
         // lanes have a row's 128 bytes, first of the rows li, then of li + 8.
-        uint32_t o[2][4];
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           const uint32_t give = low ? q[1][e] : q[0][e];
           const uint32_t got = __float_as_uint(lane_perm<0x128>(__uint_as_float(give)));
-          o[0][e] = low ? q[0][e] : got;
-          o[1][e] = low ? got : q[1][e];
+          o[0][i][e] = low ? q[0][e] : got;
+          o[1][i][e] = low ? got : q[1][e];
         }
-        const uint32_t col = at.ct * S::TC + (uint32_t)(wc * S::AB + i + (low ? 0 : STRIDE)) * 16 +
-                             (sizeof(T) == 4 ? 4 * g : 16 * (g & 1) + 8 * (g >> 1));
+      }
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          const uint32_t row = row0 + 8 * h;
-          T* const p = reinterpret_cast<T*>(a.y) + (size_t)row * a.ldy + col;
-          const Vec<T> v{make_uint4(o[h][0], o[h][1], o[h][2], o[h][3])};
-          if (stored || (row < a.n && col + EL <= a.k))
-            STREAM ? stream_vec(p, v) : store_vec(p, v);
-          else if (row < a.n && col < a.k)
-            store_some(p, v, (int)(a.k - col));
+      for (int h = 0; h < 2; h++) {
+        const uint32_t row = at.rt * S::TR + (uint32_t)(wr * S::YB + y) * 16 + (li & 7) + 8 * h;
+        T* const p = reinterpret_cast<T*>(a.y) + (size_t)row * a.ldy + col0;
+        if (sizeof(T) == 2 && a.odd) {
+          if constexpr (sizeof(T) == 2)
+            store_odd<T, PIECES>(p, o[h], place, row < a.n && col0 < a.k ? a.k - col0 : 0u);
+        } else {
+#pragma unroll
+          for (int i = 0; i < PIECES; i++) {
+            const uint32_t col = col0 + i * 8 * EL;
+            const Vec<T> v{make_uint4(o[h][i][0], o[h][i][1], o[h][i][2], o[h][i][3])};
+            if (stored || (row < a.n && col + EL <= a.k))
+              STREAM ? stream_vec(p + i * 8 * EL, v) : store_vec(p + i * 8 * EL, v);
+            else if (row < a.n && col < a.k)
+              store_some(p + i * 8 * EL, v, (int)(a.k - col));
+          }
         }
       }
     }
@@ -447,6 +490,7 @@ void launch_tiles(emh_ctx* c, const CodedIn& x, size_t n, size_t d, const CodedI
                   const MatOut& y) {
   Prod8Args a{};
   a.k = (uint32_t)k, a.d = (uint32_t)d;
+  a.odd = sizeof(T) == 2 && (y.ld % 2 != 0 || (uintptr_t)y.p % 4 != 0);
   a.ws = w.scale, a.ldws = w.lds, a.ldxs = (uint32_t)(x.lds * 4), a.ldy = y.ld;
   a.t.c = {{(const char*)w.q, nullptr}, (uint32_t)w.ld, (uint32_t)k, 0};
   a.t.slabs = (uint32_t)((d + CODE_BLOCK - 1) / CODE_BLOCK);
