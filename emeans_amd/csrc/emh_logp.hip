@@ -7,9 +7,13 @@
 // joined the same way, and lse = m + log S, H = log S - E / S, log p_t = (z_t - m) - log S.
 //
 // The likeliest classes: a wave keeps a sorted list in its lanes (lane i the i-th), the
-// larger logit first, the lower class among equals. A chunk is looked at again only where a
-// lane's largest element would enter the list; each lane offers its largest, then, where that
-// was taken, its next. The logits' own values are compared, unscaled and unrounded.
+// larger logit first, the lower class among equals: an entry is one key of 64 bits, the logit's
+// own value (unscaled and unrounded) in an order of whole numbers above the class's complement.
+// Of a chunk only lanes whose largest element would enter the list matter; of the top largest
+// of those the least is a bound that no better element is below. What reaches it, a few more
+// than top, goes to LDS beside the list, where every entry counts the ones before it: that is
+// its place. (Many equal values overflow the LDS: then each lane offers its largest, and its
+// next where that was taken.)
 //
 // Gradient: dz_v = scale (gl ([v = t] - p_v) - gh p_v (log p_v + H)), element by element.
 //
@@ -109,42 +113,137 @@ __device__ __forceinline__ float lane_value(float v, uint32_t lane) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), (int)lane));
 }
 
-// The list of the `top` best, sorted, in a wave's lanes.
+__device__ __forceinline__ uint64_t key_of(float v, uint32_t id) {
+  const uint32_t u = __float_as_uint(v + 0.f);  // (-0 is equal to 0)
+  return (uint64_t)(u & 0x80000000u ? ~u : u | 0x80000000u) << 32 | (uint32_t)~id;
+}
+__device__ __forceinline__ float key_value(uint64_t k) {
+  const uint32_t u = (uint32_t)(k >> 32);
+  return __uint_as_float(u & 0x80000000u ? u & 0x7FFFFFFFu : ~u);
+}
+__device__ __forceinline__ uint32_t key_class(uint64_t k) { return ~(uint32_t)k; }
+__device__ __forceinline__ uint64_t lane_key(uint64_t k, uint32_t lane) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(k >> 32), (int)lane) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)k, (int)lane);
+}
+// What other lanes of the wave have written to LDS is there.
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+constexpr uint32_t ROOM = 64;  // entries that a wave ranks at a time
+constexpr uint32_t ROOM_END = 4;  // zeros after them
+
+// The `top` best, sorted, in a wave's lanes; no entry: 0.
 struct Best {
-  float v = -INFINITY;
-  uint32_t id = NONE;
+  uint64_t key = 0;
+  // The least value that an entry must exceed.
+  __device__ __forceinline__ float bound(uint32_t top) const {
+    const uint64_t k = lane_key(key, top - 1);
+    return k ? key_value(k) : -INFINITY;
+  }
+  // The list's entries behind `count` others in `room` (ROOM in all), and the best of all of
+  // them the list. (Every lane reads every entry, two at a time: no lane waits for another's.)
+  __device__ __forceinline__ void merge(uint32_t top, uint64_t* room, uint32_t count) {
+    const uint32_t lane = threadIdx.x & 63;
+    const uint32_t old = (uint32_t)__popcll(__ballot(key != 0));
+    if (lane < old + 4) room[count + lane] = lane < old ? key : 0;
+    count += old;
+    wave_fence();
+    const uint64_t mine = lane < count ? room[lane] : 0;
+    uint32_t place = 0;
+    for (uint32_t j = 0; j < count; j += 4) {
+      const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(room + j);
+      const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(room + j + 2);
+      place += (a.x > mine) + (a.y > mine) + (b.x > mine) + (b.y > mine);
+    }
+    wave_fence();
+    if (lane < count && place < top) room[place] = mine;
+    wave_fence();
+    key = lane < (count < top ? count : top) ? room[lane] : 0;
+    wave_fence();
+  }
   // Every lane with `has` offers (cv, cid), cv > -infinity; the lanes whose offer was taken.
   __device__ __forceinline__ uint64_t offer(uint32_t top, float cv, uint32_t cid, bool has) {
     const uint32_t lane = threadIdx.x & 63;
     uint64_t taken = 0;
     for (;;) {
-      const float tv = lane_value(v, top - 1);
-      const uint32_t tid = (uint32_t)__builtin_amdgcn_readlane((int)id, (int)top - 1);
-      const bool better = has && (cv > tv || (cv == tv && cid < tid));
-      if (!__any(better)) return taken;
-      const float best = lanes_max<64>(better ? cv : -INFINITY);
-      uint64_t who = __ballot(better && cv == best);
+      const uint64_t mine = has ? key_of(cv, cid) : 0;
+      const uint64_t last = lane_key(key, top - 1);
+      uint64_t who = __ballot(mine > last);
+      if (!who) return taken;
       uint32_t from = (uint32_t)__ffsll((unsigned long long)who) - 1;
-      uint32_t bid = (uint32_t)__builtin_amdgcn_readlane((int)cid, (int)from);
-      for (who &= who - 1; who; who &= who - 1) {  // the lowest class of equals
+      uint64_t best = lane_key(mine, from);
+      for (who &= who - 1; who; who &= who - 1) {
         const uint32_t at = (uint32_t)__ffsll((unsigned long long)who) - 1;
-        const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)cid, (int)at);
-        if (o < bid) bid = o, from = at;
+        const uint64_t o = lane_key(mine, at);
+        if (o > best) best = o, from = at;
       }
       taken |= uint64_t(1) << from;
       if (lane == from) has = false;
-      const uint32_t r = (uint32_t)__popcll(__ballot(v > best || (v == best && id < bid)));
-      const float pv = lane_perm<0x138>(v);  // the lane below's
-      const uint32_t pid = __float_as_uint(lane_perm<0x138>(__uint_as_float(id)));
-      v = lane == r ? best : lane > r ? pv : v;
-      id = lane == r ? bid : lane > r ? pid : id;
+      const uint32_t r = (uint32_t)__popcll(__ballot(key > best));
+      const uint32_t lo = __float_as_uint(lane_perm<0x138>(__uint_as_float((uint32_t)key)));
+      const uint32_t hi = __float_as_uint(lane_perm<0x138>(__uint_as_float((uint32_t)(key >> 32))));
+      const uint64_t below = (uint64_t)hi << 32 | lo;  // the lane below's
+      key = lane == r ? best : lane > r ? below : key;
     }
   }
 };
 
+// Lanes' values v: a bound that at least `top` of them reach (-infinity where fewer than that
+// are above it), found in groups: as many as the next power of two from top; the least of the
+// groups' largest.
+__device__ __forceinline__ float group_bound(float v, uint32_t top) {
+  const uint32_t p = top <= 1 ? 0u : 32u - (uint32_t)__clz((int)(top - 1));  // log2 of the groups
+  auto join = [&](uint32_t step, float a, float b) __attribute__((always_inline)) {
+    return step + p < 6 ? fmaxf(a, b) : fminf(a, b);
+  };
+  v = join(0, v, lane_perm<0xB1>(v));
+  v = join(1, v, lane_perm<0x4E>(v));
+  v = join(2, v, lane_perm<0x141>(v));
+  v = join(3, v, lane_perm<0x140>(v));
+  const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = join(4, __uint_as_float(s[0]), __uint_as_float(s[1]));
+  const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return join(5, __uint_as_float(h[0]), __uint_as_float(h[1]));
+}
+// The top-th largest of the lanes' values among those in `who` (more than top). room: LDS for 68.
+__device__ __forceinline__ float exact_bound(float v, uint64_t who, uint32_t top, float* room) {
+  const uint32_t lane = threadIdx.x & 63, count = (uint32_t)__popcll(who);
+  const bool in = who >> lane & 1;
+  if (in)
+    room[__builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0u))] = v;
+  if (lane < 4) room[count + lane] = -INFINITY;
+  wave_fence();
+  uint32_t above = 0;
+  for (uint32_t j = 0; j < count; j += 4) {
+    const float4 o = *reinterpret_cast<const float4*>(room + j);
+    above += (o.x > v) + (o.y > v) + (o.z > v) + (o.w > v);
+  }
+  wave_fence();
+  return lanes_reduce<64>(in && above < top ? v : INFINITY,
+                          [](float a, float b) { return fminf(a, b); });
+}
+// The least f32 above v.
+__device__ __forceinline__ float next_above(float v) {
+  const uint32_t u = __float_as_uint(v);
+  return __uint_as_float(v == 0.f ? 1u : u & 0x80000000u ? u - 1 : u + 1);
+}
+
+// A row's given class and its logit: asked for before the row's sums are made.
+struct Given {
+  uint32_t t = NONE;
+  float z = 0.f;
+  __device__ __forceinline__ Given(const LogpArgs& a, int kind, size_t row) {
+    if (!a.logp) return;
+    t = a.tokens[row];
+    z = load_kind(a.z, kind, row * a.ldz + (t < a.k ? t : 0));
+  }
+};
 // The outputs of a row, by one wave.
-__device__ __forceinline__ void finish(const LogpArgs& a, int kind, size_t row, const Seen& all,
-                                       const Best& best) {
+__device__ __forceinline__ void finish(const LogpArgs& a, size_t row, const Given& given,
+                                       const Seen& all, const Best& best) {
   const uint32_t lane = threadIdx.x & 63;
   const float b = all.m == -INFINITY ? 0.f : all.m;
   const float ls = logf(all.s);
@@ -153,38 +252,39 @@ __device__ __forceinline__ void finish(const LogpArgs& a, int kind, size_t row, 
     a.lse[row] = odd ? NAN : all.m == -INFINITY ? -INFINITY : all.m + ls;
     if (a.entropy) a.entropy[row] = odd ? NAN : all.s > 0.f ? ls - all.e / all.s : 0.f;
     if (a.logp) {
-      const uint32_t t = a.tokens[row];
       float lp = 0.f;
-      if (t < a.k) {
-        lp = fmaf(load_kind(a.z, kind, row * a.ldz + t), a.scale, -b);
+      if (given.t < a.k) {
+        lp = fmaf(given.z, a.scale, -b);
         lp = odd ? NAN : all.s > 0.f ? lp - ls : -INFINITY;
-      } else if (t != NONE) {
+      } else if (given.t != NONE) {
         a.small[SW_BAD_CLASS] = 1u;
       }
       a.logp[row] = lp;
     }
   }
   if (lane < a.top) {
-    const bool is = best.id != NONE && !odd;
-    if (a.ids) a.ids[row * a.top + lane] = is ? best.id : NONE;
+    const bool is = best.key != 0 && !odd;
+    if (a.ids) a.ids[row * a.top + lane] = is ? key_class(best.key) : NONE;
     if (a.tops)
-      a.tops[row * a.top + lane] = odd ? NAN : is ? fmaf(best.v, a.scale, -b) - ls : -INFINITY;
+      a.tops[row * a.top + lane] =
+          odd ? NAN : is ? fmaf(key_value(best.key), a.scale, -b) - ls : -INFINITY;
   }
 }
 
 struct PartOut {  // [row][part]
   float4* seen;   // m, s, e
-  float2* best;   // [row][part][top]: value, class
+  uint64_t* best; // [row][part][top]
 };
 
 // W waves take a part of a row, by turns in chunks of 64 NV vectors; parts == 1: whole
-// rows, whose results they write.
+// rows, whose results they write. One wave: rows of one chunk.
 template <class T, int W, int NV, bool TOP>
 __global__ __launch_bounds__(256) void k_logp(const LogpArgs a, int kind, uint32_t parts,
                                               PartOut out) {
   constexpr int N = VecOf<T>::N, ROWS = 4 / W;
   __shared__ float4 seen[4];
-  __shared__ float2 lists[W > 1 ? 4 : 1][MAX_TOP];
+  __shared__ __attribute__((aligned(16))) uint64_t rooms[TOP ? 4 : 1][ROOM + ROOM_END];
+  __shared__ uint64_t lists[TOP && W > 1 ? 4 : 1][MAX_TOP];
   const uint32_t lane = threadIdx.x & 63;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const uint32_t w = wave % W;
@@ -196,7 +296,8 @@ __global__ __launch_bounds__(256) void k_logp(const LogpArgs a, int kind, uint32
     const uint32_t part = (uint32_t)(u - row * parts);
     const Row<T> r(a.z, row * a.ldz, a.k);
     const size_t nv = r.vectors(), chunks = (nv + 64 * NV - 1) / (64 * NV);
-    const size_t c0 = chunks * part / parts, c1 = chunks * (part + 1) / parts;
+    const size_t c0 = W == 1 ? 0 : chunks * part / parts;
+    const size_t c1 = W == 1 ? 1 : chunks * (part + 1) / parts;
     Seen all;
     Best best;
     Vec<T> next[NV];
@@ -208,11 +309,12 @@ __global__ __launch_bounds__(256) void k_logp(const LogpArgs a, int kind, uint32
       }
     };
     if (c0 + w < c1) fetch(c0 + w);
+    Given given(a, kind, row);
     for (size_t c = c0 + w; c < c1; c += W) {
       Vec<T> x[NV];
 #pragma unroll
       for (int j = 0; j < NV; j++) x[j] = next[j];
-      if (c + W < c1) fetch(c + W);
+      if (W > 1 && c + W < c1) fetch(c + W);
       const size_t v0 = c * (64 * NV) + lane;
       if (c == 0 || c == chunks - 1) {
 #pragma unroll
@@ -236,35 +338,76 @@ __global__ __launch_bounds__(256) void k_logp(const LogpArgs a, int kind, uint32
           all.e = fmaf(p, fmaxf(d, FAR), all.e);
         }
       if constexpr (TOP) {
-        // The largest of the lane's that comes after (v, id) in the list's order.
-        auto after = [&](float v, uint32_t id, float& cv, uint32_t& cid) __attribute__((always_inline)) {
+        // The largest of the lane's that comes after (v, id) in the list's order. (From memory
+        // again: registers for the few rows that come here would be every row's.)
+        auto after = [&](float v, uint32_t id, float& cv, uint32_t& cid) {
           cv = -INFINITY;
           cid = NONE;
-#pragma unroll
+#pragma unroll 1
           for (int j = 0; j < NV; j++) {
-            const uint32_t col = (uint32_t)r.column(v0 + j * 64);
+            const size_t at = v0 + (size_t)j * 64;
+            Vec<T> y = r.load(at < nv ? at : nv - 1);
+            r.mask(y, at);
+            const uint32_t col = (uint32_t)r.column(at);
 #pragma unroll
             for (int e = 0; e < N; e++) {
-              const float q = x[j].get(e);
+              const float q = y.get(e);
               const bool is = (q < v || (q == v && col + e > id)) && q > cv;
               cv = is ? q : cv;
               cid = is ? col + e : cid;
             }
           }
         };
-        if (__any(most >= lane_value(best.v, a.top - 1) && most > -INFINITY)) {
-          float lv = INFINITY;
-          uint32_t lid = 0;
-          bool may = true;
-          for (;;) {
-            float cv;
-            uint32_t cid;
-            after(lv, lid, cv, cid);
-            const uint64_t taken = best.offer(a.top, cv, cid, may && cid != NONE);
-            if (!taken) break;
-            may = taken >> lane & 1;
-            lv = cv;
-            lid = cid;
+        const float need = best.bound(a.top);
+        uint64_t who = __ballot(most > need);
+        if (who) {
+          float least = -INFINITY;
+          if ((uint32_t)__popcll(who) > a.top) {
+            const float bound = group_bound(most, a.top);
+            who &= __ballot(most >= bound);
+            least = (uint32_t)__popcll(who) > a.top
+                        ? exact_bound(most, who, a.top, reinterpret_cast<float*>(rooms[wave]))
+                        : bound;
+          }
+          least = least > need ? least : next_above(need);
+          // (A later chunk's equal of the list's last has a higher class.)
+          uint64_t* const room = rooms[wave];
+          const uint32_t old = (uint32_t)__popcll(__ballot(best.key != 0));
+          uint32_t count = 0;
+#pragma unroll
+          for (int j = 0; j < NV; j++) {
+            const uint32_t col = (uint32_t)r.column(v0 + j * 64);
+#pragma unroll
+            for (int e = 0; e < N; e++) {
+              const float q = x[j].get(e);
+              const bool is = q >= least;
+              const uint64_t them = __ballot(is);
+              if (them) {
+                const uint32_t at = count + __builtin_amdgcn_mbcnt_hi(
+                                                (uint32_t)(them >> 32),
+                                                __builtin_amdgcn_mbcnt_lo((uint32_t)them, 0u));
+                if (is && at < ROOM) room[at] = key_of(q, col + e);
+                count += (uint32_t)__popcll(them);
+              }
+            }
+          }
+          if (count + old <= ROOM) {
+            best.merge(a.top, room, count);
+          } else {
+            wave_fence();
+            float lv = INFINITY;
+            uint32_t lid = 0;
+            bool may = true;
+            for (;;) {
+              float cv;
+              uint32_t cid;
+              after(lv, lid, cv, cid);
+              const uint64_t taken = best.offer(a.top, cv, cid, may && cid != NONE);
+              if (!taken) break;
+              may = taken >> lane & 1;
+              lv = cv;
+              lid = cid;
+            }
           }
         }
       }
@@ -273,25 +416,25 @@ __global__ __launch_bounds__(256) void k_logp(const LogpArgs a, int kind, uint32
     if constexpr (W > 1) {
       __syncthreads();  // (what the last unit left has been read)
       if (lane == 0) seen[wave] = all.packed();
-      if (TOP && lane < a.top) lists[wave][lane] = make_float2(best.v, __uint_as_float(best.id));
+      if (TOP && lane < a.top) lists[wave][lane] = best.key;
       __syncthreads();
       if (wave == 0) {
         for (int i = 1; i < W; i++) {
           all.join(Seen(seen[i]));
           if constexpr (TOP) {
-            const float2 o = lane < a.top ? lists[i][lane] : make_float2(-INFINITY, 0.f);
-            (void)best.offer(a.top, o.x, __float_as_uint(o.y), o.x > -INFINITY);
+            const uint64_t o = lane < a.top ? lists[i][lane] : 0;
+            if (o) rooms[0][lane] = o;  // (a list's entries come first)
+            best.merge(a.top, rooms[0], (uint32_t)__popcll(__ballot(o != 0)));
           }
         }
       }
     }
     if (W > 1 && wave != 0) continue;
     if (parts == 1) {
-      finish(a, kind, row, all, best);
+      finish(a, row, given, all, best);
     } else {
       if (lane == 0) out.seen[u] = all.packed();
-      if (TOP && lane < a.top)
-        out.best[u * a.top + lane] = make_float2(best.v, __uint_as_float(best.id));
+      if (TOP && lane < a.top) out.best[u * a.top + lane] = best.key;
     }
   }
 }
@@ -303,18 +446,24 @@ __global__ __launch_bounds__(64) void k_logp_join(const LogpArgs a, int kind, ui
   const uint32_t lane = threadIdx.x;
   for (size_t row = blockIdx.x; row < a.n; row += gridDim.x) {
     Seen all;
+    const Given given(a, kind, row);
     for (uint32_t p = lane; p < parts; p += 64) all.join(Seen(in.seen[row * parts + p]));
     all.join_lanes();
     Best best;
     if constexpr (TOP) {
-      const uint32_t count = parts * a.top;
-      for (uint32_t i0 = 0; i0 < count; i0 += 64) {
+      __shared__ __attribute__((aligned(16))) uint64_t room[ROOM + ROOM_END];
+      const uint32_t count = parts * a.top, each = ROOM - a.top;
+      for (uint32_t i0 = 0; i0 < count; i0 += each) {
         const uint32_t i = i0 + lane;
-        const float2 o = i < count ? in.best[row * count + i] : make_float2(-INFINITY, 0.f);
-        (void)best.offer(a.top, o.x, __float_as_uint(o.y), o.x > -INFINITY);
+        const uint64_t o = lane < each && i < count ? in.best[row * count + i] : 0;
+        const uint64_t them = __ballot(o != 0);
+        const uint32_t at = __builtin_amdgcn_mbcnt_hi((uint32_t)(them >> 32),
+                                                      __builtin_amdgcn_mbcnt_lo((uint32_t)them, 0u));
+        if (o) room[at] = o;
+        best.merge(a.top, room, (uint32_t)__popcll(them));
       }
     }
-    finish(a, kind, row, all, best);
+    finish(a, row, given, all, best);
   }
 }
 
@@ -399,19 +548,21 @@ void launch_log_probs(emh_ctx* c, LogpArgs a, int kind) {
   by_kind(kind, [&](auto t) {
     using T = decltype(t);
     constexpr size_t N = VecOf<T>::N;
-    const size_t vectors = (a.k + N - 1) / N + 1;  // (of a row at any address)
-    // A wave a row where the row is a chunk or two and the rows fill the GPU; otherwise four,
-    // and parts of a row where there are few rows.
-    const bool small = vectors <= 64 * 8 && a.n >= (size_t)c->cus;
-    const size_t chunks = (vectors + 255) / 256;
+    // Of a row at any address one more than its elements fill.
+    const bool whole = a.ldz % N == 0 && (uintptr_t)a.z % 16 == 0;
+    const size_t vectors = (a.k + N - 1) / N + (whole ? 0 : 1);
+    // A wave a row where the row is a chunk; otherwise four, and parts of a row where there are
+    // few rows.
+    const bool small = vectors <= 256;
+    const size_t per = vectors <= 1024 ? 128 : 256, chunks = (vectors + per - 1) / per;
     size_t parts = 1;
     if (!small) parts = std::min((chunks + 3) / 4, std::max<size_t>(1, 4 * (size_t)c->cus / a.n));
     PartOut out{};
     if (parts > 1) {
       const size_t seen = (a.n * parts * sizeof(float4) + 255) & ~size_t(255);
-      char* p = (char*)c->logp_part.get(seen + a.n * parts * a.top * sizeof(float2), c->stream);
+      char* p = (char*)c->logp_part.get(seen + a.n * parts * a.top * sizeof(uint64_t), c->stream);
       out.seen = (float4*)p;
-      out.best = (float2*)(p + seen);
+      out.best = (uint64_t*)(p + seen);
     }
     auto go = [&](auto waves, auto nv, auto top) {
       constexpr int W = decltype(waves)::value, NV = decltype(nv)::value;
@@ -424,8 +575,12 @@ void launch_log_probs(emh_ctx* c, LogpArgs a, int kind) {
             a, kind, (uint32_t)parts, out);
     };
     auto with_top = [&](auto top) {
-      if (!small)
+      if (per == 256 && !small)
         go(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{}, top);
+      else if (!small)
+        go(std::integral_constant<int, 4>{}, std::integral_constant<int, 2>{}, top);
+      else if (vectors <= 64)
+        go(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{}, top);
       else if (vectors <= 128)
         go(std::integral_constant<int, 1>{}, std::integral_constant<int, 2>{}, top);
       else
@@ -445,7 +600,9 @@ void launch_log_probs_grad(emh_ctx* c, LogpArgs a, int kind) {
   by_kind(kind, [&](auto t) {
     using T = decltype(t);
     constexpr size_t N = VecOf<T>::N, NV = 4;
-    const size_t vectors = (a.k + N - 1) / N + 1, chunks = (vectors + 64 * NV - 1) / (64 * NV);
+    const bool whole = a.lddz % N == 0 && (uintptr_t)a.dz % 16 == 0;
+    const size_t vectors = (a.k + N - 1) / N + (whole ? 0 : 1);
+    const size_t chunks = (vectors + 64 * NV - 1) / (64 * NV);
     const size_t groups = (a.n * chunks + 3) / 4;
     k_logp_grad<T, NV><<<dim3((unsigned)std::min(groups, MAX_GROUPS)), 256, 0, c->stream>>>(
         a, (uint32_t)chunks);
