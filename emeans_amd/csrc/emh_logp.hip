@@ -280,7 +280,7 @@ struct PartOut {  // [row][part]
 // rows, whose results they write. One wave: rows of one chunk.
 template <class T, int W, int NV, bool TOP>
 __global__ __launch_bounds__(256) void k_logp(const LogpArgs a, int kind, uint32_t parts,
-                                              PartOut out) {
+                                              uint32_t each, PartOut out) {
   constexpr int N = VecOf<T>::N, ROWS = 4 / W;
   __shared__ float4 seen[4];
   __shared__ __attribute__((aligned(16))) uint64_t rooms[TOP ? 4 : 1][ROOM + ROOM_END];
@@ -292,30 +292,31 @@ __global__ __launch_bounds__(256) void k_logp(const LogpArgs a, int kind, uint32
   for (size_t u0 = (size_t)blockIdx.x * ROWS; u0 < units; u0 += (size_t)gridDim.x * ROWS) {
     const size_t u = u0 + wave / W;
     if (W == 1 && u >= units) return;  // (waves of their own)
-    const size_t row = u / parts;
-    const uint32_t part = (uint32_t)(u - row * parts);
+    // (Rows in parts are few.)
+    const size_t row = W == 1 || parts == 1 ? u : (uint32_t)u / parts;
+    const uint32_t part = W == 1 ? 0 : (uint32_t)(u - row * parts);
     const Row<T> r(a.z, row * a.ldz, a.k);
-    const size_t nv = r.vectors(), chunks = (nv + 64 * NV - 1) / (64 * NV);
-    const size_t c0 = W == 1 ? 0 : chunks * part / parts;
-    const size_t c1 = W == 1 ? 1 : chunks * (part + 1) / parts;
+    const uint32_t nv = (uint32_t)r.vectors(), chunks = (nv + 64 * NV - 1) / (64 * NV);
+    const uint32_t c0 = W == 1 ? 0 : min(chunks, part * each);
+    const uint32_t c1 = W == 1 ? 1 : min(chunks, c0 + each);
     Seen all;
     Best best;
     Vec<T> next[NV];
-    auto fetch = [&](size_t c) __attribute__((always_inline)) {
+    auto fetch = [&](uint32_t c) __attribute__((always_inline)) {
 #pragma unroll
       for (int j = 0; j < NV; j++) {
-        const size_t v = c * (64 * NV) + j * 64 + lane;
+        const uint32_t v = c * (64 * NV) + j * 64 + lane;
         next[j] = r.load(v < nv ? v : nv - 1);
       }
     };
     if (c0 + w < c1) fetch(c0 + w);
     Given given(a, kind, row);
-    for (size_t c = c0 + w; c < c1; c += W) {
+    for (uint32_t c = c0 + w; c < c1; c += W) {
       Vec<T> x[NV];
 #pragma unroll
       for (int j = 0; j < NV; j++) x[j] = next[j];
       if (W > 1 && c + W < c1) fetch(c + W);
-      const size_t v0 = c * (64 * NV) + lane;
+      const uint32_t v0 = c * (64 * NV) + lane;
       if (c == 0 || c == chunks - 1) {
 #pragma unroll
         for (int j = 0; j < NV; j++) r.mask(x[j], v0 + j * 64);
@@ -345,7 +346,7 @@ __global__ __launch_bounds__(256) void k_logp(const LogpArgs a, int kind, uint32
           cid = NONE;
 #pragma unroll 1
           for (int j = 0; j < NV; j++) {
-            const size_t at = v0 + (size_t)j * 64;
+            const uint32_t at = v0 + j * 64;
             Vec<T> y = r.load(at < nv ? at : nv - 1);
             r.mask(y, at);
             const uint32_t col = (uint32_t)r.column(at);
@@ -419,12 +420,14 @@ __global__ __launch_bounds__(256) void k_logp(const LogpArgs a, int kind, uint32
       if (TOP && lane < a.top) lists[wave][lane] = best.key;
       __syncthreads();
       if (wave == 0) {
-        for (int i = 1; i < W; i++) {
-          all.join(Seen(seen[i]));
-          if constexpr (TOP) {
-            const uint64_t o = lane < a.top ? lists[i][lane] : 0;
-            if (o) rooms[0][lane] = o;  // (a list's entries come first)
-            best.merge(a.top, rooms[0], (uint32_t)__popcll(__ballot(o != 0)));
+        for (int i = 1; i < W; i++) all.join(Seen(seen[i]));
+        if constexpr (TOP) {
+          // All lists at once where there is room (places without an entry count as least).
+          const uint32_t lists_at = (ROOM - a.top) / a.top >= W - 1 ? W - 1 : 1;
+          for (uint32_t i = 1; i < W; i += lists_at) {
+            const uint32_t n = a.top * lists_at;
+            if (lane < n) rooms[0][lane] = (&lists[i][0])[lane / a.top * MAX_TOP + lane % a.top];
+            best.merge(a.top, rooms[0], n);
           }
         }
       }
@@ -452,14 +455,15 @@ __global__ __launch_bounds__(64) void k_logp_join(const LogpArgs a, int kind, ui
     Best best;
     if constexpr (TOP) {
       __shared__ __attribute__((aligned(16))) uint64_t room[ROOM + ROOM_END];
-      const uint32_t count = parts * a.top, each = ROOM - a.top;
-      for (uint32_t i0 = 0; i0 < count; i0 += each) {
+      const uint32_t count = parts * a.top;
+      for (uint32_t i0 = 0, each = ROOM; i0 < count; i0 += each, each = ROOM - a.top) {
         const uint32_t i = i0 + lane;
         const uint64_t o = lane < each && i < count ? in.best[row * count + i] : 0;
-        const uint64_t them = __ballot(o != 0);
-        const uint32_t at = __builtin_amdgcn_mbcnt_hi((uint32_t)(them >> 32),
-                                                      __builtin_amdgcn_mbcnt_lo((uint32_t)them, 0u));
-        if (o) room[at] = o;
+        const uint64_t them = __ballot(o > lane_key(best.key, a.top - 1));
+        if (!them) continue;
+        if (them >> lane & 1)
+          room[__builtin_amdgcn_mbcnt_hi((uint32_t)(them >> 32),
+                                         __builtin_amdgcn_mbcnt_lo((uint32_t)them, 0u))] = o;
         best.merge(a.top, room, (uint32_t)__popcll(them));
       }
     }
@@ -469,17 +473,18 @@ __global__ __launch_bounds__(64) void k_logp_join(const LogpArgs a, int kind, ui
 
 // A wave takes 64 NV vectors of a row of dz.
 template <class T, int NV>
-__global__ __launch_bounds__(256) void k_logp_grad(const LogpArgs a, uint32_t chunks) {
+__global__ __launch_bounds__(256) void k_logp_grad(const LogpArgs a, uint32_t chunks,
+                                                   uint32_t units) {
   constexpr int N = VecOf<T>::N;
   const uint32_t lane = threadIdx.x & 63;
-  const size_t wave = (size_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const size_t units = a.n * chunks;
-  for (size_t u = (size_t)blockIdx.x * 4 + wave; u < units; u += (size_t)gridDim.x * 4) {
-    const size_t row = u / chunks, c = u - row * chunks;
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  for (uint32_t u = blockIdx.x * 4 + wave; u < units; u += gridDim.x * 4) {
+    const uint32_t in = chunks == 1 ? u : u / chunks, c = u - in * chunks;
+    const size_t row = in;
     const Row<T> o(a.dz, row * a.lddz, a.k);
     const T* z = reinterpret_cast<const T*>(a.z) + row * a.ldz;
     T* dz = const_cast<T*>(o.base) + o.head;
-    const size_t nv = o.vectors(), v0 = c * (64 * NV) + lane;
+    const size_t nv = o.vectors(), v0 = (size_t)c * (64 * NV) + lane;
     // Vectors that are the row's whole.
     auto whole = [&](size_t v) __attribute__((always_inline)) {
       return (v > 0 || o.head == 0) && (v + 1) * N - o.head <= o.k;
@@ -569,7 +574,7 @@ void launch_log_probs(emh_ctx* c, LogpArgs a, int kind) {
       constexpr bool TOP = decltype(top)::value;
       const size_t groups = (a.n * parts + 4 / W - 1) / (4 / W);
       k_logp<T, W, NV, TOP><<<dim3((unsigned)std::min(groups, MAX_GROUPS)), 256, 0, c->stream>>>(
-          a, kind, (uint32_t)parts, out);
+          a, kind, (uint32_t)parts, (uint32_t)((chunks + parts - 1) / parts), out);
       if (parts > 1)
         k_logp_join<TOP><<<dim3((unsigned)std::min(a.n, MAX_GROUPS)), 64, 0, c->stream>>>(
             a, kind, (uint32_t)parts, out);
@@ -603,9 +608,20 @@ void launch_log_probs_grad(emh_ctx* c, LogpArgs a, int kind) {
     const bool whole = a.lddz % N == 0 && (uintptr_t)a.dz % 16 == 0;
     const size_t vectors = (a.k + N - 1) / N + (whole ? 0 : 1);
     const size_t chunks = (vectors + 64 * NV - 1) / (64 * NV);
-    const size_t groups = (a.n * chunks + 3) / 4;
-    k_logp_grad<T, NV><<<dim3((unsigned)std::min(groups, MAX_GROUPS)), 256, 0, c->stream>>>(
-        a, (uint32_t)chunks);
+    // Bands of rows whose chunks 31 bits number.
+    const size_t band = std::max<size_t>(1, (size_t(1) << 31) / chunks - MAX_GROUPS * 4 / chunks);
+    for (size_t left = a.n; left > 0;) {
+      const size_t rows = std::min(left, band), units = rows * chunks;
+      k_logp_grad<T, NV>
+          <<<dim3((unsigned)std::min((units + 3) / 4, MAX_GROUPS)), 256, 0, c->stream>>>(
+              a, (uint32_t)chunks, (uint32_t)units);
+      left -= rows;
+      a.z = (const T*)a.z + rows * a.ldz;
+      a.dz = (T*)a.dz + rows * a.lddz;
+      a.lse_in += rows;
+      if (a.tokens) a.tokens += rows, a.glogp += rows;
+      if (a.gentropy) a.gentropy += rows, a.entropy_in += rows;
+    }
   });
   EMH_HIP(hipGetLastError());
 }
