@@ -16,26 +16,48 @@ __device__ __forceinline__ float finite_abs(float v) {
   return a < INFINITY ? a : 0.f;
 }
 
+// The code of a block's values. L lanes have it, v[count] each, and all of the wave's come here.
 struct Coder {
   float scale, by;
-  bool quick;  // (whole waves agree)
-  __device__ __forceinline__ explicit Coder(float top) {
-    scale = top / 448.f;
-    quick = __all((scale > 1e-30f && scale < 1e30f) || scale == 0.f);
-    const float r0 = __builtin_amdgcn_rcpf(scale > 0.f ? scale : 1.f);
-    by = fmaf(r0, fmaf(-scale, r0, 1.f), r0);
-    if (!(scale > 0.f)) by = 1.f;
+  bool quick;  // (the wave's)
+  // Infinite values apart, and scales whose quotients need the division, a scale is a product
+  // and its remainder, and so is every quotient by it: correctly rounded.
+  template <int L>
+  __device__ __forceinline__ static Coder of(const float* v, int count) {
+    float top = 0.f;
+#pragma unroll
+    for (int e = 0; e < count; e++) top = fmaxf(top, fabsf(v[e]));  // (passes over NaN)
+    return Coder(lanes_max<L>(top), [&]() __attribute__((always_inline)) {
+      float t = 0.f;
+#pragma unroll
+      for (int e = 0; e < count; e++) t = fmaxf(t, finite_abs(v[e]));
+      return lanes_max<L>(t);
+    });
   }
-  // A quotient: one reciprocal a block, refined, then a product and its remainder. At most
-  // 448 (1 + 2^-23), which rounds to 448. (Without a scale the values are zeros, or below
-  // what a code can hold of them.)
+  // top: the largest magnitude, infinite ones among it; finite(): without them.
+  template <class F>
+  __device__ __forceinline__ Coder(float top, F&& finite) {
+    quick = __all((top > 1e-25f && top < 1e30f) || top == 0.f);
+    if (quick) {
+      constexpr float PER = 1.f / 448.f;
+      const float q = top * PER;
+      scale = fmaf(fmaf(-448.f, q, top), PER, q);
+      const float s = top > 0.f ? scale : 1.f, r0 = __builtin_amdgcn_rcpf(s);
+      by = fmaf(r0, fmaf(-s, r0, 1.f), r0);
+    } else {
+      scale = finite() / 448.f;
+      by = 0.f;
+    }
+  }
+  // A quotient: at most 448 (1 + 2^-23), which rounds to 448.
   __device__ __forceinline__ float quotient(float v) const {
     if (quick) {
-      const float q = v * by, back = fmaf(fmaf(-scale, q, v), by, q);
+      const float q = v * by;
       // (The remainder of a negative zero is a positive one.)
-      return scale > 0.f && fabsf(v) < INFINITY ? copysignf(back, v) : v;
+      return copysignf(fmaf(fmaf(-scale, q, v), by, q), v);
     }
-    // (A scale among the last subnormal numbers may be small by half of itself.)
+    // (Without a scale the values are zeros, or below what a code can hold of them; one
+    // among the last subnormal numbers may be small by half of itself.)
     const float q = scale > 0.f ? v / scale : v;
     return fabsf(q) < INFINITY ? fminf(fmaxf(q, -448.f), 448.f) : q;
   }

@@ -46,6 +46,13 @@ struct Cols {
   __device__ __forceinline__ bool any() const { return at + N > from; }
 };
 
+// 1 / sqrt(v), to a unit of its last place: the instruction's and a Newton step.
+__device__ __forceinline__ float root_of(float v) {
+  const float r = __builtin_amdgcn_rsqf(v);
+  const float better = fmaf(r * 0.5f, fmaf(-v * r, r, 1.f), r);
+  return v > 1e-30f && v < 1e30f ? better : 1.0f / sqrtf(v);
+}
+
 template <class T>
 __device__ __forceinline__ void load_weight(const RmsArgs& a, int at, float* out) {
   constexpr int N = VecOf<T>::N;
@@ -105,7 +112,13 @@ __global__ __launch_bounds__(256) void k_rms(const RmsArgs a) {
   fetch((size_t)blockIdx.x * G + g);
   float w[NV * N];
 #pragma unroll
-  for (int j = 0; j < NV; j++) load_weight<T>(a, cols(j).at, w + j * N);
+  for (int j = 0; j < NV; j++) {
+    load_weight<T>(a, cols(j).at, w + j * N);
+    if constexpr (CODES) {  // columns that count elsewhere have no part in a block's scale
+#pragma unroll
+      for (int e = 0; e < N; e++) w[j * N + e] = cols(j).in(e) ? w[j * N + e] : 0.f;
+    }
+  }
   const float inv = 1.0f / (float)d;
   int slot = 0;
   const size_t step = (size_t)gridDim.x * G;
@@ -126,7 +139,7 @@ __global__ __launch_bounds__(256) void k_rms(const RmsArgs a) {
         q = fmaf(o, o, q);
       }
     // (h may take x's or r's place: the row is loaded by all its threads here.)
-    const float rstd = 1.0f / sqrtf(row_sum<LPR, TB>(q, red, slot) * inv + a.eps);
+    const float rstd = root_of(row_sum<LPR, TB>(q, red, slot) * inv + a.eps);
     slot ^= 1;
     if (live && a.h) {
       T* p = reinterpret_cast<T*>(a.h) + row * a.ldh;
@@ -142,12 +155,9 @@ __global__ __launch_bounds__(256) void k_rms(const RmsArgs a) {
 #pragma unroll
       for (int e = 0; e < N; e++) y[e] = h[j].get(e) * rstd * w[j * N + e];
       if constexpr (CODES) {
-        float top = 0.f;
-#pragma unroll
-        for (int e = 0; e < N; e++) top = fmaxf(top, c.in(e) ? finite_abs(y[e]) : 0.f);
         // A block's lanes (a row of 16 lanes has one block).
         constexpr int LPB = CODE_BLOCK / N < LPR ? CODE_BLOCK / N : LPR;
-        const Coder code(lanes_max<LPB>(top));
+        const Coder code = Coder::of<LPB>(y, N);
         if (live && c.any()) {
           store_codes<N>(reinterpret_cast<uint8_t*>(a.y) + row * a.ldy, c.from, c.from - c.at, d,
                          code, y);
@@ -298,8 +308,8 @@ __global__ __launch_bounds__(256) void k_rms_wide(const RmsArgs a) {
       for (int b = threadIdx.x >> 6; b < blocks; b += 4) {
         const int i = b * CODE_BLOCK + 2 * lane;
         const float y0 = i < a.d ? y_of(i) : 0.f, y1 = i + 1 < a.d ? y_of(i + 1) : 0.f;
-        const Coder code(lanes_max<64>(fmaxf(finite_abs(y0), finite_abs(y1))));
         const float v[4] = {y0, y1, 0.f, 0.f};
+        const Coder code = Coder::of<64>(v, 2);
         if (i < ((a.d + 15) & ~15))
           *reinterpret_cast<uint16_t*>(out + i) = (uint16_t)code.four(v);
         if (lane == 0) a.scale[row * a.lds + b] = code.scale;
@@ -397,13 +407,10 @@ __global__ __launch_bounds__(256) void k_codes_rows(const T* __restrict__ x, siz
       v = load_vec(p);
     else if (left > 0)
       v = load_some(p, left);
-    float f[N], top = 0.f;
+    float f[N];
 #pragma unroll
-    for (int e = 0; e < N; e++) {
-      f[e] = v.get(e);
-      top = fmaxf(top, finite_abs(f[e]));
-    }
-    const Coder code(lanes_max<LPB>(top));
+    for (int e = 0; e < N; e++) f[e] = v.get(e);
+    const Coder code = Coder::of<LPB>(f, N);
     if (left > 0) {
       store_codes<N>(q + row * ldq, col, 0, d, code, f);
       if (l == 0) scale[row * lds + b] = code.scale;
@@ -417,13 +424,13 @@ __global__ __launch_bounds__(256) void k_codes_tiles(const T* __restrict__ x, si
                                                      uint8_t* q, size_t ldq, float* scale,
                                                      size_t lds) {
   constexpr int N = VecOf<T>::N, LPB = CODE_BLOCK / N, RPP = 256 / LPB, P = CODE_BLOCK / RPP;
-  __shared__ float red[4];
+  __shared__ float2 red[4];
   const int l = threadIdx.x % LPB, r0 = threadIdx.x / LPB;
   for (size_t t = blockIdx.x; t < tiles; t += gridDim.x) {
     const size_t tr = t / blocks;
     const int b = (int)(t - tr * blocks), col = b * CODE_BLOCK + l * N, left = d - col;
     Vec<T> v[P];
-    float top = 0.f;
+    float top = 0.f, fine = 0.f;
 #pragma unroll
     for (int p = 0; p < P; p++) {
       const size_t row = tr * CODE_BLOCK + p * RPP + r0;
@@ -433,12 +440,18 @@ __global__ __launch_bounds__(256) void k_codes_tiles(const T* __restrict__ x, si
       else if (row < rows && left > 0)
         v[p] = load_some(x + row * ldx + col, left);
 #pragma unroll
-      for (int e = 0; e < N; e++) top = fmaxf(top, finite_abs(v[p].get(e)));
+      for (int e = 0; e < N; e++) {
+        top = fmaxf(top, fabsf(v[p].get(e)));
+        fine = fmaxf(fine, finite_abs(v[p].get(e)));
+      }
     }
     top = lanes_max<64>(top);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+    fine = lanes_max<64>(fine);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = make_float2(top, fine);
     __syncthreads();
-    const Coder code(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
+    const Coder code(fmaxf(fmaxf(red[0].x, red[1].x), fmaxf(red[2].x, red[3].x)), [&] {
+      return fmaxf(fmaxf(red[0].y, red[1].y), fmaxf(red[2].y, red[3].y));
+    });
     if (threadIdx.x == 0) scale[tr * lds + b] = code.scale;
 #pragma unroll
     for (int p = 0; p < P; p++) {
