@@ -17,6 +17,7 @@ struct emh_grad_norm {
   uint2* chunks = nullptr;
   double* sums = nullptr;
   size_t nchunks = 0, chunk = 0;
+  bool stream = false;
   std::vector<emh_buf*> written;
   std::vector<Range> ranges;  // of gradients and outputs
 };
@@ -317,7 +318,12 @@ int emh_grad_norm_create(emh_ctx* c, const emh_buf* const* grads, emh_buf* const
     std::vector<emh::NormTensor> table;
     std::vector<uint2> chunks;
     size_t total = 0;
-    for (size_t i = 0; i < count; i++) total += grads[i] ? grads[i]->len : 0;
+    size_t bytes = 0;
+    for (size_t i = 0; i < count; i++) {
+      total += grads[i] ? grads[i]->len : 0;
+      bytes += grads[i] ? grads[i]->len * emh::kind_bytes(grads[i]->kind) : 0;
+    }
+    plan->stream = outs && bytes >= emh::STREAM_FROM / 2;  // (with what is read, twice that)
     plan->chunk = total <= emh::NORM_FEW ? emh::NORM_CHUNK_FEW : emh::NORM_CHUNK;
     for (size_t i = 0; i < count; i++) {
       const emh_buf* g = grads[i];
@@ -395,7 +401,7 @@ void measure(emh_grad_norm* plan, float scale, float max_norm, emh_buf* out, boo
   if (clip)
     for (emh_buf* b : plan->written) ++b->gen;
   emh::launch_grad_norm(plan->ctx, plan->tensors, plan->chunks, plan->nchunks, plan->chunk,
-                        plan->sums, scale, max_norm, (float*)out->ptr, clip);
+                        plan->stream, plan->sums, scale, max_norm, (float*)out->ptr, clip);
 }
 }  // namespace
 

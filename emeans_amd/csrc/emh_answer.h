@@ -7,6 +7,9 @@
 
 namespace emh {
 
+// Bytes of results from which they go past the caches (which hold as many).
+constexpr size_t STREAM_FROM = size_t(256) << 20;
+
 // ---- emh_rms.hip
 struct RmsArgs {
   const void* x;   // forward: the rows; backward: their sums h
@@ -80,11 +83,11 @@ struct NormTensor {  // as the kernels read it
 // little as fills the GPU.
 constexpr size_t NORM_CHUNK = 16384, NORM_CHUNK_FEW = 2048, NORM_FEW = size_t(4) << 20;
 constexpr size_t NORM_SUMS = 1024;
-// chunks[i]: a tensor and the number of a chunk in it. sums: NORM_SUMS; out: the norm and the
+// chunks[i]: a tensor and the number of a chunk in it. stream: results past the caches. sums: NORM_SUMS; out: the norm and the
 // factor.
 void launch_grad_norm(emh_ctx* c, const NormTensor* tensors, const uint2* chunks, size_t nchunks,
-                      size_t chunk, double* sums, float scale, float max_norm, float* out,
-                      bool clip);
+                      size_t chunk, bool stream, double* sums, float scale, float max_norm,
+                      float* out, bool clip);
 
 // No plan made with c measures any more, and what they hold on the device is freed (c's
 // stream is idle).

@@ -7,8 +7,8 @@
 // Two launches. The first leaves one sum a workgroup (at most NORM_SUMS, over chunks that a
 // table on the device names); in the second every workgroup adds those sums, in one order, and so
 // has the norm and the factor, and scales its chunks, the last ones first: what the first launch
-// read last is what the caches may still hold. No atomics: results follow from the
-// tensors alone.
+// read last is what the caches may still hold, if results that exceed them go past them (131 M
+// bf16 elements 156 us, so 128). No atomics: results follow from the tensors alone.
 //
 // Bound by HBM: two reads and one write of an element; where the gradients are scaled in
 // place and the factor is 1 the second read and the write are left out.
@@ -73,7 +73,7 @@ __global__ __launch_bounds__(256) void k_square_sums(const NormTensor* __restric
   if (threadIdx.x == 0) sums[blockIdx.x] = s;
 }
 
-template <class T>
+template <bool STREAM, class T>
 __device__ __forceinline__ void scale_chunk(const T* p, T* o, size_t count, float f) {
   constexpr int N = VecOf<T>::N;
   const size_t whole = count / N;
@@ -83,7 +83,7 @@ __device__ __forceinline__ void scale_chunk(const T* p, T* o, size_t count, floa
     float x[N];
 #pragma unroll
     for (int e = 0; e < N; e++) x[e] = v.get(e) * f;
-    store_vec(o + i * N, x);
+    STREAM ? stream_vec(o + i * N, x) : store_vec(o + i * N, x);
   }
   const size_t i = whole * N + threadIdx.x;
   if (i < count) o[i] = from_f32<T>(to_f32(p[i]) * f);
@@ -113,6 +113,7 @@ __global__ __launch_bounds__(256) void k_norm_only(const double* sums, uint32_t 
   if (threadIdx.x == 0) out[0] = r.x, out[1] = r.y;
 }
 
+template <bool STREAM>
 __global__ __launch_bounds__(256) void k_clip(const NormTensor* __restrict__ tensors,
                                               const uint2* __restrict__ chunks, uint32_t nchunks,
                                               uint32_t chunk, const double* sums, uint32_t nsums,
@@ -127,13 +128,13 @@ __global__ __launch_bounds__(256) void k_clip(const NormTensor* __restrict__ ten
     if (f == 1.f && t.out == t.grad) continue;
     const size_t base = (size_t)at.y * chunk, count = min(t.len - base, (size_t)chunk);
     if (t.kind == EMH_F32)
-      scale_chunk(reinterpret_cast<const float*>(t.grad) + base,
+      scale_chunk<STREAM>(reinterpret_cast<const float*>(t.grad) + base,
                   reinterpret_cast<float*>(t.out) + base, count, f);
     else if (t.kind == EMH_F16)
-      scale_chunk(reinterpret_cast<const f16*>(t.grad) + base, reinterpret_cast<f16*>(t.out) + base,
+      scale_chunk<STREAM>(reinterpret_cast<const f16*>(t.grad) + base, reinterpret_cast<f16*>(t.out) + base,
                   count, f);
     else
-      scale_chunk(reinterpret_cast<const bf16*>(t.grad) + base,
+      scale_chunk<STREAM>(reinterpret_cast<const bf16*>(t.grad) + base,
                   reinterpret_cast<bf16*>(t.out) + base, count, f);
   }
 }
@@ -141,16 +142,19 @@ __global__ __launch_bounds__(256) void k_clip(const NormTensor* __restrict__ ten
 }  // namespace
 
 void launch_grad_norm(emh_ctx* c, const NormTensor* tensors, const uint2* chunks, size_t nchunks,
-                      size_t chunk, double* sums, float scale, float max_norm, float* out,
+                      size_t chunk, bool stream, double* sums, float scale, float max_norm, float* out,
                       bool clip) {
   const unsigned nsums = (unsigned)std::min(nchunks, NORM_SUMS);
   if (nsums > 0)
     k_square_sums<<<nsums, 256, 0, c->stream>>>(tensors, chunks, (uint32_t)nchunks, (uint32_t)chunk,
                                                 sums);
-  if (clip && nchunks > 0)
-    k_clip<<<(unsigned)std::min(nchunks, (size_t)2048), 256, 0, c->stream>>>(
-        tensors, chunks, (uint32_t)nchunks, (uint32_t)chunk, sums, nsums, scale, max_norm, out);
-  else
+  if (clip && nchunks > 0) {
+    auto go = [&](auto kernel) {
+      kernel<<<(unsigned)std::min(nchunks, (size_t)2048), 256, 0, c->stream>>>(
+          tensors, chunks, (uint32_t)nchunks, (uint32_t)chunk, sums, nsums, scale, max_norm, out);
+    };
+    stream ? go(k_clip<true>) : go(k_clip<false>);
+  } else
     k_norm_only<<<1, 256, 0, c->stream>>>(sums, nsums, scale, max_norm, out);
   EMH_HIP(hipGetLastError());
 }

@@ -10,10 +10,12 @@
 // results (2^-9, 2^-12) do not show. f32 results, and few rows, whose time is the classes'
 // bytes, take the f16 MFMA instead (an f16 holds every code exactly): 5e-8.
 //
-// Few rows read the classes once, as they lie. More of them go in tiles: a workgroup owns 256 x
+// Few rows read the classes as they lie. More of them go in tiles: a workgroup owns 256 x
 // 256 or 128 x 128 of the result, and a block of the depth, 128 bytes a row of both operands,
 // goes by in one step, moved to LDS by DMA into one of two stages, its 16-byte chunks
 // XOR-swizzled so that sixteen rows' equal chunks meet no bank twice.
+#include <cmath>
+
 #include "emh_answer.h"
 #include "emh_codes.h"
 #include "emh_tile.h"
@@ -61,49 +63,104 @@ __device__ __forceinline__ v4u first_codes(v4u v, int left) {
   }
   return v;
 }
-// The 16 codes of a row from column c on, zeros from column d on.
-__device__ __forceinline__ v4u codes16(const uint8_t* row, size_t c, size_t d) {
-  if (c >= d) return v4u{0u, 0u, 0u, 0u};
-  v4u v = *reinterpret_cast<const v4u*>(row + c);
-  if (c + 16 <= d) return v;
-  return first_codes(v, (int)(d - c));
+// The 16 codes at p, of which `left` are the row's, the others zeros.
+__device__ __forceinline__ v4u codes16(const uint8_t* p, int left) {
+  if (left <= 0) return v4u{0u, 0u, 0u, 0u};
+  const v4u v = *reinterpret_cast<const v4u*>(p);
+  return left >= 16 ? v : first_codes(v, left);
+}
+// The same by one 8-bit MFMA.
+__device__ __forceinline__ v8i codes_of(v4u a, v4u b) {
+  return __builtin_bit_cast(v8i, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+__device__ __forceinline__ v4f block8(v8i a, v8i b) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0,
+                                                          0, 0);
 }
 
 // Few rows: a workgroup takes 16 classes and 16 YB rows, its four waves the blocks of the depth
-// by turns; operands come from memory as they lie.
-template <int YB>
-__global__ __launch_bounds__(256) void k_few8(const CodedIn x, size_t n, size_t d, const CodedIn w,
+// by turns; operands come from memory as they lie, AHEAD blocks of a wave's on their way at once.
+template <int YB, bool EXACT>
+__global__ __launch_bounds__(256) void k_few8(const CodedIn x, size_t n, uint32_t d, const CodedIn w,
                                               size_t k, void* y, size_t ldy, int kind,
                                               uint32_t rgroups, size_t groups) {
+  constexpr int AHEAD = YB == 1 ? 4 : 2;
   __shared__ v4f sums[4][YB][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, g = lane >> 4;
-  const size_t blocks = (d + CODE_BLOCK - 1) / CODE_BLOCK;
+  const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const uint32_t blocks = (d + CODE_BLOCK - 1) / CODE_BLOCK, whole = d / CODE_BLOCK;
   for (size_t u = blockIdx.x; u < groups; u += gridDim.x) {
-    const size_t cg = u / rgroups, r0 = (u - cg * rgroups) * (16 * YB), v0 = cg * 16;
-    const uint8_t* wp = w.q + min(v0 + li, k - 1) * w.ld;
+    size_t cg = u, r0 = 0;
+    if (rgroups > 1) cg = u / rgroups, r0 = (u - cg * rgroups) * (16 * YB);
+    const size_t v0 = cg * 16;
+    const uint8_t* wp = w.q + min(v0 + li, k - 1) * w.ld + 16 * g;
     const uint8_t* xp[YB];
     const float* sp[YB];
 #pragma unroll
     for (int b = 0; b < YB; b++) {
       const size_t row = min(r0 + b * 16 + li, n - 1);
-      xp[b] = x.q + row * x.ld;
+      xp[b] = x.q + row * x.ld + 16 * g;
       sp[b] = x.scale + row * x.lds;
     }
     const float* ws = w.scale + v0 / CODE_BLOCK * w.lds;
     v4f acc[YB];
 #pragma unroll
     for (int b = 0; b < YB; b++) acc[b] = v4f{0.f, 0.f, 0.f, 0.f};
-    for (size_t s = wave; s < blocks; s += 4) {
-      const size_t c = s * CODE_BLOCK + 16 * g;
-      const Halves a(codes16(wp, c, d), codes16(wp, c + 64, d));
-      const float by = ws[s];
+    struct Block {
+      v4u w[2], x[YB][2];
+      float by, f[YB];
+    };
+    auto add = [&](const Block& o) __attribute__((always_inline)) {
+      Halves wh;
+      if constexpr (EXACT) wh = Halves(o.w[0], o.w[1]);
 #pragma unroll
       for (int b = 0; b < YB; b++) {
-        const v4f t = block16(a, Halves(codes16(xp[b], c, d), codes16(xp[b], c + 64, d)));
-        const float f = sp[b][s] * by;
+        v4f t;
+        if constexpr (EXACT)
+          t = block16(wh, Halves(o.x[b][0], o.x[b][1]));
+        else
+          t = block8(codes_of(o.w[0], o.w[1]), codes_of(o.x[b][0], o.x[b][1]));
+        const float f = o.f[b] * o.by;
 #pragma unroll
         for (int e = 0; e < 4; e++) acc[b][e] = fmaf(t[e], f, acc[b][e]);
       }
+    };
+    for (uint32_t s0 = wave; s0 < whole; s0 += 4 * AHEAD) {
+      Block o[AHEAD];
+#pragma unroll
+      for (int i = 0; i < AHEAD; i++) {
+        const uint32_t s = s0 + 4 * i;
+        if (s >= whole) continue;
+        const size_t c = (size_t)s * CODE_BLOCK;
+#pragma unroll
+        for (int h = 0; h < 2; h++) o[i].w[h] = *reinterpret_cast<const v4u*>(wp + c + 64 * h);
+        o[i].by = ws[s];
+#pragma unroll
+        for (int b = 0; b < YB; b++) {
+#pragma unroll
+          for (int h = 0; h < 2; h++)
+            o[i].x[b][h] = *reinterpret_cast<const v4u*>(xp[b] + c + 64 * h);
+          o[i].f[b] = sp[b][s];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < AHEAD; i++)
+        if (s0 + 4 * i < whole) add(o[i]);
+    }
+    if (whole < blocks && (int)(whole & 3) == wave) {  // the short last block
+      Block o;
+      const size_t c = (size_t)whole * CODE_BLOCK;
+      const int left = (int)(d - whole * CODE_BLOCK) - 16 * g;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        o.w[h] = codes16(wp + c + 64 * h, left - 64 * h);
+#pragma unroll
+        for (int b = 0; b < YB; b++) o.x[b][h] = codes16(xp[b] + c + 64 * h, left - 64 * h);
+      }
+      o.by = ws[whole];
+#pragma unroll
+      for (int b = 0; b < YB; b++) o.f[b] = sp[b][whole];
+      add(o);
     }
 #pragma unroll
     for (int b = 0; b < YB; b++) sums[wave][b][lane] = acc[b];
@@ -119,7 +176,7 @@ __global__ __launch_bounds__(256) void k_few8(const CodedIn x, size_t n, size_t 
         }
       }
     }
-    __syncthreads();  // the next group's sums take their place
+    if (gridDim.x < groups) __syncthreads();  // the next group's sums take their place
   }
 }
 
@@ -141,9 +198,6 @@ struct Shape8 {
 typedef Shape8<4, 2, 4, 8, 1> Large8;  // 256 x 256, 8 waves
 typedef Shape8<2, 2, 4, 4, 2> Small8;  // 128 x 128, 4 waves, two workgroups a CU
 
-// Bytes of results from which they go past the caches.
-constexpr size_t STREAM_FROM = size_t(256) << 20;
-
 struct Prod8Args {
   TileIn t;  // r: the rows, c: the classes; slabs: blocks of the depth
   uint32_t n, k, d;
@@ -162,9 +216,7 @@ struct Frag {  // a lane's 32 codes of a block's row
     a = *(lds_v4u)(uintptr_t)at;
     b = *(lds_v4u)(uintptr_t)(at ^ 64u);
   }
-  __device__ __forceinline__ v8i codes() const {
-    return __builtin_bit_cast(v8i, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
-  }
+  __device__ __forceinline__ v8i codes() const { return codes_of(a, b); }
 };
 typedef const float __attribute__((address_space(3)))* lds_f32;
 
@@ -186,13 +238,6 @@ __device__ __forceinline__ void sixteen(const v4f (*acc)[YB], int y, uint32_t* o
     }
   }
 }
-// A store of what no cache need keep.
-template <class T>
-__device__ __forceinline__ void stream_vec(T* p, const Vec<T>& v) {
-  typedef uint32_t any16 __attribute__((ext_vector_type(4), aligned(2)));
-  __builtin_nontemporal_store(any16{v.raw.x, v.raw.y, v.raw.z, v.raw.w}, reinterpret_cast<any16*>(p));
-}
-
 // A lane's pieces of a row (eight elements each, 64 apart; the lane has the row's `place` of
 // eight) to p, of which `left` elements from p on are the row's, where rows may begin at odd
 // multiples of two bytes: a row that does goes out an element later, by whole words.
@@ -402,8 +447,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_tile8(const Prod8Args a) {
           if constexpr (EXACT)
             t[m & 3] = block16(ch, rh[y]);
           else
-            t[m & 3] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                ca[i % SLOTS].codes(), rb[y].codes(), v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+            t[m & 3] = block8(ca[i % SLOTS].codes(), rb[y].codes());
           const float by = m < 2 ? fp[m] : f[o % S::YB];
 #pragma unroll
           for (int e = 0; e < 4; e++)
@@ -525,29 +569,46 @@ void launch_product8(emh_ctx* c, const CodedIn& x, size_t n, size_t d, const Cod
   auto few = [&](auto yb) {
     constexpr int YB = decltype(yb)::value;
     const size_t rg = (n + 16 * YB - 1) / (16 * YB), groups = (k + 15) / 16 * rg;
-    k_few8<YB><<<dim3((unsigned)std::min(groups, MAX_GROUPS)), 256, 0, c->stream>>>(
-        x, n, d, w, k, y.p, y.ld, y.kind, (uint32_t)rg, groups);
+    auto go = [&](auto exact) {
+      k_few8<YB, decltype(exact)::value>
+          <<<dim3((unsigned)std::min(groups, MAX_GROUPS)), 256, 0, c->stream>>>(
+              x, n, (uint32_t)d, w, k, y.p, y.ld, y.kind, (uint32_t)rg, groups);
+    };
+    y.kind == EMH_F32 ? go(std::true_type{}) : go(std::false_type{});
   };
-  // (A tile's offsets are 32 bits, rows of one launch too.)
+  // What each way takes, in us, from the times of 1 to 16,384 rows by 768 to 131,071 classes: few
+  // rows read the classes again for every 64 rows and the rows for every 16 classes; a tile's
+  // block of the depth takes a CU as long as here, of small tiles less where a CU has but one.
+  const double cus = c->cus, steps = (double)((d + CODE_BLOCK - 1) / CODE_BLOCK);
+  const bool f32 = y.kind == EMH_F32;
+  auto up = [](size_t v, size_t by) { return (double)((v + by - 1) / by); };
+  auto tiles_take = [&](double tiles, double slots, double start, double step, double alone) {
+    const double full = std::floor(tiles / slots), rest = tiles - full * slots;
+    return start + steps * (full * step + (rest == 0 ? 0 : rest <= cus ? alone : step));
+  };
+  const double few_take = 3.2 + ((double)n / 16 + up(n, 64)) * (double)k * (double)d / 6.5e6;
+  const double small_take = std::max(
+      tiles_take(up(n, 128) * up(k, 128), 2 * cus, 2.5, f32 ? 2.6 : 1.55, f32 ? 1.5 : 0.8),
+      (double)k * (double)d / 4.2e6);
+  const double large_take = f32 ? INFINITY : tiles_take(up(n, 256) * up(k, 256), cus, 4, 2, 2);
+  // (A tile's offsets are 32 bits.)
   const bool far = std::max({x.ld, w.ld, x.lds * 4, w.lds * 4}) >= (size_t(1) << 23);
-  if (n > 64 && !far) {
-    if (y.kind == EMH_F32) {
-      launch_tiles<float, Small8, true>(c, x, n, d, w, k, y);
-    } else {
-      const bool large = ((n + 255) / 256) * ((k + 255) / 256) >= (size_t)c->cus;
-      auto go = [&](auto t) {
-        using T = decltype(t);
-        large ? launch_tiles<T, Large8, false>(c, x, n, d, w, k, y)
-              : launch_tiles<T, Small8, false>(c, x, n, d, w, k, y);
-      };
-      y.kind == EMH_F16 ? go(f16{}) : go(bf16{});
-    }
-  } else if (n <= 16) {
-    few(std::integral_constant<int, 1>{});
-  } else if (n <= 32) {
-    few(std::integral_constant<int, 2>{});
+  if (far || few_take <= std::min(small_take, large_take)) {
+    if (n <= 16)
+      few(std::integral_constant<int, 1>{});
+    else if (n <= 32)
+      few(std::integral_constant<int, 2>{});
+    else
+      few(std::integral_constant<int, 4>{});
+  } else if (f32) {
+    launch_tiles<float, Small8, true>(c, x, n, d, w, k, y);
   } else {
-    few(std::integral_constant<int, 4>{});
+    auto go = [&](auto t) {
+      using T = decltype(t);
+      large_take < small_take ? launch_tiles<T, Large8, false>(c, x, n, d, w, k, y)
+                              : launch_tiles<T, Small8, false>(c, x, n, d, w, k, y);
+    };
+    y.kind == EMH_F16 ? go(f16{}) : go(bf16{});
   }
   EMH_HIP(hipGetLastError());
 }

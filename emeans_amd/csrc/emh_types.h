@@ -121,6 +121,25 @@ __device__ __forceinline__ void store_some(T* p, const float* v, int left) {
     if (e < left) p[e] = from_f32<T>(v[e]);
 }
 
+// Stores of what no cache need keep.
+template <class T>
+__device__ __forceinline__ void stream_vec(T* p, const Vec<T>& v) {
+  typedef uint32_t any16 __attribute__((ext_vector_type(4), aligned(2)));
+  __builtin_nontemporal_store(any16{v.raw.x, v.raw.y, v.raw.z, v.raw.w}, reinterpret_cast<any16*>(p));
+}
+template <class T>
+__device__ __forceinline__ void stream_vec(T* p, const float* v) {
+  uint32_t w[4];
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    if constexpr (sizeof(T) == 4)
+      w[e] = __float_as_uint(v[e]);
+    else
+      w[e] = pair_from_f32<T>(v[2 * e], v[2 * e + 1]);
+  }
+  stream_vec(p, Vec<T>{make_uint4(w[0], w[1], w[2], w[3])});
+}
+
 // Element i of a buffer whose kind is a run-time value (EMH_F32, EMH_F16,
 // EMH_BF16).
 __device__ __forceinline__ float load_kind(const void* p, int kind, size_t i) {

@@ -75,7 +75,15 @@ def test_types(dev, n, d, k, name):
     _run(dev, n, d, k, name, n + d + k)
 
 
-@pytest.mark.parametrize("n,d,k", [(3, 200, 50), (300, 200, 400)])
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n,d,k,pad,off", [(1500, 513, 1501, 1, 1), (2000, 100, 2001, 0, 1),
+                                           (4001, 77, 5003, 0, 0), (9001, 130, 3001, 2, 0),
+                                           (3000, 200, 3004, 0, 2)])
+def test_tiles_of_short_blocks_and_more_of_them_than_workgroups(dev, n, d, k, pad, off, name):
+    _run(dev, n, d, k, name, n + d, pad, off)
+
+
+@pytest.mark.parametrize("n,d,k", [(3, 200, 50), (300, 200, 400), (1300, 200, 1400)])
 def test_codes_and_scales_that_are_not_finite_stay_in_their_rows(dev, n, d, k):
     r = np.random.default_rng(2)
     (x, xs), (w, ws) = _codes(r, n, d, False), _codes(r, k, d, True)
