@@ -219,6 +219,11 @@ struct Frag {  // a lane's 32 codes of a block's row
   __device__ __forceinline__ v8i codes() const { return codes_of(a, b); }
 };
 typedef const float __attribute__((address_space(3)))* lds_f32;
+// Between a wave's writes to LDS and other lanes' reads, which the LDS takes in order.
+__device__ __forceinline__ void wave_fence8() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
 
 // Sixteen bytes of a lane's results in the blocks from acc[0] on: f32 as they are; of 16 bits two
 // blocks' fours swapped between lanes, so that each has eight columns of one.
@@ -238,36 +243,33 @@ __device__ __forceinline__ void sixteen(const v4f (*acc)[YB], int y, uint32_t* o
     }
   }
 }
-// A lane's pieces of a row (eight elements each, 64 apart; the lane has the row's `place` of
-// eight) to p, of which `left` elements from p on are the row's, where rows may begin at odd
-// multiples of two bytes: a row that does goes out an element later, by whole words.
-template <class T, int PIECES>
-__device__ __forceinline__ void store_odd(T* p, const uint32_t (*o)[4], uint32_t place,
-                                          uint32_t left) {
+// Sixteen bytes of a row to p; `left` elements from p on are the row's.
+template <class T, bool STREAM>
+__device__ __forceinline__ void store_row(T* p, const v4u& v, uint32_t left) {
+  const Vec<T> out{make_uint4(v[0], v[1], v[2], v[3])};
+  constexpr uint32_t EL = 16 / sizeof(T);
+  if (left >= EL)
+    STREAM ? stream_vec(p, out) : store_vec(p, out);
+  else if (left > 0)
+    store_some(p, out, (int)left);
+}
+// The same of a 16-bit row that may begin at an odd multiple of two bytes: then an element
+// later, by whole words; after: the row's next word. The first element of what a wave has of the
+// row, and the last of its last (last) sixteen bytes, are left to the caller.
+template <class T, bool STREAM>
+__device__ __forceinline__ void store_odd_row(T* p, const v4u& v, uint32_t after, bool last,
+                                              uint32_t left) {
   const uint32_t odd = (uint32_t)((uintptr_t)p >> 1) & 1, by = 16 * odd;
-  // Where the next eight of the row are: the lane of the next place.
-  const uint32_t lane = threadIdx.x & 63, q = (place + 1) & 7;
-  const uint32_t next = (lane & 7) + (q >> 2) * 8 + ((q >> 1 & 1) | (q & 1) << 1) * 16;
+  v4u s;
 #pragma unroll
-  for (int i = 0; i < PIECES; i++) {
-    const uint32_t give = place == 0 && i + 1 < PIECES ? o[i + 1 < PIECES ? i + 1 : i][0] : o[i][0];
-    const uint32_t after = (uint32_t)__builtin_amdgcn_ds_bpermute((int)(next * 4), (int)give);
-    uint32_t v[4];
-#pragma unroll
-    for (int e = 0; e < 4; e++)
-      v[e] = __builtin_amdgcn_alignbit(e < 3 ? o[i][e < 3 ? e + 1 : 3] : after, o[i][e], by);
-    const uint32_t at = (uint32_t)i * 64 + odd;
-    // The last of the pieces ends with its own eight.
-    const uint32_t have = i + 1 == PIECES && place == 7 ? 8 - odd : 8;
-    // (`left > at ? left - at : 0` lets the compiler take left for at least `odd` below.)
-    const uint32_t n = min(max(left, at) - at, have);
-    const Vec<T> out{make_uint4(v[0], v[1], v[2], v[3])};
-    if (n == 8)
-      store_vec(p + at, out);
-    else if (n > 0)
-      store_some(p + at, out, (int)n);
-    if (i == 0 && odd && place == 0 && left > 0)
-      *p = __builtin_bit_cast(T, (uint16_t)o[0][0]);
+  for (int e = 0; e < 4; e++) s[e] = __builtin_amdgcn_alignbit(e < 3 ? v[e < 3 ? e + 1 : 3] : after, v[e], by);
+  // (`left > odd ? left - odd : 0` lets the compiler take left for at least `odd` elsewhere.)
+  const uint32_t n = max(left, odd) - odd;
+  if (last && odd && n >= 7) {  // six of them; the seventh goes with the first
+    typedef uint32_t three __attribute__((ext_vector_type(3), aligned(4)));
+    *reinterpret_cast<three*>(p + 1) = three{s[0], s[1], s[2]};
+  } else {
+    store_row<T, STREAM>(p + odd, s, min(n, last ? 8 - odd : 8u));
   }
 }
 
@@ -280,6 +282,7 @@ __device__ __forceinline__ void store_odd(T* p, const uint32_t (*o)[4], uint32_t
 template <class T, class S, bool EXACT, bool STREAM>
 __global__ __launch_bounds__(S::THREADS, 2) void k_tile8(const Prod8Args a) {
   __shared__ __attribute__((aligned(1024))) char ring[2 * S::STAGE];
+  __shared__ __attribute__((aligned(16))) char out[S::NW * 16 * 144];
   const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int wr = w % S::NWR, wc = w / S::NWR;
   const uint32_t lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
@@ -480,49 +483,58 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_tile8(const Prod8Args a) {
         acc[o / S::YB][o % S::YB][e] = fmaf(t[o & 3][e], fp[m], acc[o / S::YB][o % S::YB][e]);
     }
 
-    // A row's 128 bytes go out together, sixteen a lane, `place` of eight.
+    // Through LDS, where a wave has room for 128 bytes of sixteen rows (and a word more): eight
+    // lanes side by side store a row's 128 bytes. (What a wave reads there it wrote before.)
     const TileAt at = tile_at(a.t, bid);
     stored = (at.rt + 1) * S::TR <= a.n && (at.ct + 1) * S::TC <= a.k;
-    const bool low = li < 8;
-    const uint32_t place = (low ? 0u : 4u) + (sizeof(T) == 4 ? g : 2 * (g & 1) + (g >> 1));
-    const uint32_t col0 = at.ct * S::TC + (uint32_t)(wc * S::AB) * 16 + place * EL;
     constexpr int PIECES = S::AB / (2 * STRIDE);
+    constexpr uint32_t PITCH = 144;
+    char* const mine = out + w * 16 * PITCH;
+    const uint32_t chunk_at = (sizeof(T) == 4 ? g : 2 * (g & 1) + (g >> 1)) * 16;
+    const uint32_t place = lane & 7;
+    const uint32_t col0 = at.ct * S::TC + (uint32_t)(wc * S::AB) * 16 + place * EL;
 #pragma unroll
     for (int y = 0; y < S::YB; y++) {
-      uint32_t o[2][PIECES][4];
+      uint32_t q[PIECES + 1][2][4] = {}, single[2];
+      bool some[2];
+#pragma unroll
+      for (int i = 0; i < PIECES; i++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) sixteen<T>(&acc[(2 * i + h) * STRIDE], y, q[i][h]);
 #pragma unroll
       for (int i = 0; i < PIECES; i++) {
-        uint32_t q[2][4];
 #pragma unroll
-        for (int h = 0; h < 2; h++) sixteen<T>(&acc[(2 * i + h) * STRIDE], y, q[h]);
-        // Lanes li < 8 hand their second sixteen bytes to li + 8 and get its first: then eight
-        // lanes have a row's 128 bytes, first of the rows li, then of li + 8.
+        for (int h = 0; h < 2; h++)
+          *reinterpret_cast<v4u*>(mine + li * PITCH + h * 64 + chunk_at) =
+              v4u{q[i][h][0], q[i][h][1], q[i][h][2], q[i][h][3]};
+        if (sizeof(T) == 2 && g == 0)
+          *reinterpret_cast<uint32_t*>(mine + li * PITCH + 128) = q[i + 1][0][0];
+        wave_fence8();
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const uint32_t give = low ? q[1][e] : q[0][e];
-          const uint32_t got = __float_as_uint(lane_perm<0x128>(__uint_as_float(give)));
-          o[0][i][e] = low ? q[0][e] : got;
-          o[1][i][e] = low ? got : q[1][e];
-        }
-      }
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        const uint32_t row = at.rt * S::TR + (uint32_t)(wr * S::YB + y) * 16 + (li & 7) + 8 * h;
-        T* const p = reinterpret_cast<T*>(a.y) + (size_t)row * a.ldy + col0;
-        if (sizeof(T) == 2 && a.odd) {
-          if constexpr (sizeof(T) == 2)
-            store_odd<T, PIECES>(p, o[h], place, row < a.n && col0 < a.k ? a.k - col0 : 0u);
-        } else {
-#pragma unroll
-          for (int i = 0; i < PIECES; i++) {
-            const uint32_t col = col0 + i * 8 * EL;
-            const Vec<T> v{make_uint4(o[h][i][0], o[h][i][1], o[h][i][2], o[h][i][3])};
-            if (stored || (row < a.n && col + EL <= a.k))
-              STREAM ? stream_vec(p + i * 8 * EL, v) : store_vec(p + i * 8 * EL, v);
-            else if (row < a.n && col < a.k)
-              store_some(p + i * 8 * EL, v, (int)(a.k - col));
+        for (int h = 0; h < 2; h++) {
+          const uint32_t in = (lane >> 3) + 8 * h;
+          const uint32_t row = at.rt * S::TR + (uint32_t)(wr * S::YB + y) * 16 + in;
+          const char* const from = mine + in * PITCH + place * 16;
+          const v4u v = *reinterpret_cast<const v4u*>(from);
+          const uint32_t col = col0 + i * 8 * EL;
+          T* const p = reinterpret_cast<T*>(a.y) + (size_t)row * a.ldy + col;
+          const uint32_t left = row < a.n && col < a.k ? a.k - col : 0u;
+          if (sizeof(T) == 2 && a.odd) {
+            if constexpr (sizeof(T) == 2) {
+              const bool last = i + 1 == PIECES && place == 7;
+              store_odd_row<T, STREAM>(p, v, *reinterpret_cast<const uint32_t*>(from + 16), last,
+                                       left);
+              // The first element of the wave's, from its first piece, and the last.
+              if (i == 0) single[h] = v[0], some[h] = left > 0;
+              if (last) single[h] = v[3] >> 16, some[h] = left >= 8;
+              if (i + 1 == PIECES && ((uintptr_t)p & 2) && (place == 0 || place == 7) && some[h])
+                *(p + (last ? 7 : -i * 8 * (int)EL)) = __builtin_bit_cast(T, (uint16_t)single[h]);
+            }
+          } else {
+            store_row<T, STREAM>(p, v, stored ? EL : left);
           }
         }
+        wave_fence8();
       }
     }
   }
