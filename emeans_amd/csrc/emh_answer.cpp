@@ -286,7 +286,7 @@ int emh_log_probs_grad(emh_ctx* c, const emh_buf* z, size_t ldz, size_t n, size_
     EMH_ENSURE((tokens != nullptr) == (glogp != nullptr), "tokens and glogp come together");
     EMH_ENSURE((entropy != nullptr) == (gentropy != nullptr), "entropy and gentropy come together");
     const Range rd = check_matrix(dz, n, k, lddz, "dz");
-    apart_or_same(rd, t.z, lddz == ldz, "dz", "z");
+    apart_or_same(rd, t.z, lddz == t.a.ldz, "dz", "z");
     std::vector<Named> in = {{t.tokens, "tokens"}, {check_f32(lse, n, "lse"), "lse"}};
     if (glogp) in.push_back({check_f32(glogp, n, "glogp"), "glogp"});
     if (entropy) in.push_back({check_f32(entropy, n, "entropy"), "entropy"});

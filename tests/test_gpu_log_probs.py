@@ -213,6 +213,19 @@ def test_a_class_out_of_range_is_an_error(dev):
     assert not po.read()[2].any()
 
 
+def test_gradient_in_place_without_strides(dev):
+    from emeans_amd import F32
+    n, k = 5, 40
+    z, t = np.random.default_rng(9).standard_normal((n, k)), np.arange(n, dtype=np.uint32)
+    a, b, lp, lse = dev.upload_f32(z), dev.zeros(n * k, F32), dev.zeros(n, F32), dev.zeros(n, F32)
+    one = dev.upload_f32(np.ones(n))
+    dev.log_probs(a, n, k, dev.upload_u32(t), lp, lse)
+    for to, kw in ((b, {}), (a, {}), (a, dict(ldz=k)), (a, dict(lddz=k))):
+        dev.write(a, 0, z.reshape(-1))
+        dev.log_probs_grad(a, n, k, dev.upload_u32(t), lse, to, glogp=one, **kw)
+        assert dev.read(to).tobytes() == dev.read(b).tobytes() and dev.read(to).any()
+
+
 def test_no_rows_and_refusals(dev):
     from emeans_amd import F16, F32, U32, EmeansHipInvalid
     z, f, u = dev.zeros(200, F32), dev.zeros(10, F32), dev.zeros(10, U32)
