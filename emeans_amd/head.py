@@ -11,7 +11,8 @@ labels that `assign` or a training gave, AdamW.
 layer_norm_grad and one AdamW step over all parameters, queued on the device's stream
 without a wait. `fit` uploads each batch of host rows, and waits for its losses. With
 norm="rms" the norm is rms_norm; with max_norm the gradients count as if clipped to that
-global norm, and a step whose gradients are not all finite changes nothing.
+global norm, and a step whose gradients are not all finite changes nothing (it counts as a
+step all the same).
 
 `answer` gives the likeliest clusters of resident rows, with their log probabilities and the
 answers' entropies, in 8 bits: the normalized rows and the classes as codes (rms_norm or
@@ -209,6 +210,8 @@ class ClusterHead:
             raise ValueError("answers need a positive scale")
         if n < 0 or len(x) < n * self.d or (labels is not None and len(labels) < n):
             raise ValueError("x and labels must hold n rows")
+        if x.kind != self.kind:
+            raise ValueError("x must be of the head's kind")
         if self._frozen != self.steps:
             self.freeze()
         d, k, dev = self.d, self.k, self.dev
@@ -216,7 +219,8 @@ class ClusterHead:
         stride, blocks = HipDevice.code_stride(d), HipDevice.code_blocks(d)
         codes, scales = dev.zeros(rows * stride, F8), dev.zeros(rows * blocks, F32)
         normed = None if self.rms else dev.zeros(rows * d, self.kind)
-        logits = dev.zeros(rows * k, self.kind)
+        # (F16 does not hold every logit that training's f32 does: of 65,536 and more.)
+        logits = dev.zeros(rows * k, BF16 if self.kind == BF16 else F32)
         ids, logp = dev.zeros(n * top, U32), dev.zeros(n * top, F32)
         lse, entropy = dev.zeros(n, F32), dev.zeros(n, F32)
         given = None if labels is None else dev.zeros(n, F32)

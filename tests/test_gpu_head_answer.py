@@ -146,6 +146,20 @@ def test_answers_follow_the_weights(dev):
     assert (few.ids[:, 9:] == A.NONE).all() and np.isneginf(few.logp[:, 9:]).all()
 
 
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+def test_answers_of_long_classes(dev, name):
+    """Logits of 240,000: whole in f32, of a class that is likelier than all others by
+    thousands: its log probability is 0 and so is the entropy."""
+    from emeans_amd.head import ClusterHead
+    d, k = 64, 5
+    x = np.zeros((k, d), np.float32)
+    x[np.arange(k), np.arange(k)] = 3.0
+    head = ClusterHead(d, k, kind=R.kind(name), centroids=1e4 * x, dev=dev, norm="rms")
+    got = head.answer(head.rows(x), k, 1, head.labels(np.arange(k)))
+    assert np.array_equal(got.ids[:, 0], np.arange(k))
+    assert (got.logp == 0).all() and (got.given == 0).all() and (got.entropy == 0).all()
+
+
 def test_refusals(dev):
     from emeans_amd.head import ClusterHead
     for bad in (dict(norm="batch"), dict(max_norm=0.0), dict(max_norm=-1.0),
@@ -162,6 +176,10 @@ def test_refusals(dev):
     for bad in (dict(top=0), dict(top=33), dict(n=4), dict(labels=head.labels(np.zeros(2, int)))):
         with pytest.raises(ValueError):
             head.answer(**{**dict(x=xb, n=3), **bad})
+    from emeans_amd import BF16, F16
+    for other in (F16, BF16):  # rows of another kind than the head's
+        with pytest.raises(ValueError, match="kind"):
+            head.answer(dev.zeros(24, other), 3)
 
 
 def test_all_operators_in_one_chain(dev):
