@@ -608,20 +608,10 @@ void launch_log_probs_grad(emh_ctx* c, LogpArgs a, int kind) {
     const bool whole = a.lddz % N == 0 && (uintptr_t)a.dz % 16 == 0;
     const size_t vectors = (a.k + N - 1) / N + (whole ? 0 : 1);
     const size_t chunks = (vectors + 64 * NV - 1) / (64 * NV);
-    // Bands of rows whose chunks 31 bits number.
-    const size_t band = std::max<size_t>(1, (size_t(1) << 31) / chunks - MAX_GROUPS * 4 / chunks);
-    for (size_t left = a.n; left > 0;) {
-      const size_t rows = std::min(left, band), units = rows * chunks;
-      k_logp_grad<T, NV>
-          <<<dim3((unsigned)std::min((units + 3) / 4, MAX_GROUPS)), 256, 0, c->stream>>>(
-              a, (uint32_t)chunks, (uint32_t)units);
-      left -= rows;
-      a.z = (const T*)a.z + rows * a.ldz;
-      a.dz = (T*)a.dz + rows * a.lddz;
-      a.lse_in += rows;
-      if (a.tokens) a.tokens += rows, a.glogp += rows;
-      if (a.gentropy) a.gentropy += rows, a.entropy_in += rows;
-    }
+    const size_t units = a.n * chunks;  // (2 KB of dz at least, or a row)
+    EMH_ENSURE(units < (size_t(1) << 31), "z is larger than any device's memory");
+    k_logp_grad<T, NV><<<dim3((unsigned)std::min((units + 3) / 4, MAX_GROUPS)), 256, 0, c->stream>>>(
+        a, (uint32_t)chunks, (uint32_t)units);
   });
   EMH_HIP(hipGetLastError());
 }

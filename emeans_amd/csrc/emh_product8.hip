@@ -555,22 +555,19 @@ void launch_tiles(emh_ctx* c, const CodedIn& x, size_t n, size_t d, const CodedI
   const bool stream = n * k * sizeof(T) >= STREAM_FROM && y.ld * sizeof(T) % 64 == 0 &&
                       (uintptr_t)y.p % 64 == 0;
   a.t.ctiles = (uint32_t)((k + S::TC - 1) / S::TC);
-  // Bands of rows whose tiles 32 bits number.
-  const size_t most = std::max<size_t>(1, (size_t(1) << 30) / a.t.ctiles / GROUP) * S::TR;
-  for (size_t r0 = 0; r0 < n; r0 += most) {
-    const size_t rows = std::min(n - r0, most);
-    a.n = (uint32_t)rows;
-    a.xs = x.scale + r0 * x.lds;
-    a.y = (T*)y.p + r0 * y.ld;
-    a.t.r = {{(const char*)x.q + r0 * x.ld, nullptr}, (uint32_t)x.ld, (uint32_t)rows, 0};
-    a.t.rtiles = (uint32_t)((rows + S::TR - 1) / S::TR);
-    const unsigned blocks = prepare(a.t);
-    const unsigned grid = std::min(blocks, (unsigned)(c->cus * S::PER_CU));
-    if (stream)
-      k_tile8<T, S, EXACT, true><<<grid, S::THREADS, 0, c->stream>>>(a);
-    else
-      k_tile8<T, S, EXACT, false><<<grid, S::THREADS, 0, c->stream>>>(a);
-  }
+  a.t.rtiles = (uint32_t)((n + S::TR - 1) / S::TR);
+  EMH_ENSURE((size_t)a.t.ctiles * a.t.rtiles <= (size_t(1) << 30) / GROUP,
+             "y is larger than any device's memory");
+  a.n = (uint32_t)n;
+  a.xs = x.scale;
+  a.y = y.p;
+  a.t.r = {{(const char*)x.q, nullptr}, (uint32_t)x.ld, (uint32_t)n, 0};
+  const unsigned blocks = prepare(a.t);
+  const unsigned grid = std::min(blocks, (unsigned)(c->cus * S::PER_CU));
+  if (stream)
+    k_tile8<T, S, EXACT, true><<<grid, S::THREADS, 0, c->stream>>>(a);
+  else
+    k_tile8<T, S, EXACT, false><<<grid, S::THREADS, 0, c->stream>>>(a);
 }
 
 }  // namespace
