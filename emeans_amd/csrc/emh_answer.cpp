@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstring>
 #include <memory>
 #include <mutex>
 #include <vector>
@@ -13,9 +14,9 @@
 
 struct emh_grad_norm {
   emh_ctx* ctx = nullptr;  // null once it is destroyed
-  emh::NormTensor* tensors = nullptr;  // on the device
+  double* sums = nullptr;  // a block on the device, with what follows
+  emh::NormTensor* tensors = nullptr;
   uint2* chunks = nullptr;
-  double* sums = nullptr;
   size_t nchunks = 0, chunk = 0;
   bool stream = false;
   std::vector<emh_buf*> written;
@@ -28,11 +29,7 @@ namespace {
 std::mutex g_norms_mu;
 
 void free_tables(emh_grad_norm* p) {
-  if (p->tensors) (void)hipFree(p->tensors);
-  if (p->chunks) (void)hipFree(p->chunks);
   if (p->sums) (void)hipFree(p->sums);
-  p->tensors = nullptr;
-  p->chunks = nullptr;
   p->sums = nullptr;
 }
 
@@ -365,15 +362,19 @@ int emh_grad_norm_create(emh_ctx* c, const emh_buf* const* grads, emh_buf* const
     }
     use_device(c);
     plan->nchunks = chunks.size();
+    // One block: the sums, then the tables (each entry's size is a multiple of 8).
+    const size_t first = emh::NORM_SUMS * sizeof(double);
+    const size_t named = table.size() * sizeof table[0], parts = chunks.size() * sizeof chunks[0];
     try {
-      EMH_HIP(hipMalloc(&plan->sums, emh::NORM_SUMS * sizeof(double)));
-      if (!chunks.empty()) {
-        EMH_HIP(hipMalloc(&plan->tensors, table.size() * sizeof table[0]));
-        EMH_HIP(hipMalloc(&plan->chunks, chunks.size() * sizeof chunks[0]));
-        EMH_HIP(hipMemcpyAsync(plan->tensors, table.data(), table.size() * sizeof table[0],
-                               hipMemcpyHostToDevice, c->stream));
-        EMH_HIP(hipMemcpyAsync(plan->chunks, chunks.data(), chunks.size() * sizeof chunks[0],
-                               hipMemcpyHostToDevice, c->stream));
+      EMH_HIP(hipMalloc(&plan->sums, first + named + parts));
+      char* p = (char*)plan->sums + first;
+      plan->tensors = (emh::NormTensor*)p;
+      plan->chunks = (uint2*)(p + named);
+      if (parts > 0) {
+        std::vector<char> host(named + parts);
+        memcpy(host.data(), table.data(), named);
+        memcpy(host.data() + named, chunks.data(), parts);
+        EMH_HIP(hipMemcpyAsync(p, host.data(), host.size(), hipMemcpyHostToDevice, c->stream));
         EMH_HIP(hipStreamSynchronize(c->stream));  // the host's tables go away
       }
       std::lock_guard<std::mutex> g(g_norms_mu);
