@@ -359,6 +359,7 @@ int emh_destroy(emh_ctx* c) {
     emh::drop_norms(c);
     c->rms_part.release();
     c->logp_part.release();
+    c->logp_done.release();
     for (emh::Scratch* s : {&c->cand, &c->fblist, &c->order, &c->start, &c->misc, &c->knn_tmp,
                             &c->xnorm, &c->bigj, &c->chunkcnt, &c->tickets,
                             &c->preview_ticket, &c->xsplit, &c->xsplit_norm, &c->csplit, &c->csplit_norm, &c->csplit_part,

@@ -293,6 +293,7 @@ struct emh_ctx {
   std::vector<emh_grad_norm*> norms;  // as plans (emh_answer.cpp)
   emh::Kept rms_part;      // rms_norm_grad: the workgroups' sums of dweight
   emh::Kept logp_part;     // log_probs: what the parts of a row found
+  emh::Kept logp_done;     // and how many of a row's have; zeros between calls
   emh::Scratch xent;       // cross_entropy's parts, gradients of a piece and laid-out operands
   emh::Scratch preview_ticket;  // k_mass_preview's last-block ticket (left at zero)
   // Host staging of the device loop: masses, plan, flags, epoch orders and

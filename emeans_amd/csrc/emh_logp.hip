@@ -194,8 +194,11 @@ struct Best {
 // Lanes' values v: a bound that at least `top` of them reach (-infinity where fewer than that
 // are above it), found in groups: as many as the next power of two from top; the least of the
 // groups' largest.
+__device__ __forceinline__ uint32_t group_bits(uint32_t top) {  // log2 of the groups
+  return top <= 1 ? 0u : 32u - (uint32_t)__clz((int)(top - 1));
+}
 __device__ __forceinline__ float group_bound(float v, uint32_t top) {
-  const uint32_t p = top <= 1 ? 0u : 32u - (uint32_t)__clz((int)(top - 1));  // log2 of the groups
+  const uint32_t p = group_bits(top);
   auto join = [&](uint32_t step, float a, float b) __attribute__((always_inline)) {
     return step + p < 6 ? fmaxf(a, b) : fminf(a, b);
   };
@@ -271,16 +274,115 @@ __device__ __forceinline__ void finish(const LogpArgs& a, size_t row, const Give
   }
 }
 
+// What the parts of a row leave for each other lies in memory: written and read by single
+// accesses that all of the GPU's caches let through, so that none of them is written back or
+// emptied for it (64 rows of 131,071 with top 8: 17.6 us, by fences 24.5). A second launch that
+// joins the parts took 8.0 us for a row of 131,071 without a list where this takes 4.6.
+__device__ __forceinline__ void share(uint64_t* p, uint64_t v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ uint64_t shared_value(const uint64_t* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// Counters lie a line apart: side by side 64 rows' (1,024 parts) took 10.3 us, and so 7.4.
+constexpr uint32_t DONE_STEP = 32;
 struct PartOut {  // [row][part]
-  float4* seen;   // m, s, e
-  uint64_t* best; // [row][part][top]
+  uint64_t* seen;  // two: m and s, e
+  uint64_t* best;  // [row][part][top]
+  uint32_t* done;  // [row]: its parts that are there; zeros between calls
+  __device__ __forceinline__ void put_seen(size_t u, const Seen& v) const {
+    share(seen + 2 * u, (uint64_t)__float_as_uint(v.s) << 32 | __float_as_uint(v.m));
+    share(seen + 2 * u + 1, __float_as_uint(v.e));
+  }
+  __device__ __forceinline__ Seen get_seen(size_t u) const {
+    const uint64_t ms = shared_value(seen + 2 * u), e = shared_value(seen + 2 * u + 1);
+    return Seen(make_float4(__uint_as_float((uint32_t)ms), __uint_as_float((uint32_t)(ms >> 32)),
+                            __uint_as_float((uint32_t)e), 0.f));
+  }
 };
+// One wave's, of a part of a row: whether it is the last one there.
+__device__ __forceinline__ bool last_part(uint32_t* done, uint32_t parts) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what the wave has shared is there
+  uint32_t before = 0;
+  if ((threadIdx.x & 63) == 0) {
+    before = __hip_atomic_fetch_add(done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (before == parts - 1)
+      __hip_atomic_store(done, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  const bool last = (uint32_t)__builtin_amdgcn_readfirstlane((int)before) == parts - 1;
+  asm volatile("" ::: "memory");
+  return last;
+}
+// The parts of a row, by a wave. room: LDS for ROOM + ROOM_END.
+template <bool TOP>
+__device__ __forceinline__ void join_parts(const PartOut& in, size_t row, uint32_t parts,
+                                           uint32_t top, uint64_t* room, Seen& all, Best& best) {
+  const uint32_t lane = threadIdx.x & 63;
+  // (Entries come from lists of 64 - top at a time, so that these and a list of top have room.)
+  const uint32_t count = parts * top, each = ROOM - top;
+  const uint64_t* const list = in.best + row * count;
+  auto entry = [&](uint32_t i0) __attribute__((always_inline)) {
+    const uint32_t i = i0 + lane;
+    return lane < each && i < count ? shared_value(list + i) : 0;
+  };
+  constexpr int AHEAD = 4;
+  uint64_t o[AHEAD], first = 0;
+  if constexpr (TOP) {
+#pragma unroll
+    for (int j = 0; j < AHEAD; j++) o[j] = entry(j * each);
+    // Of a group's lanes (group_bound) the first have the parts' best, others what comes next:
+    // each an entry of its own.
+    const uint32_t groups = group_bits(top), e = (lane & ((64u >> groups) - 1)) << groups | lane >> (6 - groups);
+    const uint32_t rank = e / parts, part = e - rank * parts;
+    if (rank < top) first = shared_value(list + part * top + rank);
+    for (uint32_t p = e + 64; p < parts; p += 64) {
+      const uint64_t f = shared_value(list + p * top);
+      first = f > first ? f : first;
+    }
+  }
+  all = Seen();
+  for (uint32_t p = lane; p < parts; p += 64) all.join(in.get_seen(row * parts + p));
+  all.join_lanes();
+  if constexpr (TOP) {
+    best.key = 0;
+    // (At least top entries reach it.)
+    const float bound = group_bound(first ? key_value(first) : -INFINITY, top);
+    uint32_t have = 0;
+    for (uint32_t i0 = 0; i0 < count;) {
+#pragma unroll
+      for (int j = 0; j < AHEAD; j++, i0 += each) {
+        const uint64_t them = __ballot(o[j] > lane_key(best.key, top - 1) && key_value(o[j]) >= bound);
+        if (!them) continue;
+        const uint32_t more = (uint32_t)__popcll(them);
+        if (have + more > each) {
+          best.merge(top, room, have);
+          have = 0;
+        }
+        if (them >> lane & 1)
+          room[__builtin_amdgcn_mbcnt_hi((uint32_t)(them >> 32),
+                                         __builtin_amdgcn_mbcnt_lo((uint32_t)them, have))] = o[j];
+        have += more;
+      }
+      if (i0 < count) {
+#pragma unroll
+        for (int j = 0; j < AHEAD; j++) o[j] = entry(i0 + j * each);
+      }
+    }
+    if (have > 0) best.merge(top, room, have);
+  }
+}
 
-// W waves take a part of a row, by turns in chunks of 64 NV vectors; parts == 1: whole
-// rows, whose results they write. One wave: rows of one chunk.
-template <class T, int W, int NV, bool TOP>
-__global__ __launch_bounds__(256) void k_logp(const LogpArgs a, int kind, uint32_t parts,
-                                              uint32_t each, PartOut out) {
+// W waves take a part of a row, by turns in chunks of 64 NV vectors; the last of a row's parts
+// joins them all, in their order, and writes the row's results. One wave: rows of one chunk.
+// (least_waves: with lists of the likeliest a few registers fewer than the compiler would take,
+// for a wave more on a SIMD. 16,384 rows of 2,000 bf16 with top 5: 24.5 us, without 26.3.)
+template <class T>
+constexpr int least_waves(int W, int NV, bool top, bool parts) {
+  return !top || parts ? 1 : sizeof(T) == 4 ? 6 : W == 1 && NV == 4 ? 5 : 1;
+}
+template <class T, int W, int NV, bool TOP, bool PARTS>
+__global__ __launch_bounds__(256, least_waves<T>(W, NV, TOP, PARTS)) void k_logp(
+    const LogpArgs a, int kind, uint32_t parts, uint32_t each, PartOut out) {
   constexpr int N = VecOf<T>::N, ROWS = 4 / W;
   __shared__ float4 seen[4];
   __shared__ __attribute__((aligned(16))) uint64_t rooms[TOP ? 4 : 1][ROOM + ROOM_END];
@@ -288,17 +390,17 @@ __global__ __launch_bounds__(256) void k_logp(const LogpArgs a, int kind, uint32
   const uint32_t lane = threadIdx.x & 63;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const uint32_t w = wave % W;
-  const size_t units = a.n * parts;
+  const size_t units = PARTS ? a.n * parts : a.n;
   for (size_t u0 = (size_t)blockIdx.x * ROWS; u0 < units; u0 += (size_t)gridDim.x * ROWS) {
     const size_t u = u0 + wave / W;
     if (W == 1 && u >= units) return;  // (waves of their own)
     // (Rows in parts are few.)
-    const size_t row = W == 1 || parts == 1 ? u : (uint32_t)u / parts;
-    const uint32_t part = W == 1 ? 0 : (uint32_t)(u - row * parts);
+    const size_t row = PARTS ? (uint32_t)u / parts : u;
+    const uint32_t part = PARTS ? (uint32_t)(u - row * parts) : 0;
     const Row<T> r(a.z, row * a.ldz, a.k);
     const uint32_t nv = (uint32_t)r.vectors(), chunks = (nv + 64 * NV - 1) / (64 * NV);
-    const uint32_t c0 = W == 1 ? 0 : min(chunks, part * each);
-    const uint32_t c1 = W == 1 ? 1 : min(chunks, c0 + each);
+    const uint32_t c0 = PARTS ? min(chunks, part * each) : 0;
+    const uint32_t c1 = W == 1 ? 1 : PARTS ? min(chunks, c0 + each) : chunks;
     Seen all;
     Best best;
     Vec<T> next[NV];
@@ -433,39 +535,11 @@ __global__ __launch_bounds__(256) void k_logp(const LogpArgs a, int kind, uint32
       }
     }
     if (W > 1 && wave != 0) continue;
-    if (parts == 1) {
-      finish(a, row, given, all, best);
-    } else {
-      if (lane == 0) out.seen[u] = all.packed();
-      if (TOP && lane < a.top) out.best[u * a.top + lane] = best.key;
-    }
-  }
-}
-
-// The parts of a row, by a wave.
-template <bool TOP>
-__global__ __launch_bounds__(64) void k_logp_join(const LogpArgs a, int kind, uint32_t parts,
-                                                  PartOut in) {
-  const uint32_t lane = threadIdx.x;
-  for (size_t row = blockIdx.x; row < a.n; row += gridDim.x) {
-    Seen all;
-    const Given given(a, kind, row);
-    for (uint32_t p = lane; p < parts; p += 64) all.join(Seen(in.seen[row * parts + p]));
-    all.join_lanes();
-    Best best;
-    if constexpr (TOP) {
-      __shared__ __attribute__((aligned(16))) uint64_t room[ROOM + ROOM_END];
-      const uint32_t count = parts * a.top;
-      for (uint32_t i0 = 0, each = ROOM; i0 < count; i0 += each, each = ROOM - a.top) {
-        const uint32_t i = i0 + lane;
-        const uint64_t o = lane < each && i < count ? in.best[row * count + i] : 0;
-        const uint64_t them = __ballot(o > lane_key(best.key, a.top - 1));
-        if (!them) continue;
-        if (them >> lane & 1)
-          room[__builtin_amdgcn_mbcnt_hi((uint32_t)(them >> 32),
-                                         __builtin_amdgcn_mbcnt_lo((uint32_t)them, 0u))] = o;
-        best.merge(a.top, room, (uint32_t)__popcll(them));
-      }
+    if constexpr (PARTS) {
+      if (lane == 0) out.put_seen(u, all);
+      if (TOP && lane < a.top) share(out.best + u * a.top + lane, best.key);
+      if (!last_part(out.done + row * DONE_STEP, parts)) continue;
+      join_parts<TOP>(out, row, parts, a.top, rooms[0], all, best);
     }
     finish(a, row, given, all, best);
   }
@@ -557,27 +631,36 @@ void launch_log_probs(emh_ctx* c, LogpArgs a, int kind) {
     const bool whole = a.ldz % N == 0 && (uintptr_t)a.z % 16 == 0;
     const size_t vectors = (a.k + N - 1) / N + (whole ? 0 : 1);
     // A wave a row where the row is a chunk; otherwise four, and parts of a row where there are
-    // few rows.
+    // few rows. Chunks of 128 vectors, not 256, where they leave no wave a second one anyway (a
+    // row of 16,384 bf16 8.5 us, so 9.2; 16 of them 8.7, so 9.5; 131,071 with top 8 9.0, so 9.3).
     const bool small = vectors <= 256;
-    const size_t per = vectors <= 1024 ? 128 : 256, chunks = (vectors + per - 1) / per;
+    const size_t per = vectors <= 1024 || a.n * vectors <= 512 * (size_t)c->cus ? 128 : 256;
+    const size_t chunks = (vectors + per - 1) / per;
     size_t parts = 1;
     if (!small) parts = std::min((chunks + 3) / 4, std::max<size_t>(1, 4 * (size_t)c->cus / a.n));
     PartOut out{};
     if (parts > 1) {
-      const size_t seen = (a.n * parts * sizeof(float4) + 255) & ~size_t(255);
+      const size_t seen = (a.n * parts * 2 * sizeof(uint64_t) + 255) & ~size_t(255);
       char* p = (char*)c->logp_part.get(seen + a.n * parts * a.top * sizeof(uint64_t), c->stream);
-      out.seen = (float4*)p;
+      out.seen = (uint64_t*)p;
       out.best = (uint64_t*)(p + seen);
+      // (Fewer rows than twice the CUs have parts.)
+      const bool first = c->logp_done.bytes == 0;
+      out.done = (uint32_t*)c->logp_done.get(2 * (size_t)c->cus * DONE_STEP * sizeof(uint32_t), c->stream);
+      if (first) EMH_HIP(hipMemsetAsync(out.done, 0, c->logp_done.bytes, c->stream));
     }
     auto go = [&](auto waves, auto nv, auto top) {
       constexpr int W = decltype(waves)::value, NV = decltype(nv)::value;
       constexpr bool TOP = decltype(top)::value;
       const size_t groups = (a.n * parts + 4 / W - 1) / (4 / W);
-      k_logp<T, W, NV, TOP><<<dim3((unsigned)std::min(groups, MAX_GROUPS)), 256, 0, c->stream>>>(
-          a, kind, (uint32_t)parts, (uint32_t)((chunks + parts - 1) / parts), out);
-      if (parts > 1)
-        k_logp_join<TOP><<<dim3((unsigned)std::min(a.n, MAX_GROUPS)), 64, 0, c->stream>>>(
-            a, kind, (uint32_t)parts, out);
+      auto run = [&](auto kernel) {
+        kernel<<<dim3((unsigned)std::min(groups, MAX_GROUPS)), 256, 0, c->stream>>>(
+            a, kind, (uint32_t)parts, (uint32_t)((chunks + parts - 1) / parts), out);
+      };
+      if constexpr (W > 1) {
+        if (parts > 1) return run(k_logp<T, W, NV, TOP, true>);
+      }
+      run(k_logp<T, W, NV, TOP, false>);
     };
     auto with_top = [&](auto top) {
       if (per == 256 && !small)

@@ -213,6 +213,24 @@ def test_a_class_out_of_range_is_an_error(dev):
     assert not po.read()[2].any()
 
 
+@pytest.mark.parametrize("n,k,top", [(1, 131071, 32), (5, 40001, 3), (70, 9000, 8), (400, 5000, 1)])
+def test_rows_in_parts_give_the_same_every_time(dev, n, k, top):
+    """Whichever of a row's parts is done last: with equal logits in all of them."""
+    from emeans_amd import BF16, F32, U32
+    z = np.random.default_rng(n).integers(-3, 3, (n, k)).astype(np.float32)
+    b, t = dev.zeros(n * k, BF16), dev.upload_u32(np.arange(n).astype(np.uint32))
+    dev.write(b, 0, R.encode(z, "bf16").reshape(-1))
+    out = [dev.zeros(n, F32) for _ in range(3)] + [dev.zeros(n * top, F32), dev.zeros(n * top, U32)]
+    ref, first = A.LogProbs(z), None
+    for _ in range(40):
+        dev.log_probs(b, n, k, t, out[0], out[1], entropy=out[2], top=top, top_logp=out[3],
+                      top_ids=out[4])
+        got = [dev.read(o).tobytes() for o in out]
+        first = first or got
+        assert got == first
+    assert np.array_equal(dev.read(out[4]).reshape(n, top), ref.top(top)[0])
+
+
 def test_gradient_in_place_without_strides(dev):
     from emeans_amd import F32
     n, k = 5, 40
