@@ -400,6 +400,9 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_tile8(const Prod8Args a) {
 #pragma unroll
   for (int y = 0; y < S::YB; y++) f[y] = fx[y] * fw;
 
+  Halves rh[EXACT ? S::YB : 1], ch[EXACT ? 2 : 1];  // as f16: the rows', this and the next classes'
+  if constexpr (EXACT) ch[0] = Halves(ca[0].a, ca[0].b);
+
   // Sixteen bytes of results a lane.
   constexpr int EL = 16 / sizeof(T), STRIDE = EL / 4, STORES = S::YB * S::AB / STRIDE;
   bool stored = false;  // the last tile's results went out in STORES stores of every wave
@@ -414,11 +417,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_tile8(const Prod8Args a) {
 #pragma unroll
     for (int i = 0; i < 4; i++) t[i] = v4f{0.f, 0.f, 0.f, 0.f};
     for (uint32_t s = 0; s < steps; s++) {
-      Halves rh[EXACT ? S::YB : 1];
-      if constexpr (EXACT) {
-#pragma unroll
-        for (int y = 0; y < S::YB; y++) rh[y] = Halves(rb[y].a, rb[y].b);
-      }
+      if constexpr (EXACT) rh[0] = Halves(rb[0].a, rb[0].b);
       const uint32_t other = 2 * lds0 + S::STAGE - st;
 #pragma unroll
       for (int i = 0; i < S::AB; i++) {
@@ -442,15 +441,19 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_tile8(const Prod8Args a) {
           ca[(i + AHEAD) % SLOTS].read(st + cat + (i + AHEAD) * BLOCK16);
         else
           ca[(i + AHEAD) % SLOTS].read(other + cat + (i + AHEAD - S::AB) * BLOCK16);
-        Halves ch;
-        if constexpr (EXACT) ch = Halves(ca[i % SLOTS].a, ca[i % SLOTS].b);
 #pragma unroll
         for (int y = 0; y < S::YB; y++) {
           const int m = i * S::YB + y, o = (m + ALL - 2) % ALL;  // the MFMA, and whose sums are due
-          if constexpr (EXACT)
-            t[m & 3] = block16(ch, rh[y]);
-          else
+          if constexpr (EXACT) {
+            t[m & 3] = block16(ch[i & 1], rh[y]);
+            // Between these MFMAs: the next classes' codes as f16 and, once a block, the rows'.
+            const Frag& next = ca[(i + 1) % SLOTS];
+            const v4u from = y < 2 ? next.a : next.b;
+            ch[(i + 1) & 1].v[y] = y & 1 ? halves8(from.z, from.w) : halves8(from.x, from.y);
+            if (i == 0 && y + 1 < S::YB) rh[y + 1] = Halves(rb[y + 1].a, rb[y + 1].b);
+          } else {
             t[m & 3] = block8(ca[i % SLOTS].codes(), rb[y].codes());
+          }
           const float by = m < 2 ? fp[m] : f[o % S::YB];
 #pragma unroll
           for (int e = 0; e < 4; e++)
@@ -458,6 +461,16 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_tile8(const Prod8Args a) {
           // (Here, not at the step's end, with all the blocks' sums kept until then.)
           asm volatile("" : "+v"(acc[o / S::YB][o % S::YB]));
           if (i == S::AB - 1) rb[y].read(other + rat + y * BLOCK16);
+          if constexpr (EXACT) {
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+              __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);  // an MFMA
+              if (i == 0 && y + 1 < S::YB)
+                __builtin_amdgcn_sched_group_barrier(0x2, 6, 0);  // VALU
+              else
+                __builtin_amdgcn_sched_group_barrier(0x2, 2, 0);
+            }
+          }
           __builtin_amdgcn_sched_barrier(0);
           if (i >= MEET) {
             constexpr int LEFT = (S::AB - MEET) * S::YB;
