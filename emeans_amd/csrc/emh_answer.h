@@ -83,8 +83,8 @@ struct NormTensor {  // as the kernels read it
 // little as fills the GPU.
 constexpr size_t NORM_CHUNK = 16384, NORM_CHUNK_FEW = 2048, NORM_FEW = size_t(4) << 20;
 constexpr size_t NORM_SUMS = 1024;
-// chunks[i]: a tensor and the number of a chunk in it. stream: results past the caches. sums: NORM_SUMS; out: the norm and the
-// factor.
+// chunks[i]: a tensor and the number of a chunk in it. stream: results past the caches. sums:
+// NORM_SUMS; out: the norm and the factor.
 void launch_grad_norm(emh_ctx* c, const NormTensor* tensors, const uint2* chunks, size_t nchunks,
                       size_t chunk, bool stream, double* sums, float scale, float max_norm,
                       float* out, bool clip);

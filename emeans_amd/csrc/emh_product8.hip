@@ -10,10 +10,17 @@
 // results (2^-9, 2^-12) do not show. f32 results, and few rows, whose time is the classes'
 // bytes, take the f16 MFMA instead (an f16 holds every code exactly): 5e-8.
 //
+// Bound by the matrix cores where all three sizes are large (8,192^3: 455 us, 2.4 PFLOP/s; f32 935 us,
+// 1.2), by the results' bytes where the depth is short (8,192 x 1,024 x 131,072 bf16 1.14 ms, 2.1
+// GB; k = 131,071, whose rows straddle lines and stay in the caches on their way, 1.61 ms), and
+// by the classes' bytes and latency where rows are few (1 x 1,024 x 16,384: 5.5 us; 64: 9.5 us).
+//
 // Few rows read the classes as they lie. More of them go in tiles: a workgroup owns 256 x
 // 256 or 128 x 128 of the result, and a block of the depth, 128 bytes a row of both operands,
 // goes by in one step, moved to LDS by DMA into one of two stages, its 16-byte chunks
-// XOR-swizzled so that sixteen rows' equal chunks meet no bank twice.
+// XOR-swizzled so that sixteen rows' equal chunks meet no bank twice. 256 x 256 takes 2 us a
+// block of the depth and CU where 128 x 128, two a CU, take 1.55 for half as much; but fewer of
+// them leave more of the last round idle: launch_product8 weighs that.
 #include <cmath>
 
 #include "emh_answer.h"
@@ -80,6 +87,7 @@ __device__ __forceinline__ v4f block8(v8i a, v8i b) {
 
 // Few rows: a workgroup takes 16 classes and 16 YB rows, its four waves the blocks of the depth
 // by turns; operands come from memory as they lie, AHEAD blocks of a wave's on their way at once.
+// Bound by the classes' bytes: 1 x 1,024 x 16,384 5.5 us with its launch, 16.8 MB at 3.1 TB/s.
 template <int YB, bool EXACT>
 __global__ __launch_bounds__(256) void k_few8(const CodedIn x, size_t n, uint32_t d, const CodedIn w,
                                               size_t k, void* y, size_t ldy, int kind,
@@ -262,7 +270,8 @@ __device__ __forceinline__ void store_odd_row(T* p, const v4u& v, uint32_t after
   const uint32_t odd = (uint32_t)((uintptr_t)p >> 1) & 1, by = 16 * odd;
   v4u s;
 #pragma unroll
-  for (int e = 0; e < 4; e++) s[e] = __builtin_amdgcn_alignbit(e < 3 ? v[e < 3 ? e + 1 : 3] : after, v[e], by);
+  for (int e = 0; e < 4; e++)
+    s[e] = __builtin_amdgcn_alignbit(e < 3 ? v[e < 3 ? e + 1 : 3] : after, v[e], by);
   // (`left > odd ? left - odd : 0` lets the compiler take left for at least `odd` elsewhere.)
   const uint32_t n = max(left, odd) - odd;
   if (last && odd && n >= 7) {  // six of them; the seventh goes with the first
@@ -278,7 +287,8 @@ __device__ __forceinline__ void store_odd_row(T* p, const v4u& v, uint32_t after
 //
 // A workgroup takes tiles in turn, and the blocks of all its tiles are one stream: while a
 // tile's last blocks are multiplied, the next one's first are on their way, and while its
-// results go out of the registers, too.
+// results go out of the registers, too. (A workgroup for every tile: 8,192^3 538 us, so 455;
+// 16,384 x 768 x 1,024 bf16 21.6 us, so 18.5.)
 template <class T, class S, bool EXACT, bool STREAM>
 __global__ __launch_bounds__(S::THREADS, 2) void k_tile8(const Prod8Args a) {
   __shared__ __attribute__((aligned(1024))) char ring[2 * S::STAGE];
