@@ -491,15 +491,16 @@ template <class T, class F>
 bool by_shape(size_t d, F&& f) {
   constexpr size_t N = VecOf<T>::N;
   const size_t v = (d + N - 1) / N;
-  // Two vectors on 16 lanes where a block of codes is 16 lanes' (100,000 x 256 bf16 to codes 30.3
-  // us, on 64 lanes 36.5).
-  constexpr int PAIR = N == 8 ? 16 : 64;
+  // A row on as many lanes as one block of codes has: 100,000 x 256 bf16 to codes 30.2 us, x 128
+  // f32 26.3 (on 64 lanes 36.9 and 29.1). Longer rows, two vectors on 32 lanes, take as long
+  // or longer (10,007 x 300 f16 6.9, so 6.6).
+  constexpr int PAIR = N == 8 ? 16 : 32;
   if (d < N)
     return false;
   else if (v <= 16)
     f(Shape<16, 1>{});
   else if (v <= 32)
-    f(Shape<PAIR, 32 / PAIR + (PAIR == 64)>{});
+    f(Shape<PAIR, 32 / PAIR>{});
   else if (v <= 64)
     f(Shape<64, 1>{});
   else if (v <= 128)
