@@ -19,7 +19,7 @@
 // 256 or 128 x 128 of the result, and a block of the depth, 128 bytes a row of both operands,
 // goes by in one step, moved to LDS by DMA into one of two stages, its 16-byte chunks
 // XOR-swizzled so that sixteen rows' equal chunks meet no bank twice. 256 x 256 takes 2 us a
-// block of the depth and CU where 128 x 128, two a CU, take 1.55 for half as much; but fewer of
+// block of the depth and CU where 128 x 128, two a CU, take 1.3 for half as much; but fewer of
 // them leave more of the last round idle: launch_product8 weighs that.
 #include <cmath>
 
@@ -608,9 +608,10 @@ void launch_product8(emh_ctx* c, const CodedIn& x, size_t n, size_t d, const Cod
     };
     y.kind == EMH_F32 ? go(std::true_type{}) : go(std::false_type{});
   };
-  // What each way takes, in us, from the times of 1 to 16,384 rows by 768 to 131,071 classes: few
-  // rows read the classes again for every 64 rows and the rows for every 16 classes; a tile's
-  // block of the depth takes a CU as long as here, of small tiles less where a CU has but one.
+  // What each way takes, in us, from the times of 1 to 2,000 rows (tiles: 16,384) by 1,000 to 131,071
+  // classes of 128 to 4,096: few rows read the classes again for every 64 rows and the rows for
+  // every 16 classes, or take what their workgroups take; a tile's block of the depth takes a CU
+  // as long as here, of small tiles less where a CU has but one.
   const double cus = c->cus, steps = (double)((d + CODE_BLOCK - 1) / CODE_BLOCK);
   const bool f32 = y.kind == EMH_F32;
   auto up = [](size_t v, size_t by) { return (double)((v + by - 1) / by); };
@@ -618,9 +619,12 @@ void launch_product8(emh_ctx* c, const CodedIn& x, size_t n, size_t d, const Cod
     const double full = std::floor(tiles / slots), rest = tiles - full * slots;
     return start + steps * (full * step + (rest == 0 ? 0 : rest <= cus ? alone : step));
   };
-  const double few_take = 3.2 + ((double)n / 16 + up(n, 64)) * (double)k * (double)d / 6.5e6;
+  const double reads = n <= 64 ? (double)n / 16 + 1 : 5 * up(n, 64);
+  const double few_take = 2.5 + std::max(reads * (double)k * (double)d / 5.8e6,
+                                         up(k, 16) * up(n, 64) * 1.3e-3);
   const double small_take = std::max(
-      tiles_take(up(n, 128) * up(k, 128), 2 * cus, 2.5, f32 ? 2.6 : 1.55, f32 ? 1.5 : 0.8),
+      tiles_take(up(n, 128) * up(k, 128), 2 * cus, f32 ? 4.5 : 4.2, f32 ? 2.05 : 1.3,
+                 f32 ? 1.05 : 0.64),
       (double)k * (double)d / 4.2e6);
   const double large_take = f32 ? INFINITY : tiles_take(up(n, 256) * up(k, 256), cus, 4, 2, 2);
   // (A tile's offsets are 32 bits.)
