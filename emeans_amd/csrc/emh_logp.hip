@@ -270,11 +270,10 @@ __device__ __forceinline__ void finish(const LogpArgs& a, size_t row, const Give
     }
   }
   if (lane < a.top) {
-    const bool is = best.key != 0 && !odd;
+    const float z = key_value(best.key);
+    const bool is = best.key != 0 && !odd && z * a.scale > -INFINITY;
     if (a.ids) a.ids[row * a.top + lane] = is ? key_class(best.key) : NONE;
-    if (a.tops)
-      a.tops[row * a.top + lane] =
-          odd ? NAN : is ? fmaf(key_value(best.key), a.scale, -b) - ls : -INFINITY;
+    if (a.tops) a.tops[row * a.top + lane] = odd ? NAN : is ? fmaf(z, a.scale, -b) - ls : -INFINITY;
   }
 }
 

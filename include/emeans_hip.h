@@ -507,7 +507,7 @@ int emh_product8(emh_ctx* ctx, const emh_buf* x, size_t ldx, const emh_buf* xsca
                  size_t n, size_t d, const emh_buf* w, size_t ldw, const emh_buf* wscales,
                  size_t ldws, size_t k, emh_buf* y, size_t ldy);
 /* Of rows of logits z (n x k, f32, f16 or bf16), times scale (positive: an inverse
- * temperature): lse = log sum_v exp z_v; logp = z_t - lse of the row's class t = tokens[i] (u32,
+ * temperature; a product beyond f32 counts as infinite): lse = log sum_v exp z_v; logp = z_t - lse of the row's class t = tokens[i] (u32,
  * 0xFFFFFFFF for none: 0; any other t >= k is an error at the next synchronizing call, and
  * counts as none); entropy = -sum_v p_v log p_v with p_v = exp(z_v - lse); the `top` (at most
  * EMH_MAX_TOP) likeliest classes and their log probabilities, the likeliest first, of equal logits

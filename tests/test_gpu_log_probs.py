@@ -195,6 +195,40 @@ def test_rows_with_few_classes_and_values_that_are_not_finite(dev, n, k, name):
     assert np.isnan(g[3:6]).all()
 
 
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("k", [40, 9000])
+def test_masks_of_the_lowest_value(dev, name, k):
+    """Masked by the type's lowest value, and by twice it through the scale: infinite in f32 and
+    bf16, where a class has no probability then, and not in f16. Rows: all masked; all but two."""
+    from emeans_amd import F32, U32
+    low = {"f32": np.finfo(np.float32).min, "f16": -65504.0, "bf16": -(2.0 - 2.0 ** -7) * 2.0 ** 127}[name]
+    z = np.full((2, k), low)
+    z[1, [3, k - 2]] = 1.0, 2.0
+    p, t = R.Padded(dev, z, name), dev.upload_u32(np.array([7, k - 2], np.uint32))
+    out = [dev.zeros(c, F32) for c in (2, 2, 2, 8)] + [dev.zeros(8, U32)]
+    one, dz = dev.upload_f32(np.ones(2)), R.Padded(dev, 0 * z, name)
+    for scale in (1.0, 2.0):
+        dev.log_probs(p.buf, 2, k, t, out[0], out[1], entropy=out[2], top=4, top_logp=out[3],
+                      top_ids=out[4], scale=scale)
+        lp, lse, h, tops, ids = (dev.read(o) for o in out)
+        none = scale == 2 and name != "f16"
+        if none:
+            assert np.isneginf([lp[0], lse[0]]).all() and h[0] == 0
+            assert (ids[:4] == A.NONE).all() and np.isneginf(tops[:4]).all()
+        else:  # all alike
+            assert np.allclose([lp[0], -h[0], *tops[:4]], -np.log(k), rtol=1e-6)
+            assert np.array_equal(ids[:4], [0, 1, 2, 3])
+        q = 1 / (1 + np.exp(-scale))
+        assert np.allclose([lp[1], *tops[4:6]], np.log([q, q, 1 - q]), rtol=1e-6)
+        assert np.allclose(h[1], -q * np.log(q) - (1 - q) * np.log(1 - q), rtol=1e-6)
+        assert np.array_equal(ids[4:], [k - 2, 3] + ([A.NONE] * 2 if none else [0, 1]))
+        dev.log_probs_grad(p.buf, 2, k, t, out[1], dz.buf, entropy=out[2], glogp=one,
+                           gentropy=one, scale=scale)
+        g = dz.read()
+        assert (g[1, [c for c in range(k) if c not in (3, k - 2)]] == 0).all()
+        assert np.isfinite(g).all() and (not none or (g[0] == 0).all())
+
+
 def test_a_class_out_of_range_is_an_error(dev):
     from emeans_amd import F32, EmeansHipInvalid
     z, tokens, _ = _inputs(5, 30, 1, masks=False)
