@@ -22,10 +22,10 @@
 // element of the row.
 //
 // Bound by HBM (one read; one read and one write): 4,096 x 131,071 bf16 190 us, 5.7 TB/s, with
-// the 8 likeliest 209 us; the gradient 408 us, 5.3 TB/s. Next by the instructions, 11 issue slots an
+// the 8 likeliest 212 us; the gradient 408 us, 5.3 TB/s. Next by the instructions, 11 issue slots an
 // element forward, and with a list some 450 a row and chunk, which bound short rows: 10,007 x
-// 1,000 f32 8.8 us, with the 5 likeliest 13.0. A few rows are latency: of 131,071 4.5 us, with
-// the 8 likeliest 9.1.
+// 1,000 f32 8.8 us, with the 5 likeliest 13.1. A few rows are latency: of 131,071 4.5 us, with
+// the 8 likeliest 8.9.
 #include "emh_answer.h"
 #include "emh_types.h"
 
@@ -481,22 +481,24 @@ __global__ __launch_bounds__(256, least_waves<T>(W, NV, TOP, PARTS)) void k_logp
           uint64_t* const room = rooms[wave];
           const uint32_t old = (uint32_t)__popcll(__ballot(best.key != 0));
           uint32_t count = 0;
+          // A bit for every element of the lane's, the first the highest.
+          uint32_t bits = 0;
 #pragma unroll
-          for (int j = 0; j < NV; j++) {
-            const uint32_t col = (uint32_t)r.column(v0 + j * 64);
+          for (int j = 0; j < NV; j++)
 #pragma unroll
-            for (int e = 0; e < N; e++) {
-              const float q = x[j].get(e);
-              const bool is = q >= least;
-              const uint64_t them = __ballot(is);
-              if (them) {
-                const uint32_t at = count + __builtin_amdgcn_mbcnt_hi(
-                                                (uint32_t)(them >> 32),
-                                                __builtin_amdgcn_mbcnt_lo((uint32_t)them, 0u));
-                if (is && at < ROOM) room[at] = key_of(q, col + e);
-                count += (uint32_t)__popcll(them);
-              }
+            for (int e = 0; e < N; e++) bits = bits + bits + (x[j].get(e) >= least ? 1u : 0u);
+          const bool single = (bits & (bits - 1)) == 0;  // then it is the lane's largest
+          for (uint64_t them; count <= ROOM && (them = __ballot(bits != 0));) {
+            const uint32_t at = __builtin_amdgcn_mbcnt_hi(
+                (uint32_t)(them >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)them, count));
+            const uint32_t bit = 31u - (uint32_t)__clz((int)bits), slot = NV * N - 1 - bit;
+            const uint32_t v = v0 + slot / N * 64, e = slot % N;
+            if (bits != 0 && at < ROOM) {
+              const float q = single ? most : to_f32(r.base[(size_t)v * N + e]);
+              room[at] = key_of(q, (uint32_t)r.column(v) + e);
             }
+            bits &= ~(1u << bit);
+            count += (uint32_t)__popcll(them);
           }
           if (count + old <= ROOM) {
             best.merge(a.top, room, count);
