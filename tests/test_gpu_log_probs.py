@@ -345,3 +345,32 @@ def test_a_captured_call_replays(dev, n, k):
         call()
         assert got == [dev.read(b).tobytes() for b in outs]
     g.close()
+
+
+def test_two_contexts_at_once(dev):
+    """Rows in parts on two contexts, queued in turns without a wait: each has counters and
+    parts of its own. A first call may not be captured: they do not exist yet."""
+    from emeans_amd import BF16, F32, U32, EmeansHipInvalid, HipDevice
+    n, k, top = 40, 30000, 8
+    other = HipDevice()
+    z = np.random.default_rng(8).standard_normal((2, n, k))
+    b = []
+    for d, v in zip((dev, other), z):
+        o = dict(z=d.zeros(n * k, BF16), lse=d.zeros(n, F32), h=d.zeros(n, F32),
+                 ids=d.zeros(n * top, U32))
+        d.write(o["z"], 0, R.encode(v, "bf16").reshape(-1))
+        d.sync()
+        b.append(o)
+    call = lambda d, o: d.log_probs(o["z"], n, k, None, None, o["lse"], entropy=o["h"],  # noqa: E731
+                                    top=top, top_ids=o["ids"])
+    with pytest.raises(EmeansHipInvalid, match="before the capture"):
+        A.Graph(other, lambda: call(other, b[1]))
+    for _ in range(20):
+        for d, o in zip((dev, other), b):
+            call(d, o)
+    for d, o, v in zip((dev, other), b, z):
+        ref = A.LogProbs(R.decode(R.encode(v, "bf16"), "bf16"))
+        assert np.array_equal(d.read(o["ids"]).reshape(n, top), ref.top(top)[0])
+        assert np.abs(d.read(o["lse"]) - ref.lse).max() <= 1e-5 * np.abs(ref.lse).max()
+        assert np.abs(d.read(o["h"]) - ref.h).max() <= 1e-5 * ref.h.max()
+    other.close()
