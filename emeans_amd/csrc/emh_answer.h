@@ -31,6 +31,8 @@ struct RmsArgs {
   size_t lds;
   float* rstd;     // forward: or null
   float* part;     // backward: [workgroup][d], or null
+  void* dw;        // backward: dweight, where one workgroup has all of its sums; or null
+  int dwkind;
 };
 void launch_rms_norm(emh_ctx* c, const RmsArgs& a);
 void launch_rms_norm_grad(emh_ctx* c, RmsArgs a, const MatOut& dweight);

@@ -259,7 +259,7 @@ __global__ __launch_bounds__(TB, TB / 256) void k_rms_grad(const RmsArgs a) {
       one(now, r0 + g);
     }
   }
-  if (!a.part) return;
+  if (!a.part && !a.dw) return;
   // The groups' sums of a column, added through LDS.
   static_assert(G > 1, "groups to add");
 #pragma unroll
@@ -275,7 +275,10 @@ __global__ __launch_bounds__(TB, TB / 256) void k_rms_grad(const RmsArgs a) {
     float s = 0.f;
 #pragma unroll 8
     for (int k = 0; k < G; k++) s += fold[i * TB + k * LPR + l];
-    out[c.at + i % N] = s;
+    if (a.dw)
+      store_kind(a.dw, a.dwkind, c.at + i % N, s);
+    else
+      out[c.at + i % N] = s;
   }
 }
 
@@ -557,7 +560,10 @@ void launch_rms_norm_grad(emh_ctx* c, RmsArgs a, const MatOut& dweight) {
           constexpr int TB = decltype(threads)::value;
           constexpr size_t G = TB / S::LPR;
           parts = std::min((a.rows + G - 1) / G, (size_t)c->cus);
-          if (dweight.p) a.part = (float*)c->rms_part.get(parts * d * 4, c->stream);
+          if (parts == 1)
+            a.dw = dweight.p, a.dwkind = dweight.kind;
+          else if (dweight.p)
+            a.part = (float*)c->rms_part.get(parts * d * 4, c->stream);
           k_rms_grad<T, S::LPR, S::NV, TB><<<dim3((unsigned)parts), TB, 0, c->stream>>>(a);
         };
         constexpr int HELD = S::NV * VecOf<T>::N;
@@ -577,7 +583,8 @@ void launch_rms_norm_grad(emh_ctx* c, RmsArgs a, const MatOut& dweight) {
       if (a.y)
         k_rms_grad_wide<T><<<dim3((unsigned)std::min(a.rows, MAX_GROUPS)), 256, 0, c->stream>>>(a);
     });
-  if (dweight.p)
+  // (One workgroup's sums are dweight: 8 rows of 1,024 bf16 4.4 us, with a second launch 8.0.)
+  if (dweight.p && !a.dw)
     k_rms_sums<<<dim3((unsigned)std::min((d + 15) / 16, MAX_GROUPS)), 1024, 0, c->stream>>>(
         a.part, (int)parts, (int)d, dweight.p, dweight.kind);
   EMH_HIP(hipGetLastError());
