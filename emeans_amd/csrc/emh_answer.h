@@ -30,11 +30,12 @@ struct RmsArgs {
   float* scale;    // not null: y is codes
   size_t lds;
   float* rstd;     // forward: or null
+  bool through;    // forward: h and y pass through the caches
   float* part;     // backward: [workgroup][d], or null
   void* dw;        // backward: dweight, where one workgroup has all of its sums; or null
   int dwkind;
 };
-void launch_rms_norm(emh_ctx* c, const RmsArgs& a);
+void launch_rms_norm(emh_ctx* c, RmsArgs a);
 void launch_rms_norm_grad(emh_ctx* c, RmsArgs a, const MatOut& dweight);
 // Codes of x (rows x d), a scale for every `tall` rows (1 or CODE_BLOCK) by CODE_BLOCK columns.
 void launch_quantize(emh_ctx* c, const MatIn& x, size_t rows, size_t d, bool tall, uint8_t* q,

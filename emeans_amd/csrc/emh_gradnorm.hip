@@ -85,7 +85,7 @@ __device__ __forceinline__ void scale_chunk(const T* p, T* o, size_t count, floa
     float x[N];
 #pragma unroll
     for (int e = 0; e < N; e++) x[e] = v.get(e) * f;
-    STREAM ? stream_vec(o + i * N, x) : store_vec(o + i * N, x);
+    STREAM ? stream_vec(o + i * N, x) : put_vec(true, o + i * N, x);
   }
   const size_t i = whole * N + threadIdx.x;
   if (i < count) o[i] = from_f32<T>(to_f32(p[i]) * f);

@@ -251,20 +251,22 @@ __device__ __forceinline__ void sixteen(const v4f (*acc)[YB], int y, uint32_t* o
     }
   }
 }
+// Where results go: into the caches, through them or past them.
+enum Way { CACHED, THROUGH, PAST };
 // Sixteen bytes of a row to p; `left` elements from p on are the row's.
-template <class T, bool STREAM>
+template <class T, Way WAY>
 __device__ __forceinline__ void store_row(T* p, const v4u& v, uint32_t left) {
   const Vec<T> out{make_uint4(v[0], v[1], v[2], v[3])};
   constexpr uint32_t EL = 16 / sizeof(T);
   if (left >= EL)
-    STREAM ? stream_vec(p, out) : store_vec(p, out);
+    WAY == PAST ? stream_vec(p, out) : put_vec(WAY == THROUGH, p, out);
   else if (left > 0)
     store_some(p, out, (int)left);
 }
 // The same of a 16-bit row that may begin at an odd multiple of two bytes: then an element
 // later, by whole words; after: the row's next word. The first element of what a wave has of the
 // row, and the last of its last (last) sixteen bytes, are left to the caller.
-template <class T, bool STREAM>
+template <class T, Way WAY>
 __device__ __forceinline__ void store_odd_row(T* p, const v4u& v, uint32_t after, bool last,
                                               uint32_t left) {
   const uint32_t odd = (uint32_t)((uintptr_t)p >> 1) & 1, by = 16 * odd;
@@ -278,18 +280,17 @@ __device__ __forceinline__ void store_odd_row(T* p, const v4u& v, uint32_t after
     typedef uint32_t three __attribute__((ext_vector_type(3), aligned(4)));
     *reinterpret_cast<three*>(p + 1) = three{s[0], s[1], s[2]};
   } else {
-    store_row<T, STREAM>(p + odd, s, min(n, last ? 8 - odd : 8u));
+    store_row<T, WAY>(p + odd, s, min(n, last ? 8 - odd : 8u));
   }
 }
 
-// EXACT: f32 results by f16 MFMAs; else T results by 8-bit ones. STREAM: results that are
-// larger than the caches go past them.
+// EXACT: f32 results by f16 MFMAs; else T results by 8-bit ones.
 //
 // A workgroup takes tiles in turn, and the blocks of all its tiles are one stream: while a
 // tile's last blocks are multiplied, the next one's first are on their way, and while its
 // results go out of the registers, too. (A workgroup for every tile: 8,192^3 538 us, so 455;
 // 16,384 x 768 x 1,024 bf16 21.6 us, so 18.5.)
-template <class T, class S, bool EXACT, bool STREAM>
+template <class T, class S, bool EXACT, Way WAY>
 __global__ __launch_bounds__(S::THREADS, 2) void k_tile8(const Prod8Args a) {
   __shared__ __attribute__((aligned(1024))) char ring[2 * S::STAGE];
   __shared__ __attribute__((aligned(16))) char out[S::NW * 16 * 144];
@@ -545,7 +546,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_tile8(const Prod8Args a) {
           if (sizeof(T) == 2 && a.odd) {
             if constexpr (sizeof(T) == 2) {
               const bool last = i + 1 == PIECES && place == 7;
-              store_odd_row<T, STREAM>(p, v, *reinterpret_cast<const uint32_t*>(from + 16), last,
+              store_odd_row<T, WAY>(p, v, *reinterpret_cast<const uint32_t*>(from + 16), last,
                                        left);
               // The first element of the wave's, from its first piece, and the last.
               if (i == 0) single[h] = v[0], some[h] = left > 0;
@@ -554,7 +555,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_tile8(const Prod8Args a) {
                 *(p + (last ? 7 : -i * 8 * (int)EL)) = __builtin_bit_cast(T, (uint16_t)single[h]);
             }
           } else {
-            store_row<T, STREAM>(p, v, stored ? EL : left);
+            store_row<T, WAY>(p, v, stored ? EL : left);
           }
         }
         wave_fence8();
@@ -574,9 +575,10 @@ void launch_tiles(emh_ctx* c, const CodedIn& x, size_t n, size_t d, const CodedI
   a.t.c = {{(const char*)w.q, nullptr}, (uint32_t)w.ld, (uint32_t)k, 0};
   a.t.slabs = (uint32_t)((d + CODE_BLOCK - 1) / CODE_BLOCK);
   a.t.passes = 1, a.t.splits = 1;
-  // Where rows begin at whole 64 bytes: pieces of them are put together in the caches.
-  const bool stream = n * k * sizeof(T) >= STREAM_FROM && y.ld * sizeof(T) % 64 == 0 &&
-                      (uintptr_t)y.p % 64 == 0;
+  // Rows that do not begin at whole 64 bytes: their pieces are put together in the caches. Others
+  // go through them (16,384 x 768 x 1,024 bf16 17.0 us, written back at the end 18.5), and past
+  // them where they are larger.
+  const bool whole = y.ld * sizeof(T) % 64 == 0 && (uintptr_t)y.p % 64 == 0;
   a.t.ctiles = (uint32_t)((k + S::TC - 1) / S::TC);
   a.t.rtiles = (uint32_t)((n + S::TR - 1) / S::TR);
   EMH_ENSURE((size_t)a.t.ctiles * a.t.rtiles <= (size_t(1) << 30) / GROUP,
@@ -587,10 +589,13 @@ void launch_tiles(emh_ctx* c, const CodedIn& x, size_t n, size_t d, const CodedI
   a.t.r = {{(const char*)x.q, nullptr}, (uint32_t)x.ld, (uint32_t)n, 0};
   const unsigned blocks = prepare(a.t);
   const unsigned grid = std::min(blocks, (unsigned)(c->cus * S::PER_CU));
-  if (stream)
-    k_tile8<T, S, EXACT, true><<<grid, S::THREADS, 0, c->stream>>>(a);
+  auto go = [&](auto kernel) { kernel<<<grid, S::THREADS, 0, c->stream>>>(a); };
+  if (!whole)
+    go(k_tile8<T, S, EXACT, CACHED>);
+  else if (n * k * sizeof(T) < STREAM_FROM)
+    go(k_tile8<T, S, EXACT, THROUGH>);
   else
-    k_tile8<T, S, EXACT, false><<<grid, S::THREADS, 0, c->stream>>>(a);
+    go(k_tile8<T, S, EXACT, PAST>);
 }
 
 }  // namespace

@@ -121,6 +121,16 @@ __device__ __forceinline__ void store_some(T* p, const float* v, int left) {
     if (e < left) p[e] = from_f32<T>(v[e]);
 }
 
+// Stores that pass through the caches to memory at once: what a kernel leaves in them is written
+// back at its end, when nothing else is left to do (a few us for the 32 MB that they hold). Where
+// lines are stored in parts they cost more than they save. (Two idle cycles: the data's registers
+// may be written next.)
+template <class T>
+__device__ __forceinline__ void through_vec(T* p, const Vec<T>& v) {
+  typedef uint32_t any16 __attribute__((ext_vector_type(4)));
+  const any16 q{v.raw.x, v.raw.y, v.raw.z, v.raw.w};
+  asm volatile("global_store_dwordx4 %0, %1, off sc1\n\ts_nop 1" ::"v"(p), "v"(q) : "memory");
+}
 // Stores of what no cache need keep.
 template <class T>
 __device__ __forceinline__ void stream_vec(T* p, const Vec<T>& v) {
@@ -128,7 +138,7 @@ __device__ __forceinline__ void stream_vec(T* p, const Vec<T>& v) {
   __builtin_nontemporal_store(any16{v.raw.x, v.raw.y, v.raw.z, v.raw.w}, reinterpret_cast<any16*>(p));
 }
 template <class T>
-__device__ __forceinline__ void stream_vec(T* p, const float* v) {
+__device__ __forceinline__ Vec<T> vec_of(const float* v) {
   uint32_t w[4];
 #pragma unroll
   for (int e = 0; e < 4; e++) {
@@ -137,7 +147,19 @@ __device__ __forceinline__ void stream_vec(T* p, const float* v) {
     else
       w[e] = pair_from_f32<T>(v[2 * e], v[2 * e + 1]);
   }
-  stream_vec(p, Vec<T>{make_uint4(w[0], w[1], w[2], w[3])});
+  return Vec<T>{make_uint4(w[0], w[1], w[2], w[3])};
+}
+template <class T>
+__device__ __forceinline__ void stream_vec(T* p, const float* v) {
+  stream_vec(p, vec_of<T>(v));
+}
+template <class T>
+__device__ __forceinline__ void put_vec(bool through, T* p, const Vec<T>& v) {
+  through ? through_vec(p, v) : store_vec(p, v);
+}
+template <class T>
+__device__ __forceinline__ void put_vec(bool through, T* p, const float* v) {
+  put_vec(through, p, vec_of<T>(v));
 }
 
 // Element i of a buffer whose kind is a run-time value (EMH_F32, EMH_F16,
