@@ -79,14 +79,22 @@ template <bool STREAM, class T>
 __device__ __forceinline__ void scale_chunk(const T* p, T* o, size_t count, float f) {
   constexpr int N = VecOf<T>::N;
   const size_t whole = count / N;
-#pragma unroll 4
-  for (size_t i = threadIdx.x; i < whole; i += 256) {
-    const Vec<T> v = load_vec(p + i * N);
+  auto put = [&](size_t i, const Vec<T>& v) __attribute__((always_inline)) {
     float x[N];
 #pragma unroll
     for (int e = 0; e < N; e++) x[e] = v.get(e) * f;
     STREAM ? stream_vec(o + i * N, x) : put_vec(true, o + i * N, x);
+  };
+  constexpr int AT_ONCE = 4;
+  size_t at = threadIdx.x;
+  for (; at + (AT_ONCE - 1) * 256 < whole; at += AT_ONCE * 256) {
+    Vec<T> v[AT_ONCE];
+#pragma unroll
+    for (int b = 0; b < AT_ONCE; b++) v[b] = load_vec(p + (at + b * 256) * N);
+#pragma unroll
+    for (int b = 0; b < AT_ONCE; b++) put(at + b * 256, v[b]);
   }
+  for (; at < whole; at += 256) put(at, load_vec(p + at * N));
   const size_t i = whole * N + threadIdx.x;
   if (i < count) o[i] = from_f32<T>(to_f32(p[i]) * f);
 }

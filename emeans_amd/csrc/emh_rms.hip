@@ -164,7 +164,7 @@ __global__ __launch_bounds__(256) void k_rms(const RmsArgs a) {
         const Coder code = Coder::of<LPB>(y, N);
         if (live && c.any()) {
           store_codes<N>(reinterpret_cast<uint8_t*>(a.y) + row * a.ldy, c.from, c.from - c.at, d,
-                         code, y);
+                         code, y, a.through);
           if (c.from % CODE_BLOCK == 0) a.scale[row * a.lds + c.from / CODE_BLOCK] = code.scale;
         }
       } else {
@@ -401,6 +401,7 @@ __global__ __launch_bounds__(256) void k_codes_rows(const T* __restrict__ x, siz
                                                     int d, int blocks, uint8_t* q, size_t ldq,
                                                     float* scale, size_t lds) {
   constexpr int N = VecOf<T>::N, LPB = CODE_BLOCK / N;
+  const bool whole = ldq % 64 == 0 && (uintptr_t)q % 64 == 0;
   const size_t units = rows * blocks, step = (size_t)gridDim.x * (256 / LPB);
   const int l = threadIdx.x % LPB;
   // (Whole waves leave together: lanes_max and Coder take all lanes.)
@@ -421,7 +422,7 @@ __global__ __launch_bounds__(256) void k_codes_rows(const T* __restrict__ x, siz
     for (int e = 0; e < N; e++) f[e] = v.get(e);
     const Coder code = Coder::of<LPB>(f, N);
     if (left > 0) {
-      store_codes<N>(q + row * ldq, col, 0, d, code, f);
+      store_codes<N>(q + row * ldq, col, 0, d, code, f, whole);
       if (l == 0) scale[row * lds + b] = code.scale;
     }
   }
@@ -435,6 +436,7 @@ __global__ __launch_bounds__(256) void k_codes_tiles(const T* __restrict__ x, si
                                                      size_t lds) {
   constexpr int N = VecOf<T>::N, LPB = CODE_BLOCK / N, RPP = 256 / LPB, P = CODE_BLOCK / RPP;
   __shared__ float2 red[4];
+  const bool whole = ldq % 64 == 0 && (uintptr_t)q % 64 == 0;
   const int l = threadIdx.x % LPB, r0 = threadIdx.x / LPB;
   for (size_t t = blockIdx.x; t < tiles; t += gridDim.x) {
     const size_t tr = t / blocks;
@@ -469,7 +471,7 @@ __global__ __launch_bounds__(256) void k_codes_tiles(const T* __restrict__ x, si
       float f[N];
 #pragma unroll
       for (int e = 0; e < N; e++) f[e] = v[p].get(e);
-      if (row < rows && left > 0) store_codes<N>(q + row * ldq, col, 0, d, code, f);
+      if (row < rows && left > 0) store_codes<N>(q + row * ldq, col, 0, d, code, f, whole);
     }
     __syncthreads();  // red is the next tile's
   }
