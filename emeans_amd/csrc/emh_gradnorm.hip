@@ -8,10 +8,11 @@
 // table on the device names); in the second every workgroup adds those sums, in one order, and so
 // has the norm and the factor, and scales its chunks, the last ones first: what the first launch
 // read last is what the caches may still hold, if results that exceed them go past them (131 M
-// bf16 elements 156 us, so 128). No atomics: results follow from the tensors alone.
+// bf16 elements 156 us, then 128). No atomics: results follow from the tensors alone.
 //
-// Bound by HBM: two reads and one write of an element (131,071 x 1,001 bf16 128 us, 6.1 TB/s of
-// those three, the second read in part from the caches; 99,072 f32, two launches, 5.6 to 7.5 us).
+// Bound by HBM: two reads and one write of an element (131,071 x 1,001 bf16 124 us, 6.3 TB/s of
+// those three, the second read in part from the caches; 99,072 f32, two launches, 5.6 to 7.5 us; 4 M
+// f32 10.1, results through the caches, without that 12.6).
 // Where the gradients are scaled in place and the factor is 1 the second read and the write are
 // left out.
 #include "emh_answer.h"

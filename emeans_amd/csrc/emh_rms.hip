@@ -14,7 +14,7 @@
 //
 // Bound by HBM: 3 elements and a byte, or 4 elements, moved per element forward, 4 backward.
 // 200,000 x 768 bf16: 239 us either way, 5.1 TB/s; to codes 220 us, 4.9 TB/s; codes alone 89 us,
-// 5.2 TB/s. 16,384 x 768, which the caches hold in part: 16.1, 21.8 and 17.9 us. One row of 1,024:
+// 5.2 TB/s. 16,384 x 768, which the caches hold in part: 16.1, 21.8, 17.9 and 7.9 us. One row of 1,024:
 // 4.6 us, its launch.
 #include "emh_answer.h"
 #include "emh_codes.h"
