@@ -255,7 +255,9 @@ __device__ __forceinline__ void finish(const LogpArgs& a, size_t row, const Give
   const uint32_t lane = threadIdx.x & 63;
   const float b = all.m == -INFINITY ? 0.f : all.m;
   const float ls = logf(all.s);
-  const bool odd = !(all.s < INFINITY);  // a NaN, or an infinite logit
+  // A NaN, an infinite logit, or one that the scale makes infinite (m: the others are
+  // -infinity beside it, and S is zero).
+  const bool odd = !(all.s < INFINITY) || all.m == INFINITY;
   if (lane == 0) {
     a.lse[row] = odd ? NAN : all.m == -INFINITY ? -INFINITY : all.m + ls;
     if (a.entropy) a.entropy[row] = odd ? NAN : all.s > 0.f ? ls - all.e / all.s : 0.f;
