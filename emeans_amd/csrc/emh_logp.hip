@@ -2,9 +2,12 @@
 // logits, and the gradient of the logits.
 //
 // With z = scale logits: lse = log sum exp z_v, log p_v = z_v - lse, H = -sum p_v log p_v. One
-// pass: a lane keeps the maximum m of what it has seen, S = sum exp(z - m) and E = sum exp(z -
-// m) (z - m), both moved to a new maximum by exp(m - m'); lanes, waves and parts of a row are
-// joined the same way, and lse = m + log S, H = log S - E / S, log p_t = (z_t - m) - log S.
+// pass: a lane keeps the largest logit m of what it has seen (before the scale), S = sum exp(d)
+// and E = sum exp(d) d with d = scale (x - m), both moved to a new largest by exp(scale (m - m'));
+// lanes, waves and parts of a row are joined the same way, and lse = scale m + log S, H = log S - E
+// / S, log p_t = scale (x_t - m) - log S. (The difference comes before the scale: then d of the
+// largest is 0 however large it is. Off by a rounding of scale m, it was 1e31 in a row masked by
+// f32's lowest value.) Exponents and E are in base 2.
 //
 // The likeliest classes: a wave keeps a sorted list in its lanes (lane i the i-th), the
 // larger logit first, the lower class among equals: an entry is one key of 64 bits, the logit's
@@ -27,13 +30,15 @@
 // to LDS a row and chunk, which short rows feel: 10,007 x 1,000 f32 8.8 us, with the 5
 // likeliest 13.1. A few rows are latency: of 131,071 4.5 us, with
 // the 8 likeliest 8.9.
+#include <cfloat>
+
 #include "emh_answer.h"
 #include "emh_types.h"
 
 namespace emh {
 namespace {
 
-constexpr float LOG2E = 1.44269504f;
+constexpr float LOG2E = 1.44269504f, LN2 = 0.693147181f;
 constexpr float FAR = -1e4f;  // below any logarithm of a positive f32
 constexpr uint32_t NONE = 0xFFFFFFFFu;
 
@@ -83,31 +88,38 @@ struct Row {
   }
 };
 
-// What a lane, a wave or a part of a row has seen: maximum, S and E (see above).
+// exp(scale (x - m)) = 2^power(x, half_of(m), base2(scale)). (Halves: the difference of two finite
+// logits does not overflow. Where the scale's product does it stays finite: 0 times it is 0.)
+__device__ __forceinline__ float base2(float scale) { return fminf(scale * (2.f * LOG2E), FLT_MAX); }
+__device__ __forceinline__ float half_of(float m) { return m == -INFINITY ? 0.f : 0.5f * m; }
+__device__ __forceinline__ float power(float x, float half, float by) {
+  return fmaf(x, 0.5f, -half) * by;
+}
+
+// What a lane, a wave or a part of a row has seen: the largest, S and E (see above).
 struct Seen {
   float m = -INFINITY, s = 0.f, e = 0.f;
   __device__ __forceinline__ Seen() {}
   __device__ __forceinline__ explicit Seen(float4 v) : m(v.x), s(v.y), e(v.z) {}
   __device__ __forceinline__ float4 packed() const { return make_float4(m, s, e, 0.f); }
-  // To the maximum `to`, at least m.
-  __device__ __forceinline__ void move(float to) {
-    const float b = to == -INFINITY ? 0.f : to;
-    const float d = fmaxf(m - b, -1e30f);  // (nothing seen: s is zero)
-    const float f = __builtin_amdgcn_exp2f(d * LOG2E);
+  // To the largest `to`, at least m.
+  __device__ __forceinline__ void move(float to, float by) {
+    const float d = fmaxf(power(m, half_of(to), by), FAR);  // (nothing seen: s is zero)
+    const float f = __builtin_amdgcn_exp2f(d);
     e = f * fmaf(s, d, e);
     s *= f;
     m = to;
   }
-  __device__ __forceinline__ void join(const Seen& o) {
+  __device__ __forceinline__ void join(const Seen& o, float by) {
     Seen t = o;
     const float to = fmaxf(m, o.m);
-    move(to);
-    t.move(to);
+    move(to, by);
+    t.move(to, by);
     s += t.s;
     e += t.e;
   }
-  __device__ __forceinline__ void join_lanes() {
-    move(lanes_max<64>(m));
+  __device__ __forceinline__ void join_lanes(float by) {
+    move(lanes_max<64>(m), by);
     s = lanes_sum<64>(s);
     e = lanes_sum<64>(e);
   }
@@ -253,30 +265,33 @@ struct Given {
 __device__ __forceinline__ void finish(const LogpArgs& a, size_t row, const Given& given,
                                        const Seen& all, const Best& best) {
   const uint32_t lane = threadIdx.x & 63;
-  const float b = all.m == -INFINITY ? 0.f : all.m;
+  // top + off: the scaled largest, exactly.
+  const float m = all.m == -INFINITY ? 0.f : all.m;
+  const float top = m * a.scale, off = fmaf(m, a.scale, -top);
+  // A NaN, an infinite logit, or one that the scale makes infinite.
+  const bool odd = !(all.s < INFINITY) || top == INFINITY;
+  const bool none = all.m == -INFINITY || top == -INFINITY;
   const float ls = logf(all.s);
-  // A NaN, an infinite logit, or one that the scale makes infinite (m: the others are
-  // -infinity beside it, and S is zero).
-  const bool odd = !(all.s < INFINITY) || all.m == INFINITY;
+  auto logp_of = [&](float z) __attribute__((always_inline)) {
+    if (odd) return (float)NAN;
+    return none || z * a.scale == -INFINITY ? -INFINITY : fmaf(z, a.scale, -top) - off - ls;
+  };
   if (lane == 0) {
-    a.lse[row] = odd ? NAN : all.m == -INFINITY ? -INFINITY : all.m + ls;
-    if (a.entropy) a.entropy[row] = odd ? NAN : all.s > 0.f ? ls - all.e / all.s : 0.f;
+    a.lse[row] = odd ? NAN : none ? -INFINITY : top + (off + ls);
+    if (a.entropy) a.entropy[row] = odd ? NAN : none ? 0.f : fmaf(-LN2, all.e / all.s, ls);
     if (a.logp) {
       float lp = 0.f;
-      if (given.t < a.k) {
-        lp = fmaf(given.z, a.scale, -b);
-        lp = odd ? NAN : all.s > 0.f ? lp - ls : -INFINITY;
-      } else if (given.t != NONE) {
+      if (given.t < a.k)
+        lp = logp_of(given.z);
+      else if (given.t != NONE)
         a.small[SW_BAD_CLASS] = 1u;
-      }
       a.logp[row] = lp;
     }
   }
   if (lane < a.top) {
-    const float z = key_value(best.key);
-    const bool is = best.key != 0 && !odd && z * a.scale > -INFINITY;
-    if (a.ids) a.ids[row * a.top + lane] = is ? key_class(best.key) : NONE;
-    if (a.tops) a.tops[row * a.top + lane] = odd ? NAN : is ? fmaf(z, a.scale, -b) - ls : -INFINITY;
+    const float lp = best.key != 0 ? logp_of(key_value(best.key)) : odd ? NAN : -INFINITY;
+    if (a.ids) a.ids[row * a.top + lane] = lp > -INFINITY ? key_class(best.key) : NONE;
+    if (a.tops) a.tops[row * a.top + lane] = lp;
   }
 }
 
@@ -322,7 +337,8 @@ __device__ __forceinline__ bool last_part(uint32_t* done, uint32_t parts) {
 // The parts of a row, by a wave. room: LDS for ROOM + ROOM_END.
 template <bool TOP>
 __device__ __forceinline__ void join_parts(const PartOut& in, size_t row, uint32_t parts,
-                                           uint32_t top, uint64_t* room, Seen& all, Best& best) {
+                                           uint32_t top, float by, uint64_t* room, Seen& all,
+                                           Best& best) {
   const uint32_t lane = threadIdx.x & 63;
   // (Entries come from lists of 64 - top at a time, so that these and a list of top have room.)
   const uint32_t count = parts * top, each = ROOM - top;
@@ -348,8 +364,8 @@ __device__ __forceinline__ void join_parts(const PartOut& in, size_t row, uint32
     }
   }
   all = Seen();
-  for (uint32_t p = lane; p < parts; p += 64) all.join(in.get_seen(row * parts + p));
-  all.join_lanes();
+  for (uint32_t p = lane; p < parts; p += 64) all.join(in.get_seen(row * parts + p), by);
+  all.join_lanes(by);
   if constexpr (TOP) {
     best.key = 0;
     // (At least top entries reach it.)
@@ -397,6 +413,7 @@ __global__ __launch_bounds__(256, least_waves<T>(W, NV, TOP, PARTS)) void k_logp
   const uint32_t lane = threadIdx.x & 63;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const uint32_t w = wave % W;
+  const float by = base2(a.scale);
   const size_t units = PARTS ? a.n * parts : a.n;
   for (size_t u0 = (size_t)blockIdx.x * ROWS; u0 < units; u0 += (size_t)gridDim.x * ROWS) {
     const size_t u = u0 + wave / W;
@@ -435,15 +452,14 @@ __global__ __launch_bounds__(256, least_waves<T>(W, NV, TOP, PARTS)) void k_logp
       for (int j = 0; j < NV; j++)
 #pragma unroll
         for (int e = 0; e < N; e++) most = fmaxf(most, x[j].get(e));
-      const float to = fmaxf(all.m, most * a.scale);
-      all.move(to);
-      const float b = to == -INFINITY ? 0.f : to;
+      all.move(fmaxf(all.m, most), by);
+      const float half = half_of(all.m);
 #pragma unroll
       for (int j = 0; j < NV; j++)
 #pragma unroll
         for (int e = 0; e < N; e++) {
-          const float d = fmaf(x[j].get(e), a.scale, -b);
-          const float p = __builtin_amdgcn_exp2f(d * LOG2E);
+          const float d = power(x[j].get(e), half, by);
+          const float p = __builtin_amdgcn_exp2f(d);
           all.s += p;
           all.e = fmaf(p, fmaxf(d, FAR), all.e);
         }
@@ -524,14 +540,14 @@ __global__ __launch_bounds__(256, least_waves<T>(W, NV, TOP, PARTS)) void k_logp
         }
       }
     }
-    all.join_lanes();
+    all.join_lanes(by);
     if constexpr (W > 1) {
       __syncthreads();  // (what the last unit left has been read)
       if (lane == 0) seen[wave] = all.packed();
       if (TOP && lane < a.top) lists[wave][lane] = best.key;
       __syncthreads();
       if (wave == 0) {
-        for (int i = 1; i < W; i++) all.join(Seen(seen[i]));
+        for (int i = 1; i < W; i++) all.join(Seen(seen[i]), by);
         if constexpr (TOP) {
           // All lists at once where there is room (places without an entry count as least).
           const uint32_t lists_at = (ROOM - a.top) / a.top >= W - 1 ? W - 1 : 1;
@@ -548,7 +564,7 @@ __global__ __launch_bounds__(256, least_waves<T>(W, NV, TOP, PARTS)) void k_logp
       if (lane == 0) out.put_seen(u, all);
       if (TOP && lane < a.top) share(out.best + u * a.top + lane, best.key);
       if (!last_part(out.done + row * DONE_STEP, parts)) continue;
-      join_parts<TOP>(out, row, parts, a.top, rooms[0], all, best);
+      join_parts<TOP>(out, row, parts, a.top, by, rooms[0], all, best);
     }
     finish(a, row, given, all, best);
   }

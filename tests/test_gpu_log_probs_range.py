@@ -70,3 +70,68 @@ def test_a_logit_that_the_scale_makes_infinite(dev, n, k, name, large, scale, to
         assert (ids[~bad] == ([0, 2, 3, 4, 5] if less else [0, 1, 2, 3, 4])).all()
     g = _grad(dev, bufs, scale, np.full(n, 1 / scale), np.full(n, 1 / scale))
     assert np.isnan(g[[0, 2]]).all() and np.isfinite(g[~bad]).all()
+
+
+LOW = {"f32": float(np.finfo(np.float32).min), "f16": -65504.0, "bf16": -(2.0 - 2.0 ** -7) * 2.0 ** 127}
+
+
+def _large_rows(n, k, name):
+    """Rows masked by the lowest value, wholly or but for one; two alike far above the others;
+    one among masked ones; all far below zero, two of them less so; large ones of both signs."""
+    low, big, far = LOW[name], *((60000.0, 60000.0) if name == "f16" else (1e10, 1e30))
+    z = np.zeros((n, k))
+    z[0] = low
+    z[1] = low
+    z[1, 7] = 5.0
+    z[2, [3, k - 2]] = big
+    z[3] = low
+    z[3, k // 2] = far
+    z[4] = -far
+    z[4, [1, k - 1]] = -far / 2
+    z[5] = np.random.default_rng(k).choice([-far, far, far / 4], k)
+    return z, np.array([7, 7, 3, k // 2, 1, 0] + [0] * (n - 6))
+
+
+class Exact:
+    """The same in 64 bits from differences (beside 1e38 these hold no logarithm of a sum)."""
+
+    def __init__(self, z, scale):
+        with np.errstate(invalid="ignore"):
+            m = z.max(1)
+            self.none = np.isneginf(m)
+            self.d = np.where(self.none[:, None], -np.inf, scale * (z - m[:, None]))
+        s = np.where(self.none, 1.0, np.exp(self.d).sum(1))
+        self.lp = self.d - np.log(s)[:, None]
+        self.lse = scale * m + np.log(s)
+        self.p = np.exp(self.lp)
+        self.h = -np.where(self.p > 0, self.p * np.where(self.p > 0, self.lp, 0), 0.0).sum(1)
+        self.order = np.argsort(-z, axis=1, kind="stable")
+
+    def top(self, m):
+        lp = np.take_along_axis(self.lp, self.order[:, :m], 1)
+        return np.where(np.isneginf(lp), A.NONE, self.order[:, :m]), lp
+
+
+@pytest.mark.parametrize("n,k", SHAPES)
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("scale", [0.7, 0.3, 1.3, 1e-30])
+def test_large_logits_and_a_scale_whose_products_are_not_exact(dev, n, k, name, scale):
+    """d = scale (z - m) is 0 for the largest, by each of k classes that are as large; a logit that
+    the scale makes -infinite is none."""
+    scale = float(np.float32(scale))
+    z, tokens = _large_rows(n, k, name)
+    (lp, lse, h, ids, tops), bufs = _call(dev, z, tokens, name, scale, 5)
+    v = bufs[0].value
+    with np.errstate(over="ignore"):
+        v = np.where(np.isneginf((v * scale).astype(np.float32)), -np.inf, v)
+    ref = Exact(v, scale)
+    # Sums of equal terms, or of one and what rounds to nothing beside it (1e-30: of k alike).
+    s = 4 * (k / 64 + 96) * U * (1 + np.log(k))
+
+    def near(a, b):
+        with np.errstate(invalid="ignore"):
+            return (a == b) | (np.abs(a - b) <= s + 4 * U * np.abs(b))
+    wi, wl = ref.top(5)
+    assert near(lse, ref.lse).all() and near(h, ref.h).all()
+    assert near(lp, ref.lp[np.arange(n), tokens]).all()
+    assert np.array_equal(ids, wi) and near(tops, wl).all()
