@@ -373,7 +373,8 @@ class HipDevice:
                        glogp: Optional[DevBuf] = None, gentropy: Optional[DevBuf] = None,
                        scale: float = 1.0, ldz: int = 0, lddz: int = 0):
         """The logits' gradient (z's kind, may be z) of the log probabilities weighted by glogp
-        and the entropies weighted by gentropy (F32, n entries)."""
+        and the entropies weighted by gentropy (F32, n entries). Probabilities are exp(z - lse)
+        of f32 values: off by a factor within exp(2^-23 |lse|)."""
         check(lib().emh_log_probs_grad(self._ctx, z.h, ldz, n, k, _h(tokens), scale, lse.h,
                                        _h(entropy), _h(glogp), _h(gentropy), dz.h, lddz))
 

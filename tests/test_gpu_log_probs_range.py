@@ -135,3 +135,20 @@ def test_large_logits_and_a_scale_whose_products_are_not_exact(dev, n, k, name, 
     assert near(lse, ref.lse).all() and near(h, ref.h).all()
     assert near(lp, ref.lp[np.arange(n), tokens]).all()
     assert np.array_equal(ids, wi) and near(tops, wl).all()
+
+
+@pytest.mark.parametrize("n,k", SHAPES)
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("scale", [0.7, 0.3, 1.0])
+def test_gradients_of_large_logits(dev, n, k, name, scale):
+    """Rows that count nothing get zeros whatever their logits, and all of them finite values; a
+    class that is alone has p = 1, and its row no gradient."""
+    scale = float(np.float32(scale))
+    z, tokens = _large_rows(n, k, name)
+    _, bufs = _call(dev, z, tokens, name, scale, 0)
+    zero, one = np.zeros(n), np.random.default_rng(3).standard_normal(n)
+    assert (_grad(dev, bufs, scale, zero, zero) == 0).all()
+    g = _grad(dev, bufs, scale, one, one)
+    assert np.isfinite(g).all()
+    assert (g[[1, 3]] == 0).all()
+    assert g[6:].any() or n == 6
