@@ -612,7 +612,7 @@ class GradNorm:
 
     def norm(self, out: DevBuf, max_norm: float = float("inf"), scale: float = 1.0):
         """out (F32, 2 entries) = the norm of scale times the gradients, and the factor that
-        brings it to max_norm (1 where it is below; NaN where it is not finite)."""
+        brings it to max_norm (1 where it is below; NaN where it is not finite in F32)."""
         check(lib().emh_grad_norm_measure(self._h, scale, max_norm, out.h))
 
     def clip(self, out: DevBuf, max_norm: float, scale: float = 1.0):

@@ -108,7 +108,7 @@ __device__ __forceinline__ float2 norm_of(const double* sums, uint32_t nsums, fl
   for (uint32_t i = threadIdx.x; i < nsums; i += 256) s += sums[i];
   s = group_sum(s, red);
   const double norm = fabs((double)scale) * sqrt(s);
-  finite = norm < (double)INFINITY;  // (f32 squares do not overflow f64)
+  finite = (float)norm < INFINITY;  // (as out holds it)
   float f = 1.f;
   if (!finite)
     f = NAN;

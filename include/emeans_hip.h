@@ -541,7 +541,7 @@ int emh_grad_norm_create(emh_ctx* ctx, const emh_buf* const* grads, emh_buf* con
                          size_t count, emh_grad_norm** out);
 /* out[0] = norm = |scale| sqrt(sum of all elements' squares) (summed in f64), out[1] = min(1,
  * max_norm / norm) (f32, 2 entries; max_norm may be infinite; scale: 1 / the loss's, if it was
- * scaled). A norm that is not finite has a NaN as out[1]. */
+ * scaled). A norm that is not finite in f32 has a NaN as out[1]. */
 int emh_grad_norm_measure(emh_grad_norm* plan, float scale, float max_norm, emh_buf* out);
 /* The same, and every gradient times out[1] (where that is a NaN, as it is) to its output. */
 int emh_grad_norm_clip(emh_grad_norm* plan, float scale, float max_norm, emh_buf* out);
