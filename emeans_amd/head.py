@@ -16,7 +16,7 @@ step all the same).
 
 `answer` gives the likeliest clusters of resident rows, with their log probabilities and the
 answers' entropies, in 8 bits: the normalized rows and the classes as codes (rms_norm or
-quantize), their product8, log_probs.
+quantize), their product8 in F32, log_probs.
 
 `python -m emeans_amd.head` runs this on synthetic rows.
 """
@@ -219,8 +219,9 @@ class ClusterHead:
         stride, blocks = HipDevice.code_stride(d), HipDevice.code_blocks(d)
         codes, scales = dev.zeros(rows * stride, F8), dev.zeros(rows * blocks, F32)
         normed = None if self.rms else dev.zeros(rows * d, self.kind)
-        # (F16 does not hold every logit that training's f32 does: of 65,536 and more.)
-        logits = dev.zeros(rows * k, BF16 if self.kind == BF16 else F32)
+        # F32 whatever the head's kind, as in training: in BF16 logits of 256 are 2 apart, and F16
+        # ends at 65,504.
+        logits = dev.zeros(rows * k, F32)
         ids, logp = dev.zeros(n * top, U32), dev.zeros(n * top, F32)
         lse, entropy = dev.zeros(n, F32), dev.zeros(n, F32)
         given = None if labels is None else dev.zeros(n, F32)
