@@ -284,7 +284,8 @@ __global__ __launch_bounds__(TB, TB / 256) void k_rms_grad(const RmsArgs a) {
 
 // Rows too long for the registers of a workgroup (or shorter than a vector): one workgroup a
 // row, which it reads twice. What it writes an element's own thread has read (h may be x or r, y
-// may be x).
+// may be x). A thread's sum is f64 here, of up to 65,536 elements: in f32 equal ones were off by
+// 0.1 %.
 template <class T, bool CODES>
 __global__ __launch_bounds__(256) void k_rms_wide(const RmsArgs a) {
   __shared__ float red[2][4];
@@ -296,12 +297,12 @@ __global__ __launch_bounds__(256) void k_rms_wide(const RmsArgs a) {
     auto sum = [&](int i) __attribute__((always_inline)) {
       return r ? from_f32<T>(to_f32(x[i]) + to_f32(r[i])) : x[i];
     };
-    float q = 0.f;
+    double q = 0.0;
     for (int i = threadIdx.x; i < a.d; i += 256) {
-      const float o = to_f32(sum(i));
-      q = fmaf(o, o, q);
+      const double o = to_f32(sum(i));
+      q = fma(o, o, q);
     }
-    const float rstd = 1.0f / sqrtf(row_sum<256, 256>(q, red, slot) / (float)a.d + a.eps);
+    const float rstd = 1.0f / sqrtf(row_sum<256, 256>((float)q, red, slot) / (float)a.d + a.eps);
     slot ^= 1;
     if (threadIdx.x == 0 && a.rstd) a.rstd[row] = rstd;
     auto y_of = [&](int i) __attribute__((always_inline)) {
@@ -341,10 +342,11 @@ __global__ __launch_bounds__(256) void k_rms_grad_wide(const RmsArgs a) {
     const T* dh = a.r ? reinterpret_cast<const T*>(a.r) + row * a.ldr : nullptr;
     T* o = reinterpret_cast<T*>(a.y) + row * a.ldy;
     const float rstd = a.rstd[row];
-    float c = 0.f;
+    double sum = 0.0;
     for (int i = threadIdx.x; i < a.d; i += 256)
-      c = fmaf(to_f32(dy[i]) * (a.w ? load_kind(a.w, a.wkind, i) : 1.f), to_f32(h[i]) * rstd, c);
-    c = row_sum<256, 256>(c, red, slot) / (float)a.d;
+      sum = fma((double)(to_f32(dy[i]) * (a.w ? load_kind(a.w, a.wkind, i) : 1.f)),
+                (double)(to_f32(h[i]) * rstd), sum);
+    const float c = row_sum<256, 256>((float)sum, red, slot) / (float)a.d;
     slot ^= 1;
     for (int i = threadIdx.x; i < a.d; i += 256) {
       const float g = to_f32(dy[i]) * (a.w ? load_kind(a.w, a.wkind, i) : 1.f);
@@ -354,19 +356,20 @@ __global__ __launch_bounds__(256) void k_rms_grad_wide(const RmsArgs a) {
     }
   }
 }
-// Their sums over rows: a thread a column, blockIdx.y a share of the rows.
+// Their sums over rows: a thread a column, blockIdx.y a share of the rows (f64: rows shorter than
+// a vector may be many millions).
 template <class T>
 __global__ __launch_bounds__(256) void k_rms_cols(const RmsArgs a) {
   const int col = blockIdx.x * 256 + threadIdx.x;
   if (col >= a.d) return;
   const size_t per = (a.rows + gridDim.y - 1) / gridDim.y;
   const size_t lo = min(a.rows, blockIdx.y * per), hi = min(a.rows, lo + per);
-  float s = 0.f;
+  double s = 0.0;
 #pragma unroll 4
   for (size_t r = lo; r < hi; r++)
-    s = fmaf(to_f32(reinterpret_cast<const T*>(a.dy)[r * a.lddy + col]),
-             to_f32(reinterpret_cast<const T*>(a.x)[r * a.ldx + col]) * a.rstd[r], s);
-  a.part[(size_t)blockIdx.y * a.d + col] = s;
+    s = fma((double)to_f32(reinterpret_cast<const T*>(a.dy)[r * a.lddy + col]),
+            (double)(to_f32(reinterpret_cast<const T*>(a.x)[r * a.ldx + col]) * a.rstd[r]), s);
+  a.part[(size_t)blockIdx.y * a.d + col] = (float)s;
 }
 
 // out = the nparts rows of sums added: 16 columns a workgroup, 64 shares of the rows in step
