@@ -284,8 +284,8 @@ __global__ __launch_bounds__(TB, TB / 256) void k_rms_grad(const RmsArgs a) {
 
 // Rows too long for the registers of a workgroup (or shorter than a vector): one workgroup a
 // row, which it reads twice. What it writes an element's own thread has read (h may be x or r, y
-// may be x). A thread's sum is f64 here, of up to 65,536 elements: in f32 equal ones were off by
-// 0.1 %.
+// may be x). A thread's sum is f64 here, of up to 65,536 elements: in f32 equal ones' sum was
+// off by 0.06 %.
 template <class T, bool CODES>
 __global__ __launch_bounds__(256) void k_rms_wide(const RmsArgs a) {
   __shared__ float red[2][4];

@@ -481,8 +481,8 @@ int emh_adamw_destroy(emh_adamw* plan);
  * their kind; rstd = 1 / sqrt(mean(h^2) + eps), y = h rstd weight. weight (d entries, x's kind or
  * f32) may be NULL (ones). h may be NULL, x or residual. y: x's kind, may be x or residual (not
  * what h is), scales NULL; or f8 codes of the unrounded result with a scale for every row and
- * block. rstd (f32, rows entries; may be NULL) is for the gradient. Squares are f32: a row's
- * largest element lies below 2^63. d <= 2^24. */
+ * block. rstd (f32, rows entries; may be NULL) is for the gradient. The sum of a row's squares is
+ * f32: elements below 2^64 / sqrt(d) do not exceed it; a row whose sum does has rstd 0. d <= 2^24. */
 int emh_rms_norm(emh_ctx* ctx, const emh_buf* x, size_t ldx, const emh_buf* residual, size_t ldr,
                  size_t rows, size_t d, const emh_buf* weight, float eps, emh_buf* h, size_t ldh,
                  emh_buf* y, size_t ldy, emh_buf* scales, size_t lds, emh_buf* rstd);

@@ -57,3 +57,23 @@ def test_many_short_rows(dev, rows, d):
     dev.rms_norm_grad(dy, x, rows, d, None, rstd, None, dw)
     want = rows * float(np.float32(0.9)) * float(np.float32(1.1)) * _rstd(1.1)
     assert np.all(np.abs(dev.read(dw) - want) <= (64 + 24) * U * want)
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [64, 1000, 9001])
+def test_the_largest_sums_of_squares(dev, name, d):
+    """Elements just below 2^64 / sqrt(d) have a norm; a row whose sum exceeds f32 has rstd 0."""
+    from emeans_amd import F32
+    r = np.random.default_rng(d)
+    x = r.choice([-1.0, 1.0], (2, d)) * 0.98 * 2.0 ** 64 / np.sqrt(d)
+    x[1] *= 1.1
+    px, py = R.Padded(dev, x, name), R.Padded(dev, 0 * x, name)
+    rstd = dev.zeros(2, F32)
+    dev.rms_norm(px.buf, 2, d, None, py.buf, rstd=rstd, eps=EPS)
+    v = px.value[0]
+    want = 1 / np.sqrt((v * v).mean())
+    got = dev.read(rstd)
+    assert abs(got[0] - want) <= 2 * (d / 16 + 32) * U * want and got[1] == 0
+    y = py.read()
+    assert np.all(np.abs(y[0] - v * want) <= (2 * (d / 16 + 32) * U + R.UNIT[name]) * 1.01)
+    assert not y[1].any()
