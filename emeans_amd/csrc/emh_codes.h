@@ -69,9 +69,10 @@ struct Coder {
 
 // The codes of N (4 or 8) columns from `col` on, the first `skip` of v other columns', to a
 // row of codes (its start 16-byte aligned); zeros from the row's d columns to its next
-// multiple of 16. through: eight codes pass through the caches at once (emh_types.h): 16,384 x
-// 768 bf16 coded in 7.7 us, written back at the end in 8.6; but 30,000 x 1,000, whose rows of
-// 1,008 bytes straddle lines, 19.9 and 17.4.
+// multiple of 16. through: eight codes pass through the caches at once (emh_types.h). Coding alone does
+// that where rows of codes are whole 64 bytes (16,384 x 768 bf16 7.8 us, written back at the end 8.6;
+// 30,000 x 1,000, whose 1,008 bytes straddle lines, 19.9 and 17.4); the norm by its rows' size
+// (launch_rms_norm).
 template <int N>
 __device__ __forceinline__ void store_codes(uint8_t* row, int col, int skip, int d, const Coder& c,
                                             const float* v, bool through) {

@@ -12,7 +12,8 @@
 //
 // Bound by HBM: two reads and one write of an element (131,071 x 1,001 bf16 124 us, 6.3 TB/s of
 // those three, the second read in part from the caches; 99,072 f32, two launches, 5.6 to 7.5 us; 4 M
-// f32 10.1, results through the caches, without that 12.6).
+// f32 10.1, results through the caches, without that 12.6; at odd addresses 10.9 and 12.7, and 50 M
+// bf16 50.6 and 50.1).
 // Where the gradients are scaled in place and the factor is 1 the second read and the write are
 // left out.
 #include "emh_answer.h"

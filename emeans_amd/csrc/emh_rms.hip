@@ -531,7 +531,9 @@ bool by_shape(size_t d, F&& f) {
 void launch_rms_norm(emh_ctx* c, RmsArgs a) {
   if (a.rows == 0) return;
   // Up to 16 MB of rows through the caches: 4,096 x 1,024 f32 8.2 us, written back 10.3; to codes 7.3
-  // and 10.5; 25 MB take the same time either way, longer rows longer.
+  // and 10.5; 25 MB take the same time either way, longer rows longer. At any address: 10,007 x 300
+  // f16 to codes 5.8, with codes written back 6.3, h too 6.9; 8,000 x 999 bf16 10.0 and 12.1 (codes
+  // 10.5 and 13.6); f32 4,000 x 1,001 9.7 and 9.3, the only one slower of a dozen.
   a.through = a.rows * (size_t)a.d * kind_bytes(a.kind) <= size_t(16) << 20;
   by_kind(a.kind, [&](auto t) {
     using T = decltype(t);
