@@ -70,7 +70,7 @@ struct Coder {
 // The codes of N (4 or 8) columns from `col` on, the first `skip` of v other columns', to a
 // row of codes (its start 16-byte aligned); zeros from the row's d columns to its next
 // multiple of 16. through: eight codes pass through the caches at once (emh_types.h). Coding alone does
-// that where rows of codes are whole 64 bytes (16,384 x 768 bf16 7.8 us, written back at the end 8.6;
+// that where rows of codes are whole 64 bytes (16,384 x 768 bf16 7.9 us, written back at the end 8.6;
 // 30,000 x 1,000, whose 1,008 bytes straddle lines, 19.9 and 17.4); the norm by its rows' size
 // (launch_rms_norm).
 template <int N>

@@ -28,11 +28,11 @@
 // element of the row.
 //
 // Bound by HBM (one read; one read and one write): 4,096 x 131,071 bf16 190 us, 5.7 TB/s, with
-// the 8 likeliest 212 us; the gradient 408 us, 5.3 TB/s. Next by the instructions, 11 issue slots an
+// the 8 likeliest 215 us; the gradient 409 us, 5.3 TB/s. Next by the instructions, 11 issue slots an
 // element forward, and with a list by its steps, a chain of some 400 instructions and ten visits
 // to LDS a row and chunk, which short rows feel: 10,007 x 1,000 f32 8.8 us, with the 5
-// likeliest 13.1. A few rows are latency: of 131,071 4.5 us, with
-// the 8 likeliest 8.9.
+// likeliest 13.4. A few rows are latency: of 131,071 4.5 us, with
+// the 8 likeliest 9.1.
 #include <cfloat>
 
 #include "emh_answer.h"

@@ -12,10 +12,11 @@
 // f32 results take the f16 MFMA (an f16 holds every code exactly): 5e-8. For 16-bit results of few
 // rows that costs 5.6 us instead of 5.1 (1 x 1,024 x 16,384), and 29.3 instead of 22.2 (131,071 classes).
 //
-// Bound by the matrix cores where all three sizes are large (8,192^3: 455 us, 2.4 PFLOP/s; f32 935 us,
+// Bound by the matrix cores where all three sizes are large (8,192^3: 458 us, 2.4 PFLOP/s; f32 935 us,
 // 1.2), by the results' bytes where the depth is short (8,192 x 1,024 x 131,072 bf16 1.14 ms, 2.1
 // GB; k = 131,071, whose rows straddle lines and stay in the caches on their way, 1.61 ms), and
-// by the classes' bytes and latency where rows are few (1 x 1,024 x 16,384: 5.5 us; 64: 9.5 us).
+// by the classes' bytes and latency where rows are few (1 x 1,024 x 16,384: 5.1 us, from memory 5.8; 64
+// rows: 9.3, f32 12.5).
 //
 // Few rows read the classes as they lie. More of them go in tiles: a workgroup owns 256 x
 // 256 or 128 x 128 of the result, and a block of the depth, 128 bytes a row of both operands,
@@ -89,7 +90,7 @@ __device__ __forceinline__ v4f block8(v8i a, v8i b) {
 
 // Few rows: a workgroup takes 16 classes and 16 YB rows, its four waves the blocks of the depth
 // by turns; operands come from memory as they lie, AHEAD blocks of a wave's on their way at once.
-// Bound by the classes' bytes: 1 x 1,024 x 16,384 5.5 us with its launch, 16.8 MB at 3.1 TB/s.
+// Bound by the classes' bytes: 1 x 1,024 x 16,384 5.1 us with its launch, 16.8 MB at 3.3 TB/s.
 template <int YB, bool EXACT>
 __global__ __launch_bounds__(256) void k_few8(const CodedIn x, size_t n, uint32_t d, const CodedIn w,
                                               size_t k, void* y, size_t ldy, int kind,

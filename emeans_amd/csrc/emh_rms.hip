@@ -13,9 +13,10 @@
 // added by a second launch, in an order that follows from the sizes.
 //
 // Bound by HBM: 3 elements and a byte, or 4 elements, moved per element forward, 4 backward.
-// 200,000 x 768 bf16: 239 us either way, 5.1 TB/s; to codes 220 us, 4.9 TB/s; codes alone 89 us,
-// 5.2 TB/s. 16,384 x 768, which the caches hold in part: 16.1, 21.8, 17.9 and 7.9 us. One row of 1,024:
-// 4.6 us, its launch.
+// 200,000 x 768 bf16: 236 us and 240, 5.2 TB/s; to codes 221 us, 4.9 TB/s; codes alone 89 us, 5.2
+// TB/s. 16,384 x 768, which the caches hold in part: 16.3, 21.9, 17.9 and 7.9 us. One row of 1,024:
+// 4.5 us, its launch. Rows that no workgroup holds (k_rms_wide and what follows it) are read by single
+// elements: 4,096 x 16,384 bf16 206 us, backward 385, to codes 280.
 #include "emh_answer.h"
 #include "emh_codes.h"
 
@@ -501,7 +502,7 @@ bool by_shape(size_t d, F&& f) {
   const size_t v = (d + N - 1) / N;
   // A row on as many lanes as one block of codes has: 100,000 x 256 bf16 to codes 30.2 us, x 128
   // f32 26.3 (on 64 lanes 36.9 and 29.1). Longer rows, two vectors on 32 lanes, take as long
-  // or longer (10,007 x 300 f16 6.9, so 6.6).
+  // or longer (10,007 x 300 f16 6.9, so 6.6, both with stores that were written back).
   constexpr int PAIR = N == 8 ? 16 : 32;
   if (d < N)
     return false;

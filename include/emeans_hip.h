@@ -464,7 +464,8 @@ int emh_adamw_destroy(emh_adamw* plan);
  * in the reference): a root-mean-square norm, 8-bit codes and their product, log probabilities
  * of logits, their gradients, and the norm of all gradients. The conventions are those of the
  * learning operators. A graph captured from the context's stream may be replayed as long
- * as the buffers live; graphs of one context share its workspace, so one replay follows another.
+ * as the buffers and plans live; graphs of one context share its workspace, so one replay follows
+ * another.
  * A call whose workspace does not exist yet is refused during a capture: make it once before.
  *
  * Codes: an f8 matrix has rows that begin at multiples of 16 bytes (its address and its
