@@ -152,3 +152,22 @@ def test_gradients_of_large_logits(dev, n, k, name, scale):
     assert np.isfinite(g).all()
     assert (g[[1, 3]] == 0).all()
     assert g[6:].any() or n == 6
+
+
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("scale", [1.0, 0.7])
+@pytest.mark.parametrize("size", [20.0, 3000.0, 60000.0])
+def test_how_far_a_gradient_of_large_logits_is_off(dev, name, scale, size):
+    """Two classes alike far above the others: p is a half, off by a factor within exp(2^-23 |lse|)
+    and the roundings of lse's own logarithm and of the result."""
+    scale = float(np.float32(scale))
+    n, k = 3, 1000
+    z = np.full((n, k), -size)
+    z[:, [1, 998]] = size
+    (lp, lse, h, _, _), bufs = _call(dev, z, np.ones(n), name, scale, 0)
+    assert np.abs(lp + np.log(2)).max() <= 200 * U and np.abs(h - np.log(2)).max() <= 200 * U
+    g = _grad(dev, bufs, scale, np.ones(n), np.zeros(n))
+    off = np.expm1(2.0 ** -23 * scale * size) + 200 * U
+    want = np.array([0.5, -0.5]) * scale
+    assert np.all(np.abs(g[:, [1, 998]] - want) <= scale * 0.5 * off + R.UNIT[name] * scale)
+    assert (np.delete(g, [1, 998], 1) == 0).all() or size == 20.0
