@@ -275,9 +275,11 @@ __device__ __forceinline__ void finish(const LogpArgs& a, size_t row, const Give
   const bool odd = !(all.s < INFINITY) || top == INFINITY;
   const bool none = all.m == -INFINITY || top == -INFINITY;
   const float ls = logf(all.s);
+  auto some = [&](float z) __attribute__((always_inline)) {  // it has a probability
+    return !odd && !none && z * a.scale > -INFINITY;
+  };
   auto logp_of = [&](float z) __attribute__((always_inline)) {
-    if (odd) return (float)NAN;
-    return none || z * a.scale == -INFINITY ? -INFINITY : fmaf(z, a.scale, -top) - off - ls;
+    return odd ? (float)NAN : some(z) ? fmaf(z, a.scale, -top) - off - ls : -INFINITY;
   };
   if (lane == 0) {
     a.lse[row] = odd ? NAN : none ? -INFINITY : top + (off + ls);
@@ -292,9 +294,10 @@ __device__ __forceinline__ void finish(const LogpArgs& a, size_t row, const Give
     }
   }
   if (lane < a.top) {
-    const float lp = best.key != 0 ? logp_of(key_value(best.key)) : odd ? NAN : -INFINITY;
-    if (a.ids) a.ids[row * a.top + lane] = lp > -INFINITY ? key_class(best.key) : NONE;
-    if (a.tops) a.tops[row * a.top + lane] = lp;
+    // (Of a finite logit it may be -infinity: 6e38 below the largest.)
+    const float z = best.key != 0 ? key_value(best.key) : -INFINITY;
+    if (a.ids) a.ids[row * a.top + lane] = some(z) ? key_class(best.key) : NONE;
+    if (a.tops) a.tops[row * a.top + lane] = logp_of(z);
   }
 }
 

@@ -171,3 +171,15 @@ def test_how_far_a_gradient_of_large_logits_is_off(dev, name, scale, size):
     want = np.array([0.5, -0.5]) * scale
     assert np.all(np.abs(g[:, [1, 998]] - want) <= scale * 0.5 * off + R.UNIT[name] * scale)
     assert (np.delete(g, [1, 998], 1) == 0).all() or size == 20.0
+
+
+@pytest.mark.parametrize("n,k", SHAPES)
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+def test_classes_whose_log_probability_is_beyond_f32(dev, n, k, name):
+    """Their logits are finite: they are among the likeliest, in their order, with -infinity."""
+    z = np.full((n, k), -np.inf)
+    z[:, [2, 5, k - 1]] = -3e38, -2e38, 3e38
+    (lp, lse, h, ids, tops), _ = _call(dev, z, np.full(n, 2), name, 1.0, 4)
+    assert np.isneginf(lp).all() and (h == 0).all() and np.isfinite(lse).all()
+    assert (ids == [k - 1, 5, 2, A.NONE]).all()
+    assert (tops[:, 0] == 0).all() and np.isneginf(tops[:, 1:]).all()
