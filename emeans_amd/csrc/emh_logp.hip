@@ -610,12 +610,13 @@ __global__ __launch_bounds__(256) void k_logp_grad(const LogpArgs a, uint32_t ch
     float gh = a.gentropy ? a.gentropy[row] * a.scale : 0.f;
     const float h = a.gentropy ? a.entropy_in[row] : 0.f;
     if (lse == -INFINITY) lse = gl = gh = 0.f;  // no class may be answered: zeros
+    if (lse != lse) gl = NAN;                   // (the bounds of d hold no NaN)
+    const float glh = fmaf(gh, h, gl);
     auto one = [&](float q, bool own) __attribute__((always_inline)) {
-      // (Rounded as lse's largest was: a class alone has p = 1 at any size of logits. At most 0,
-      // which a NaN passes.)
-      const float z1 = q * a.scale - lse, d = z1 > 0.f ? 0.f : z1;
+      // (Rounded as lse's largest was: a class alone has p = 1 at any size of logits. From FAR to 0.)
+      const float d = __builtin_amdgcn_fmed3f(q * a.scale - lse, FAR, 0.f);
       const float p = __builtin_amdgcn_exp2f(d * LOG2E);
-      const float g = -p * fmaf(gh, fmaxf(d, FAR) + h, gl);
+      const float g = -p * fmaf(gh, d, glh);
       return own ? g + gl : g;
     };
 #pragma unroll
