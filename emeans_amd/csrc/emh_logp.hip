@@ -31,7 +31,7 @@
 // the 8 likeliest 215 us; the gradient 409 us, 5.3 TB/s. Next by the instructions, 11 issue slots an
 // element forward, and with a list by its steps, a chain of some 400 instructions and ten visits
 // to LDS a row and chunk, which short rows feel: 10,007 x 1,000 f32 8.8 us, with the 5
-// likeliest 13.4. A few rows are latency: of 131,071 4.5 us, with
+// likeliest 13.3. A few rows are latency: of 131,071 4.5 us, with
 // the 8 likeliest 9.1.
 #include <cfloat>
 
@@ -458,7 +458,10 @@ __global__ __launch_bounds__(256, least_waves<T>(W, NV, TOP, PARTS)) void k_logp
       for (int j = 0; j < NV; j++)
 #pragma unroll
         for (int e = 0; e < N; e++) most = fmaxf(most, x[j].get(e));
-      all.move(fmaxf(all.m, most), by);
+      if constexpr (W == 1)
+        all.m = most;  // (a row's only chunk: nothing to move)
+      else
+        all.move(fmaxf(all.m, most), by);
       const float half = half_of(all.m);
 #pragma unroll
       for (int j = 0; j < NV; j++)
